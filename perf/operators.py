@@ -73,6 +73,15 @@ def _width(rng, low, high):
 
 MAX_FLOPS = 6.8e10   # of the largest listed product
 MAX_BYTES = 1.2e8    # of the largest listed product's weights; of the longest listed cache
+MAX_APPEND = 7e7     # of the largest listed append
+MAX_HELD = 1.35e8    # of the longest listed cache's keys
+
+
+def _large(case):
+    """Whether an attention case passes the largest listed ones, in what it moves, computes or holds."""
+    queries, values = case["heads"] * case["queries"], case["kv_heads"] * case["head_dim"]
+    return (work(case)["bytes"] > MAX_BYTES or work(case)["flops"] > MAX_FLOPS
+            or case["batch"] * case["capacity"] * max(values, queries) > MAX_HELD)
 
 
 def draw(rng):
@@ -89,16 +98,19 @@ def draw(rng):
     kv_heads = rng.choice([1, 2, 4, 8, 12])
     if kind == "append":
         capacity = _log_int(rng, 64, 8192)
-        return dict(kind=kind, batch=_log_int(rng, 1, 16), time=rng.choice([1, _log_int(rng, 1, min(capacity, 2000))]),
+        case = dict(kind=kind, batch=_log_int(rng, 1, 16), time=rng.choice([1, _log_int(rng, 1, min(capacity, 2000))]),
                     kv_heads=min(kv_heads, 8), head_dim=head_dim, capacity=capacity, ragged=rng.randint(1, 10 ** 6))
+        while work(case)["bytes"] > MAX_APPEND:
+            case["time"] = case["time"] * 2 // 3
+        return case
     queries = 1 if rng.random() < 0.6 else _log_int(rng, 2, 1000)
     longest = _log_int(rng, max(16, queries), 65536 if queries == 1 else 4096)
     case = dict(kind=kind, batch=_log_int(rng, 1, 16 if queries == 1 else 3), heads=kv_heads * rng.choice([1, 1, 2, 4, 8]),
                 kv_heads=kv_heads, head_dim=head_dim, queries=queries, capacity=longest + rng.randint(0, 512),
                 longest=longest, ragged=rng.randint(0, 10 ** 6))
-    while case["batch"] > 1 and (work(case)["bytes"] > MAX_BYTES or work(case)["flops"] > MAX_FLOPS):
+    while _large(case) and case["batch"] > 1:
         case["batch"] -= 1
-    while case["kv_heads"] > 1 and (work(case)["bytes"] > MAX_BYTES or work(case)["flops"] > MAX_FLOPS):
+    if _large(case):
         case["heads"], case["kv_heads"] = case["heads"] // case["kv_heads"], 1
     return case
 
