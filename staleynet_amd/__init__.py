@@ -6,8 +6,9 @@ This package holds its sources (``csrc/``), the build (``build.py``), the
 C++ host mirror (``host/``) and the Python mirror of the reference API
 (``gemm.py``).
 """
-from .gemm import (BatchStrides, Gpu, GpuError, Mask, MatmulKernel, MatmulPanic, MatmulSpec, Precision, Shape,
-                   Storage, Tensor, WriteMode, library, status_string, validate)
+from .gemm import (BatchStrides, ByteBuffer, Fp4Cache, Fp4Matrix, Gpu, GpuError, Mask, MatmulKernel, MatmulPanic,
+                   MatmulSpec, Precision, Shape, Storage, Tensor, WriteMode, library, status_string, validate)
 
-__all__ = ["BatchStrides", "Gpu", "GpuError", "Mask", "MatmulKernel", "MatmulPanic", "MatmulSpec", "Precision",
-           "Shape", "Storage", "Tensor", "WriteMode", "library", "status_string", "validate"]
+__all__ = ["BatchStrides", "ByteBuffer", "Fp4Cache", "Fp4Matrix", "Gpu", "GpuError", "Mask", "MatmulKernel",
+           "MatmulPanic", "MatmulSpec", "Precision", "Shape", "Storage", "Tensor", "WriteMode", "library",
+           "status_string", "validate"]

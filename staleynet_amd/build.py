@@ -21,7 +21,7 @@ INCLUDE = os.path.join(REPO_ROOT, "include")
 SOURCES = ["context.cpp", "gemm_f32.hip", "gemm_f32_unaligned.hip", "gemm_dma.hip", "gemm_bf16.hip",
            "gemm_simple.hip", "gemv.hip", "bias.hip", "softmax.hip", "loss.hip", "heads.hip", "attention.hip", "attention_forward.hip", "bf16_stage.hip",
            "synth.hip", "route.hip", "noalloc.hip", "attention_backward.hip",
-           "gemm_bf16_wide.hip"]
+           "gemm_bf16_wide.hip", "fp4.cpp", "fp4_quantize.hip", "fp4_matmul.hip", "fp4_attention.hip"]
 
 # Packed-fp32 instructions are switched off: some of their forms have given
 # wrong results on these machines, and the kernels here never need them.

@@ -12,14 +12,8 @@
 #include <cstring>
 #include <new>
 
+#include "context_internal.h"
 #include "gemm_internal.h"
-
-struct sn_context {
-    int device = 0;
-    hipStream_t stream = nullptr;
-    uint32_t kernel = SN_KERNEL_MFMA_F32;
-    sn::Env env;
-};
 
 // The C structs' layouts are part of the ABI a Rust #[repr(C)] binding
 // mirrors (x86-64 / aarch64 LP64): sizes and field offsets pinned here.

@@ -1,0 +1,266 @@
+// fp32 to 4-bit blocks and back (staleynet_fp4.h has the format): weights
+// (sn_quantize_fp4, sn_dequantize_fp4) and rows of a key/value cache
+// (sn_fp4_cache_append, sn_fp4_cache_read).
+//
+// For a block of 32 values with largest magnitude A = m 2^x, m in [0.5, 1): the
+// factor is 2^e, e = x - 3 (which puts A in [4, 8) factors), or x - 2 where
+// m >= 7/8; codes are the values times 2^-e rounded to nearest, ties to even.
+// The scaling is by a power of two, so each step is exact but the one rounding,
+// which v_cvt_scalef32_pk_fp4_f32 does (its result was compared at every tie, its
+// neighbours, past the largest code and at -0).
+//
+// All are bound by memory: 4 bytes a value on the fp32 side against 0.53. Four
+// lanes take a block, eight values each: 32-byte loads or stores, a word of codes a
+// lane, so a wave's codes are 256 contiguous bytes; the maximum is exchanged over
+// four lanes.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "fp4_device.h"
+#include "fp4_internal.h"
+
+namespace sn {
+namespace fp4 {
+namespace {
+
+constexpr int kThreads = 256;
+
+// The block's scale byte from its largest magnitude's bits (as an integer, so
+// that infinities and NaN are the largest).
+__device__ __forceinline__ uint32_t scale_byte(uint32_t magnitude) {
+    if (magnitude == 0) return 0;
+    if (magnitude >= 0x7f800000u) return 255;
+    // A >= 2^-126: its exponent field is x + 126, and its fraction is at least 3/4
+    // where m >= 7/8. Subnormals are under 2^-126, where the factor is at its least.
+    const int32_t s = int32_t(magnitude >> 23) - 2 + ((magnitude & 0x007fffffu) >= 0x00600000u ? 1 : 0);
+    return uint32_t(min(max(s, 0), int32_t(kLargestScale)));
+}
+
+// Eight values of a block, four neighbouring lanes a block: this lane's word of
+// codes, and the block's scale byte. Every lane of the four has to call it.
+__device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t& s) {
+    uint32_t magnitude = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) magnitude = max(magnitude, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+    magnitude = max(magnitude, uint32_t(__shfl_xor(int(magnitude), 1)));
+    magnitude = max(magnitude, uint32_t(__shfl_xor(int(magnitude), 2)));
+    s = scale_byte(magnitude);
+    if (s > kLargestScale) return 0;
+    const float factor = factor_of(s);
+    uint32_t word = 0;
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], factor, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], factor, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], factor, 2);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], factor, 3);
+    return word;
+}
+
+__device__ __forceinline__ void dequantize8(uint32_t word, uint32_t s, float (&v)[8]) {
+    const float factor = factor_of(s);
+    const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, factor, 0);
+    const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, factor, 1);
+    const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, factor, 2);
+    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, factor, 3);
+    v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
+}
+
+// One weight block a thread where the operand's columns are contiguous (reads
+// of neighbouring threads are neighbouring columns), else four lanes a block.
+__global__ __launch_bounds__(kThreads) void quantize_columns_kernel(WeightArgs a) {
+    const int64_t blocks = blocks_of(a.inner);
+    const int64_t c = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+    if (c >= a.cols) return;
+    for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
+        const float* from = a.source + c * a.col_step + b * kBlock * a.inner_step;
+        float v[32];
+        uint32_t magnitude = 0;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            v[i] = b * kBlock + i < a.inner ? from[i * a.inner_step] : 0.f;
+            magnitude = max(magnitude, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+        }
+        const uint32_t s = scale_byte(magnitude);
+        const float factor = factor_of(s);
+        u32x4 words = {0, 0, 0, 0};
+        if (s <= kLargestScale) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t word = 0;
+                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * w], v[8 * w + 1], factor, 0);
+                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * w + 2], v[8 * w + 3], factor, 1);
+                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * w + 4], v[8 * w + 5], factor, 2);
+                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * w + 6], v[8 * w + 7], factor, 3);
+                words[w] = word;
+            }
+        }
+        *reinterpret_cast<u32x4*>(a.codes + (c * blocks + b) * kBlockBytes) = words;
+        a.scales[c * blocks + b] = uint8_t(s);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(WeightArgs a) {
+    const int64_t blocks = blocks_of(a.inner);
+    const int64_t eighths = a.cols * blocks * 4;
+    const int64_t stride = int64_t(gridDim.x) * kThreads;
+    // eighths is a multiple of 4: the four lanes of a block leave the loop together.
+    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < eighths; e += stride) {
+        const int64_t block = e >> 2, c = block / blocks, k = (block % blocks) * kBlock + 8 * (e & 3);
+        const float* from = a.source + c * a.col_step + k;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + i < a.inner ? from[i] : 0.f;
+        uint32_t s;
+        const uint32_t word = quantize8(v, s);
+        reinterpret_cast<uint32_t*>(a.codes)[e] = word;
+        if ((e & 3) == 0) a.scales[block] = uint8_t(s);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void dequantize_kernel(WeightArgs a) {
+    const int64_t blocks = blocks_of(a.inner);
+    const int64_t rows = blocks * 4;  // eights of values a column
+    const int64_t total = a.cols * rows;
+    const int64_t stride = int64_t(gridDim.x) * kThreads;
+    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < total; e += stride) {
+        // The contiguous side of the output first.
+        const bool columns = a.inner_step != 1;
+        const int64_t c = columns ? e % a.cols : e / rows, eighth = columns ? e / a.cols : e % rows;
+        const int64_t k = 8 * eighth;
+        float v[8];
+        dequantize8(reinterpret_cast<const uint32_t*>(a.codes)[c * rows + eighth],
+                    a.scales[c * blocks + eighth / 4], v);
+        float* to = a.output + c * a.col_step + k * a.inner_step;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (k + i < a.inner) to[i * a.inner_step] = v[i];
+    }
+}
+
+// Where eight values of a cache row are: e counts (sequence, time, head, eighth)
+// of keys and then of values, so that neighbouring lanes read neighbouring columns
+// of a packed row.
+struct CachePlace {
+    bool values, held;
+    int64_t b, t, h, eighth;
+    int64_t row;  // of the cache
+};
+__device__ __forceinline__ CachePlace cache_place(const CacheRowsArgs& a, int64_t e) {
+    const int64_t eighths = a.head_dim / 8;
+    CachePlace p;
+    p.eighth = e % eighths;
+    e /= eighths;
+    p.h = e % a.kv_heads;
+    e /= a.kv_heads;
+    p.values = e % 2 != 0;
+    e /= 2;
+    p.t = e % a.time;
+    p.b = e / a.time;
+    const int64_t at = (a.positions != nullptr ? int64_t(a.positions[p.b]) : a.position) + p.t;
+    p.held = at < a.capacity;
+    p.row = (p.b * a.kv_heads + p.h) * a.capacity + at;
+    return p;
+}
+
+template <bool VECTOR>
+__global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheRowsArgs a, int64_t total) {
+    const int64_t stride = int64_t(gridDim.x) * kThreads;
+    // total is a multiple of 4 and a block's four lanes share b and t: they go together.
+    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < total; e += stride) {
+        const CachePlace p = cache_place(a, e);
+        if (!p.held) continue;
+        const float* from = a.packed + (p.b * a.time + p.t) * a.width + (p.values ? a.value_column : a.key_column) +
+                            p.h * a.head_dim + 8 * p.eighth;
+        float v[8];
+        if (VECTOR) {
+            const f32x4 lo = reinterpret_cast<const f32x4*>(from)[0], hi = reinterpret_cast<const f32x4*>(from)[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = from[i];
+        }
+        uint32_t s;
+        const uint32_t word = quantize8(v, s);
+        uint8_t* codes = p.values ? a.v_codes : a.k_codes;
+        uint8_t* scales = p.values ? a.v_scales : a.k_scales;
+        reinterpret_cast<uint32_t*>(codes)[p.row * (a.head_dim / 8) + p.eighth] = word;
+        if ((p.eighth & 3) == 0) scales[p.row * (a.head_dim / kBlock) + p.eighth / 4] = uint8_t(s);
+    }
+}
+
+template <bool VECTOR>
+__global__ __launch_bounds__(kThreads) void cache_read_kernel(CacheRowsArgs a, int64_t total) {
+    const int64_t stride = int64_t(gridDim.x) * kThreads;
+    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < total; e += stride) {
+        const CachePlace p = cache_place(a, e);
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (p.held) {
+            const uint8_t* codes = p.values ? a.v_codes : a.k_codes;
+            const uint8_t* scales = p.values ? a.v_scales : a.k_scales;
+            dequantize8(reinterpret_cast<const uint32_t*>(codes)[p.row * (a.head_dim / 8) + p.eighth],
+                        scales[p.row * (a.head_dim / kBlock) + p.eighth / 4], v);
+        }
+        float* to = (p.values ? a.values : a.keys) + ((p.b * a.kv_heads + p.h) * a.time + p.t) * a.head_dim +
+                    8 * p.eighth;
+        if (VECTOR) {
+            reinterpret_cast<f32x4*>(to)[0] = f32x4{v[0], v[1], v[2], v[3]};
+            reinterpret_cast<f32x4*>(to)[1] = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[i] = v[i];
+        }
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Enough workgroups for every thread to have one item, at most 2^20 (the
+// kernels loop over the rest).
+unsigned grid_of(int64_t items) {
+    const int64_t groups = (items + kThreads - 1) / kThreads;
+    return unsigned(groups < (int64_t(1) << 20) ? groups : int64_t(1) << 20);
+}
+
+}  // namespace
+
+hipError_t launch_quantize(const WeightArgs& a, hipStream_t stream) {
+    const int64_t blocks = blocks_of(a.inner);
+    if (a.cols == 0 || blocks == 0) return hipSuccess;
+    if (a.inner_step == 1) {
+        hipLaunchKernelGGL(quantize_rows_kernel, dim3(grid_of(a.cols * blocks * 4)), dim3(kThreads), 0, stream, a);
+    } else {
+        const dim3 grid(unsigned((a.cols + kThreads - 1) / kThreads), unsigned(blocks < 65535 ? blocks : 65535));
+        hipLaunchKernelGGL(quantize_columns_kernel, grid, dim3(kThreads), 0, stream, a);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_dequantize(const WeightArgs& a, hipStream_t stream) {
+    const int64_t blocks = blocks_of(a.inner);
+    if (a.cols == 0 || blocks == 0) return hipSuccess;
+    hipLaunchKernelGGL(dequantize_kernel, dim3(grid_of(a.cols * blocks * 4)), dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_append(const CacheRowsArgs& a, hipStream_t stream) {
+    const int64_t total = 2 * a.batch * a.time * a.kv_heads * (a.head_dim / 8);
+    if (total == 0) return hipSuccess;
+    const bool vector =
+        aligned16(a.packed) && a.width % 4 == 0 && a.key_column % 4 == 0 && a.value_column % 4 == 0;
+    hipLaunchKernelGGL(vector ? cache_append_kernel<true> : cache_append_kernel<false>, dim3(grid_of(total)),
+                       dim3(kThreads), 0, stream, a, total);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_read(const CacheRowsArgs& a, hipStream_t stream) {
+    const int64_t total = 2 * a.batch * a.time * a.kv_heads * (a.head_dim / 8);
+    if (total == 0) return hipSuccess;
+    const bool vector = aligned16(a.keys) && aligned16(a.values);
+    hipLaunchKernelGGL(vector ? cache_read_kernel<true> : cache_read_kernel<false>, dim3(grid_of(total)),
+                       dim3(kThreads), 0, stream, a, total);
+    return hipGetLastError();
+}
+
+}  // namespace fp4
+}  // namespace sn

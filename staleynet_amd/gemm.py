@@ -258,6 +258,88 @@ class CHeadLayout(ctypes.Structure):
                                                      "time_capacity", "time_offset")]
 
 
+FP4_BLOCK = 32  # SN_FP4_BLOCK (include/staleynet_fp4.h): values of a 4-bit block
+FP4_FEW_ROWS = 64  # SN_FP4_FEW_ROWS
+
+
+class CFp4CacheShape(ctypes.Structure):
+    """``sn_fp4_cache_shape`` (include/staleynet_fp4.h)."""
+
+    _fields_ = [(name, ctypes.c_size_t) for name in ("batch", "kv_heads", "capacity", "head_dim")]
+
+
+class CFp4CacheRows(ctypes.Structure):
+    """``sn_fp4_cache_rows``."""
+
+    _fields_ = [(name, ctypes.c_size_t) for name in ("time", "position", "width", "key_column", "value_column")]
+
+
+class CFp4AttentionShape(ctypes.Structure):
+    """``sn_fp4_attention_shape``."""
+
+    _fields_ = [(name, ctypes.c_size_t) for name in ("heads", "queries", "keys", "q_sequence", "q_head", "q_row",
+                                                     "out_sequence", "out_head", "out_row")] + \
+        [("scale", ctypes.c_float)]
+
+
+class ByteBuffer:
+    """Bytes in device memory: the codes or the scales of 4-bit blocks."""
+
+    def __init__(self, gpu: "Gpu", pointer: int, count: int):
+        self._gpu = gpu
+        self.pointer = pointer
+        self._count = count
+
+    def __len__(self) -> int:
+        return self._count
+
+    def free(self) -> None:
+        if self.pointer and self._gpu._ctx:  # as Tensor.free
+            self._gpu._check(_library().sn_free_bytes(self._gpu._ctx, ctypes.c_void_p(self.pointer)), "free_bytes")
+        self.pointer = 0
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+@dataclass(frozen=True)
+class Fp4Matrix:
+    """A product's right operand ``[inner, cols]`` in 4 bits (include/staleynet_fp4.h): per column
+    ``ceil(inner / 32)`` blocks of 16 bytes of codes, and one scale byte a block."""
+
+    cols: int
+    inner: int
+    codes: ByteBuffer
+    scales: ByteBuffer
+
+
+@dataclass(frozen=True)
+class Fp4Cache:
+    """A key/value cache ``[batch][kv_heads][capacity][head_dim]`` in 4 bits (include/staleynet_fp4.h)."""
+
+    batch: int
+    kv_heads: int
+    capacity: int
+    head_dim: int
+    k_codes: ByteBuffer
+    k_scales: ByteBuffer
+    v_codes: ByteBuffer
+    v_scales: ByteBuffer
+
+    def to_c(self) -> CFp4CacheShape:
+        return CFp4CacheShape(self.batch, self.kv_heads, self.capacity, self.head_dim)
+
+    def buffers(self) -> list:
+        """The four buffers as the C ABI takes them: pointer and bytes each."""
+        out = []
+        for b in (self.k_codes, self.k_scales, self.v_codes, self.v_scales):
+            out += [ctypes.c_void_p(b.pointer), len(b)]
+        return out
+
+
 class TokenBuffer:
     """Token ids (u32) in device memory (``TokenBuffer``, device.rs:35-36)."""
 
@@ -372,6 +454,21 @@ def _library() -> ctypes.CDLL:
         lib.sn_plan_matmul_column_sums.argtypes = lib.sn_plan_matmul.argtypes
         lib.sn_matmul_noalloc.argtypes = [ctypes.POINTER(CMatmulSpec), ctypes.c_void_p, size, ctypes.c_void_p, size,
                                           ctypes.c_void_p, size, ctypes.c_void_p]
+        u8p = ctypes.POINTER(ctypes.c_uint8)
+        operand = [ctypes.c_void_p, size]
+        lib.sn_alloc_bytes.argtypes = [ctx, size, ctypes.POINTER(ctypes.c_void_p)]
+        lib.sn_upload_bytes.argtypes = [ctx, u8p, size, ctypes.POINTER(ctypes.c_void_p)]
+        lib.sn_download_bytes.argtypes = [ctx, ctypes.c_void_p, size, u8p]
+        lib.sn_free_bytes.argtypes = [ctx, ctypes.c_void_p]
+        lib.sn_fp4_sizes.argtypes = [size, size, ctypes.POINTER(size), ctypes.POINTER(size)]
+        lib.sn_quantize_fp4.argtypes = [ctx, size, size, ctypes.c_uint32] + operand * 3
+        lib.sn_dequantize_fp4.argtypes = lib.sn_quantize_fp4.argtypes
+        lib.sn_matmul_fp4.argtypes = [ctx, ctypes.POINTER(CMatmulSpec)] + operand * 5
+        cache_and_rows = [ctx, ctypes.POINTER(CFp4CacheShape), ctypes.POINTER(CFp4CacheRows)]
+        lib.sn_fp4_cache_append.argtypes = cache_and_rows + operand * 6
+        lib.sn_fp4_cache_read.argtypes = cache_and_rows + operand * 7
+        lib.sn_fp4_attention.argtypes = [ctx, ctypes.POINTER(CFp4CacheShape), ctypes.POINTER(CFp4AttentionShape)] + \
+            operand * 7
         u32p = ctypes.POINTER(ctypes.c_uint32)
         lib.sn_tile_map.argtypes = [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, u32p, u32p,
                                     u32p, u32p]
@@ -383,7 +480,9 @@ def _library() -> ctypes.CDLL:
                      "sn_softmax_backward", "sn_cross_entropy", "sn_upload_tokens", "sn_download_tokens",
                      "sn_free_tokens", "sn_split_heads", "sn_merge_heads", "sn_causal_attention",
                      "sn_causal_attention_score_grad", "sn_plan_matmul", "sn_plan_matmul_column_sums", "sn_matmul_column_sums", "sn_tile_map", "sn_matmul_noalloc", "sn_causal_attention_with_stats",
-                     "sn_causal_attention_backward"):
+                     "sn_causal_attention_backward", "sn_alloc_bytes", "sn_upload_bytes", "sn_download_bytes",
+                     "sn_free_bytes", "sn_fp4_sizes", "sn_quantize_fp4", "sn_dequantize_fp4", "sn_matmul_fp4",
+                     "sn_fp4_cache_append", "sn_fp4_cache_read", "sn_fp4_attention"):
             getattr(lib, name).restype = ctypes.c_int
         _lib = lib
     return _lib
@@ -392,6 +491,15 @@ def _library() -> ctypes.CDLL:
 def library() -> ctypes.CDLL:
     """The loaded ``libstaleynet_gemm.so`` (raises if it has not been built)."""
     return _library()
+
+
+def fp4_sizes(rows: int, inner: int) -> tuple[int, int]:
+    """``sn_fp4_sizes``: bytes of the codes and of the scales of ``rows`` rows of ``inner`` values."""
+    codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
+    rc = _library().sn_fp4_sizes(rows, inner, ctypes.byref(codes), ctypes.byref(scales))
+    if rc != SN_OK:
+        raise GpuError(rc, "fp4_sizes")
+    return codes.value, scales.value
 
 
 def status_string(status: int) -> str:
@@ -796,6 +904,127 @@ class Gpu:
                                          ctypes.c_void_p(logits_grad.pointer), logits_grad.shape().rows,
                                          logits_grad.shape().cols)
         self._check(rc, "cross_entropy")
+
+    def zeros_bytes(self, count: int) -> ByteBuffer:
+        """``sn_alloc_bytes``: zeroed bytes."""
+        out = ctypes.c_void_p()
+        self._check(_library().sn_alloc_bytes(self._ctx, count, ctypes.byref(out)), "zeros_bytes")
+        return ByteBuffer(self, out.value or 0, count)
+
+    def upload_bytes(self, values) -> ByteBuffer:
+        """``sn_upload_bytes``."""
+        host = np.ascontiguousarray(values, dtype=np.uint8).ravel()
+        out = ctypes.c_void_p()
+        self._check(_library().sn_upload_bytes(self._ctx, host.ctypes.data_as(ctypes.POINTER(ctypes.c_uint8)),
+                                               host.size, ctypes.byref(out)), "upload_bytes")
+        return ByteBuffer(self, out.value or 0, host.size)
+
+    def download_bytes(self, buffer: ByteBuffer) -> np.ndarray:
+        """``sn_download_bytes``."""
+        host = np.empty(len(buffer), np.uint8)
+        self._check(_library().sn_download_bytes(self._ctx, ctypes.c_void_p(buffer.pointer), host.size,
+                                                 host.ctypes.data_as(ctypes.POINTER(ctypes.c_uint8))),
+                    "download_bytes")
+        return host
+
+    def fp4_matrix(self, cols: int, inner: int) -> Fp4Matrix:
+        """An ``Fp4Matrix`` of zeros."""
+        codes, scales = fp4_sizes(cols, inner)
+        return Fp4Matrix(cols, inner, self.zeros_bytes(codes), self.zeros_bytes(scales))
+
+    def quantize_fp4(self, source: Tensor, matrix: Fp4Matrix, storage: Storage = Storage.RowMajor) -> None:
+        """``sn_quantize_fp4``: a right operand ``[inner, cols]`` (``RowMajor`` as Linear keeps its weight,
+        or ``Transposed``) rounded to 4-bit blocks along ``inner``."""
+        rc = _library().sn_quantize_fp4(self._ctx, matrix.cols, matrix.inner, int(storage),
+                                        ctypes.c_void_p(source.pointer), len(source),
+                                        ctypes.c_void_p(matrix.codes.pointer), len(matrix.codes),
+                                        ctypes.c_void_p(matrix.scales.pointer), len(matrix.scales))
+        if rc in _VALIDATION_CODES:
+            raise MatmulPanic(rc)
+        self._check(rc, "quantize_fp4")
+
+    def dequantize_fp4(self, matrix: Fp4Matrix, output: Tensor, storage: Storage = Storage.RowMajor) -> None:
+        """``sn_dequantize_fp4``: the values ``matrix`` stands for, exactly, stored as ``storage`` says."""
+        rc = _library().sn_dequantize_fp4(self._ctx, matrix.cols, matrix.inner, int(storage),
+                                          ctypes.c_void_p(matrix.codes.pointer), len(matrix.codes),
+                                          ctypes.c_void_p(matrix.scales.pointer), len(matrix.scales),
+                                          ctypes.c_void_p(output.pointer), len(output))
+        if rc in _VALIDATION_CODES:
+            raise MatmulPanic(rc)
+        self._check(rc, "dequantize_fp4")
+
+    def matmul_fp4(self, spec: MatmulSpec, left: Tensor, right: Fp4Matrix, output: Tensor,
+                   bias: Tensor | None = None) -> None:
+        """``matmul`` (with ``bias``: ``matmul_bias``) against a 4-bit right operand (``sn_matmul_fp4``); the
+        spec's ``right`` is ``Transposed``, as the operand's columns are contiguous."""
+        if (right.cols, right.inner) != (spec.cols, spec.inner):
+            raise MatmulPanic(SN_ERR_RIGHT_TOO_SMALL)
+        c = spec.to_c()
+        b_pointer, b_len = (None, 0) if bias is None else (bias.pointer, len(bias))
+        rc = _library().sn_matmul_fp4(self._ctx, ctypes.byref(c), ctypes.c_void_p(left.pointer), len(left),
+                                      ctypes.c_void_p(right.codes.pointer), len(right.codes),
+                                      ctypes.c_void_p(right.scales.pointer), len(right.scales),
+                                      ctypes.c_void_p(b_pointer), b_len, ctypes.c_void_p(output.pointer),
+                                      len(output))
+        if rc in _VALIDATION_CODES:
+            raise MatmulPanic(rc)
+        self._check(rc, "matmul_fp4")
+
+    def fp4_cache(self, batch: int, kv_heads: int, capacity: int, head_dim: int) -> Fp4Cache:
+        """An ``Fp4Cache`` of zeros."""
+        codes, scales = fp4_sizes(batch * kv_heads * capacity, head_dim)
+        return Fp4Cache(batch, kv_heads, capacity, head_dim, self.zeros_bytes(codes), self.zeros_bytes(scales),
+                        self.zeros_bytes(codes), self.zeros_bytes(scales))
+
+    def fp4_cache_append(self, cache: Fp4Cache, packed: Tensor, time: int, width: int, key_column: int,
+                         value_column: int, position: int = 0, positions: TokenBuffer | None = None) -> None:
+        """``split_heads`` of the keys and values of packed rows into a 4-bit cache (``sn_fp4_cache_append``):
+        each sequence's ``time`` rows from ``positions[sequence]`` (or ``position``) on."""
+        rows = CFp4CacheRows(time, position, width, key_column, value_column)
+        c = cache.to_c()
+        p_pointer, p_len = (None, 0) if positions is None else (positions.pointer, len(positions))
+        rc = _library().sn_fp4_cache_append(self._ctx, ctypes.byref(c), ctypes.byref(rows),
+                                            ctypes.c_void_p(packed.pointer), len(packed), ctypes.c_void_p(p_pointer),
+                                            p_len, *cache.buffers())
+        self._check_cache(rc, "fp4_cache_append")
+
+    def fp4_cache_read(self, cache: Fp4Cache, time: int, keys: Tensor, values: Tensor, position: int = 0,
+                       positions: TokenBuffer | None = None) -> None:
+        """The values held at those positions (``sn_fp4_cache_read``): ``keys`` and ``values``
+        ``[batch][kv_heads][time][head_dim]``."""
+        rows = CFp4CacheRows(time, position, 0, 0, 0)
+        c = cache.to_c()
+        p_pointer, p_len = (None, 0) if positions is None else (positions.pointer, len(positions))
+        rc = _library().sn_fp4_cache_read(self._ctx, ctypes.byref(c), ctypes.byref(rows), *cache.buffers(),
+                                          ctypes.c_void_p(p_pointer), p_len, ctypes.c_void_p(keys.pointer), len(keys),
+                                          ctypes.c_void_p(values.pointer), len(values))
+        self._check_cache(rc, "fp4_cache_read")
+
+    def fp4_attention(self, cache: Fp4Cache, q: Tensor, out: Tensor, heads: int, queries: int, scale: float,
+                      keys: int = 0, lengths: TokenBuffer | None = None,
+                      q_strides: tuple[int, int, int] | None = None,
+                      out_strides: tuple[int, int, int] | None = None) -> None:
+        """Causal attention over a 4-bit cache (``sn_fp4_attention``): the last ``queries`` of the positions
+        each sequence holds (``lengths``, or ``keys`` for all). Strides are floats between sequences, heads and
+        queries; the default is head-major ``[batch][heads][queries][head_dim]``, and
+        ``(queries * width, head_dim, width)`` are columns of packed rows."""
+        h = cache.head_dim
+        head_major = (heads * queries * h, queries * h, h)
+        shape = CFp4AttentionShape(heads, queries, keys, *(q_strides or head_major), *(out_strides or head_major),
+                                   scale)
+        c = cache.to_c()
+        n_pointer, n_len = (None, 0) if lengths is None else (lengths.pointer, len(lengths))
+        rc = _library().sn_fp4_attention(self._ctx, ctypes.byref(c), ctypes.byref(shape), ctypes.c_void_p(q.pointer),
+                                         len(q), *cache.buffers(), ctypes.c_void_p(n_pointer), n_len,
+                                         ctypes.c_void_p(out.pointer), len(out))
+        self._check_cache(rc, "fp4_attention")
+
+    def _check_cache(self, rc: int, what: str) -> None:
+        if rc == SN_ERR_SHAPE:
+            raise AssertionError(f"{what}: heads, columns or positions do not fit the shape")
+        if rc == SN_ERR_LENGTH_MISMATCH:
+            raise AssertionError(f"{what}: a buffer is too small for the shape")
+        self._check(rc, what)
 
     def matmul_raw(self, spec: MatmulSpec, left: int, left_len: int, right: int, right_len: int, output: int,
                    output_len: int) -> None:
