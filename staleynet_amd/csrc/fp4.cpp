@@ -28,6 +28,7 @@ using namespace sn::fp4;
 // Sizes and offsets stay below this, so that byte offsets fit the kernels' signed arithmetic.
 constexpr size_t kLimit = size_t(1) << 60;
 constexpr size_t kMaxDimension = size_t(1) << 31;
+constexpr size_t kMaxPositions = size_t(1) << 30;  // of a cache: attention counts them in 32 bits
 
 int status(hipError_t err) { return err == hipSuccess ? SN_OK : int(err); }
 
@@ -87,7 +88,7 @@ int cache_need(const sn_fp4_cache_shape& c, size_t* codes, size_t* scales) {
     if (c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 128) return SN_ERR_UNSUPPORTED;
     size_t heads, rows, values;
     if (!product(c.batch, c.kv_heads, &heads) || !product(heads, c.capacity, &rows) ||
-        !product(rows, c.head_dim, &values) || heads >= kMaxDimension || c.capacity >= kMaxDimension)
+        !product(rows, c.head_dim, &values) || heads >= kMaxDimension || c.capacity >= kMaxPositions)
         return SN_ERR_OVERFLOW;
     *codes = values / 2;
     *scales = values / SN_FP4_BLOCK;
@@ -396,6 +397,8 @@ int sn_fp4_attention(sn_context* ctx, const sn_fp4_cache_shape* cache, const sn_
     args.scale = s.scale;
     args.workspace = ctx->env.workspace;
     args.workspace_bytes = ctx->env.workspace_bytes;
+    args.counters = ctx->env.counters;
+    args.counter_count = ctx->env.counter_count;
     args.cu_count = ctx->env.cu_count;
     hipError_t err = hipSetDevice(ctx->device);
     if (err == hipSuccess) err = launch_attention(args, ctx->stream);

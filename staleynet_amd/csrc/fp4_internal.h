@@ -77,6 +77,8 @@ struct AttentionArgs {
     float scale = 1.f;
     float* workspace = nullptr;
     size_t workspace_bytes = 0;
+    uint32_t* counters = nullptr;  // zero between calls
+    size_t counter_count = 0;
     int cu_count = 256;
 };
 hipError_t launch_attention(const AttentionArgs& args, hipStream_t stream);
