@@ -25,6 +25,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "fp4_device.h"
 #include "fp4_internal.h"
@@ -36,8 +37,10 @@ namespace {
 
 constexpr int kRows = 16;  // queries of a wave
 constexpr int kKeys = 32;  // keys of a step
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
+constexpr int kSplitWaves = 8;   // of a workgroup whose waves share rows
+constexpr int kSplitThreads = 64 * kSplitWaves;
+constexpr int kRowWaves = 4;     // of one whose waves have rows of their own
+constexpr int kRowThreads = 64 * kRowWaves;
 
 struct KernelArgs {
     AttentionArgs a;
@@ -45,7 +48,7 @@ struct KernelArgs {
     int32_t group;          // query heads of a key/value head
     int32_t row_tiles;      // of a key/value head
     int32_t workgroups;     // about as many workgroups as share the keys (0: one to a row tile)
-    int32_t least_keys;     // of a workgroup, a multiple of kKeys kWaves
+    int32_t least_keys;     // of a workgroup, a multiple of kKeys kSplitWaves
     uint32_t* counters;     // one a row tile of every key/value head, zero between calls
     float* records;         // [workgroup][row][H + 4]: O, m, l
 };
@@ -65,7 +68,6 @@ struct WaveStage {
     static constexpr int O_ROW = H + 4;
     static constexpr int O_BYTES = (kRows * O_ROW + 2 * kRows) * 4;
     static constexpr int BYTES = kKeys * ROW > O_BYTES ? kKeys * ROW : O_BYTES;
-    static constexpr int MAX_SPLITS = kWaves * BYTES / (kRows * 4);  // workgroups whose weights fit the stages
     static constexpr int Q_BYTES = H / 32 * kParts * 64 * 16;  // q's fragments, [fragment][part][lane]
 };
 
@@ -142,9 +144,14 @@ struct Running {
 };
 
 // Keys key0, key0 + step, .. before `end`, 32 at a time. q(i, part): the fragments of q.
-template <int H, class Query>
+// The scores of the next step are formed beside the softmax and O of this one, so that the
+// matrix cores and the vector units have work of their own; codes are loaded two steps
+// (K) and one (V) ahead. m is raised only where a score passes it by 8 (numerators up to
+// 2^8 are as exact), which after a few steps is never: O is hardly rescaled.
+// ready() makes them usable, while the first codes are on their way.
+template <int H, class Ready, class Query>
 __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t key0, int32_t step, int32_t end,
-                                     char* stage, int n, int g, uint32_t upper, Query&& q,
+                                     char* stage, int n, int g, uint32_t upper, Ready&& ready, Query&& q,
                                      Running<H>& run) {
 #pragma clang fp contract(off)
     using Stage = WaveStage<H>;
@@ -153,102 +160,105 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
     const AttentionArgs& a = p.a;
 #pragma unroll
     for (int d = 0; d < TILES; ++d) run.o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (key0 >= end) return;
 
     // The step's rows from a base the wave shares, and the lane's offsets from it.
     const int64_t cache_row = (r.b * a.kv_heads + r.kv_head) * a.capacity;
-    const uint8_t* k_codes = a.k_codes + (cache_row + key0) * (H / 2);
-    const uint8_t* v_codes = a.v_codes + (cache_row + key0) * (H / 2);
-    const uint8_t* k_scales = a.k_scales + (cache_row + key0) * (H / 32);
-    const uint8_t* v_scales = a.v_scales + (cache_row + key0) * (H / 32);
     const uint32_t code_at = g * (H / 8), scale_at = g * (H / 4) / 32;
     struct Words {
-        uint32_t k[2][NF], v[2][NF];
-        uint32_t ks[2], vs[2];
+        uint32_t w[2][NF];
+        uint32_t s[2];
     };
-    auto load_words = [](const uint8_t* from, uint32_t (&w)[NF]) __attribute__((always_inline)) {
-        if constexpr (NF == 4) {
-            const u32x4 x = *reinterpret_cast<const u32x4*>(from);
-            w[0] = x[0], w[1] = x[1], w[2] = x[2], w[3] = x[3];
-        } else if constexpr (NF == 2) {
-            const u32x2 x = *reinterpret_cast<const u32x2*>(from);
-            w[0] = x[0], w[1] = x[1];
-        } else {
-            w[0] = *reinterpret_cast<const uint32_t*>(from);
-        }
-    };
-    // Keys past the end read the last key (their scores and values are replaced).
-    auto load = [&](int32_t first, Words& x) __attribute__((always_inline)) {
+    // The 32 keys from `first` on (a step's, so `first` is under `end`); keys past the end
+    // read the last key (their scores and values are replaced).
+    auto load = [&](const uint8_t* codes, const uint8_t* scales, int32_t first, Words& x)
+                    __attribute__((always_inline)) {
+        codes += (cache_row + first) * (H / 2);
+        scales += (cache_row + first) * (H / 32);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const uint32_t key = uint32_t(min(16 * u + n, end - 1 - first));
-            load_words(k_codes + (key * (H / 2) + code_at), x.k[u]);
-            load_words(v_codes + (key * (H / 2) + code_at), x.v[u]);
-            x.ks[u] = k_scales[key * (H / 32) + scale_at];
-            x.vs[u] = v_scales[key * (H / 32) + scale_at];
+            const uint8_t* from = codes + (key * (H / 2) + code_at);
+            if constexpr (NF == 4) {
+                const u32x4 v = *reinterpret_cast<const u32x4*>(from);
+                x.w[u][0] = v[0], x.w[u][1] = v[1], x.w[u][2] = v[2], x.w[u][3] = v[3];
+            } else if constexpr (NF == 2) {
+                const u32x2 v = *reinterpret_cast<const u32x2*>(from);
+                x.w[u][0] = v[0], x.w[u][1] = v[1];
+            } else {
+                x.w[u][0] = *reinterpret_cast<const uint32_t*>(from);
+            }
+            x.s[u] = scales[key * (H / 32) + scale_at];
         }
-        k_codes += int64_t(step) * (H / 2);
-        v_codes += int64_t(step) * (H / 2);
-        k_scales += int64_t(step) * (H / 32);
-        v_scales += int64_t(step) * (H / 32);
+    };
+    struct Scores {
+        f32x4 s[2];
+    };
+    // Two chains of sums a tile (the first parts, and the others), so that they overlap.
+    auto scores = [&](const Words& k) __attribute__((always_inline)) {
+        f32x4 most[2], rest[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) most[u] = rest[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float factor[2] = {factor_of(k.s[0]), factor_of(k.s[1])};
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            bf16x8 f[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) f[u] = fragment_of(k.w[u][i], factor[u]);
+#pragma unroll
+            for (int part = kParts - 1; part >= 0; --part) {
+                const bf16x8 x = q(i, part);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    f32x4& to = part == 0 ? most[u] : rest[u];
+                    to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[u], x, to, 0, 0, 0);
+                }
+            }
+        }
+        Scores out;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) out.s[u] = most[u] + rest[u];
+        return out;
     };
     char* const v_write = stage + n * Stage::ROW + g * (H / 2);
     const char* const v_read = stage + (4 * g + (n >> 2)) * Stage::ROW + 8 * (n & 3);
 
-    Words next;
-    load(key0, next);
+    Words k_next, v_next;
+    if (key0 < end) {
+        load(a.k_codes, a.k_scales, key0, k_next);
+        load(a.v_codes, a.v_scales, key0, v_next);
+    }
+    ready();
+    if (key0 >= end) return;
+    Scores s_next = scores(k_next);
+    if (key0 + step < end) load(a.k_codes, a.k_scales, key0 + step, k_next);
     for (; key0 < end; key0 += step) {
-        Words now = next;
-        if (key0 + step < end) load(key0 + step, next);
-        const bool masked = key0 + kKeys > r.all_see || key0 + kKeys > end;  // of the wave
-
-        f32x4 s[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const float k_factor[2] = {factor_of(now.ks[0]), factor_of(now.ks[1])};
-#pragma unroll
-        for (int i = 0; i < NF; ++i) {
-            const bf16x8 k0 = fragment_of(now.k[0][i], k_factor[0]), k1 = fragment_of(now.k[1][i], k_factor[1]);
-#pragma unroll
-            for (int part = kParts - 1; part >= 0; --part) {
-                const bf16x8 x = q(i, part);
-                s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k0, x, s[0], 0, 0, 0);
-                s[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k1, x, s[1], 0, 0, 0);
-            }
-        }
-        // Values a query does not see must not reach it through 0 x NaN: in a step at the
-        // end of what some query sees, NaN blocks are taken out here and the queries
-        // that see them given NaN below.
+        Scores s = s_next;
+        Words v = v_next;
+        // What queries do not see is replaced: -inf for its scores, 0 for its values, since
+        // 0 x NaN would reach them. NaN blocks of keys that some queries see are taken out as
+        // well, and those queries given NaN below.
         uint64_t poison[2] = {0, 0};
-        if (masked) {
+        if (key0 + kKeys > r.all_see || key0 + kKeys > end) {  // of the wave
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int32_t key = key0 + 16 * u + n;
-                const bool nan = now.vs[u] > kLargestScale;
+                const bool nan = v.s[u] > kLargestScale;
                 poison[u] = __ballot(nan && key < end);
                 if (nan || key >= end) {
-                    now.vs[u] = 127;
+                    v.s[u] = 127;
 #pragma unroll
-                    for (int i = 0; i < NF; ++i) now.v[u][i] = 0;
+                    for (int i = 0; i < NF; ++i) v.w[u][i] = 0;
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int32_t k = key0 + 16 * u + 4 * g + e;
-                    s[u][e] = k <= r.last && k < end ? s[u][e] : -INFINITY;
+                    s.s[u][e] = k <= r.last && k < end ? s.s[u][e] : -INFINITY;
                 }
             }
         }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const float factor = factor_of(now.vs[u]);
-#pragma unroll
-            for (int i = 0; i < NF; ++i)
-                *reinterpret_cast<bf16x8*>(v_write + 16 * u * Stage::ROW + 16 * i) = fragment_of(now.v[u][i], factor);
-        }
-
-        const float top = largest_of_four(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                                                fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3]))));
-        if (__any(top > run.m)) {
+        const float top = largest_of_four(fmaxf(fmaxf(fmaxf(s.s[0][0], s.s[0][1]), fmaxf(s.s[0][2], s.s[0][3])),
+                                                fmaxf(fmaxf(s.s[1][0], s.s[1][1]), fmaxf(s.s[1][2], s.s[1][3]))));
+        if (__any(top > run.m + 8.f)) {
             const float m_new = fmaxf(run.m, top);
             const float alpha = m_new == -INFINITY ? 1.f : exp2_of(run.m - m_new);
             run.m = m_new;
@@ -256,21 +266,34 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
 #pragma unroll
             for (int d = 0; d < TILES; ++d) run.o[d] = run.o[d] * alpha;
         }
+        const bool more = key0 + step < end;
+        if (more) load(a.v_codes, a.v_scales, key0 + step, v_next);
+        // (After the last step these scores are of the last keys again, and not used.)
+        s_next = scores(k_next);
+        if (key0 + 2 * step < end) load(a.k_codes, a.k_scales, key0 + 2 * step, k_next);
+
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float factor = factor_of(v.s[u]);
+#pragma unroll
+            for (int i = 0; i < NF; ++i)
+                *reinterpret_cast<bf16x8*>(v_write + 16 * u * Stage::ROW + 16 * i) = fragment_of(v.w[u][i], factor);
+        }
         const float base = run.m == -INFINITY ? 0.f : run.m;
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            x[e] = exp2_of(s[e / 4][e % 4] - base);
+            x[e] = exp2_of(s.s[e / 4][e % 4] - base);
             run.l = run.l + x[e];
         }
-        const SplitVector pr = split_exact(x, upper);
+        const SplitVector pr = split_finite(x, upper);  // a NaN reaches the result through l
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int d = 0; d < TILES; ++d) {
-            const bf16x8 v = transposed(v_read + 32 * d, v_read + 16 * Stage::ROW + 32 * d);
+            const bf16x8 f = transposed(v_read + 32 * d, v_read + 16 * Stage::ROW + 32 * d);
 #pragma unroll
             for (int part = kParts - 1; part >= 0; --part)
-                run.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pr.part[part], run.o[d], 0, 0, 0);
+                run.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pr.part[part], run.o[d], 0, 0, 0);
         }
         __builtin_amdgcn_wave_barrier();
         if (poison[0] | poison[1]) {
@@ -292,10 +315,31 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
     }
 }
 
-// A workgroup's share of the keys, from the lengths as the device has them: sequence
-// b's n keys go to max(1, ceil(n / share)) workgroups for each of its row tiles, where
-// share makes them about p.workgroups in all; then consecutive workgroups take
-// consecutive shares of a tile, tiles of a sequence, sequences.
+// Sums over lanes 0 .. this one (neighbours within rows of 16, then rows: data-parallel
+// moves, no LDS).
+__device__ __forceinline__ uint32_t sums_up_to_lane(uint32_t x) {
+    auto move = [](auto control, auto rows, uint32_t v) __attribute__((always_inline)) {
+        return uint32_t(
+            __builtin_amdgcn_update_dpp(0, int(v), decltype(control)::value, decltype(rows)::value, 0xf, false));
+    };
+    using std::integral_constant;
+    x += move(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{}, x);  // from the lane before
+    x += move(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{}, x);  // two before
+    x += move(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{}, x);
+    x += move(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{}, x);
+    x += move(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{}, x);  // lane 15 to row 1, 47 to row 3
+    x += move(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{}, x);  // lane 31 to rows 2 and 3
+    return x;
+}
+
+// A workgroup's share of the keys, from the lengths as the device has them. Sequence b's
+// n keys go to ceil(n / share) workgroups for each of its row tiles, or to one where n
+// is at most two least shares (merging two records costs what they save: 300 keys 7.2 us
+// in one, 8.7 in two; 701 8.8 and 8.6). share is an even share of all keys, raised by
+// eighths until the workgroups that have over half a share number at most p.workgroups,
+// so that none of them waits for another to end (80 tiles of 4000 keys on 256
+// workgroups: 33 us with 320 shares, 21 with 240). Consecutive workgroups take consecutive
+// shares of a tile, tiles of a sequence, sequences.
 struct Share {
     int32_t b, length, keys;  // keys: that a workgroup takes
     int32_t tile;             // of the sequence: kv_head * row_tiles + row tile
@@ -303,10 +347,10 @@ struct Share {
     int32_t first;            // the tile's first workgroup
     bool ok;
 };
-__device__ __forceinline__ Share share_of(const KernelArgs& p, int32_t most_splits, int lane) {
+__device__ __forceinline__ Share share_of(const KernelArgs& p, int lane) {
     const AttentionArgs& a = p.a;
     const int32_t tiles = int32_t(a.kv_heads) * p.row_tiles;  // of a sequence
-    constexpr int32_t kUnit = kKeys * kWaves;
+    constexpr int32_t kUnit = kKeys * kSplitWaves;
     const int32_t index = int32_t(blockIdx.x);
     Share s = {};
     s.splits = 1;
@@ -318,39 +362,38 @@ __device__ __forceinline__ Share share_of(const KernelArgs& p, int32_t most_spli
         s.ok = true;
         return s;
     }
-    int64_t total = 0;
-    int32_t longest = 0;
-    for (int64_t b0 = 0; b0 < a.batch; b0 += 64) {
-        const int32_t n = b0 + lane < a.batch ? held_by(a, b0 + lane) : 0;
-        int64_t sum = n;
-        int32_t most = n;
-#pragma unroll
-        for (int step = 32; step > 0; step >>= 1) {
-            sum += __shfl_xor(sum, step);
-            most = max(most, __shfl_xor(most, step));
+    const int32_t batch = int32_t(a.batch);  // under p.workgroups
+    auto held = [&](int32_t b) __attribute__((always_inline)) { return b < batch ? held_by(a, b) : 0; };
+    const int32_t n0 = held(lane);
+    // The sum over the sequences of f(keys held).
+    auto sum_over = [&](auto f) __attribute__((always_inline)) {
+        if (batch == 1) return int64_t(uint32_t(__builtin_amdgcn_readfirstlane(f(n0))));
+        int64_t sum = 0;
+        for (int32_t b0 = 0; b0 < batch; b0 += 64) {
+            const int32_t n = b0 == 0 ? n0 : held(b0 + lane);
+            sum += uint32_t(__builtin_amdgcn_readlane(sums_up_to_lane(b0 + lane < batch ? f(n) : 0), 63));
         }
-        total += sum;
-        longest = max(longest, most);
-    }
-    const int64_t even = (total * tiles + p.workgroups - 1) / p.workgroups;
-    const int64_t share = min(max(even, int64_t((longest + most_splits - 1) / most_splits)), int64_t(longest));
-    s.keys = __builtin_amdgcn_readfirstlane(max(p.least_keys, int32_t((share + kUnit - 1) / kUnit) * kUnit));
+        return sum;
+    };
+    const int64_t even = sum_over([](int32_t n) { return n / kKeys; }) * tiles / p.workgroups * kKeys;
+    int32_t keys = max(p.least_keys, int32_t((min(even, a.capacity) + kUnit - 1) / kUnit) * kUnit);
+    auto splits_of = [&](int32_t n) __attribute__((always_inline)) {
+        return n <= 2 * p.least_keys ? 1 : (n + keys - 1) / keys;
+    };
+    auto filled = [&](int32_t n) __attribute__((always_inline)) { return n > keys / 2 ? splits_of(n) : 0; };
+    while (keys < a.capacity && sum_over(filled) * tiles > p.workgroups)
+        keys = min(int32_t(a.capacity) + kUnit, (keys + keys / 8 + kUnit - 1) / kUnit * kUnit);
+    s.keys = __builtin_amdgcn_readfirstlane(keys);
     int32_t before = 0;  // workgroups of the sequences so far
-    for (int64_t b0 = 0; b0 < a.batch; b0 += 64) {
-        const bool here = b0 + lane < a.batch;
-        const int32_t n = here ? held_by(a, b0 + lane) : 0;
-        const int32_t splits = here ? max(1, (n + s.keys - 1) / s.keys) : 0;
-        int32_t sum = splits * tiles;  // inclusive over the lanes
-#pragma unroll
-        for (int step = 1; step < 64; step <<= 1) {
-            const int32_t other = __shfl_up(sum, step);
-            if (lane >= step) sum += other;
-        }
+    for (int32_t b0 = 0; b0 < batch; b0 += 64) {
+        const int32_t n = b0 == 0 ? n0 : held(b0 + lane);
+        const int32_t splits = b0 + lane < batch ? splits_of(n) : 0;
+        const int32_t sum = int32_t(sums_up_to_lane(splits * tiles));
         const int32_t start = before + sum - splits * tiles;
         const uint64_t mine = __ballot(index >= start && index < start + splits * tiles);
         if (mine != 0) {
             const int from = __builtin_ctzll(mine);
-            s.b = int32_t(b0) + from;
+            s.b = b0 + from;
             s.length = __builtin_amdgcn_readlane(n, from);
             s.splits = __builtin_amdgcn_readlane(splits, from);
             const int32_t at = index - __builtin_amdgcn_readlane(start, from);
@@ -365,18 +408,18 @@ __device__ __forceinline__ Share share_of(const KernelArgs& p, int32_t most_spli
     return s;
 }
 
-// A decode step: the workgroup's waves share 16 rows and take every fourth 32 keys of
+// A decode step: the workgroup's waves share 16 rows and take every eighth 32 keys of
 // its share; their m, l and O are merged through LDS in wave order, and those of a
 // tile's workgroups by the last of them to arrive, in the workgroups' order (records
 // and counter as in attention.hip's decode form: device-coherent stores, completed
 // before the counter is raised).
 template <int H>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(3, 3)))
-void split_attention_kernel(KernelArgs p) {
+__global__ __launch_bounds__(kSplitThreads) void split_attention_kernel(KernelArgs p) {
 #pragma clang fp contract(off)
     using Stage = WaveStage<H>;
     constexpr int RECORD = H + 4;
-    __shared__ __attribute__((aligned(16))) char stages[kWaves * Stage::BYTES];
+    constexpr int PIECES = H / 4;
+    __shared__ __attribute__((aligned(16))) char stages[kSplitWaves * Stage::BYTES];
     __shared__ __attribute__((aligned(16))) char q_lds[Stage::Q_BYTES];
     __shared__ uint32_t arrived_last;
     const AttentionArgs& a = p.a;
@@ -384,24 +427,24 @@ void split_attention_kernel(KernelArgs p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
     const uint32_t upper = upper_half_mask();
-    const Share share = share_of(p, Stage::MAX_SPLITS, lane);
+    const Share share = share_of(p, lane);
     if (!share.ok) return;
     const int32_t tile = share.tile % p.row_tiles;
     const Rows r = rows_of(p, share.b, share.tile / p.row_tiles, tile, share.length, n);
-
-    // q's fragments, one a wave at a time.
-    for (int i = wave; i < H / 32; i += kWaves) {
-        const SplitVector x = query_fragment<H>(p, r, g, i, upper);
-#pragma unroll
-        for (int part = 0; part < kParts; ++part)
-            *reinterpret_cast<bf16x8*>(q_lds + ((i * kParts + part) * 64 + lane) * 16) = x.part[part];
-    }
-    __syncthreads();
     const int32_t key_first = share.split * share.keys;
     const int32_t end = min(r.some_see, share.splits > 1 ? key_first + share.keys : r.some_see);
     char* const stage = stages + wave * Stage::BYTES;
     Running<H> run;
-    walk<H>(p, r, key_first + wave * kKeys, kKeys * kWaves, end, stage, n, g, upper,
+    walk<H>(p, r, key_first + wave * kKeys, kKeys * kSplitWaves, end, stage, n, g, upper,
+            [&]() __attribute__((always_inline)) {  // q's fragments, one a wave
+                if (wave < H / 32) {
+                    const SplitVector x = query_fragment<H>(p, r, g, wave, upper);
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part)
+                        *reinterpret_cast<bf16x8*>(q_lds + ((wave * kParts + part) * 64 + lane) * 16) = x.part[part];
+                }
+                __syncthreads();
+            },
             [&](int i, int part) __attribute__((always_inline)) {
                 return *reinterpret_cast<const bf16x8*>(q_lds + ((i * kParts + part) * 64 + lane) * 16);
             },
@@ -419,32 +462,34 @@ void split_attention_kernel(KernelArgs p) {
     __syncthreads();
     const uint32_t first_row = uint32_t(tile) * kRows;
     const int rows = int(min(uint32_t(a.queries) * uint32_t(p.group) - first_row, uint32_t(kRows)));
-    auto out_of = [&](int row) __attribute__((always_inline)) {
-        const uint32_t at = first_row + row;
-        return a.out + r.b * a.out_sequence + (r.kv_head * p.group + at % uint32_t(p.group)) * a.out_head +
-               int64_t(at / uint32_t(p.group)) * a.out_row;
+    const int units = rows * PIECES;  // of four floats of a row, at most 512
+    static_assert(kRows * PIECES <= kSplitThreads, "a thread has at most one unit");
+    auto store = [&](int unit, float total, f32x4 sum) __attribute__((always_inline)) {
+        const uint32_t at = first_row + uint32_t(unit / PIECES);
+        float* to = a.out + r.b * a.out_sequence + (r.kv_head * p.group + at % uint32_t(p.group)) * a.out_head +
+                    int64_t(at / uint32_t(p.group)) * a.out_row + 4 * (unit % PIECES);
+        const float inverse = 1.f / total;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) to[c] = total == 0.f ? 0.f : sum[c] * inverse;
     };
     const __amdgpu_buffer_rsrc_t records = gemm::buffer_of(p.records + int64_t(share.first) * kRows * RECORD);
-    for (int e = tid; e < rows * (H / 4); e += kThreads) {
-        const int row = e / (H / 4), piece = e % (H / 4);
+    if (tid < units) {
+        const int row = tid / PIECES, piece = tid % PIECES;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w)
+        for (int w = 0; w < kSplitWaves; ++w)
             top = fmaxf(top, reinterpret_cast<const float*>(stages + w * Stage::BYTES)[kRows * Stage::O_ROW + row]);
         float total = 0.f;
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < kSplitWaves; ++w) {
             const float* from = reinterpret_cast<const float*>(stages + w * Stage::BYTES);
             const float weight = top == -INFINITY ? 1.f : exp2_of(from[kRows * Stage::O_ROW + row] - top);
             total = total + weight * from[kRows * Stage::O_ROW + kRows + row];
             sum = sum + weight * *reinterpret_cast<const f32x4*>(from + row * Stage::O_ROW + 4 * piece);
         }
         if (share.splits == 1) {
-            const float inverse = 1.f / total;
-            float* to = out_of(row) + 4 * piece;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) to[c] = total == 0.f ? 0.f : sum[c] * inverse;
+            store(tid, total, sum);
         } else {
             const int32_t at = (share.split * kRows + row) * RECORD;
             gemm::buffer_store4_coherent(records, (at + 4 * piece) * 4, sum);
@@ -461,60 +506,82 @@ void split_attention_kernel(KernelArgs p) {
     __syncthreads();
     if (!arrived_last) return;
 
-    // Weights of the workgroups' records: 2^(m - the largest m), and the sums l so weighted.
-    float* const weights = reinterpret_cast<float*>(stages);  // [row][split]
-    float* const sums = reinterpret_cast<float*>(q_lds);      // [row]
-    const int splits = share.splits;
-    // 16 lanes a row.
-    for (int row = tid / 16; row < rows; row += kThreads / 16) {
-        float top = -INFINITY;
-        for (int s = tid % 16; s < splits; s += 16) {
-            const f32x4 ml = gemm::buffer_load4_coherent(records, ((s * kRows + row) * RECORD + H) * 4);
-            weights[row * splits + s] = ml[0];
-            top = fmaxf(top, ml[0]);
-        }
+    // Threads of group j fold records j, j + groups, .. of their unit, eight in flight, and
+    // group 0 the groups' results, in that order.
+    constexpr int kBatch = 8;
+    const int groups = min(kSplitThreads / units, (share.splits + kBatch - 1) / kBatch);
+    const int group = tid / units, unit = tid % units;
+    float m = -INFINITY, l = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    if (group < groups) {
+        const int32_t row_at = unit / PIECES * RECORD, piece_at = 4 * (unit % PIECES);
+        for (int s0 = group; s0 < share.splits; s0 += kBatch * groups) {
+            f32x4 ml[kBatch], part[kBatch];
 #pragma unroll
-        for (int step = 8; step > 0; step >>= 1) top = fmaxf(top, __shfl_xor(top, step));
-        float total = 0.f;
-        for (int s = tid % 16; s < splits; s += 16) {
-            const f32x4 ml = gemm::buffer_load4_coherent(records, ((s * kRows + row) * RECORD + H) * 4);
-            const float weight = top == -INFINITY ? 1.f : exp2_of(ml[0] - top);
-            weights[row * splits + s] = weight;
-            total = total + weight * ml[1];
-        }
+            for (int u = 0; u < kBatch; ++u) {
+                const int s = s0 + u * groups;
+                const int32_t at = s * kRows * RECORD + row_at;
+                ml[u] = gemm::buffer_load4_coherent(records, s < share.splits ? (at + H) * 4 : gemm::kOutOfRange);
+                part[u] =
+                    gemm::buffer_load4_coherent(records, s < share.splits ? (at + piece_at) * 4 : gemm::kOutOfRange);
+            }
+            float top = m;
 #pragma unroll
-        for (int step = 8; step > 0; step >>= 1) total = total + __shfl_xor(total, step);
-        if (tid % 16 == 0) sums[row] = total;
+            for (int u = 0; u < kBatch; ++u) {
+                if (s0 + u * groups >= share.splits) ml[u][0] = -INFINITY;  // read as zeros: weight 0
+                top = fmaxf(top, ml[u][0]);
+            }
+            const float base = top == -INFINITY ? 0.f : top, kept = exp2_of(m - base);
+            m = top;
+            l = l * kept;
+            sum = sum * kept;
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const float weight = exp2_of(ml[u][0] - base);
+                l = l + weight * ml[u][1];
+                sum = sum + weight * part[u];
+            }
+        }
+    }
+    if (groups == 1) {
+        if (group == 0) store(unit, l, sum);
+        if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return;
+    }
+    // (Every thread is past its last read of the stages: two barriers ago.)
+    float* const folded = reinterpret_cast<float*>(stages);  // [group][unit]: O, m, l
+    static_assert(kSplitThreads * 24 <= kSplitWaves * Stage::BYTES, "the groups' results fit the stages");
+    if (group < groups) {
+        float* to = folded + 6 * tid;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) to[c] = sum[c];
+        to[4] = m;
+        to[5] = l;
     }
     __syncthreads();
-    for (int e = tid; e < rows * (H / 4); e += kThreads) {
-        const int row = e / (H / 4), piece = e % (H / 4);
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        constexpr int kBatch = 8;
-        for (int s0 = 0; s0 < splits; s0 += kBatch) {
-            f32x4 part[kBatch];
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u)
-                part[u] = gemm::buffer_load4_coherent(
-                    records, s0 + u < splits ? (((s0 + u) * kRows + row) * RECORD + 4 * piece) * 4 : gemm::kOutOfRange);
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u)
-                if (s0 + u < splits) sum = sum + weights[row * splits + s0 + u] * part[u];
+    if (group == 0) {
+        float top = m;
+        for (int j = 1; j < groups; ++j) top = fmaxf(top, folded[6 * (j * units + unit) + 4]);
+        const float base = top == -INFINITY ? 0.f : top, kept = exp2_of(m - base);
+        l = l * kept;
+        sum = sum * kept;
+        for (int j = 1; j < groups; ++j) {
+            const float* from = folded + 6 * (j * units + unit);
+            const float weight = exp2_of(from[4] - base);
+            l = l + weight * from[5];
+            sum = sum + weight * f32x4{from[0], from[1], from[2], from[3]};
         }
-        const float total = sums[row], inverse = 1.f / total;
-        float* to = out_of(row) + 4 * piece;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) to[c] = total == 0.f ? 0.f : sum[c] * inverse;
+        store(unit, l, sum);
     }
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // A prompt chunk: each wave has 16 rows of its own and walks over all their keys.
 template <int H>
-__global__ __launch_bounds__(kThreads) void row_attention_kernel(KernelArgs p) {
+__global__ __launch_bounds__(kRowThreads) void row_attention_kernel(KernelArgs p) {
 #pragma clang fp contract(off)
     using Stage = WaveStage<H>;
-    __shared__ __attribute__((aligned(16))) char stages[kWaves * Stage::BYTES];
+    __shared__ __attribute__((aligned(16))) char stages[kRowWaves * Stage::BYTES];
     const AttentionArgs& a = p.a;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -523,8 +590,8 @@ __global__ __launch_bounds__(kThreads) void row_attention_kernel(KernelArgs p) {
     // The last rows, which see the most keys, first; neighbouring workgroups are
     // key/value heads, so that one XCD's read few of them.
     const uint32_t kv_all = uint32_t(a.batch * a.kv_heads), kv = blockIdx.x % kv_all;
-    const int32_t groups = (p.row_tiles + kWaves - 1) / kWaves;
-    const int32_t tile = (groups - 1 - int32_t(blockIdx.x / kv_all)) * kWaves + wave;
+    const int32_t groups = (p.row_tiles + kRowWaves - 1) / kRowWaves;
+    const int32_t tile = (groups - 1 - int32_t(blockIdx.x / kv_all)) * kRowWaves + wave;
     if (tile >= p.row_tiles) return;  // the kernel has no barrier
     const uint32_t b = kv / uint32_t(a.kv_heads);
     const Rows r = rows_of(p, b, kv % uint32_t(a.kv_heads), tile, held_by(a, b), n);
@@ -532,7 +599,7 @@ __global__ __launch_bounds__(kThreads) void row_attention_kernel(KernelArgs p) {
 #pragma unroll
     for (int i = 0; i < H / 32; ++i) q[i] = query_fragment<H>(p, r, g, i, upper);
     Running<H> run;
-    walk<H>(p, r, 0, kKeys, r.some_see, stages + wave * Stage::BYTES, n, g, upper,
+    walk<H>(p, r, 0, kKeys, r.some_see, stages + wave * Stage::BYTES, n, g, upper, []() {},
             [&](int i, int part) __attribute__((always_inline)) { return q[i].part[part]; }, run);
     run.l = run.l + __shfl_xor(run.l, 16);
     run.l = run.l + __shfl_xor(run.l, 32);
@@ -549,26 +616,26 @@ template <int H>
 hipError_t launch(const AttentionArgs& a, KernelArgs p, hipStream_t stream) {
     const int64_t tiles = a.batch * a.kv_heads * p.row_tiles;
     const int64_t longest = a.lengths != nullptr ? a.capacity : a.keys;
-    if (tiles >= 4 * a.cu_count && p.row_tiles >= kWaves) {
-        const int64_t grid = a.batch * a.kv_heads * ((p.row_tiles + kWaves - 1) / kWaves);
+    if (tiles >= 4 * a.cu_count && p.row_tiles >= kRowWaves) {
+        const int64_t grid = a.batch * a.kv_heads * ((p.row_tiles + kRowWaves - 1) / kRowWaves);
         if (grid > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL(row_attention_kernel<H>, dim3(unsigned(grid)), dim3(kThreads), 0, stream, p);
+        hipLaunchKernelGGL(row_attention_kernel<H>, dim3(unsigned(grid)), dim3(kRowThreads), 0, stream, p);
         return hipGetLastError();
     }
-    // Three workgroups a CU are resident (registers and LDS); the keys go to about as many.
-    const int64_t resident = 3 * int64_t(a.cu_count);
+    // Workgroups a CU has room for (LDS at h = 128, registers else); the keys go to as many.
+    const int64_t resident = (H == 128 ? 1 : 2) * int64_t(a.cu_count);
     const int64_t record_bytes = kRows * (H + 4) * int64_t(sizeof(float));
     const int64_t room = a.workspace != nullptr ? int64_t(a.workspace_bytes) / record_bytes : 0;
     const int64_t wanted = std::min(resident, room - tiles);
-    p.least_keys = kKeys * kWaves;
+    p.least_keys = kKeys * kSplitWaves;
     int64_t grid = tiles;
-    if (wanted > 0 && tiles < resident && size_t(tiles) <= a.counter_count && longest > p.least_keys) {
-        // At most `wanted` shares that are full and one a tile that is not.
+    if (wanted > tiles && size_t(tiles) <= a.counter_count && longest > 2 * p.least_keys) {
+        // Besides the shares over half full, which are at most `wanted`, one a tile.
         p.workgroups = int32_t(wanted);
         grid = std::min(wanted + tiles, tiles * ((longest + p.least_keys - 1) / p.least_keys));
     }
     if (grid > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(split_attention_kernel<H>, dim3(unsigned(grid)), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(split_attention_kernel<H>, dim3(unsigned(grid)), dim3(kSplitThreads), 0, stream, p);
     return hipGetLastError();
 }
 

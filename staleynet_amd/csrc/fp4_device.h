@@ -54,6 +54,26 @@ __device__ __forceinline__ float cut(float x, uint32_t upper) {
 __device__ __forceinline__ float quiet(float x) {  // a NaN whose upper half is one
     return x != x ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) | 0x00400000u) : x;
 }
+__device__ __forceinline__ SplitVector split_vector_of(const u32x4 (&w)[kParts]) {
+    SplitVector out;
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) out.part[q] = __builtin_bit_cast(bf16x8, w[q]);
+    return out;
+}
+// Finite values only.
+__device__ __forceinline__ SplitVector split_finite(const float (&x)[8], uint32_t upper) {
+#pragma clang fp contract(off)
+    u32x4 w[kParts];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const float a = x[2 * p], b = x[2 * p + 1];
+        const float a1 = a - cut(a, upper), b1 = b - cut(b, upper);
+        w[0][p] = upper_halves(a, b);
+        w[1][p] = upper_halves(a1, b1);
+        w[2][p] = upper_halves(a1 - cut(a1, upper), b1 - cut(b1, upper));
+    }
+    return split_vector_of(w);
+}
 __device__ __forceinline__ SplitVector split_exact(const float (&x)[8], uint32_t upper) {
 #pragma clang fp contract(off)
     u32x4 w[kParts];
@@ -62,11 +82,10 @@ __device__ __forceinline__ SplitVector split_exact(const float (&x)[8], uint32_t
     for (int p = 0; p < 4; ++p) {
         const float a = x[2 * p], b = x[2 * p + 1];
         const float a1 = a - cut(a, upper), b1 = b - cut(b, upper);
-        const float a2 = a1 - cut(a1, upper), b2 = b1 - cut(b1, upper);
         odd |= __builtin_isunordered(a1, b1);
         w[0][p] = upper_halves(a, b);
         w[1][p] = upper_halves(a1, b1);
-        w[2][p] = upper_halves(a2, b2);
+        w[2][p] = upper_halves(a1 - cut(a1, upper), b1 - cut(b1, upper));
     }
     if (__any(odd)) {
 #pragma unroll
@@ -84,10 +103,7 @@ __device__ __forceinline__ SplitVector split_exact(const float (&x)[8], uint32_t
             for (int q = 0; q < kParts; ++q) w[q][p] = upper_halves(part[0][q], part[1][q]);
         }
     }
-    SplitVector out;
-#pragma unroll
-    for (int q = 0; q < kParts; ++q) out.part[q] = __builtin_bit_cast(bf16x8, w[q]);
-    return out;
+    return split_vector_of(w);
 }
 
 }  // namespace fp4

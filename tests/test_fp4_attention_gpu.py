@@ -145,6 +145,16 @@ def test_long_caches_and_every_workspace(gpu, head_dim, heads, kv_heads, queries
             other.close()
 
 
+@pytest.mark.parametrize("batch,longest,head_dim", [(150, 3000, 32), (65, 9000, 64), (300, 700, 32)])
+def test_many_sequences(gpu, batch, longest, head_dim):
+    """More sequences than a wave has lanes, lengths from 0 to long: the shares of every one are found."""
+    rng = np.random.default_rng(batch)
+    lengths = np.minimum(longest, np.exp(rng.uniform(0, np.log(longest + 1), batch)).astype(int) - 1)
+    lengths[[0, 63, 64, batch - 1]] = [longest, 0, longest, longest - 1]
+    case = Case(batch, 2, 1, 1, longest, head_dim, lengths, seed=batch)
+    case.check(case.run(gpu))
+
+
 def test_one_length_for_all(gpu):
     case = Case(3, 6, 3, 4, 77, 64, [60, 60, 60], seed=8)
     got = case.run(gpu, uniform=60)
