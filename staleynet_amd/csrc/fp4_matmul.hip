@@ -16,7 +16,7 @@
 // passes the parts through LDS of its own. D = W x^T: a lane holds four consecutive
 // columns of one part's sums. The codes and the x of the next step are on their way
 // while this one's are used.
-// More rows: 16 R rows to a wave, x split as it is used.
+// More rows: tiles staged in LDS, below.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -24,18 +24,16 @@
 
 #include "fp4_device.h"
 #include "fp4_internal.h"
+#include "gemm_common.h"
 
 namespace sn {
 namespace fp4 {
 namespace {
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
 constexpr int kStep = 128;        // inner values of a step: four blocks
 constexpr int kMaxWaves = 8;
-
-__device__ __forceinline__ bf16x8 rounded8(const float (&x)[8]) {
-    const u32x4 w = {pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3]), pack2_bf16(x[4], x[5]), pack2_bf16(x[6], x[7])};
-    return __builtin_bit_cast(bf16x8, w);
-}
 
 __device__ __forceinline__ void store_output(const ProductArgs& a, int64_t row, int64_t col, float sum) {
 #pragma clang fp contract(off)
@@ -45,6 +43,38 @@ __device__ __forceinline__ void store_output(const ProductArgs& a, int64_t row, 
     if (a.bias != nullptr) out = out + a.bias[col];
     *y = out;
 }
+
+// How rows of x are read, four values from k (a multiple of 4) on, zeros where `ok` is not
+// set or past `inner`. No branch, so that the loads of a step stay in flight: quads are whole
+// (inner a multiple of 4), or the last ones are read from the row's end and shifted
+// (rows start at any 4-byte address then; 16-byte loads need no more), or, under
+// 4 values, one by one.
+enum class Quads { kWhole, kShifted, kSingle };
+template <Quads Q>
+__device__ __forceinline__ f32x4 load4(const float* row, int64_t k, int64_t inner, bool ok) {
+    typedef f32x4 f32x4_unaligned __attribute__((aligned(4)));
+    const f32x4 zeros = {0.f, 0.f, 0.f, 0.f};
+    f32x4 v = zeros;
+    if constexpr (Q == Quads::kWhole) {
+        v = ok && k < inner ? f32x4(*reinterpret_cast<const f32x4_unaligned*>(row + k)) : zeros;
+    } else if constexpr (Q == Quads::kShifted) {
+        const int64_t past = k + 4 - inner;  // values past the end, of these four
+        const f32x4 got = *reinterpret_cast<const f32x4_unaligned*>(row + (past > 0 ? inner - 4 : k));
+        const int shift = past <= 0 ? 0 : past >= 4 ? 4 : int(past);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float x = 0.f;
+#pragma unroll
+            for (int s = 0; s + e < 4; ++s) x = shift == s ? got[e + s] : x;
+            v[e] = ok ? x : 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ok && k + e < inner ? row[k + e] : 0.f;
+    }
+    return v;
+}
+Quads quads_of(int64_t inner) { return inner < 4 ? Quads::kSingle : inner % 4 == 0 ? Quads::kWhole : Quads::kShifted; }
 
 // A step's weights: per column tile the lane's block, 16 bytes of codes and the scale byte.
 template <int C>
@@ -69,7 +99,7 @@ __device__ __forceinline__ void load_weights(const ProductArgs& a, const int64_t
 
 // Four values as PARTS parts, packed in pairs (split_exact has the arithmetic).
 template <int PARTS>
-__device__ __forceinline__ void split_four(const float (&x)[4], uint32_t upper, u32x2 (&w)[PARTS]) {
+__device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[PARTS]) {
 #pragma clang fp contract(off)
     if constexpr (PARTS == 1) {
         w[0] = u32x2{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
@@ -97,7 +127,7 @@ __device__ __forceinline__ void split_four(const float (&x)[4], uint32_t upper, 
 }
 
 // At most 16 T / PARTS rows. PARTS: 3, or 1 for x rounded to bf16.
-template <int C, int T, int PARTS, bool VECTOR>
+template <int C, int T, int PARTS, Quads Q>
 __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a) {
     // Parts [wave][PARTS rows][kStep + 8], then the waves' sums [wave][C][T][16 parts][16 columns].
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -122,7 +152,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
         for (int o = 0; o < T; ++o) acc[c][o] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // x of a step: four values of rows 2 pair + half.
-    float x[PAIRS][4];
+    f32x4 x[PAIRS];
     const int half = lane >> 5, quad = 4 * (lane & 31);
     auto load_x = [&](int64_t step) __attribute__((always_inline)) {
         const int64_t k = step * kStep + quad;
@@ -130,15 +160,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
         for (int pair = 0; pair < PAIRS; ++pair) {
             if (2 * pair >= rows) break;
             const int row = 2 * pair + half;
-            const float* from = a.x + row * a.inner + k;
-            if (VECTOR) {
-                const f32x4 v = row < rows && k < a.inner ? *reinterpret_cast<const f32x4*>(from) : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[pair][e] = v[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[pair][e] = row < rows && k + e < a.inner ? from[e] : 0.f;
-            }
+            x[pair] = load4<Q>(a.x + (row < rows ? row : 0) * a.inner, k, a.inner, row < rows);
         }
     };
     char* const parts = lds + wave * (PARTS * rows * PART_ROW);
@@ -208,118 +230,214 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
     }
 }
 
-// Eight values of a row of x from k on, zeros past `inner`.
-template <bool VECTOR>
-__device__ __forceinline__ void load8(const float* row, int64_t k, int64_t inner, bool ok, float (&v)[8]) {
-    if (VECTOR && ok && k + 8 <= inner) {
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(row + k), hi = *reinterpret_cast<const f32x4*>(row + k + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = ok && k + i < inner ? row[k + i] : 0.f;
-    }
-}
+// Many rows: tiles of 32 RT WR rows x 32 CT WC columns, WR x WC waves. x is split as it is
+// staged in LDS, 64 inner values at a time, in two stages: while the matrix cores work
+// on one, the next is split and written, and the one after is on its way in registers. A
+// lane's 16 bytes of codes are a block of one column: 64 inner values of 32 columns a
+// load. D = x W: a lane holds one column. Inner value 8 i + j of half h of a stage is
+// element j of operand i of lanes h (as the block's words hold the codes).
+template <int RT, int CT, int WR, int WC, int PARTS>
+struct TileShape {
+    static constexpr int THREADS = 64 * WR * WC;
+    static constexpr int ROWS = 32 * RT * WR, COLS = 32 * CT * WC;
+    static constexpr int K = 64;
+    static constexpr int ROW = 2 * K + 16;  // bytes of a staged row: 8 rows' reads on distinct banks
+    static constexpr int PART = ROWS * ROW, STAGE = PARTS * PART;
+    static constexpr int QUADS = ROWS * K / 4 / THREADS;  // of x a thread
+    static_assert(QUADS * THREADS * 4 == ROWS * K, "whole quads");
+};
 
-// 16 R rows a workgroup.
-template <int C, int R, int PARTS, bool VECTOR>
-__global__ __launch_bounds__(64 * kMaxWaves) void rows_kernel(ProductArgs a) {
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    float* const sums = reinterpret_cast<float*>(lds);  // [wave][C][R][16 rows][16 columns]
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int waves = blockDim.x >> 6;
-    const int n = lane & 15, g = lane >> 4;
+// Slices of the inner dimension, `stages` stages each; with more than one the sums go to
+// `sums` [slice][rows][cols], and another kernel adds them.
+struct TileLaunch {
+    int32_t tiles_m, tiles_n, slices, stages;
+    float* sums;
+};
+
+template <int RT, int CT, int WR, int WC, int PARTS, Quads Q>
+__global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileLaunch launch) {
+    using S = TileShape<RT, CT, WR, WC, PARTS>;
+    __shared__ __attribute__((aligned(16))) char stages[2 * S::STAGE];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
     const uint32_t upper = upper_half_mask();
-    const int64_t col0 = int64_t(blockIdx.x) * (16 * C);
-    const int64_t row0 = int64_t(blockIdx.y) * (16 * R);
-    const int64_t rows = min(a.rows - row0, int64_t(16 * R));
-    const int64_t steps = (a.blocks + 3) / 4;
-    const float* xr[R];
-    bool row_ok[R];
+    int unused, slice, tile_m, tile_n;
+    gemm::tile_coordinates(blockIdx.x, gridDim.x, launch.tiles_m, launch.tiles_n, launch.slices, unused, slice, tile_m,
+                           tile_n);
+    const int64_t row0 = int64_t(tile_m) * S::ROWS, col0 = int64_t(tile_n) * S::COLS;
+    const int64_t wave_col = col0 + wave % WC * (32 * CT);
+    const int wave_row = wave / WC * (32 * RT);
+    // The slice's stages.
+    const int32_t begin = slice * launch.stages;
+    const int32_t end = min(begin + launch.stages, int32_t((a.blocks + 1) / 2));
+
+    // x: QUADS of four values a thread, 16 threads to a row's stage.
+    const int quad = 4 * (tid % 16), first_row = tid / 16;
+    constexpr int APART = S::THREADS / 16;
+    f32x4 x[S::QUADS];
+    auto load_x = [&](int32_t stage) __attribute__((always_inline)) {
+        const int64_t k = int64_t(stage) * S::K + quad;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        row_ok[r] = 16 * r + n < rows;
-        xr[r] = a.x + (row0 + (row_ok[r] ? 16 * r + n : 0)) * a.inner;
+        for (int u = 0; u < S::QUADS; ++u) {
+            const int64_t row = row0 + first_row + u * APART;
+            x[u] = load4<Q>(a.x + (row < a.rows ? row : 0) * a.inner, k, a.inner, row < a.rows);
+        }
+    };
+    auto store_x = [&](char* stage) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < S::QUADS; ++u) {
+            u32x2 w[PARTS];
+            split_four<PARTS>(x[u], upper, w);
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q)
+                *reinterpret_cast<u32x2*>(stage + q * S::PART + (first_row + u * APART) * S::ROW + 2 * quad) = w[q];
+        }
+    };
+    int64_t block0[CT];  // columns past the last read the last
+#pragma unroll
+    for (int c = 0; c < CT; ++c) block0[c] = min(wave_col + 32 * c + n, a.cols - 1) * a.blocks;
+
+    f32x16 acc[RT][CT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[r][c][e] = 0.f;
+
+    StepWeights<CT> next;
+    if (begin < end) {
+        load_weights<CT>(a, block0, 2 * int64_t(begin) + h, next);
+        load_x(begin);
+        store_x(stages);
+        if (begin + 1 < end) load_x(begin + 1);
     }
-    int64_t block0[C];
+    __syncthreads();
+    for (int32_t s = begin; s < end; ++s) {
+        const StepWeights<CT> now = next;
+        if (s + 1 < end) {
+            load_weights<CT>(a, block0, 2 * int64_t(s + 1) + h, next);
+            store_x(stages + (s + 1 - begin) % 2 * S::STAGE);
+        }
+        if (s + 2 < end) load_x(s + 2);
+        const char* const from = stages + (s - begin) % 2 * S::STAGE + (wave_row + n) * S::ROW + 64 * h;
+        float factor[CT];
 #pragma unroll
-    for (int c = 0; c < C; ++c) block0[c] = min(col0 + 16 * c + n, a.cols - 1) * a.blocks;
-    f32x4 acc[C][R];
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc[c][r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    StepWeights<C> next;
-    if (wave < steps) load_weights<C>(a, block0, 4 * wave + g, next);
-    for (int64_t step = wave; step < steps; step += waves) {
-        const StepWeights<C> now = next;
-        if (step + waves < steps) load_weights<C>(a, block0, 4 * (step + waves) + g, next);
-        float factor[C];
-#pragma unroll
-        for (int c = 0; c < C; ++c) factor[c] = factor_of(now.s[c]);
-        const int64_t k = step * kStep + g * kBlock;
+        for (int c = 0; c < CT; ++c) factor[c] = factor_of(now.s[c]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            bf16x8 wf[C];
+            bf16x8 wf[CT];
 #pragma unroll
-            for (int c = 0; c < C; ++c) wf[c] = fragment_of(now.w[c][i], factor[c]);
+            for (int c = 0; c < CT; ++c) wf[c] = fragment_of(now.w[c][i], factor[c]);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float v[8];
-                load8<VECTOR>(xr[r], k + 8 * i, a.inner, row_ok[r], v);
-                if (PARTS == 1) {
-                    const bf16x8 xf = rounded8(v);
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int c = 0; c < C; ++c)
-                        acc[c][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[c], xf, acc[c][r], 0, 0, 0);
-                } else {
-                    const SplitVector xf = split_exact(v, upper);
+                for (int q = PARTS - 1; q >= 0; --q) {
+                    const bf16x8 xf =
+                        *reinterpret_cast<const bf16x8*>(from + q * S::PART + 32 * r * S::ROW + 16 * i);
 #pragma unroll
-                    for (int c = 0; c < C; ++c)
-#pragma unroll
-                        for (int q = kParts - 1; q >= 0; --q)
-                            acc[c][r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf[c], xf.part[q], acc[c][r], 0, 0, 0);
+                    for (int c = 0; c < CT; ++c)
+                        acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xf, wf[c], acc[r][c], 0, 0, 0);
                 }
-            }
         }
+        __syncthreads();
     }
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < CT; ++c) {
+        const int64_t col = wave_col + 32 * c + n;
+        if (col >= a.cols) continue;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
-            *reinterpret_cast<f32x4*>(&sums[((wave * C + c) * R + r) * 256 + n * 16 + 4 * g]) = acc[c][r];
-    __syncthreads();
-    constexpr int tile_floats = C * R * 256;
-    for (int e = threadIdx.x; e < tile_floats; e += blockDim.x) {
-        const int64_t row = 16 * ((e >> 8) % R) + ((e >> 4) & 15), col = col0 + 16 * ((e >> 8) / R) + (e & 15);
-        if (row >= rows || col >= a.cols) continue;
-        float sum = 0.f;
-        for (int w = 0; w < waves; ++w) sum += sums[w * tile_floats + e];
-        store_output(a, row0 + row, col, sum);
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int64_t row = row0 + wave_row + 32 * r + 8 * (e / 4) + 4 * h + e % 4;
+                if (row >= a.rows) continue;
+                if (launch.slices > 1)
+                    launch.sums[(slice * a.rows + row) * a.cols + col] = acc[r][c][e];
+                else
+                    store_output(a, row, col, acc[r][c][e]);
+            }
     }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// The slices' sums, added in slice order.
+__global__ __launch_bounds__(256) void slice_sums_kernel(ProductArgs a, TileLaunch launch) {
+    const int64_t total = a.rows * a.cols;
+    for (int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x; e < total; e += int64_t(gridDim.x) * 256) {
+        float sum = 0.f;
+        for (int s = 0; s < launch.slices; ++s) sum += launch.sums[s * total + e];
+        store_output(a, e / a.cols, e % a.cols, sum);
+    }
+}
 
 template <int C, int T, int PARTS>
 hipError_t few_rows(const ProductArgs& a, int waves, hipStream_t stream) {
-    const bool vector = aligned16(a.x) && a.inner % 4 == 0;
     const dim3 grid(unsigned((a.cols + 16 * C - 1) / (16 * C)));
     const size_t lds = waves * std::max<size_t>(C * T * 256 * sizeof(float), PARTS * a.rows * 2 * (kStep + 8));
-    hipLaunchKernelGGL((vector ? few_rows_kernel<C, T, PARTS, true> : few_rows_kernel<C, T, PARTS, false>), grid,
-                       dim3(64 * waves), lds, stream, a);
+    hipLaunchKernelGGL((quads_of(a.inner) == Quads::kWhole ? few_rows_kernel<C, T, PARTS, Quads::kWhole>
+                                                           : few_rows_kernel<C, T, PARTS, Quads::kShifted>),
+                       grid, dim3(64 * waves), lds, stream, a);
     return hipGetLastError();
 }
 
-template <int C, int R, int PARTS>
-hipError_t many_rows(const ProductArgs& a, int waves, hipStream_t stream) {
-    const bool vector = aligned16(a.x) && a.inner % 4 == 0;
-    const dim3 grid(unsigned((a.cols + 16 * C - 1) / (16 * C)), unsigned((a.rows + 16 * R - 1) / (16 * R)));
-    const size_t lds = size_t(waves) * C * R * 256 * sizeof(float);
-    hipLaunchKernelGGL((vector ? rows_kernel<C, R, PARTS, true> : rows_kernel<C, R, PARTS, false>), grid,
-                       dim3(64 * waves), lds, stream, a);
-    return hipGetLastError();
+template <int RT, int CT, int WR, int WC, int PARTS>
+hipError_t tiles(ProductArgs a, int64_t wanted, hipStream_t stream) {
+    using S = TileShape<RT, CT, WR, WC, PARTS>;
+    const int64_t tiles_n = (a.cols + S::COLS - 1) / S::COLS;
+    const int64_t stages = (a.blocks + 1) / 2;
+    // As many rows a launch as its grid (under 2^32 threads) holds.
+    const int64_t most = std::max<int64_t>(1, ((int64_t(1) << 32) - 1) / S::THREADS / tiles_n) * S::ROWS;
+    const ProductArgs all = a;
+    for (int64_t row = 0; row < all.rows; row += most) {
+        a.rows = std::min(most, all.rows - row);
+        a.x = all.x + row * all.inner;
+        a.y = all.y + row * all.cols;
+        TileLaunch launch;
+        launch.tiles_m = int32_t((a.rows + S::ROWS - 1) / S::ROWS);
+        launch.tiles_n = int32_t(tiles_n);
+        const int64_t tiles = launch.tiles_m * tiles_n;
+        const int64_t bytes = a.rows * a.cols * int64_t(sizeof(float));
+        const int64_t room = a.workspace != nullptr ? int64_t(a.workspace_bytes) / bytes : 0;
+        int64_t slices = std::min({wanted / tiles, stages / 4, room});
+        slices = std::max<int64_t>(1, slices);
+        launch.stages = int32_t((stages + slices - 1) / slices);
+        launch.slices = int32_t(std::max<int64_t>(1, (stages + launch.stages - 1) / std::max(1, launch.stages)));
+        launch.sums = static_cast<float*>(a.workspace);
+        auto* const kernel = quads_of(a.inner) == Quads::kWhole     ? tile_kernel<RT, CT, WR, WC, PARTS, Quads::kWhole>
+                             : quads_of(a.inner) == Quads::kShifted ? tile_kernel<RT, CT, WR, WC, PARTS, Quads::kShifted>
+                                                                    : tile_kernel<RT, CT, WR, WC, PARTS, Quads::kSingle>;
+        hipLaunchKernelGGL(kernel, dim3(unsigned(tiles * launch.slices)),
+                           dim3(S::THREADS), 0, stream, a, launch);
+        hipError_t err = hipGetLastError();
+        if (err == hipSuccess && launch.slices > 1) {
+            const int64_t groups = std::min<int64_t>((a.rows * a.cols + 255) / 256, int64_t(1) << 20);
+            hipLaunchKernelGGL(slice_sums_kernel, dim3(unsigned(groups)), dim3(256), 0, stream, a, launch);
+            err = hipGetLastError();
+        }
+        if (err != hipSuccess) return err;
+    }
+    return hipSuccess;
+}
+
+// Tiles of 32 x 128 (27 KB of LDS, five workgroups a CU) hide their stages' latency best where
+// there are few of them, and the inner dimension is sliced until they fill the CUs twice.
+// Three parts: tiles of 128 x 256 (one a CU; 188 us at 2048 x 4096 x 4096 against 233) where the CUs' last
+// round is full enough to keep that quarter: 2000 x 4096 x 4100 would be 346 us of them, 245 of small ones.
+// One part: 64 x 128 where they fill the CUs twice (2000 x 4096 x 4100: 141 us, 187 of small ones and 222 of
+// 128 x 256; 777 x 1001 x 1537, of which there are 169: 23 us against 19).
+template <int PARTS>
+hipError_t many_rows(const ProductArgs& a, hipStream_t stream) {
+    const int64_t cus = a.cu_count;
+    const auto up = [](int64_t x, int64_t unit) { return (x + unit - 1) / unit; };
+    if constexpr (PARTS == 3) {
+        const int64_t rounds = up(up(a.rows, 128) * up(a.cols, 256), cus);
+        if (rounds * cus * (128 * 256) * 4 <= up(a.rows, 32) * 32 * up(a.cols, 128) * 128 * 5)
+            return tiles<2, 2, 2, 4, PARTS>(a, 0, stream);
+    } else {
+        if (up(a.rows, 64) * up(a.cols, 128) >= 2 * cus) return tiles<2, 1, 1, 4, PARTS>(a, 0, stream);
+    }
+    return tiles<1, 1, 1, 4, PARTS>(a, 2 * cus, stream);
 }
 
 template <int T, int PARTS>
@@ -336,12 +454,13 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
     if (a.rows == 0 || a.cols == 0) return hipSuccess;
     const int64_t steps = std::max<int64_t>(1, (a.blocks + 3) / 4);
     const int waves = int(std::min<int64_t>(8, steps));
-    if (a.bf16 && a.rows <= 16) return few_rows_by_columns<1, 1>(a, waves, stream);
-    if (!a.bf16 && a.rows <= 5) return few_rows_by_columns<1, 3>(a, waves, stream);
-    if (!a.bf16 && a.rows <= 10) return few_rows_by_columns<2, 3>(a, waves, stream);
-    if (!a.bf16 && a.rows <= 16) return few_rows_by_columns<3, 3>(a, waves, stream);
-    const int many = int(std::min<int64_t>(4, steps));
-    return a.bf16 ? many_rows<2, 4, 1>(a, many, stream) : many_rows<2, 4, 3>(a, many, stream);
+    if (a.rows <= 16 && a.inner >= 4) {
+        if (a.bf16) return few_rows_by_columns<1, 1>(a, waves, stream);
+        return a.rows <= 5    ? few_rows_by_columns<1, 3>(a, waves, stream)
+               : a.rows <= 10 ? few_rows_by_columns<2, 3>(a, waves, stream)
+                              : few_rows_by_columns<3, 3>(a, waves, stream);
+    }
+    return a.bf16 ? many_rows<1>(a, stream) : many_rows<3>(a, stream);
 }
 
 }  // namespace fp4

@@ -259,7 +259,6 @@ class CHeadLayout(ctypes.Structure):
 
 
 FP4_BLOCK = 32  # SN_FP4_BLOCK (include/staleynet_fp4.h): values of a 4-bit block
-FP4_FEW_ROWS = 64  # SN_FP4_FEW_ROWS
 
 
 class CFp4CacheShape(ctypes.Structure):

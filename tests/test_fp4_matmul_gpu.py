@@ -88,6 +88,22 @@ def test_long_and_wide(gpu, rows, inner, cols):
     assert error < MatmulKernel.MfmaF32.tolerance()
 
 
+@pytest.mark.parametrize("rows,inner,cols,bf16", [
+    (2000, 203, 3900, False),   # tiles of 128 x 256, quads shifted at the rows' ends
+    (1990, 64, 4001, False),    # the same, one stage
+    (1100, 130, 3900, True),    # tiles of 64 x 128
+    (1100, 3, 3900, True),      # values read one by one
+    (70, 2, 300, False),
+    (300, 1000, 200, True)])    # sliced
+def test_tiles(gpu, rows, inner, cols, bf16):
+    rng = np.random.default_rng(rows)
+    codes, scales, w = weights(cols, inner, rows)
+    x = rng.standard_normal((rows, inner)).astype(np.float32)
+    bias = rng.standard_normal(cols).astype(np.float32)
+    spec = MatmulSpec.new(rows, cols, inner).with_precision(Precision.Bf16 if bf16 else Precision.F32)
+    check(run(gpu, spec, x, codes, scales, bias=bias, offset=1), to_bf16(x) if bf16 else x, w, inner, bias=bias)
+
+
 @pytest.mark.parametrize("rows", [1, 5, 9, 40, 100])
 @pytest.mark.parametrize("with_bias", [False, True])
 def test_scale_accumulate_and_bias(gpu, rows, with_bias):
