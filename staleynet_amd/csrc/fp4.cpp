@@ -28,6 +28,8 @@ using namespace sn::fp4;
 // Sizes and offsets stay below this, so that byte offsets fit the kernels' signed arithmetic.
 constexpr size_t kLimit = size_t(1) << 60;
 constexpr size_t kMaxDimension = size_t(1) << 31;
+constexpr size_t kMaxCols = size_t(1) << 28;       // of a product: 2^32 threads a launch
+constexpr size_t kMaxInner = size_t(1) << 25;      // of a product: its kernels count blocks in 32 bits
 constexpr size_t kMaxPositions = size_t(1) << 30;  // of a cache: attention counts them in 32 bits
 
 int status(hipError_t err) { return err == hipSuccess ? SN_OK : int(err); }
@@ -279,7 +281,9 @@ int sn_matmul_fp4(sn_context* ctx, const sn_matmul_spec* spec, const float* left
         spec->mask != SN_MASK_NONE)
         return SN_ERR_UNSUPPORTED;
     size_t codes_need, scales_need;
-    if (sn_fp4_sizes(spec->cols, spec->inner, &codes_need, &scales_need) != SN_OK) return SN_ERR_OVERFLOW;
+    if (sn_fp4_sizes(spec->cols, spec->inner, &codes_need, &scales_need) != SN_OK || spec->inner >= kMaxInner ||
+        spec->cols >= kMaxCols)
+        return SN_ERR_OVERFLOW;
     if (codes_len < codes_need || scales_len < scales_need) return SN_ERR_RIGHT_TOO_SMALL;
     if (bias != nullptr && bias_len != spec->cols) return SN_ERR_LENGTH_MISMATCH;
     if (ctx == nullptr) return SN_ERR_NULL_ARGUMENT;

@@ -76,24 +76,23 @@ __device__ __forceinline__ f32x4 load4(const float* row, int64_t k, int64_t inne
 }
 Quads quads_of(int64_t inner) { return inner < 4 ? Quads::kSingle : inner % 4 == 0 ? Quads::kWhole : Quads::kShifted; }
 
-// A step's weights: per column tile the lane's block, 16 bytes of codes and the scale byte.
+// Weights of some 16 or 32 column tiles for a run of inner values: per tile the lane's
+// block, 16 bytes of codes and the scale byte. `codes` and `scales` are a workgroup's first
+// column, at its first block of the run; `column` counts blocks from there to the lane's
+// columns (under 2^28 and 32-bit byte offsets: inner < 2^25, at most 256 columns), `block`
+// is the lane's of the run. Past a row's last block, where x is 0, the last is read again.
 template <int C>
 struct StepWeights {
     u32x4 w[C];
     uint32_t s[C];
 };
 template <int C>
-__device__ __forceinline__ void load_weights(const ProductArgs& a, const int64_t (&block0)[C], int64_t block,
-                                             StepWeights<C>& x) {
-    // Past the row's last block: zeros (x is 0 there too).
-    const bool ok = block < a.blocks;
+__device__ __forceinline__ void load_weights(const uint8_t* codes, const uint8_t* scales, const uint32_t (&column)[C],
+                                             uint32_t block, StepWeights<C>& x) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const int64_t at = block0[c] + (ok ? block : 0);
-        const u32x4 got = *reinterpret_cast<const u32x4*>(a.codes + at * kBlockBytes);
-        const uint32_t byte = a.scales[at];
-        x.w[c] = ok ? got : u32x4{0, 0, 0, 0};
-        x.s[c] = ok ? byte : 127u;
+        x.w[c] = *reinterpret_cast<const u32x4*>(codes + (column[c] + block) * uint32_t(kBlockBytes));
+        x.s[c] = scales[column[c] + block];
     }
 }
 
@@ -126,13 +125,12 @@ __device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[P
     }
 }
 
-// At most 16 T / PARTS rows. PARTS: 3, or 1 for x rounded to bf16.
-template <int C, int T, int PARTS, Quads Q>
+// At most 2 PAIRS rows, which PARTS (3, or 1 for x rounded to bf16) make at most 16 T.
+template <int C, int T, int PAIRS, int PARTS, Quads Q>
 __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a) {
     // Parts [wave][PARTS rows][kStep + 8], then the waves' sums [wave][C][T][16 parts][16 columns].
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int PART_ROW = 2 * (kStep + 8);
-    constexpr int PAIRS = (16 * T / PARTS + 1) / 2;  // of rows: 32 lanes load a row's step
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6;
@@ -140,10 +138,17 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
     const uint32_t upper = upper_half_mask();
     const int64_t col0 = int64_t(blockIdx.x) * (16 * C);
     const int rows = int(a.rows);
-    const int64_t steps = (a.blocks + 3) / 4;
-    int64_t block0[C];  // of this lane's columns; columns past the last read the last
+    const int32_t blocks = int32_t(a.blocks), steps = (blocks + 3) / 4;
+    const int32_t last_col = int32_t(min(a.cols - col0, int64_t(16 * C))) - 1;
+    uint32_t column[C];  // columns past the last read the last
 #pragma unroll
-    for (int c = 0; c < C; ++c) block0[c] = min(col0 + 16 * c + n, a.cols - 1) * a.blocks;
+    for (int c = 0; c < C; ++c) column[c] = uint32_t(min(16 * c + n, last_col)) * uint32_t(blocks);
+    const uint8_t* const codes = a.codes + col0 * a.blocks * kBlockBytes;
+    const uint8_t* const scales = a.scales + col0 * a.blocks;
+    auto load = [&](int32_t step, StepWeights<C>& w) __attribute__((always_inline)) {
+        load_weights<C>(codes + int64_t(step) * (4 * kBlockBytes), scales + int64_t(step) * 4, column,
+                        uint32_t(min(g, blocks - 1 - 4 * step)), w);
+    };
 
     f32x4 acc[C][T];
 #pragma unroll
@@ -151,17 +156,15 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 #pragma unroll
         for (int o = 0; o < T; ++o) acc[c][o] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // x of a step: four values of rows 2 pair + half.
+    // x of a step: four values of rows 2 pair + half, 32 lanes a row. Rows past the last are the
+    // last again, written to its place.
     f32x4 x[PAIRS];
     const int half = lane >> 5, quad = 4 * (lane & 31);
-    auto load_x = [&](int64_t step) __attribute__((always_inline)) {
-        const int64_t k = step * kStep + quad;
+    auto load_x = [&](int32_t step) __attribute__((always_inline)) {
+        const int64_t k = int64_t(step) * kStep + quad;
 #pragma unroll
-        for (int pair = 0; pair < PAIRS; ++pair) {
-            if (2 * pair >= rows) break;
-            const int row = 2 * pair + half;
-            x[pair] = load4<Q>(a.x + (row < rows ? row : 0) * a.inner, k, a.inner, row < rows);
-        }
+        for (int pair = 0; pair < PAIRS; ++pair)
+            x[pair] = load4<Q>(a.x + min(2 * pair + half, rows - 1) * a.inner, k, a.inner, true);
     };
     char* const parts = lds + wave * (PARTS * rows * PART_ROW);
     int part_read[T];  // lanes past the last part read the last; their sums are not used
@@ -170,27 +173,25 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 
     StepWeights<C> next;
     if (wave < steps) {
-        load_weights<C>(a, block0, 4 * wave + g, next);
         load_x(wave);
+        load(wave, next);
     }
-    for (int64_t step = wave; step < steps; step += waves) {
-        const StepWeights<C> now = next;
+    for (int32_t step = wave; step < steps; step += waves) {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int pair = 0; pair < PAIRS; ++pair) {
-            if (2 * pair >= rows) break;
-            u32x2 w[PARTS];
-            split_four<PARTS>(x[pair], upper, w);
-            const int row = 2 * pair + half;
-            if (row < rows)
+            u32x2 split[PARTS];
+            split_four<PARTS>(x[pair], upper, split);
 #pragma unroll
-                for (int q = 0; q < PARTS; ++q)
-                    *reinterpret_cast<u32x2*>(parts + (q * rows + row) * PART_ROW + 2 * quad) = w[q];
+            for (int q = 0; q < PARTS; ++q)
+                *reinterpret_cast<u32x2*>(parts + (q * rows + min(2 * pair + half, rows - 1)) * PART_ROW + 2 * quad) =
+                    split[q];
         }
         __builtin_amdgcn_wave_barrier();
+        const StepWeights<C> now = next;
         if (step + waves < steps) {
-            load_weights<C>(a, block0, 4 * (step + waves) + g, next);
-            load_x(step + waves);
+            load_x(step + waves);  // first: the next step splits x while its codes may be on their way
+            load(step + waves, next);
         }
         float factor[C];
 #pragma unroll
@@ -294,9 +295,18 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
                 *reinterpret_cast<u32x2*>(stage + q * S::PART + (first_row + u * APART) * S::ROW + 2 * quad) = w[q];
         }
     };
-    int64_t block0[CT];  // columns past the last read the last
+    const int32_t blocks = int32_t(a.blocks);
+    const int32_t last_col = int32_t(min(a.cols - col0, int64_t(S::COLS))) - 1;
+    uint32_t column[CT];  // columns past the last read the last
 #pragma unroll
-    for (int c = 0; c < CT; ++c) block0[c] = min(wave_col + 32 * c + n, a.cols - 1) * a.blocks;
+    for (int c = 0; c < CT; ++c)
+        column[c] = uint32_t(min(wave % WC * (32 * CT) + 32 * c + n, last_col)) * uint32_t(blocks);
+    const uint8_t* const codes = a.codes + col0 * a.blocks * kBlockBytes;
+    const uint8_t* const scales = a.scales + col0 * a.blocks;
+    auto load = [&](int32_t stage, StepWeights<CT>& w) __attribute__((always_inline)) {
+        load_weights<CT>(codes + int64_t(stage) * (2 * kBlockBytes), scales + int64_t(stage) * 2, column,
+                         uint32_t(min(h, blocks - 1 - 2 * stage)), w);
+    };
 
     f32x16 acc[RT][CT];
 #pragma unroll
@@ -308,7 +318,7 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
 
     StepWeights<CT> next;
     if (begin < end) {
-        load_weights<CT>(a, block0, 2 * int64_t(begin) + h, next);
+        load(begin, next);
         load_x(begin);
         store_x(stages);
         if (begin + 1 < end) load_x(begin + 1);
@@ -317,7 +327,7 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
     for (int32_t s = begin; s < end; ++s) {
         const StepWeights<CT> now = next;
         if (s + 1 < end) {
-            load_weights<CT>(a, block0, 2 * int64_t(s + 1) + h, next);
+            load(s + 1, next);
             store_x(stages + (s + 1 - begin) % 2 * S::STAGE);
         }
         if (s + 2 < end) load_x(s + 2);
@@ -371,12 +381,12 @@ __global__ __launch_bounds__(256) void slice_sums_kernel(ProductArgs a, TileLaun
     }
 }
 
-template <int C, int T, int PARTS>
+template <int C, int T, int PAIRS, int PARTS>
 hipError_t few_rows(const ProductArgs& a, int waves, hipStream_t stream) {
     const dim3 grid(unsigned((a.cols + 16 * C - 1) / (16 * C)));
     const size_t lds = waves * std::max<size_t>(C * T * 256 * sizeof(float), PARTS * a.rows * 2 * (kStep + 8));
-    hipLaunchKernelGGL((quads_of(a.inner) == Quads::kWhole ? few_rows_kernel<C, T, PARTS, Quads::kWhole>
-                                                           : few_rows_kernel<C, T, PARTS, Quads::kShifted>),
+    hipLaunchKernelGGL((quads_of(a.inner) == Quads::kWhole ? few_rows_kernel<C, T, PAIRS, PARTS, Quads::kWhole>
+                                                           : few_rows_kernel<C, T, PAIRS, PARTS, Quads::kShifted>),
                        grid, dim3(64 * waves), lds, stream, a);
     return hipGetLastError();
 }
@@ -440,25 +450,25 @@ hipError_t many_rows(const ProductArgs& a, hipStream_t stream) {
     return tiles<1, 1, 1, 4, PARTS>(a, 2 * cus, stream);
 }
 
-template <int T, int PARTS>
-hipError_t few_rows_by_columns(const ProductArgs& a, int waves, hipStream_t stream) {
+template <int T, int PAIRS, int PARTS>
+hipError_t few_rows_by_columns(const ProductArgs& a, hipStream_t stream) {
+    const int waves = int(std::max<int64_t>(1, std::min<int64_t>(kMaxWaves, (a.blocks + 3) / 4)));
     const int64_t tiles = (a.cols + 15) / 16;
-    if (tiles >= 3 * a.cu_count) return few_rows<4, T, PARTS>(a, waves, stream);
-    if (4 * tiles >= 5 * a.cu_count) return few_rows<2, T, PARTS>(a, waves, stream);
-    return few_rows<1, T, PARTS>(a, waves, stream);
+    if (tiles >= 3 * a.cu_count) return few_rows<4, T, PAIRS, PARTS>(a, waves, stream);
+    if (4 * tiles >= 5 * a.cu_count) return few_rows<2, T, PAIRS, PARTS>(a, waves, stream);
+    return few_rows<1, T, PAIRS, PARTS>(a, waves, stream);
 }
 
 }  // namespace
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
     if (a.rows == 0 || a.cols == 0) return hipSuccess;
-    const int64_t steps = std::max<int64_t>(1, (a.blocks + 3) / 4);
-    const int waves = int(std::min<int64_t>(8, steps));
     if (a.rows <= 16 && a.inner >= 4) {
-        if (a.bf16) return few_rows_by_columns<1, 1>(a, waves, stream);
-        return a.rows <= 5    ? few_rows_by_columns<1, 3>(a, waves, stream)
-               : a.rows <= 10 ? few_rows_by_columns<2, 3>(a, waves, stream)
-                              : few_rows_by_columns<3, 3>(a, waves, stream);
+        if (a.bf16) return a.rows <= 2 ? few_rows_by_columns<1, 1, 1>(a, stream) : few_rows_by_columns<1, 8, 1>(a, stream);
+        return a.rows <= 2    ? few_rows_by_columns<1, 1, 3>(a, stream)
+               : a.rows <= 5  ? few_rows_by_columns<1, 3, 3>(a, stream)
+               : a.rows <= 10 ? few_rows_by_columns<2, 5, 3>(a, stream)
+                              : few_rows_by_columns<3, 8, 3>(a, stream);
     }
     return a.bf16 ? many_rows<1>(a, stream) : many_rows<3>(a, stream);
 }
