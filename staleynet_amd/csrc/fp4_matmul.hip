@@ -8,14 +8,18 @@
 // 32 codes become matrix operands with 16 conversions, scale included; nothing is
 // multiplied per group.
 //
-// Few rows: a wave takes 16 C columns and steps of 128 inner values (lane n, g: block g
-// of the step for column n). The workgroup's waves take the steps in turn, and add their
-// sums through LDS in wave order. The parts of all rows, 3 rows (bf16: 1) to each row of x, are
-// the rows of T operands of 16: at most 5 rows need one matrix instruction for 512
-// weights, 10 two, 16 three. The wave splits a step's x once, four values a lane, and
+// Few rows: a wave takes 16 C columns and a run of steps of 128 inner values (lane n, g:
+// block g of the step for column n); the workgroup's waves take consecutive runs, and add
+// their sums through LDS in wave order. The parts of all rows, 3 rows (bf16: 1) to each row
+// of x, are the rows of T operands of 16: at most 5 rows need one matrix instruction for
+// 512 weights, 10 two, 16 three. The wave splits a step's x once, four values a lane, and
 // passes the parts through LDS of its own. D = W x^T: a lane holds four consecutive
 // columns of one part's sums. The codes and the x of the next step are on their way
 // while this one's are used.
+//   Scale bytes: a column's are 1 / 16 of its codes, and read byte by byte beside them they cost the
+// address units as much as the codes do (1 x 8192 x 28672: 39 us, 28 without any). So a
+// lane reads 16 of one column at once, for the next 16 / C steps, and the bytes
+// pass through LDS.
 // More rows: tiles staged in LDS, below.
 #include <hip/hip_runtime.h>
 
@@ -34,6 +38,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kStep = 128;        // inner values of a step: four blocks
 constexpr int kMaxWaves = 8;
+constexpr int kScaleBytes = 1024;  // 16 of each lane
 
 __device__ __forceinline__ void store_output(const ProductArgs& a, int64_t row, int64_t col, float sum) {
 #pragma clang fp contract(off)
@@ -76,26 +81,6 @@ __device__ __forceinline__ f32x4 load4(const float* row, int64_t k, int64_t inne
 }
 Quads quads_of(int64_t inner) { return inner < 4 ? Quads::kSingle : inner % 4 == 0 ? Quads::kWhole : Quads::kShifted; }
 
-// Weights of some 16 or 32 column tiles for a run of inner values: per tile the lane's
-// block, 16 bytes of codes and the scale byte. `codes` and `scales` are a workgroup's first
-// column, at its first block of the run; `column` counts blocks from there to the lane's
-// columns (under 2^28 and 32-bit byte offsets: inner < 2^25, at most 256 columns), `block`
-// is the lane's of the run. Past a row's last block, where x is 0, the last is read again.
-template <int C>
-struct StepWeights {
-    u32x4 w[C];
-    uint32_t s[C];
-};
-template <int C>
-__device__ __forceinline__ void load_weights(const uint8_t* codes, const uint8_t* scales, const uint32_t (&column)[C],
-                                             uint32_t block, StepWeights<C>& x) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        x.w[c] = *reinterpret_cast<const u32x4*>(codes + (column[c] + block) * uint32_t(kBlockBytes));
-        x.s[c] = scales[column[c] + block];
-    }
-}
-
 // Four values as PARTS parts, packed in pairs (split_exact has the arithmetic).
 template <int PARTS>
 __device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[PARTS]) {
@@ -128,9 +113,10 @@ __device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[P
 // At most 2 PAIRS rows, which PARTS (3, or 1 for x rounded to bf16) make at most 16 T.
 template <int C, int T, int PAIRS, int PARTS, Quads Q>
 __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a) {
-    // Parts [wave][PARTS rows][kStep + 8], then the waves' sums [wave][C][T][16 parts][16 columns].
+    // Scales and parts [wave][PARTS rows][kStep + 8], then the waves' sums [wave][C][T][16 parts][16 columns].
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int PART_ROW = 2 * (kStep + 8);
+    constexpr int SCALES = kScaleBytes;  // [step of the run][column][block]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6;
@@ -139,15 +125,44 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
     const int64_t col0 = int64_t(blockIdx.x) * (16 * C);
     const int rows = int(a.rows);
     const int32_t blocks = int32_t(a.blocks), steps = (blocks + 3) / 4;
+    // The wave's run of steps.
+    const int32_t each = (steps + waves - 1) / waves;
+    const int32_t begin = wave * each, end = min(begin + each, steps);
+    // The lane's columns, in blocks from the workgroup's first (32-bit byte offsets: inner < 2^25);
+    // columns past the last read the last. Past a row's last block, where x is 0, the last
+    // is read again.
     const int32_t last_col = int32_t(min(a.cols - col0, int64_t(16 * C))) - 1;
-    uint32_t column[C];  // columns past the last read the last
+    uint32_t column[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) column[c] = uint32_t(min(16 * c + n, last_col)) * uint32_t(blocks);
     const uint8_t* const codes = a.codes + col0 * a.blocks * kBlockBytes;
-    const uint8_t* const scales = a.scales + col0 * a.blocks;
-    auto load = [&](int32_t step, StepWeights<C>& w) __attribute__((always_inline)) {
-        load_weights<C>(codes + int64_t(step) * (4 * kBlockBytes), scales + int64_t(step) * 4, column,
-                        uint32_t(min(g, blocks - 1 - 4 * step)), w);
+    auto load = [&](int32_t step, u32x4 (&w)[C]) __attribute__((always_inline)) {
+        const uint8_t* from = codes + int64_t(step) * (4 * kBlockBytes);
+        const uint32_t block = uint32_t(min(g, blocks - 1 - 4 * step));
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            w[c] = *reinterpret_cast<const u32x4*>(from + (column[c] + block) * uint32_t(kBlockBytes));
+    };
+    // Scale bytes of RUN steps from `step` on: lane -> column lane % 16 C, 16 bytes of it. What
+    // lies past the column's end is not used; past the buffer's, not read.
+    constexpr int RUN = 16 / C;
+    const int scale_col = lane % (16 * C), scale_part = lane / (16 * C);
+    const int64_t scale_row = (col0 + min(scale_col, last_col)) * a.blocks + 16 * scale_part;
+    auto load_scales = [&](int32_t step) __attribute__((always_inline)) {
+        typedef u32x4 u32x4_bytes __attribute__((aligned(1)));
+        const int64_t at = scale_row + 4 * step, total = a.cols * a.blocks;
+        u32x4 s;
+        if (at + 16 <= total) {
+            s = *reinterpret_cast<const u32x4_bytes*>(a.scales + at);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[i] = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) s[i] |= uint32_t(a.scales[min(at + 4 * i + b, total - 1)]) << (8 * b);
+            }
+        }
+        return s;
     };
 
     f32x4 acc[C][T];
@@ -166,17 +181,26 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
         for (int pair = 0; pair < PAIRS; ++pair)
             x[pair] = load4<Q>(a.x + min(2 * pair + half, rows - 1) * a.inner, k, a.inner, true);
     };
-    char* const parts = lds + wave * (PARTS * rows * PART_ROW);
+    char* const wave_lds = lds + wave * (SCALES + PARTS * rows * PART_ROW);
+    char* const parts = wave_lds + SCALES;
     int part_read[T];  // lanes past the last part read the last; their sums are not used
 #pragma unroll
     for (int o = 0; o < T; ++o) part_read[o] = min(16 * o + n, PARTS * rows - 1) * PART_ROW + g * (2 * kBlock);
 
-    StepWeights<C> next;
-    if (wave < steps) {
-        load_x(wave);
-        load(wave, next);
+    u32x4 next[C], next_scales;
+    if (begin < end) {
+        next_scales = load_scales(begin);
+        load_x(begin);
+        load(begin, next);
     }
-    for (int32_t step = wave; step < steps; step += waves) {
+    for (int32_t step = begin; step < end; ++step) {
+        const int32_t in_run = (step - begin) % RUN;
+        if (in_run == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<uint32_t*>(wave_lds + ((4 * scale_part + i) * (16 * C) + scale_col) * 4) = next_scales[i];
+            if (step + RUN < end) next_scales = load_scales(step + RUN);
+        }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int pair = 0; pair < PAIRS; ++pair) {
@@ -188,14 +212,18 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
                     split[q];
         }
         __builtin_amdgcn_wave_barrier();
-        const StepWeights<C> now = next;
-        if (step + waves < steps) {
-            load_x(step + waves);  // first: the next step splits x while its codes may be on their way
-            load(step + waves, next);
+        u32x4 now[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) now[c] = next[c];
+        if (step + 1 < end) {
+            load_x(step + 1);  // first: the next step splits x while its codes may be on their way
+            load(step + 1, next);
         }
         float factor[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) factor[c] = factor_of(now.s[c]);
+        for (int c = 0; c < C; ++c)
+            factor[c] = factor_of(uint8_t(
+                wave_lds[(in_run * (16 * C) + 16 * c + n) * 4 + min(g, blocks - 1 - 4 * step)]));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             bf16x8 xf[T];
@@ -203,7 +231,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
             for (int o = 0; o < T; ++o) xf[o] = *reinterpret_cast<const bf16x8*>(parts + part_read[o] + 16 * i);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const bf16x8 wf = fragment_of(now.w[c][i], factor[c]);
+                const bf16x8 wf = fragment_of(now[c][i], factor[c]);
 #pragma unroll
                 for (int o = 0; o < T; ++o)
                     acc[c][o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[o], acc[c][o], 0, 0, 0);
@@ -297,15 +325,24 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
     };
     const int32_t blocks = int32_t(a.blocks);
     const int32_t last_col = int32_t(min(a.cols - col0, int64_t(S::COLS))) - 1;
-    uint32_t column[CT];  // columns past the last read the last
+    uint32_t column[CT];  // as in few_rows_kernel
 #pragma unroll
     for (int c = 0; c < CT; ++c)
         column[c] = uint32_t(min(wave % WC * (32 * CT) + 32 * c + n, last_col)) * uint32_t(blocks);
     const uint8_t* const codes = a.codes + col0 * a.blocks * kBlockBytes;
     const uint8_t* const scales = a.scales + col0 * a.blocks;
-    auto load = [&](int32_t stage, StepWeights<CT>& w) __attribute__((always_inline)) {
-        load_weights<CT>(codes + int64_t(stage) * (2 * kBlockBytes), scales + int64_t(stage) * 2, column,
-                         uint32_t(min(h, blocks - 1 - 2 * stage)), w);
+    struct Weights {
+        u32x4 w[CT];
+        uint32_t s[CT];
+    };
+    auto load = [&](int32_t stage, Weights& x) __attribute__((always_inline)) {
+        const uint32_t block = uint32_t(min(h, blocks - 1 - 2 * stage));
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+            x.w[c] = *reinterpret_cast<const u32x4*>(codes + int64_t(stage) * (2 * kBlockBytes) +
+                                                     (column[c] + block) * uint32_t(kBlockBytes));
+            x.s[c] = (scales + int64_t(stage) * 2)[column[c] + block];
+        }
     };
 
     f32x16 acc[RT][CT];
@@ -316,7 +353,7 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[r][c][e] = 0.f;
 
-    StepWeights<CT> next;
+    Weights next;
     if (begin < end) {
         load(begin, next);
         load_x(begin);
@@ -325,7 +362,7 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
     }
     __syncthreads();
     for (int32_t s = begin; s < end; ++s) {
-        const StepWeights<CT> now = next;
+        const Weights now = next;
         if (s + 1 < end) {
             load(s + 1, next);
             store_x(stages + (s + 1 - begin) % 2 * S::STAGE);
@@ -384,7 +421,8 @@ __global__ __launch_bounds__(256) void slice_sums_kernel(ProductArgs a, TileLaun
 template <int C, int T, int PAIRS, int PARTS>
 hipError_t few_rows(const ProductArgs& a, int waves, hipStream_t stream) {
     const dim3 grid(unsigned((a.cols + 16 * C - 1) / (16 * C)));
-    const size_t lds = waves * std::max<size_t>(C * T * 256 * sizeof(float), PARTS * a.rows * 2 * (kStep + 8));
+    const size_t lds =
+        waves * std::max<size_t>(C * T * 256 * sizeof(float), kScaleBytes + PARTS * a.rows * 2 * (kStep + 8));
     hipLaunchKernelGGL((quads_of(a.inner) == Quads::kWhole ? few_rows_kernel<C, T, PAIRS, PARTS, Quads::kWhole>
                                                            : few_rows_kernel<C, T, PAIRS, PARTS, Quads::kShifted>),
                        grid, dim3(64 * waves), lds, stream, a);
