@@ -16,10 +16,10 @@
 //    own, no barrier) and are read back transposed in that order.
 // Every product is exact; sums, maxima and probabilities are fp32.
 //
-// Two forms. With few rows to a key/value head (a decode step) a workgroup's waves share 16
-// rows and take every fourth 32 keys, q's parts in LDS; the keys are split over
-// workgroups (split_attention_kernel). With many (a prompt chunk) each wave has 16
-// rows of its own and all their keys (row_attention_kernel).
+// A workgroup's waves share 16 rows and take the steps in turn, q's parts in LDS. (Waves with
+// rows of their own, each walking over all keys, left two waves a SIMD in step with the
+// longest sequence: 292 us for two 1000-query chunks against up to 6001 positions, 197 so.)
+// Where there are few rows (a decode step) workgroups share a tile's keys as well.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -37,10 +37,8 @@ namespace {
 
 constexpr int kRows = 16;  // queries of a wave
 constexpr int kKeys = 32;  // keys of a step
-constexpr int kSplitWaves = 8;   // of a workgroup whose waves share rows
-constexpr int kSplitThreads = 64 * kSplitWaves;
-constexpr int kRowWaves = 4;     // of one whose waves have rows of their own
-constexpr int kRowThreads = 64 * kRowWaves;
+constexpr int kSplitWaves = 8;  // of a workgroup where several share a tile's keys
+constexpr int kTileWaves = 4;   // of one that has a tile to itself, where there are many
 
 struct KernelArgs {
     AttentionArgs a;
@@ -230,7 +228,7 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
     ready();
     if (key0 >= end) return;
     Scores s_next = scores(k_next);
-    if (key0 + step < end) load(a.k_codes, a.k_scales, key0 + step, k_next);
+    load(a.k_codes, a.k_scales, min(key0 + step, end - 1), k_next);
     for (; key0 < end; key0 += step) {
         Scores s = s_next;
         Words v = v_next;
@@ -266,11 +264,11 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
 #pragma unroll
             for (int d = 0; d < TILES; ++d) run.o[d] = run.o[d] * alpha;
         }
-        const bool more = key0 + step < end;
-        if (more) load(a.v_codes, a.v_scales, key0 + step, v_next);
-        // (After the last step these scores are of the last keys again, and not used.)
+        // Past the last step these are the last key again, and not used: no branch divides the
+        // matrix instructions from the vector ones.
+        load(a.v_codes, a.v_scales, min(key0 + step, end - 1), v_next);
         s_next = scores(k_next);
-        if (key0 + 2 * step < end) load(a.k_codes, a.k_scales, key0 + 2 * step, k_next);
+        load(a.k_codes, a.k_scales, min(key0 + 2 * step, end - 1), k_next);
 
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -355,9 +353,13 @@ __device__ __forceinline__ Share share_of(const KernelArgs& p, int lane) {
     Share s = {};
     s.splits = 1;
     if (p.workgroups == 0) {
-        s.b = index / tiles;
+        // The last rows, which see the most keys, first; a head's next rows go to the next XCD, so
+        // that each has rows of long and of short sequences (one XCD a head: 289 us for two
+        // chunks of different lengths, 197 so).
+        const int32_t heads = int32_t(a.batch * a.kv_heads), head = (index % heads + index / heads) % heads;
+        s.b = head / int32_t(a.kv_heads);
         s.length = held_by(a, s.b);
-        s.tile = index % tiles;
+        s.tile = head % int32_t(a.kv_heads) * p.row_tiles + (p.row_tiles - 1 - index / heads);
         s.first = index;
         s.ok = true;
         return s;
@@ -408,18 +410,17 @@ __device__ __forceinline__ Share share_of(const KernelArgs& p, int lane) {
     return s;
 }
 
-// A decode step: the workgroup's waves share 16 rows and take every eighth 32 keys of
-// its share; their m, l and O are merged through LDS in wave order, and those of a
-// tile's workgroups by the last of them to arrive, in the workgroups' order (records
-// and counter as in attention.hip's decode form: device-coherent stores, completed
-// before the counter is raised).
-template <int H>
-__global__ __launch_bounds__(kSplitThreads) void split_attention_kernel(KernelArgs p) {
+// 16 rows: the waves' m, l and O are merged through LDS in wave order, and, where
+// workgroups share the tile's keys, those of the workgroups by the last of them to
+// arrive, in the workgroups' order (records and counter as in attention.hip's decode
+// form: device-coherent stores, completed before the counter is raised).
+template <int H, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) void attention_kernel(KernelArgs p) {
 #pragma clang fp contract(off)
     using Stage = WaveStage<H>;
     constexpr int RECORD = H + 4;
     constexpr int PIECES = H / 4;
-    __shared__ __attribute__((aligned(16))) char stages[kSplitWaves * Stage::BYTES];
+    __shared__ __attribute__((aligned(16))) char stages[W * Stage::BYTES];
     __shared__ __attribute__((aligned(16))) char q_lds[Stage::Q_BYTES];
     __shared__ uint32_t arrived_last;
     const AttentionArgs& a = p.a;
@@ -435,8 +436,9 @@ __global__ __launch_bounds__(kSplitThreads) void split_attention_kernel(KernelAr
     const int32_t end = min(r.some_see, share.splits > 1 ? key_first + share.keys : r.some_see);
     char* const stage = stages + wave * Stage::BYTES;
     Running<H> run;
-    walk<H>(p, r, key_first + wave * kKeys, kKeys * kSplitWaves, end, stage, n, g, upper,
+    walk<H>(p, r, key_first + wave * kKeys, kKeys * W, end, stage, n, g, upper,
             [&]() __attribute__((always_inline)) {  // q's fragments, one a wave
+                static_assert(H / 32 <= W, "a wave has at most one");
                 if (wave < H / 32) {
                     const SplitVector x = query_fragment<H>(p, r, g, wave, upper);
 #pragma unroll
@@ -463,7 +465,6 @@ __global__ __launch_bounds__(kSplitThreads) void split_attention_kernel(KernelAr
     const uint32_t first_row = uint32_t(tile) * kRows;
     const int rows = int(min(uint32_t(a.queries) * uint32_t(p.group) - first_row, uint32_t(kRows)));
     const int units = rows * PIECES;  // of four floats of a row, at most 512
-    static_assert(kRows * PIECES <= kSplitThreads, "a thread has at most one unit");
     auto store = [&](int unit, float total, f32x4 sum) __attribute__((always_inline)) {
         const uint32_t at = first_row + uint32_t(unit / PIECES);
         float* to = a.out + r.b * a.out_sequence + (r.kv_head * p.group + at % uint32_t(p.group)) * a.out_head +
@@ -473,30 +474,31 @@ __global__ __launch_bounds__(kSplitThreads) void split_attention_kernel(KernelAr
         for (int c = 0; c < 4; ++c) to[c] = total == 0.f ? 0.f : sum[c] * inverse;
     };
     const __amdgpu_buffer_rsrc_t records = gemm::buffer_of(p.records + int64_t(share.first) * kRows * RECORD);
-    if (tid < units) {
-        const int row = tid / PIECES, piece = tid % PIECES;
+    for (int unit = tid; unit < units; unit += 64 * W) {
+        const int row = unit / PIECES, piece = unit % PIECES;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kSplitWaves; ++w)
+        for (int w = 0; w < W; ++w)
             top = fmaxf(top, reinterpret_cast<const float*>(stages + w * Stage::BYTES)[kRows * Stage::O_ROW + row]);
         float total = 0.f;
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kSplitWaves; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float* from = reinterpret_cast<const float*>(stages + w * Stage::BYTES);
             const float weight = top == -INFINITY ? 1.f : exp2_of(from[kRows * Stage::O_ROW + row] - top);
             total = total + weight * from[kRows * Stage::O_ROW + kRows + row];
             sum = sum + weight * *reinterpret_cast<const f32x4*>(from + row * Stage::O_ROW + 4 * piece);
         }
         if (share.splits == 1) {
-            store(tid, total, sum);
+            store(unit, total, sum);
         } else {
             const int32_t at = (share.split * kRows + row) * RECORD;
             gemm::buffer_store4_coherent(records, (at + 4 * piece) * 4, sum);
             if (piece == 0) gemm::buffer_store4_coherent(records, (at + H) * 4, f32x4{top, total, 0.f, 0.f});
         }
     }
-    if (share.splits == 1) return;
+    if (W != kSplitWaves || share.splits == 1) return;
+    static_assert(W != kSplitWaves || kRows * PIECES <= 64 * W, "a thread has at most one unit below");
     __builtin_amdgcn_s_waitcnt(0);  // this thread's record is complete device-wide
     __syncthreads();
     uint32_t* const counter = p.counters + int64_t(share.b) * a.kv_heads * p.row_tiles + share.tile;
@@ -509,7 +511,7 @@ __global__ __launch_bounds__(kSplitThreads) void split_attention_kernel(KernelAr
     // Threads of group j fold records j, j + groups, .. of their unit, eight in flight, and
     // group 0 the groups' results, in that order.
     constexpr int kBatch = 8;
-    const int groups = min(kSplitThreads / units, (share.splits + kBatch - 1) / kBatch);
+    const int groups = min(64 * W / units, (share.splits + kBatch - 1) / kBatch);
     const int group = tid / units, unit = tid % units;
     float m = -INFINITY, l = 0.f;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -550,7 +552,7 @@ __global__ __launch_bounds__(kSplitThreads) void split_attention_kernel(KernelAr
     }
     // (Every thread is past its last read of the stages: two barriers ago.)
     float* const folded = reinterpret_cast<float*>(stages);  // [group][unit]: O, m, l
-    static_assert(kSplitThreads * 24 <= kSplitWaves * Stage::BYTES, "the groups' results fit the stages");
+    static_assert(64 * W * 24 <= W * Stage::BYTES, "the groups' results fit the stages");
     if (group < groups) {
         float* to = folded + 6 * tid;
 #pragma unroll
@@ -576,53 +578,11 @@ __global__ __launch_bounds__(kSplitThreads) void split_attention_kernel(KernelAr
     if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// A prompt chunk: each wave has 16 rows of its own and walks over all their keys.
-template <int H>
-__global__ __launch_bounds__(kRowThreads) void row_attention_kernel(KernelArgs p) {
-#pragma clang fp contract(off)
-    using Stage = WaveStage<H>;
-    __shared__ __attribute__((aligned(16))) char stages[kRowWaves * Stage::BYTES];
-    const AttentionArgs& a = p.a;
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = lane & 15, g = lane >> 4;
-    const uint32_t upper = upper_half_mask();
-    // The last rows, which see the most keys, first; neighbouring workgroups are
-    // key/value heads, so that one XCD's read few of them.
-    const uint32_t kv_all = uint32_t(a.batch * a.kv_heads), kv = blockIdx.x % kv_all;
-    const int32_t groups = (p.row_tiles + kRowWaves - 1) / kRowWaves;
-    const int32_t tile = (groups - 1 - int32_t(blockIdx.x / kv_all)) * kRowWaves + wave;
-    if (tile >= p.row_tiles) return;  // the kernel has no barrier
-    const uint32_t b = kv / uint32_t(a.kv_heads);
-    const Rows r = rows_of(p, b, kv % uint32_t(a.kv_heads), tile, held_by(a, b), n);
-    SplitVector q[H / 32];
-#pragma unroll
-    for (int i = 0; i < H / 32; ++i) q[i] = query_fragment<H>(p, r, g, i, upper);
-    Running<H> run;
-    walk<H>(p, r, 0, kKeys, r.some_see, stages + wave * Stage::BYTES, n, g, upper, []() {},
-            [&](int i, int part) __attribute__((always_inline)) { return q[i].part[part]; }, run);
-    run.l = run.l + __shfl_xor(run.l, 16);
-    run.l = run.l + __shfl_xor(run.l, 32);
-    if (!r.ok) return;
-    float* out = a.out + r.b * a.out_sequence + r.head * a.out_head + int64_t(r.t) * a.out_row;
-    const float inverse = 1.f / run.l;
-#pragma unroll
-    for (int d = 0; d < H / 16; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[16 * d + 4 * g + e] = run.l == 0.f ? 0.f : run.o[d][e] * inverse;
-}
-
 template <int H>
 hipError_t launch(const AttentionArgs& a, KernelArgs p, hipStream_t stream) {
     const int64_t tiles = a.batch * a.kv_heads * p.row_tiles;
     const int64_t longest = a.lengths != nullptr ? a.capacity : a.keys;
-    if (tiles >= 4 * a.cu_count && p.row_tiles >= kRowWaves) {
-        const int64_t grid = a.batch * a.kv_heads * ((p.row_tiles + kRowWaves - 1) / kRowWaves);
-        if (grid > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL(row_attention_kernel<H>, dim3(unsigned(grid)), dim3(kRowThreads), 0, stream, p);
-        return hipGetLastError();
-    }
-    // Workgroups a CU has room for (LDS at h = 128, registers else); the keys go to as many.
+    // Workgroups of eight waves that a CU has room for (LDS at h = 128, registers else).
     const int64_t resident = (H == 128 ? 1 : 2) * int64_t(a.cu_count);
     const int64_t record_bytes = kRows * (H + 4) * int64_t(sizeof(float));
     const int64_t room = a.workspace != nullptr ? int64_t(a.workspace_bytes) / record_bytes : 0;
@@ -635,7 +595,10 @@ hipError_t launch(const AttentionArgs& a, KernelArgs p, hipStream_t stream) {
         grid = std::min(wanted + tiles, tiles * ((longest + p.least_keys - 1) / p.least_keys));
     }
     if (grid > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(split_attention_kernel<H>, dim3(unsigned(grid)), dim3(kSplitThreads), 0, stream, p);
+    if (tiles > 2 * resident)
+        hipLaunchKernelGGL((attention_kernel<H, kTileWaves>), dim3(unsigned(grid)), dim3(64 * kTileWaves), 0, stream, p);
+    else
+        hipLaunchKernelGGL((attention_kernel<H, kSplitWaves>), dim3(unsigned(grid)), dim3(64 * kSplitWaves), 0, stream, p);
     return hipGetLastError();
 }
 
