@@ -30,6 +30,8 @@ constexpr size_t kLimit = size_t(1) << 60;
 constexpr size_t kMaxDimension = size_t(1) << 31;
 constexpr size_t kMaxCols = size_t(1) << 28;       // of a product: 2^32 threads a launch
 constexpr size_t kMaxInner = size_t(1) << 25;      // of a product: its kernels count blocks in 32 bits
+constexpr size_t kMaxRows = size_t(1) << 28;        // query rows of an attention call
+constexpr size_t kMaxHeads = size_t(1) << 21;       // of a cache, over its sequences: 2^32 threads a launch
 constexpr size_t kMaxPositions = size_t(1) << 30;  // of a cache: attention counts them in 32 bits
 
 int status(hipError_t err) { return err == hipSuccess ? SN_OK : int(err); }
@@ -90,7 +92,7 @@ int cache_need(const sn_fp4_cache_shape& c, size_t* codes, size_t* scales) {
     if (c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 128) return SN_ERR_UNSUPPORTED;
     size_t heads, rows, values;
     if (!product(c.batch, c.kv_heads, &heads) || !product(heads, c.capacity, &rows) ||
-        !product(rows, c.head_dim, &values) || heads >= kMaxDimension || c.capacity >= kMaxPositions)
+        !product(rows, c.head_dim, &values) || heads >= kMaxHeads || c.capacity >= kMaxPositions)
         return SN_ERR_OVERFLOW;
     *codes = values / 2;
     *scales = values / SN_FP4_BLOCK;
@@ -351,7 +353,7 @@ int sn_fp4_attention(sn_context* ctx, const sn_fp4_cache_shape* cache, const sn_
     if (lengths == nullptr && s.keys > cache->capacity) return SN_ERR_SHAPE;
     size_t head_rows, all_rows;
     if (!product(s.heads, s.queries, &head_rows) || !product(cache->batch, head_rows, &all_rows) ||
-        all_rows >= kMaxDimension)
+        all_rows >= kMaxRows)
         return SN_ERR_OVERFLOW;
     const size_t counts[3] = {cache->batch, s.heads, s.queries};
     const size_t q_strides[3] = {s.q_sequence, s.q_head, s.q_row};

@@ -265,11 +265,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 // lane's 16 bytes of codes are a block of one column: 64 inner values of 32 columns a
 // load. D = x W: a lane holds one column. Inner value 8 i + j of half h of a stage is
 // element j of operand i of lanes h (as the block's words hold the codes).
-template <int RT, int CT, int WR, int WC, int PARTS>
+template <int RT, int CT, int WR, int WC, int PARTS, int SUBS>
 struct TileShape {
     static constexpr int THREADS = 64 * WR * WC;
     static constexpr int ROWS = 32 * RT * WR, COLS = 32 * CT * WC;
-    static constexpr int K = 64;
+    static constexpr int K = 64 * SUBS;     // of a stage
     static constexpr int ROW = 2 * K + 16;  // bytes of a staged row: 8 rows' reads on distinct banks
     static constexpr int PART = ROWS * ROW, STAGE = PARTS * PART;
     static constexpr int QUADS = ROWS * K / 4 / THREADS;  // of x a thread
@@ -283,9 +283,9 @@ struct TileLaunch {
     float* sums;
 };
 
-template <int RT, int CT, int WR, int WC, int PARTS, Quads Q>
+template <int RT, int CT, int WR, int WC, int PARTS, int SUBS, Quads Q>
 __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileLaunch launch) {
-    using S = TileShape<RT, CT, WR, WC, PARTS>;
+    using S = TileShape<RT, CT, WR, WC, PARTS, SUBS>;
     __shared__ __attribute__((aligned(16))) char stages[2 * S::STAGE];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -299,11 +299,11 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
     const int wave_row = wave / WC * (32 * RT);
     // The slice's stages.
     const int32_t begin = slice * launch.stages;
-    const int32_t end = min(begin + launch.stages, int32_t((a.blocks + 1) / 2));
+    const int32_t end = min(begin + launch.stages, int32_t((a.blocks + 2 * SUBS - 1) / (2 * SUBS)));
 
-    // x: QUADS of four values a thread, 16 threads to a row's stage.
-    const int quad = 4 * (tid % 16), first_row = tid / 16;
-    constexpr int APART = S::THREADS / 16;
+    // x: QUADS of four values a thread, 16 SUBS threads to a row's stage.
+    const int quad = 4 * (tid % (16 * SUBS)), first_row = tid / (16 * SUBS);
+    constexpr int APART = S::THREADS / (16 * SUBS);
     f32x4 x[S::QUADS];
     auto load_x = [&](int32_t stage) __attribute__((always_inline)) {
         const int64_t k = int64_t(stage) * S::K + quad;
@@ -332,16 +332,21 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
     const uint8_t* const codes = a.codes + col0 * a.blocks * kBlockBytes;
     const uint8_t* const scales = a.scales + col0 * a.blocks;
     struct Weights {
-        u32x4 w[CT];
-        uint32_t s[CT];
+        u32x4 w[SUBS][CT];
+        uint32_t s[SUBS][CT];
     };
     auto load = [&](int32_t stage, Weights& x) __attribute__((always_inline)) {
-        const uint32_t block = uint32_t(min(h, blocks - 1 - 2 * stage));
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-            x.w[c] = *reinterpret_cast<const u32x4*>(codes + int64_t(stage) * (2 * kBlockBytes) +
-                                                     (column[c] + block) * uint32_t(kBlockBytes));
-            x.s[c] = (scales + int64_t(stage) * 2)[column[c] + block];
+        for (int sub = 0; sub < SUBS; ++sub) {
+            const int32_t first = min(2 * (SUBS * stage + sub), blocks - 1);  // past the last in a partial stage
+            const uint32_t block = uint32_t(min(h, blocks - 1 - first));
+            const uint8_t* const from = codes + first * kBlockBytes;
+            const uint8_t* const bytes = scales + first;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+                x.w[sub][c] = *reinterpret_cast<const u32x4*>(from + (column[c] + block) * uint32_t(kBlockBytes));
+                x.s[sub][c] = bytes[column[c] + block];
+            }
         }
     };
 
@@ -369,24 +374,27 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
         }
         if (s + 2 < end) load_x(s + 2);
         const char* const from = stages + (s - begin) % 2 * S::STAGE + (wave_row + n) * S::ROW + 64 * h;
-        float factor[CT];
 #pragma unroll
-        for (int c = 0; c < CT; ++c) factor[c] = factor_of(now.s[c]);
+        for (int sub = 0; sub < SUBS; ++sub) {
+            float factor[CT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bf16x8 wf[CT];
+            for (int c = 0; c < CT; ++c) factor[c] = factor_of(now.s[sub][c]);
 #pragma unroll
-            for (int c = 0; c < CT; ++c) wf[c] = fragment_of(now.w[c][i], factor[c]);
+            for (int i = 0; i < 4; ++i) {
+                bf16x8 wf[CT];
 #pragma unroll
-            for (int r = 0; r < RT; ++r)
+                for (int c = 0; c < CT; ++c) wf[c] = fragment_of(now.w[sub][c][i], factor[c]);
 #pragma unroll
-                for (int q = PARTS - 1; q >= 0; --q) {
-                    const bf16x8 xf =
-                        *reinterpret_cast<const bf16x8*>(from + q * S::PART + 32 * r * S::ROW + 16 * i);
+                for (int r = 0; r < RT; ++r)
 #pragma unroll
-                    for (int c = 0; c < CT; ++c)
-                        acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xf, wf[c], acc[r][c], 0, 0, 0);
-                }
+                    for (int q = PARTS - 1; q >= 0; --q) {
+                        const bf16x8 xf = *reinterpret_cast<const bf16x8*>(from + q * S::PART + 32 * r * S::ROW +
+                                                                           128 * sub + 16 * i);
+#pragma unroll
+                        for (int c = 0; c < CT; ++c)
+                            acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xf, wf[c], acc[r][c], 0, 0, 0);
+                    }
+            }
         }
         __syncthreads();
     }
@@ -429,11 +437,11 @@ hipError_t few_rows(const ProductArgs& a, int waves, hipStream_t stream) {
     return hipGetLastError();
 }
 
-template <int RT, int CT, int WR, int WC, int PARTS>
+template <int RT, int CT, int WR, int WC, int PARTS, int SUBS>
 hipError_t tiles(ProductArgs a, int64_t wanted, hipStream_t stream) {
-    using S = TileShape<RT, CT, WR, WC, PARTS>;
+    using S = TileShape<RT, CT, WR, WC, PARTS, SUBS>;
     const int64_t tiles_n = (a.cols + S::COLS - 1) / S::COLS;
-    const int64_t stages = (a.blocks + 1) / 2;
+    const int64_t stages = (a.blocks + 2 * SUBS - 1) / (2 * SUBS);
     // As many rows a launch as its grid (under 2^32 threads) holds.
     const int64_t most = std::max<int64_t>(1, ((int64_t(1) << 32) - 1) / S::THREADS / tiles_n) * S::ROWS;
     const ProductArgs all = a;
@@ -447,14 +455,14 @@ hipError_t tiles(ProductArgs a, int64_t wanted, hipStream_t stream) {
         const int64_t tiles = launch.tiles_m * tiles_n;
         const int64_t bytes = a.rows * a.cols * int64_t(sizeof(float));
         const int64_t room = a.workspace != nullptr ? int64_t(a.workspace_bytes) / bytes : 0;
-        int64_t slices = std::min({wanted / tiles, stages / 4, room});
+        int64_t slices = std::min({wanted / tiles, stages * SUBS / 4, room});
         slices = std::max<int64_t>(1, slices);
         launch.stages = int32_t((stages + slices - 1) / slices);
         launch.slices = int32_t(std::max<int64_t>(1, (stages + launch.stages - 1) / std::max(1, launch.stages)));
         launch.sums = static_cast<float*>(a.workspace);
-        auto* const kernel = quads_of(a.inner) == Quads::kWhole     ? tile_kernel<RT, CT, WR, WC, PARTS, Quads::kWhole>
-                             : quads_of(a.inner) == Quads::kShifted ? tile_kernel<RT, CT, WR, WC, PARTS, Quads::kShifted>
-                                                                    : tile_kernel<RT, CT, WR, WC, PARTS, Quads::kSingle>;
+        auto* const kernel = quads_of(a.inner) == Quads::kWhole     ? tile_kernel<RT, CT, WR, WC, PARTS, SUBS, Quads::kWhole>
+                             : quads_of(a.inner) == Quads::kShifted ? tile_kernel<RT, CT, WR, WC, PARTS, SUBS, Quads::kShifted>
+                                                                    : tile_kernel<RT, CT, WR, WC, PARTS, SUBS, Quads::kSingle>;
         hipLaunchKernelGGL(kernel, dim3(unsigned(tiles * launch.slices)),
                            dim3(S::THREADS), 0, stream, a, launch);
         hipError_t err = hipGetLastError();
@@ -481,11 +489,11 @@ hipError_t many_rows(const ProductArgs& a, hipStream_t stream) {
     if constexpr (PARTS == 3) {
         const int64_t rounds = up(up(a.rows, 128) * up(a.cols, 256), cus);
         if (rounds * cus * (128 * 256) * 4 <= up(a.rows, 32) * 32 * up(a.cols, 128) * 128 * 5)
-            return tiles<2, 2, 2, 4, PARTS>(a, 0, stream);
+            return tiles<2, 2, 2, 4, PARTS, 1>(a, 0, stream);
     } else {
-        if (up(a.rows, 64) * up(a.cols, 128) >= 2 * cus) return tiles<2, 1, 1, 4, PARTS>(a, 0, stream);
+        if (up(a.rows, 64) * up(a.cols, 128) >= 2 * cus) return tiles<2, 1, 1, 4, PARTS, 2>(a, 0, stream);
     }
-    return tiles<1, 1, 1, 4, PARTS>(a, 2 * cus, stream);
+    return tiles<1, 1, 1, 4, PARTS, PARTS == 1 ? 2 : 1>(a, 2 * cus, stream);
 }
 
 template <int T, int PAIRS, int PARTS>

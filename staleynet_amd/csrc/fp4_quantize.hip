@@ -15,6 +15,7 @@
 // four lanes.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "fp4_device.h"
@@ -137,78 +138,83 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(WeightArgs a) {
     }
 }
 
-// Where eight values of a cache row are: e counts (sequence, time, head, eighth)
-// of keys and then of values, so that neighbouring lanes read neighbouring columns
-// of a packed row.
+// A workgroup takes packed rows (sequence b, token t), its threads the row's eights of
+// values: those of the keys, head by head, then of the values, so that neighbouring lanes
+// have neighbouring columns.
 struct CachePlace {
-    bool values, held;
-    int64_t b, t, h, eighth;
-    int64_t row;  // of the cache
+    bool values;
+    int32_t h, eighth;
 };
-__device__ __forceinline__ CachePlace cache_place(const CacheRowsArgs& a, int64_t e) {
-    const int64_t eighths = a.head_dim / 8;
+template <int H>
+__device__ __forceinline__ CachePlace cache_place(int32_t item, int32_t kv_heads) {
+    const int32_t half = kv_heads * (H / 8);
     CachePlace p;
-    p.eighth = e % eighths;
-    e /= eighths;
-    p.h = e % a.kv_heads;
-    e /= a.kv_heads;
-    p.values = e % 2 != 0;
-    e /= 2;
-    p.t = e % a.time;
-    p.b = e / a.time;
-    const int64_t at = (a.positions != nullptr ? int64_t(a.positions[p.b]) : a.position) + p.t;
-    p.held = at < a.capacity;
-    p.row = (p.b * a.kv_heads + p.h) * a.capacity + at;
+    p.values = item >= half;
+    item -= p.values ? half : 0;
+    p.h = item / (H / 8);
+    p.eighth = item % (H / 8);
     return p;
 }
+// The cache position of a packed row, or -1 past the capacity.
+__device__ __forceinline__ int64_t position_of(const CacheRowsArgs& a, int64_t b, int64_t t) {
+    const int64_t at = (a.positions != nullptr ? int64_t(a.positions[b]) : a.position) + t;
+    return at < a.capacity ? at : -1;
+}
 
-template <bool VECTOR>
-__global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheRowsArgs a, int64_t total) {
-    const int64_t stride = int64_t(gridDim.x) * kThreads;
-    // total is a multiple of 4 and a block's four lanes share b and t: they go together.
-    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < total; e += stride) {
-        const CachePlace p = cache_place(a, e);
-        if (!p.held) continue;
-        const float* from = a.packed + (p.b * a.time + p.t) * a.width + (p.values ? a.value_column : a.key_column) +
-                            p.h * a.head_dim + 8 * p.eighth;
-        float v[8];
-        if (VECTOR) {
-            const f32x4 lo = reinterpret_cast<const f32x4*>(from)[0], hi = reinterpret_cast<const f32x4*>(from)[1];
+template <int H, bool VECTOR>
+__global__ __launch_bounds__(kThreads) void cache_append_kernel(CacheRowsArgs a) {
+    const int32_t heads = int32_t(a.kv_heads), items = 2 * heads * (H / 8);  // under 2^26
+    for (int64_t row = blockIdx.x; row < a.batch * a.time; row += gridDim.x) {
+        const int64_t b = row / a.time, at = position_of(a, b, row % a.time);
+        if (at < 0) continue;
+        // items is a multiple of 4: the four lanes of a block leave the loop together.
+        for (int32_t item = threadIdx.x; item < items; item += blockDim.x) {
+            const CachePlace p = cache_place<H>(item, heads);
+            const float* from =
+                a.packed + row * a.width + (p.values ? a.value_column : a.key_column) + p.h * H + 8 * p.eighth;
+            float v[8];
+            if (VECTOR) {
+                const f32x4 lo = reinterpret_cast<const f32x4*>(from)[0], hi = reinterpret_cast<const f32x4*>(from)[1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
-        } else {
+                for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = from[i];
+                for (int i = 0; i < 8; ++i) v[i] = from[i];
+            }
+            uint32_t s;
+            const uint32_t word = quantize8(v, s);
+            const int64_t cache_row = (b * heads + p.h) * a.capacity + at;
+            uint8_t* codes = p.values ? a.v_codes : a.k_codes;
+            uint8_t* scales = p.values ? a.v_scales : a.k_scales;
+            reinterpret_cast<uint32_t*>(codes)[cache_row * (H / 8) + p.eighth] = word;
+            if ((p.eighth & 3) == 0) scales[cache_row * (H / 32) + p.eighth / 4] = uint8_t(s);
         }
-        uint32_t s;
-        const uint32_t word = quantize8(v, s);
-        uint8_t* codes = p.values ? a.v_codes : a.k_codes;
-        uint8_t* scales = p.values ? a.v_scales : a.k_scales;
-        reinterpret_cast<uint32_t*>(codes)[p.row * (a.head_dim / 8) + p.eighth] = word;
-        if ((p.eighth & 3) == 0) scales[p.row * (a.head_dim / kBlock) + p.eighth / 4] = uint8_t(s);
     }
 }
 
-template <bool VECTOR>
-__global__ __launch_bounds__(kThreads) void cache_read_kernel(CacheRowsArgs a, int64_t total) {
-    const int64_t stride = int64_t(gridDim.x) * kThreads;
-    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < total; e += stride) {
-        const CachePlace p = cache_place(a, e);
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (p.held) {
-            const uint8_t* codes = p.values ? a.v_codes : a.k_codes;
-            const uint8_t* scales = p.values ? a.v_scales : a.k_scales;
-            dequantize8(reinterpret_cast<const uint32_t*>(codes)[p.row * (a.head_dim / 8) + p.eighth],
-                        scales[p.row * (a.head_dim / kBlock) + p.eighth / 4], v);
-        }
-        float* to = (p.values ? a.values : a.keys) + ((p.b * a.kv_heads + p.h) * a.time + p.t) * a.head_dim +
-                    8 * p.eighth;
-        if (VECTOR) {
-            reinterpret_cast<f32x4*>(to)[0] = f32x4{v[0], v[1], v[2], v[3]};
-            reinterpret_cast<f32x4*>(to)[1] = f32x4{v[4], v[5], v[6], v[7]};
-        } else {
+template <int H, bool VECTOR>
+__global__ __launch_bounds__(kThreads) void cache_read_kernel(CacheRowsArgs a) {
+    const int32_t heads = int32_t(a.kv_heads), items = 2 * heads * (H / 8);
+    for (int64_t row = blockIdx.x; row < a.batch * a.time; row += gridDim.x) {
+        const int64_t b = row / a.time, t = row % a.time, at = position_of(a, b, t);
+        for (int32_t item = threadIdx.x; item < items; item += blockDim.x) {
+            const CachePlace p = cache_place<H>(item, heads);
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (at >= 0) {
+                const int64_t cache_row = (b * heads + p.h) * a.capacity + at;
+                const uint8_t* codes = p.values ? a.v_codes : a.k_codes;
+                const uint8_t* scales = p.values ? a.v_scales : a.k_scales;
+                dequantize8(reinterpret_cast<const uint32_t*>(codes)[cache_row * (H / 8) + p.eighth],
+                            scales[cache_row * (H / 32) + p.eighth / 4], v);
+            }
+            float* to = (p.values ? a.values : a.keys) + ((b * heads + p.h) * a.time + t) * H + 8 * p.eighth;
+            if (VECTOR) {
+                reinterpret_cast<f32x4*>(to)[0] = f32x4{v[0], v[1], v[2], v[3]};
+                reinterpret_cast<f32x4*>(to)[1] = f32x4{v[4], v[5], v[6], v[7]};
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[i] = v[i];
+                for (int i = 0; i < 8; ++i) to[i] = v[i];
+            }
         }
     }
 }
@@ -243,23 +249,37 @@ hipError_t launch_dequantize(const WeightArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-hipError_t launch_cache_append(const CacheRowsArgs& a, hipStream_t stream) {
-    const int64_t total = 2 * a.batch * a.time * a.kv_heads * (a.head_dim / 8);
-    if (total == 0) return hipSuccess;
-    const bool vector =
-        aligned16(a.packed) && a.width % 4 == 0 && a.key_column % 4 == 0 && a.value_column % 4 == 0;
-    hipLaunchKernelGGL(vector ? cache_append_kernel<true> : cache_append_kernel<false>, dim3(grid_of(total)),
-                       dim3(kThreads), 0, stream, a, total);
+namespace {
+
+// One workgroup a packed row, up to 2^20 of them (they loop over the rest).
+template <int H>
+hipError_t launch_rows(const CacheRowsArgs& a, bool append, bool vector, hipStream_t stream) {
+    const int64_t rows = a.batch * a.time, items = 2 * a.kv_heads * (H / 8);
+    if (rows == 0 || items == 0) return hipSuccess;
+    const dim3 grid(unsigned(std::min<int64_t>(rows, int64_t(1) << 20)));
+    const dim3 threads(unsigned(std::min<int64_t>(kThreads, (items + 63) / 64 * 64)));
+    auto* const kernel = append ? (vector ? cache_append_kernel<H, true> : cache_append_kernel<H, false>)
+                                : (vector ? cache_read_kernel<H, true> : cache_read_kernel<H, false>);
+    hipLaunchKernelGGL(kernel, grid, threads, 0, stream, a);
     return hipGetLastError();
+}
+hipError_t launch_rows(const CacheRowsArgs& a, bool append, bool vector, hipStream_t stream) {
+    switch (a.head_dim) {
+        case 32: return launch_rows<32>(a, append, vector, stream);
+        case 64: return launch_rows<64>(a, append, vector, stream);
+        default: return launch_rows<128>(a, append, vector, stream);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_cache_append(const CacheRowsArgs& a, hipStream_t stream) {
+    const bool vector = aligned16(a.packed) && a.width % 4 == 0 && a.key_column % 4 == 0 && a.value_column % 4 == 0;
+    return launch_rows(a, true, vector, stream);
 }
 
 hipError_t launch_cache_read(const CacheRowsArgs& a, hipStream_t stream) {
-    const int64_t total = 2 * a.batch * a.time * a.kv_heads * (a.head_dim / 8);
-    if (total == 0) return hipSuccess;
-    const bool vector = aligned16(a.keys) && aligned16(a.values);
-    hipLaunchKernelGGL(vector ? cache_read_kernel<true> : cache_read_kernel<false>, dim3(grid_of(total)),
-                       dim3(kThreads), 0, stream, a, total);
-    return hipGetLastError();
+    return launch_rows(a, false, aligned16(a.keys) && aligned16(a.values), stream);
 }
 
 }  // namespace fp4
