@@ -188,6 +188,73 @@ def test_nan_reaches_only_the_queries_that_see_it(gpu, head_dim):
     assert np.isnan(got[0, 2, 39, :32]).all() and not np.isnan(got[0, 2, 38, :min(32, head_dim - 32)]).any()
 
 
+def test_a_cache_whose_offsets_pass_32_bits(gpu):
+    """4.3 GB of codes a buffer. Positions never written hold zeros: their scores and values are 0, so
+    a query's result is known from the last 40 positions alone."""
+    batch, kv_heads, capacity, head_dim, time = 2, 8, 1 << 22, 128, 40
+    rng = np.random.default_rng(12)
+    cache = gpu.fp4_cache(batch, kv_heads, capacity, head_dim)
+    columns = kv_heads * head_dim
+    packed = rng.standard_normal((batch * time, 2 * columns)).astype(np.float32)
+    rows = gpu.upload(Shape(batch * time, 2 * columns), packed)
+    first = [capacity - time, capacity - time - 1000]
+    positions = gpu.upload_tokens(first)
+    gpu.fp4_cache_append(cache, rows, time, 2 * columns, 0, columns, positions=positions)
+    keys, values = (gpu.zeros(Shape.vector(batch * kv_heads * time * head_dim)) for _ in range(2))
+    gpu.fp4_cache_read(cache, time, keys, values, positions=positions)
+    held = [ref.dequantize(*ref.quantize(packed[:, i * columns:(i + 1) * columns].reshape(-1, head_dim)))
+            .reshape(batch, time, kv_heads, head_dim).transpose(0, 2, 1, 3) for i in range(2)]
+    for got, expected in zip((keys, values), held):
+        assert np.array_equal(gpu.download(got), expected.astype(np.float32).ravel())
+    q = rng.standard_normal((batch, kv_heads, 1, head_dim)).astype(np.float32)
+    out = gpu.zeros(Shape.vector(q.size))
+    lengths = [n + time for n in first]
+    scale = 1.5 * head_dim ** -0.5 * 4
+    gpu.fp4_attention(cache, gpu.upload(Shape.vector(q.size), q), out, kv_heads, 1, scale,
+                      lengths=gpu.upload_tokens(lengths))
+    got = gpu.download(out).reshape(batch, kv_heads, head_dim)
+    for b in range(batch):
+        for head in range(kv_heads):
+            s = held[0][b, head] @ q[b, head, 0].astype(np.float64) * scale
+            top = max(s.max(), 0.0)
+            p = np.exp(s - top)
+            expected = p @ held[1][b, head] / (p.sum() + first[b] * np.exp(-top))
+            # Within the module's bound: A under 100, chains of 4e6 / 32 / 8 / 32 keys a wave, V under 6.
+            assert np.abs(got[b, head] - expected).max() <= 1e-3 * np.abs(expected).max() + 1e-6
+
+
+def test_two_contexts_do_not_share_their_splits(gpu):
+    """Split caches on two contexts at once: each merges its own records."""
+    case = Case(2, 8, 2, 1, 5000, 64, [5000, 3000], seed=9)
+    expected = case.run(gpu)
+    other = Gpu(0, workspace_bytes=64 << 20)
+    try:
+        cases = [Case(2, 8, 2, 1, 5000, 64, [5000, 3000], seed=9) for _ in range(2)]
+        runs = []
+        for context, c in zip((gpu, other), cases):
+            cache = c.cache(context)
+            q = context.upload(Shape.vector(c.q.size), c.q)
+            out = context.zeros(Shape.vector(c.q.size))
+            lengths = context.upload_tokens(c.lengths)
+            runs.append((context, c, cache, q, out, lengths))
+        for _ in range(20):
+            for context, c, cache, q, out, lengths in runs:
+                context.fp4_attention(cache, q, out, c.heads, 1, c.scale, lengths=lengths)
+        for context, c, cache, q, out, lengths in runs:
+            assert np.array_equal(context.download(out).reshape(c.q.shape), expected)
+        del runs, cache, q, out, lengths
+    finally:
+        other.close()
+
+
+def test_an_empty_cache(gpu):
+    cache = gpu.fp4_cache(2, 2, 0, 64)
+    q = gpu.upload(Shape.vector(256), np.ones(256))
+    out = gpu.upload(Shape.vector(256), np.ones(256))
+    gpu.fp4_attention(cache, q, out, 2, 1, 1.0, lengths=gpu.upload_tokens([7, 0]))
+    assert not gpu.download(out).any()
+
+
 def test_refusals_on_the_device(gpu):
     case = Case(1, 2, 2, 2, 8, 32, [8])
     cache = case.cache(gpu)

@@ -11,7 +11,7 @@ import pytest
 
 import fp4_reference as ref
 from fp4_reference import View
-from staleynet_amd.gemm import Fp4Matrix, Gpu, MatmulKernel, MatmulPanic, MatmulSpec, Precision, Shape
+from staleynet_amd.gemm import Fp4Matrix, Gpu, MatmulKernel, MatmulPanic, MatmulSpec, Precision, Shape, Storage
 
 pytestmark = pytest.mark.gpu
 
@@ -180,6 +180,27 @@ def test_precision_goes_by_the_context_and_the_spec():
             assert np.array_equal(run(gpu, spec.with_precision(Precision.Bf16), x, codes, scales), bf16)
     finally:
         gpu.close()
+
+
+@pytest.mark.parametrize("rows", [2, 9, 20])
+def test_codes_past_32_bits(gpu, rows):
+    """5 GB of codes, zeros but for the last 40 columns."""
+    cols, inner, some = 300_000, 32_768, 40
+    rng = np.random.default_rng(rows)
+    matrix = gpu.fp4_matrix(cols, inner)
+    w = rng.standard_normal((some, inner)).astype(np.float32)
+    blocks = inner // 32
+    part = Fp4Matrix(some, inner, View(matrix.codes, (cols - some) * blocks * 16, some * blocks * 16, 1),
+                     View(matrix.scales, (cols - some) * blocks, some * blocks, 1))
+    gpu.quantize_fp4(gpu.upload(Shape.vector(w.size), w), part, Storage.Transposed)
+    x = rng.standard_normal((rows, inner)).astype(np.float32)
+    out = gpu.upload(Shape(rows, cols), np.ones(rows * cols))
+    gpu.matmul_fp4(MatmulSpec.new(rows, cols, inner).right_transposed(), gpu.upload(Shape(rows, inner), x), matrix, out)
+    got = gpu.download(out).reshape(rows, cols)
+    assert not got[:, :-some].any()
+    values = ref.dequantize(gpu.download_bytes(part.codes).reshape(some, -1),
+                            gpu.download_bytes(part.scales).reshape(some, -1), inner)
+    check(got[:, -some:], x, values, inner)
 
 
 def test_empty_products_and_refusals_on_the_device(gpu):
