@@ -27,6 +27,9 @@
 //   Gpu::causal_attention_with_stats, Gpu::causal_attention_backward (the forward keeping per-query
 //                     statistics instead of the probabilities, and the backward that recomputes
 //                     them; no reference counterpart: layers/attention.rs:206-213 and :238-260)
+//   ByteBuffer, Fp4Matrix, Fp4Cache, Gpu::quantize_fp4 / dequantize_fp4 / matmul_fp4 /
+//   fp4_cache_append / fp4_cache_read / fp4_attention (4-bit weights and cache, staleynet_fp4.h; no
+//                     reference counterpart)
 // The reference panics on undersized operands; here that is a thrown
 // staleynet_cuda::Panic carrying the same message. Driver errors (the
 // reference's Err(DriverError)) are thrown as staleynet_cuda::GpuError.
@@ -40,6 +43,7 @@
 #include <utility>
 #include <vector>
 
+#include "staleynet_fp4.h"
 #include "staleynet_gemm.h"
 
 namespace staleynet_cuda {
@@ -239,6 +243,51 @@ class TokenBuffer {
     sn_context* context_ = nullptr;
     uint32_t* buffer_ = nullptr;
     size_t count_ = 0;
+};
+
+// Bytes in device memory: the codes or the scales of 4-bit blocks; owns its buffer (move-only).
+class ByteBuffer {
+   public:
+    ByteBuffer() = default;
+    ByteBuffer(sn_context* context, uint8_t* buffer, size_t count) : context_(context), buffer_(buffer), count_(count) {}
+    ByteBuffer(const ByteBuffer&) = delete;
+    ByteBuffer& operator=(const ByteBuffer&) = delete;
+    ByteBuffer(ByteBuffer&& other) noexcept { *this = std::move(other); }
+    ByteBuffer& operator=(ByteBuffer&& other) noexcept {
+        if (this != &other) {
+            release();
+            context_ = std::exchange(other.context_, nullptr);
+            buffer_ = std::exchange(other.buffer_, nullptr);
+            count_ = std::exchange(other.count_, 0);
+        }
+        return *this;
+    }
+    ~ByteBuffer() { release(); }
+
+    size_t len() const { return count_; }
+    const uint8_t* data() const { return buffer_; }
+    uint8_t* data() { return buffer_; }
+
+   private:
+    void release() {
+        if (buffer_ != nullptr) sn_free_bytes(context_, buffer_);
+        buffer_ = nullptr;
+    }
+    sn_context* context_ = nullptr;
+    uint8_t* buffer_ = nullptr;
+    size_t count_ = 0;
+};
+
+// A product's right operand [inner, cols] in 4 bits (staleynet_fp4.h).
+struct Fp4Matrix {
+    size_t cols = 0, inner = 0;
+    ByteBuffer codes, scales;
+};
+
+// A key/value cache [batch][kv_heads][capacity][head_dim] in 4 bits (staleynet_fp4.h).
+struct Fp4Cache {
+    sn_fp4_cache_shape shape{};
+    ByteBuffer k_codes, k_scales, v_codes, v_scales;
 };
 
 // Where a group of attention heads sits in the packed activations and in the
@@ -461,9 +510,83 @@ class Gpu {
                                            v_grad.len()));
     }
 
+    // Zeroed bytes (sn_alloc_bytes), and the 4-bit operands made of them.
+    ByteBuffer zeros_bytes(size_t count) const {
+        uint8_t* buffer = nullptr;
+        check(sn_alloc_bytes(context_, count, &buffer));
+        return ByteBuffer(context_, buffer, count);
+    }
+    Fp4Matrix fp4_matrix(size_t cols, size_t inner) const {
+        size_t codes = 0, scales = 0;
+        check(sn_fp4_sizes(cols, inner, &codes, &scales));
+        return Fp4Matrix{cols, inner, zeros_bytes(codes), zeros_bytes(scales)};
+    }
+    Fp4Cache fp4_cache(const sn_fp4_cache_shape& shape) const {
+        size_t codes = 0, scales = 0;
+        check(sn_fp4_sizes(shape.batch * shape.kv_heads * shape.capacity, shape.head_dim, &codes, &scales));
+        return Fp4Cache{shape, zeros_bytes(codes), zeros_bytes(scales), zeros_bytes(codes), zeros_bytes(scales)};
+    }
+
+    // A right operand [inner, cols], stored as `storage` says, to 4 bits and back (sn_quantize_fp4,
+    // sn_dequantize_fp4).
+    void quantize_fp4(const Tensor& source, Fp4Matrix& matrix, Storage storage = Storage::RowMajor) const {
+        check(sn_quantize_fp4(context_, matrix.cols, matrix.inner, abi_storage(storage), source.data(), source.len(),
+                              matrix.codes.data(), matrix.codes.len(), matrix.scales.data(), matrix.scales.len()));
+    }
+    void dequantize_fp4(const Fp4Matrix& matrix, Tensor& output, Storage storage = Storage::RowMajor) const {
+        check(sn_dequantize_fp4(context_, matrix.cols, matrix.inner, abi_storage(storage), matrix.codes.data(),
+                                matrix.codes.len(), matrix.scales.data(), matrix.scales.len(), output.data(),
+                                output.len()));
+    }
+
+    // `Gpu::matmul`, or with a bias matmul_bias, against a 4-bit right operand (sn_matmul_fp4); the spec
+    // is right_transposed.
+    void matmul_fp4(const MatmulSpec& spec, const Tensor& left, const Fp4Matrix& right, Tensor& output,
+                    const Tensor* bias = nullptr) const {
+        if (right.cols != spec.cols || right.inner != spec.inner)
+            throw Panic(SN_ERR_RIGHT_TOO_SMALL, "matmul_fp4: the operand's columns and inner length are not the spec's");
+        const sn_matmul_spec c = spec.to_ffi();
+        check(sn_matmul_fp4(context_, &c, left.data(), left.len(), right.codes.data(), right.codes.len(),
+                            right.scales.data(), right.scales.len(), bias ? bias->data() : nullptr,
+                            bias ? bias->len() : 0, output.data(), output.len()));
+    }
+
+    // split_heads of the keys and values of packed rows into a 4-bit cache, at each sequence's own
+    // position where `positions` is given (sn_fp4_cache_append), and their values (sn_fp4_cache_read).
+    void fp4_cache_append(Fp4Cache& cache, const sn_fp4_cache_rows& rows, const Tensor& packed,
+                          const TokenBuffer* positions = nullptr) const {
+        check(sn_fp4_cache_append(context_, &cache.shape, &rows, packed.data(), packed.len(),
+                                  positions ? positions->data() : nullptr, positions ? positions->len() : 0,
+                                  cache.k_codes.data(), cache.k_codes.len(), cache.k_scales.data(),
+                                  cache.k_scales.len(), cache.v_codes.data(), cache.v_codes.len(),
+                                  cache.v_scales.data(), cache.v_scales.len()));
+    }
+    void fp4_cache_read(const Fp4Cache& cache, const sn_fp4_cache_rows& rows, Tensor& keys, Tensor& values,
+                        const TokenBuffer* positions = nullptr) const {
+        check(sn_fp4_cache_read(context_, &cache.shape, &rows, cache.k_codes.data(), cache.k_codes.len(),
+                                cache.k_scales.data(), cache.k_scales.len(), cache.v_codes.data(),
+                                cache.v_codes.len(), cache.v_scales.data(), cache.v_scales.len(),
+                                positions ? positions->data() : nullptr, positions ? positions->len() : 0,
+                                keys.data(), keys.len(), values.data(), values.len()));
+    }
+
+    // Causal attention over a 4-bit cache (sn_fp4_attention); `lengths` null: shape.keys for every sequence.
+    void fp4_attention(const Fp4Cache& cache, const sn_fp4_attention_shape& shape, const Tensor& q, Tensor& out,
+                       const TokenBuffer* lengths = nullptr) const {
+        check(sn_fp4_attention(context_, &cache.shape, &shape, q.data(), q.len(), cache.k_codes.data(),
+                               cache.k_codes.len(), cache.k_scales.data(), cache.k_scales.len(),
+                               cache.v_codes.data(), cache.v_codes.len(), cache.v_scales.data(),
+                               cache.v_scales.len(), lengths ? lengths->data() : nullptr,
+                               lengths ? lengths->len() : 0, out.data(), out.len()));
+    }
+
     sn_context* raw() const { return context_; }
 
    private:
+    static uint32_t abi_storage(Storage storage) {
+        return storage == Storage::Transposed ? SN_TRANSPOSED : SN_ROW_MAJOR;
+    }
+
     // check_layout (ops/attention.rs:11-18).
     static void check_layout(const HeadLayout& layout, const Tensor& packed, const Tensor& head_major) {
         if (layout.time_offset + layout.time > layout.time_capacity)
