@@ -79,10 +79,9 @@ int weight_call(sn_context* ctx, bool quantize, size_t cols, size_t inner, uint3
     args.scales = const_cast<uint8_t*>(scales);
     args.cols = int64_t(cols);
     args.inner = int64_t(inner);
-    args.col_step = storage == SN_TRANSPOSED ? args.inner : 1;
-    args.inner_step = storage == SN_TRANSPOSED ? 1 : args.cols;
+    args.transposed = storage == SN_TRANSPOSED;
     hipError_t err = hipSetDevice(ctx->device);
-    if (err == hipSuccess) err = quantize ? launch_quantize(args, ctx->stream) : launch_dequantize(args, ctx->stream);
+    if (err == hipSuccess) err = launch_weights(args, quantize, ctx->stream);
     return status(err);
 }
 

@@ -10,7 +10,7 @@
 namespace sn {
 namespace fp4 {
 
-// Bytes of a block's codes; values past the largest scale byte that is not NaN.
+// Values and bytes of codes of a block; the largest scale byte that is not NaN's.
 constexpr int64_t kBlock = SN_FP4_BLOCK;
 constexpr int64_t kBlockBytes = kBlock / 2;
 constexpr uint32_t kLargestScale = 252;
@@ -18,17 +18,16 @@ constexpr uint32_t kLargestScale = 252;
 constexpr int64_t blocks_of(int64_t inner) { return (inner + kBlock - 1) / kBlock; }
 
 // Weights to 4 bits and back (fp4_quantize.hip): `cols` rows of the format with
-// `inner` values each, element k of row c at c * col_step + k * inner_step of the
-// fp32 side.
+// `inner` values each; the fp32 side is [inner, cols], or transposed [cols, inner].
 struct WeightArgs {
-    const float* source = nullptr;
-    float* output = nullptr;
+    const float* source = nullptr;  // to quantize
+    float* output = nullptr;        // else
     uint8_t* codes = nullptr;
     uint8_t* scales = nullptr;
-    int64_t cols = 0, inner = 0, col_step = 0, inner_step = 0;
+    int64_t cols = 0, inner = 0;
+    bool transposed = false;
 };
-hipError_t launch_quantize(const WeightArgs& args, hipStream_t stream);
-hipError_t launch_dequantize(const WeightArgs& args, hipStream_t stream);
+hipError_t launch_weights(const WeightArgs& args, bool quantize, hipStream_t stream);
 
 // Rows of a cache from packed fp32 rows, and back to dense fp32.
 struct CacheRowsArgs {

@@ -9,10 +9,12 @@
 // which v_cvt_scalef32_pk_fp4_f32 does (its result was compared at every tie, its
 // neighbours, past the largest code and at -0).
 //
-// All are bound by memory: 4 bytes a value on the fp32 side against 0.53. Four
-// lanes take a block, eight values each: 32-byte loads or stores, a word of codes a
-// lane, so a wave's codes are 256 contiguous bytes; the maximum is exchanged over
-// four lanes.
+// All are bound by memory: 4 bytes a value on the fp32 side against 0.53. Where the fp32 values of
+// a block are contiguous four lanes take it, eight values each: 32-byte loads or stores, a word of
+// codes a lane, so a wave's codes are 256 contiguous bytes; the maximum is exchanged over
+// four lanes. 8192 x 28672 weights: 183 us (5.8 TB/s) to 4 bits, 198 back, transposed; 308 and 232
+// with contiguous columns, where a wave writes 16 bytes each to 64 rows of codes (blocks taken in
+// runs of 4, 8 or 16 by a thread, to fill those rows' lines sooner: 331 to 342).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -38,6 +40,16 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t magnitude) {
     return uint32_t(min(max(s, 0), int32_t(kLargestScale)));
 }
 
+// Eight values' codes, lowest first.
+__device__ __forceinline__ uint32_t codes_of(const float* v, float factor) {
+    uint32_t word = 0;
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], factor, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], factor, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], factor, 2);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], factor, 3);
+    return word;
+}
+
 // Eight values of a block, four neighbouring lanes a block: this lane's word of
 // codes, and the block's scale byte. Every lane of the four has to call it.
 __device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t& s) {
@@ -47,14 +59,7 @@ __device__ __forceinline__ uint32_t quantize8(const float (&v)[8], uint32_t& s) 
     magnitude = max(magnitude, uint32_t(__shfl_xor(int(magnitude), 1)));
     magnitude = max(magnitude, uint32_t(__shfl_xor(int(magnitude), 2)));
     s = scale_byte(magnitude);
-    if (s > kLargestScale) return 0;
-    const float factor = factor_of(s);
-    uint32_t word = 0;
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[0], v[1], factor, 0);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[2], v[3], factor, 1);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[4], v[5], factor, 2);
-    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[6], v[7], factor, 3);
-    return word;
+    return s > kLargestScale ? 0 : codes_of(v, factor_of(s));
 }
 
 __device__ __forceinline__ void dequantize8(uint32_t word, uint32_t s, float (&v)[8]) {
@@ -66,75 +71,105 @@ __device__ __forceinline__ void dequantize8(uint32_t word, uint32_t s, float (&v
     v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1], v[4] = c[0], v[5] = c[1], v[6] = d[0], v[7] = d[1];
 }
 
-// One weight block a thread where the operand's columns are contiguous (reads
-// of neighbouring threads are neighbouring columns), else four lanes a block.
+// Weights whose columns are contiguous (SN_ROW_MAJOR): a block a thread, so that a wave reads or
+// writes 64 neighbouring columns at once.
 __global__ __launch_bounds__(kThreads) void quantize_columns_kernel(WeightArgs a) {
     const int64_t blocks = blocks_of(a.inner);
     const int64_t c = int64_t(blockIdx.x) * kThreads + threadIdx.x;
     if (c >= a.cols) return;
     for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
-        const float* from = a.source + c * a.col_step + b * kBlock * a.inner_step;
+        const float* from = a.source + b * kBlock * a.cols + c;
         float v[32];
         uint32_t magnitude = 0;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            v[i] = b * kBlock + i < a.inner ? from[i * a.inner_step] : 0.f;
+            v[i] = b * kBlock + i < a.inner ? from[i * a.cols] : 0.f;
             magnitude = max(magnitude, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
         }
         const uint32_t s = scale_byte(magnitude);
-        const float factor = factor_of(s);
         u32x4 words = {0, 0, 0, 0};
         if (s <= kLargestScale) {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t word = 0;
-                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * w], v[8 * w + 1], factor, 0);
-                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * w + 2], v[8 * w + 3], factor, 1);
-                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * w + 4], v[8 * w + 5], factor, 2);
-                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, v[8 * w + 6], v[8 * w + 7], factor, 3);
-                words[w] = word;
-            }
+            for (int w = 0; w < 4; ++w) words[w] = codes_of(&v[8 * w], factor_of(s));
         }
         *reinterpret_cast<u32x4*>(a.codes + (c * blocks + b) * kBlockBytes) = words;
         a.scales[c * blocks + b] = uint8_t(s);
     }
 }
-
-__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(WeightArgs a) {
+__global__ __launch_bounds__(kThreads) void dequantize_columns_kernel(WeightArgs a) {
     const int64_t blocks = blocks_of(a.inner);
-    const int64_t eighths = a.cols * blocks * 4;
-    const int64_t stride = int64_t(gridDim.x) * kThreads;
-    // eighths is a multiple of 4: the four lanes of a block leave the loop together.
-    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < eighths; e += stride) {
-        const int64_t block = e >> 2, c = block / blocks, k = (block % blocks) * kBlock + 8 * (e & 3);
-        const float* from = a.source + c * a.col_step + k;
-        float v[8];
+    const int64_t c = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+    if (c >= a.cols) return;
+    for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
+        const u32x4 words = *reinterpret_cast<const u32x4*>(a.codes + (c * blocks + b) * kBlockBytes);
+        const uint32_t s = a.scales[c * blocks + b];
+        float* to = a.output + b * kBlock * a.cols + c;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < a.inner ? from[i] : 0.f;
-        uint32_t s;
-        const uint32_t word = quantize8(v, s);
-        reinterpret_cast<uint32_t*>(a.codes)[e] = word;
-        if ((e & 3) == 0) a.scales[block] = uint8_t(s);
+        for (int w = 0; w < 4; ++w) {
+            float v[8];
+            dequantize8(words[w], s, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (b * kBlock + 8 * w + i < a.inner) to[(8 * w + i) * a.cols] = v[i];
+        }
     }
 }
 
-__global__ __launch_bounds__(kThreads) void dequantize_kernel(WeightArgs a) {
-    const int64_t blocks = blocks_of(a.inner);
-    const int64_t rows = blocks * 4;  // eights of values a column
-    const int64_t total = a.cols * rows;
+// Weights whose inner dimension is contiguous (SN_TRANSPOSED): four lanes a block. Rows start at any
+// 4-byte address; wide loads and stores need no more.
+typedef f32x4 f32x4_unaligned __attribute__((aligned(4)));
+__device__ __forceinline__ void eighth_of(int64_t e, int64_t per_row, bool narrow, int64_t& row, int64_t& at) {
+    if (narrow) {  // the division of 32-bit numbers is a fifth of the other's instructions
+        row = uint32_t(e) / uint32_t(per_row);
+        at = uint32_t(e) - uint32_t(row) * uint32_t(per_row);
+    } else {
+        row = e / per_row;
+        at = e - row * per_row;
+    }
+}
+__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(WeightArgs a) {
+    const int64_t per_row = 4 * blocks_of(a.inner), total = a.cols * per_row;
+    const int64_t stride = int64_t(gridDim.x) * kThreads;
+    // total is a multiple of 4: the four lanes of a block leave the loop together.
+    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < total; e += stride) {
+        int64_t c, eighth;
+        eighth_of(e, per_row, total <= int64_t(UINT32_MAX), c, eighth);
+        const int64_t k = 8 * eighth;
+        const float* from = a.source + c * a.inner + k;
+        float v[8];
+        if (k + 8 <= a.inner) {
+            const f32x4 lo = *reinterpret_cast<const f32x4_unaligned*>(from);
+            const f32x4 hi = *reinterpret_cast<const f32x4_unaligned*>(from + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = lo[i], v[4 + i] = hi[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = k + i < a.inner ? from[i] : 0.f;
+        }
+        uint32_t s;
+        const uint32_t word = quantize8(v, s);
+        reinterpret_cast<uint32_t*>(a.codes)[e] = word;
+        if ((e & 3) == 0) a.scales[e >> 2] = uint8_t(s);
+    }
+}
+__global__ __launch_bounds__(kThreads) void dequantize_rows_kernel(WeightArgs a) {
+    const int64_t per_row = 4 * blocks_of(a.inner), total = a.cols * per_row;
     const int64_t stride = int64_t(gridDim.x) * kThreads;
     for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < total; e += stride) {
-        // The contiguous side of the output first.
-        const bool columns = a.inner_step != 1;
-        const int64_t c = columns ? e % a.cols : e / rows, eighth = columns ? e / a.cols : e % rows;
+        int64_t c, eighth;
+        eighth_of(e, per_row, total <= int64_t(UINT32_MAX), c, eighth);
         const int64_t k = 8 * eighth;
         float v[8];
-        dequantize8(reinterpret_cast<const uint32_t*>(a.codes)[c * rows + eighth],
-                    a.scales[c * blocks + eighth / 4], v);
-        float* to = a.output + c * a.col_step + k * a.inner_step;
+        dequantize8(reinterpret_cast<const uint32_t*>(a.codes)[e], a.scales[e >> 2], v);
+        float* to = a.output + c * a.inner + k;
+        if (k + 8 <= a.inner) {
+            *reinterpret_cast<f32x4_unaligned*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4_unaligned*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (k + i < a.inner) to[i * a.inner_step] = v[i];
+            for (int i = 0; i < 8; ++i)
+                if (k + i < a.inner) to[i] = v[i];
+        }
     }
 }
 
@@ -230,22 +265,18 @@ unsigned grid_of(int64_t items) {
 
 }  // namespace
 
-hipError_t launch_quantize(const WeightArgs& a, hipStream_t stream) {
+hipError_t launch_weights(const WeightArgs& a, bool quantize, hipStream_t stream) {
     const int64_t blocks = blocks_of(a.inner);
     if (a.cols == 0 || blocks == 0) return hipSuccess;
-    if (a.inner_step == 1) {
-        hipLaunchKernelGGL(quantize_rows_kernel, dim3(grid_of(a.cols * blocks * 4)), dim3(kThreads), 0, stream, a);
+    if (a.transposed) {
+        hipLaunchKernelGGL((quantize ? quantize_rows_kernel : dequantize_rows_kernel), dim3(grid_of(a.cols * blocks * 4)),
+                           dim3(kThreads), 0, stream, a);
     } else {
-        const dim3 grid(unsigned((a.cols + kThreads - 1) / kThreads), unsigned(blocks < 65535 ? blocks : 65535));
-        hipLaunchKernelGGL(quantize_columns_kernel, grid, dim3(kThreads), 0, stream, a);
+        const int64_t groups = (a.cols + kThreads - 1) / kThreads;
+        const dim3 grid(unsigned(groups), unsigned(std::min<int64_t>(blocks, 65535)));
+        hipLaunchKernelGGL((quantize ? quantize_columns_kernel : dequantize_columns_kernel), grid, dim3(kThreads), 0,
+                           stream, a);
     }
-    return hipGetLastError();
-}
-
-hipError_t launch_dequantize(const WeightArgs& a, hipStream_t stream) {
-    const int64_t blocks = blocks_of(a.inner);
-    if (a.cols == 0 || blocks == 0) return hipSuccess;
-    hipLaunchKernelGGL(dequantize_kernel, dim3(grid_of(a.cols * blocks * 4)), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
