@@ -25,6 +25,11 @@
  * keep their sign (also of zero). A block of zeros has s = 0; one with an
  * infinity or NaN has s = 255 and codes 0.
  *
+ * Limits, past which a call is SN_ERR_OVERFLOW: columns and inner length of a
+ * matrix to quantize under 2^31; of a product, columns under 2^28 and inner
+ * length under 2^25; a cache's batch * kv_heads under 2^21 and its capacity
+ * under 2^30; batch * heads * queries of an attention call under 2^28.
+ *
  * Buffers are bytes in device memory (sn_alloc_bytes, sn_upload_bytes, or any
  * other). Code buffers are 16-byte aligned (SN_ERR_UNSUPPORTED otherwise).
  * Every call is asynchronous on the context's stream, allocates nothing and
@@ -155,7 +160,7 @@ typedef struct sn_fp4_attention_shape {
 /* out = softmax(scale * q K^T) V per query over the positions it sees, the
  * 4-bit form of sn_causal_attention (decode step and prompt chunk alike). A
  * query that sees no position (a sequence of length 0; padding ahead of a
- * shorter prompt) gives zeros. Positions a query does not see do not enter its
+ * shorter prompt) gives zeros; one whose scores are all -inf gives NaN. Positions a query does not see do not enter its
  * result, whatever they hold (also NaN blocks). fp32 arithmetic as in
  * sn_matmul_fp4. lengths over the capacity count as the capacity; `keys` over
  * it is SN_ERR_SHAPE. Buffers too short for the strides are SN_ERR_LENGTH_MISMATCH; out

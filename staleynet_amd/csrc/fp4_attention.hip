@@ -38,15 +38,15 @@ namespace {
 constexpr int kRows = 16;  // queries of a wave
 constexpr int kKeys = 32;  // keys of a step
 constexpr int kSplitWaves = 8;  // of a workgroup where several share a tile's keys
-constexpr int kTileWaves = 4;   // of one that has a tile to itself, where there are many
+constexpr int kTileWaves = 4;   // of one that has a tile to itself, where tiles fill the CUs
 
 struct KernelArgs {
     AttentionArgs a;
     float q_scale;          // scale log2 e
     int32_t group;          // query heads of a key/value head
     int32_t row_tiles;      // of a key/value head
-    int32_t workgroups;     // about as many workgroups as share the keys (0: one to a row tile)
-    int32_t least_keys;     // of a workgroup, a multiple of kKeys kSplitWaves
+    int32_t workgroups;     // that share the keys, but for one more a tile (0: one to a tile)
+    int32_t least_keys;     // of a workgroup's share, a multiple of kKeys kSplitWaves
     uint32_t* counters;     // one a row tile of every key/value head, zero between calls
     float* records;         // [workgroup][row][H + 4]: O, m, l
 };
@@ -285,7 +285,7 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
             run.l = run.l + x[e];
         }
         const SplitVector pr = split_finite(x, upper);  // a NaN reaches the result through l
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int d = 0; d < TILES; ++d) {
             const bf16x8 f = transposed(v_read + 32 * d, v_read + 16 * Stage::ROW + 32 * d);
@@ -293,7 +293,7 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
             for (int part = kParts - 1; part >= 0; --part)
                 run.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, pr.part[part], run.o[d], 0, 0, 0);
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
         if (poison[0] | poison[1]) {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -470,8 +470,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
         float* to = a.out + r.b * a.out_sequence + (r.kv_head * p.group + at % uint32_t(p.group)) * a.out_head +
                     int64_t(at / uint32_t(p.group)) * a.out_row + 4 * (unit % PIECES);
         const float inverse = 1.f / total;
+        // No term: nothing is seen, or every score is -inf, of which there is no softmax.
+        const float nothing = share.length - int32_t(a.queries) + int32_t(at / uint32_t(p.group)) < 0 ? 0.f : NAN;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) to[c] = total == 0.f ? 0.f : sum[c] * inverse;
+        for (int c = 0; c < 4; ++c) to[c] = total == 0.f ? nothing : sum[c] * inverse;
     };
     const __amdgpu_buffer_rsrc_t records = gemm::buffer_of(p.records + int64_t(share.first) * kRows * RECORD);
     for (int unit = tid; unit < units; unit += 64 * W) {
@@ -595,7 +597,11 @@ hipError_t launch(const AttentionArgs& a, KernelArgs p, hipStream_t stream) {
         grid = std::min(wanted + tiles, tiles * ((longest + p.least_keys - 1) / p.least_keys));
     }
     if (grid > INT32_MAX) return hipErrorInvalidValue;
-    if (tiles > 2 * resident)
+    // Tiles that fill the CUs by themselves need no eight waves each: of 3000 keys with h = 128, 400 tiles
+    // take 45.4 us of eight waves and 41.2 of four, 1600 tiles 147 and 125. (Fewer tiles are
+    // shared where the workspace allows it, else each has what one workgroup can give; 48 of 300 keys: 6.8
+    // either way.)
+    if (tiles > resident)
         hipLaunchKernelGGL((attention_kernel<H, kTileWaves>), dim3(unsigned(grid)), dim3(64 * kTileWaves), 0, stream, p);
     else
         hipLaunchKernelGGL((attention_kernel<H, kSplitWaves>), dim3(unsigned(grid)), dim3(64 * kSplitWaves), 0, stream, p);

@@ -17,6 +17,14 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// Between a wave's writes of LDS and its other lanes' reads of them, and back: the hardware
+// keeps the order of one wave's accesses, the fences the compiler's (no instruction comes of them).
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 // The factor a scale byte stands for: 2^(s - 127), subnormal for 0, NaN past
 // the largest. The conversions below read its exponent; a product code * factor
 // is exact in bf16 and in fp32 over that whole range (checked for every code and
@@ -41,8 +49,7 @@ __device__ __forceinline__ bf16x8 fragment_of(uint32_t word, float factor) {
 // An fp32 value as the exact sum of three bf16 values of its sign, each the
 // leading 8 significant bits of what is left (cut off, not rounded: the largest
 // float stays finite, and 24 = 8 + 8 + 8). Exact from 2^-110 on; below, what is
-// lost is under 2^-133.
-// Eight consecutive values of a fragment. An infinity or NaN leaves NaN in the
+// lost is under 2^-133. An infinity or NaN leaves NaN in the
 // rest, which one comparison a pair finds; then it is its own first part
 // and the others are 0, so that products follow IEEE arithmetic.
 __device__ __forceinline__ uint32_t upper_halves(float x0, float x1) {

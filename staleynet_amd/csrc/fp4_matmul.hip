@@ -201,7 +201,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
                 *reinterpret_cast<uint32_t*>(wave_lds + ((4 * scale_part + i) * (16 * C) + scale_col) * 4) = next_scales[i];
             if (step + RUN < end) next_scales = load_scales(step + RUN);
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int pair = 0; pair < PAIRS; ++pair) {
             u32x2 split[PARTS];
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
                 *reinterpret_cast<u32x2*>(parts + (q * rows + min(2 * pair + half, rows - 1)) * PART_ROW + 2 * quad) =
                     split[q];
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
         u32x4 now[C];
 #pragma unroll
         for (int c = 0; c < C; ++c) now[c] = next[c];
@@ -496,6 +496,11 @@ hipError_t many_rows(const ProductArgs& a, hipStream_t stream) {
     return tiles<1, 1, 1, 4, PARTS, PARTS == 1 ? 2 : 1>(a, 2 * cus, stream);
 }
 
+// C = 4 tiles of 16 columns a wave use x's parts four times, but want 4 x as many columns: of 4096
+// inner values, with 1 row and with 16, C = 1, 2 and 4 take
+//   4096 columns:   5.3,  6.0,  7.6 us and 10.1, 10.8, 14.2 us
+//   6144 columns:   7.0,  6.2,  7.7        18.4, 10.9, 14.3
+//   12288 columns:  9.0,  9.3,  9.2        27.3, 20.5, 15.3
 template <int T, int PAIRS, int PARTS>
 hipError_t few_rows_by_columns(const ProductArgs& a, hipStream_t stream) {
     const int waves = int(std::max<int64_t>(1, std::min<int64_t>(kMaxWaves, (a.blocks + 3) / 4)));
@@ -510,6 +515,8 @@ hipError_t few_rows_by_columns(const ProductArgs& a, hipStream_t stream) {
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
     if (a.rows == 0 || a.cols == 0) return hipSuccess;
     if (a.rows <= 16 && a.inner >= 4) {
+        // As few operands and loads of x as hold the rows (4096 x 8192: 2 rows 6.7 us, as 16 would be 11.3; one
+        // rounded to bf16 6.1, and 7.4).
         if (a.bf16) return a.rows <= 2 ? few_rows_by_columns<1, 1, 1>(a, stream) : few_rows_by_columns<1, 8, 1>(a, stream);
         return a.rows <= 2    ? few_rows_by_columns<1, 1, 3>(a, stream)
                : a.rows <= 5  ? few_rows_by_columns<1, 3, 3>(a, stream)

@@ -132,6 +132,23 @@ def test_attention_refusals():
     assert attention(q=(1 << 62, 64, 64)) == gemm.SN_ERR_OVERFLOW
 
 
+def test_limits():
+    """Sizes whose counts the kernels or their grids would not hold; the largest below are not refused as such."""
+    over = gemm.SN_ERR_OVERFLOW
+    assert product(MatmulSpec.new(1, 1, 1 << 25).right_transposed(), left_len=1 << 25) == over
+    assert product(MatmulSpec.new(1, 1, (1 << 25) - 1).right_transposed(),
+                   left_len=1 << 25) == gemm.SN_ERR_RIGHT_TOO_SMALL
+    assert product(MatmulSpec.new(1, 1 << 28, 1).right_transposed(), out_len=1 << 28) == over
+    assert product(MatmulSpec.new(1, (1 << 28) - 1, 1).right_transposed(),
+                   out_len=1 << 28) == gemm.SN_ERR_RIGHT_TOO_SMALL
+    for call in (append, attention):
+        assert call(cache=dict(batch=1 << 20, kv_heads=2)) == over
+        assert call(cache=dict(capacity=1 << 30)) == over
+        assert call(cache=dict(capacity=(1 << 30) - 1)) == gemm.SN_ERR_NULL_ARGUMENT  # the context
+    assert attention(queries=1 << 25) == over  # 2 * 6 heads
+    assert attention(queries=1 << 24) == gemm.SN_ERR_LENGTH_MISMATCH
+
+
 def test_the_reference_form_on_known_blocks():
     block = np.zeros((1, 32), np.float32)
     block[0, :8] = [6, -6, 0.25, 0.75, 5, -0.1, -0.0, 3.5]

@@ -188,6 +188,20 @@ def test_nan_reaches_only_the_queries_that_see_it(gpu, head_dim):
     assert np.isnan(got[0, 2, 39, :32]).all() and not np.isnan(got[0, 2, 38, :min(32, head_dim - 32)]).any()
 
 
+@pytest.mark.parametrize("length", [40, 3000])
+def test_scores_that_are_all_minus_infinity(gpu, length):
+    """q is infinite where every key is -1: no softmax, NaN; a query that sees no key is zeros all the same."""
+    case = Case(2, 2, 1, 4, length, 32, [length, 2], seed=length)
+    case.codes[0][..., 0] = case.codes[0][..., 0] & 0xF0 | 0xA  # -1 in the first place
+    case.q[:, 0, :, 0] = np.inf
+    got = case.run(gpu)
+    assert np.isnan(got[0, 0]).all() and np.isnan(got[1, 0, 2:]).all()
+    assert not got[1, :, :2].any()
+    case.q[:, 0] = 0
+    got[:, 0] = case.run(gpu)[:, 0]
+    case.check(got)
+
+
 def test_a_cache_whose_offsets_pass_32_bits(gpu):
     """4.3 GB of codes a buffer. Positions never written hold zeros: their scores and values are 0, so
     a query's result is known from the last 40 positions alone."""
