@@ -20,6 +20,9 @@
 // address units as much as the codes do (1 x 8192 x 28672: 39 us, 28 without any). So a
 // lane reads 16 of one column at once, for the next 16 / C steps, and the bytes
 // pass through LDS.
+//   What bounds it: W's bytes where there are many (1 x 8192 x 28672: 31.5 us, 125 MB at 4.0 TB/s), one
+// launch where there are few (1 x 768 x 2304: 3.8 us), and the parts' LDS reads and matrix instructions at 16
+// rows (16 x 4096 x 14336: 15.3 us for 31 MB).
 // More rows: tiles staged in LDS, below.
 #include <hip/hip_runtime.h>
 
@@ -263,7 +266,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 // staged in LDS, 64 inner values at a time, in two stages: while the matrix cores work
 // on one, the next is split and written, and the one after is on its way in registers. A
 // lane's 16 bytes of codes are a block of one column: 64 inner values of 32 columns a
-// load. D = x W: a lane holds one column. Inner value 8 i + j of half h of a stage is
+// load. D = x W: a lane holds one column. 2048 x 4096 x 4096 with fp32 inputs: 181 us, 380 TFLOP/s of products
+// (1140 of bf16 ones, matrix cores busy half the cycles; 130 us without any load, 150 without x's, and 175 to 177 with
+// the next stage's split spread between the matrix instructions, which costs one part a tenth). Inner value 8 i + j of half h of a stage is
 // element j of operand i of lanes h (as the block's words hold the codes).
 template <int RT, int CT, int WR, int WC, int PARTS, int SUBS>
 struct TileShape {
@@ -478,10 +483,11 @@ hipError_t tiles(ProductArgs a, int64_t wanted, hipStream_t stream) {
 
 // Tiles of 32 x 128 (27 KB of LDS, five workgroups a CU) hide their stages' latency best where
 // there are few of them, and the inner dimension is sliced until they fill the CUs twice.
-// Three parts: tiles of 128 x 256 (one a CU; 188 us at 2048 x 4096 x 4096 against 233) where the CUs' last
+// Three parts: tiles of 128 x 256 (one a CU; 181 us at 2048 x 4096 x 4096 against 233) where the CUs' last
 // round is full enough to keep that quarter: 2000 x 4096 x 4100 would be 346 us of them, 245 of small ones.
-// One part: 64 x 128 where they fill the CUs twice (2000 x 4096 x 4100: 141 us, 187 of small ones and 222 of
-// 128 x 256; 777 x 1001 x 1537, of which there are 169: 23 us against 19).
+// One part: 64 x 128 where they fill the CUs twice (2000 x 4096 x 4100: 134 us, 187 of small ones and 222 of
+// 128 x 256; 777 x 1001 x 1537, of which there are 169: 23 us against 15). Stages of 128 inner values there, whose
+// three parts LDS has no room for (64: 141 and 19 us).
 template <int PARTS>
 hipError_t many_rows(const ProductArgs& a, hipStream_t stream) {
     const int64_t cus = a.cu_count;
