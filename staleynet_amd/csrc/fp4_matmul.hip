@@ -8,8 +8,8 @@
 // 32 codes become matrix operands with 16 conversions, scale included; nothing is
 // multiplied per group.
 //
-// Few rows: a wave takes 16 C columns and a run of steps of 128 inner values (lane n, g:
-// block g of the step for column n); the workgroup's waves take consecutive runs, and add
+// Few rows: a wave takes 16 C columns and a run of steps of 128 or 256 inner values (lane n, g:
+// block g of the step for column n, or two); the workgroup's waves take consecutive runs, and add
 // their sums through LDS in wave order. The parts of all rows, 3 rows (bf16: 1) to each row
 // of x, are the rows of T operands of 16: at most 5 rows need one matrix instruction for
 // 512 weights, 10 two, 16 three. The wave splits a step's x once, four values a lane, and
@@ -17,12 +17,12 @@
 // columns of one part's sums. The codes and the x of the next step are on their way
 // while this one's are used.
 //   Scale bytes: a column's are 1 / 16 of its codes, and read byte by byte beside them they cost the
-// address units as much as the codes do (1 x 8192 x 28672: 39 us, 28 without any). So a
-// lane reads 16 of one column at once, for the next 16 / C steps, and the bytes
+// address units as much as the codes do (1 x 8192 x 28672: 39 us, 28 without any; 31.5 so). So a
+// lane reads 16 of one column at once, for the next steps, and the bytes
 // pass through LDS.
-//   What bounds it: W's bytes where there are many (1 x 8192 x 28672: 31.5 us, 125 MB at 4.0 TB/s), one
-// launch where there are few (1 x 768 x 2304: 3.8 us), and the parts' LDS reads and matrix instructions at 16
-// rows (16 x 4096 x 14336: 15.3 us for 31 MB).
+//   What bounds it: W's bytes where there are many (1 x 8192 x 28672: 29.3 us, 125 MB at 4.3 TB/s), one
+// launch where there are few (1 x 768 x 2304: 3.8 us), and at 16 rows (16 x 4096 x 14336: 15.3 us
+// for 31 MB) the vector units, busy half the cycles with the split of x, which every workgroup does again.
 // More rows: tiles staged in LDS, below.
 #include <hip/hip_runtime.h>
 
@@ -39,7 +39,7 @@ namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kStep = 128;        // inner values of a step: four blocks
+constexpr int kStep = 128;        // inner values the matrix instructions take at once: four blocks
 constexpr int kMaxWaves = 8;
 constexpr int kScaleBytes = 1024;  // 16 of each lane
 
@@ -113,13 +113,22 @@ __device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[P
     }
 }
 
+// Blocks of a column a lane takes in a step, as neighbours. Two make the four lanes of a column read 128 bytes of it,
+// a cache line, at once; with one, the line is read for the first half and, where the codes in flight do not
+// fit the caches, again for the other: 1 x 8192 x 28672 31.5 us, 29.3 with two (149 MB fetched for 125). With three
+// operands, or fewer columns and so fewer codes in flight, the registers and the longer steps cost
+// as much or more (16 x 4096 x 14336: 15.8 and 16.2 us; 1 x 4096 x 8192: 6.7 and 7.2).
+constexpr int blocks_of_lane(int c, int t) { return c == 4 && t == 1 ? 2 : 1; }
+
 // At most 2 PAIRS rows, which PARTS (3, or 1 for x rounded to bf16) make at most 16 T.
 template <int C, int T, int PAIRS, int PARTS, Quads Q>
 __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a) {
+    constexpr int J = blocks_of_lane(C, T);
+    constexpr int STEP_BLOCKS = 4 * J;
     // Scales and parts [wave][PARTS rows][kStep + 8], then the waves' sums [wave][C][T][16 parts][16 columns].
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int PART_ROW = 2 * (kStep + 8);
-    constexpr int SCALES = kScaleBytes;  // [step of the run][column][block]
+    constexpr int SCALES = kScaleBytes;  // [four blocks of the run][column][block]
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int waves = blockDim.x >> 6;
@@ -127,7 +136,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
     const uint32_t upper = upper_half_mask();
     const int64_t col0 = int64_t(blockIdx.x) * (16 * C);
     const int rows = int(a.rows);
-    const int32_t blocks = int32_t(a.blocks), steps = (blocks + 3) / 4;
+    const int32_t blocks = int32_t(a.blocks), steps = (blocks + STEP_BLOCKS - 1) / STEP_BLOCKS;
     // The wave's run of steps.
     const int32_t each = (steps + waves - 1) / waves;
     const int32_t begin = wave * each, end = min(begin + each, steps);
@@ -139,21 +148,24 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 #pragma unroll
     for (int c = 0; c < C; ++c) column[c] = uint32_t(min(16 * c + n, last_col)) * uint32_t(blocks);
     const uint8_t* const codes = a.codes + col0 * a.blocks * kBlockBytes;
-    auto load = [&](int32_t step, u32x4 (&w)[C]) __attribute__((always_inline)) {
-        const uint8_t* from = codes + int64_t(step) * (4 * kBlockBytes);
-        const uint32_t block = uint32_t(min(g, blocks - 1 - 4 * step));
+    auto load = [&](int32_t step, u32x4 (&w)[J][C]) __attribute__((always_inline)) {
+        const uint8_t* from = codes + int64_t(step) * (STEP_BLOCKS * kBlockBytes);
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            w[c] = *reinterpret_cast<const u32x4*>(from + (column[c] + block) * uint32_t(kBlockBytes));
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const uint32_t block = uint32_t(min(J * g + j, blocks - 1 - STEP_BLOCKS * step));
+                w[j][c] = *reinterpret_cast<const u32x4*>(from + (column[c] + block) * uint32_t(kBlockBytes));
+            }
     };
     // Scale bytes of RUN steps from `step` on: lane -> column lane % 16 C, 16 bytes of it. What
     // lies past the column's end is not used; past the buffer's, not read.
-    constexpr int RUN = 16 / C;
+    constexpr int RUN = 16 / (C * J);
     const int scale_col = lane % (16 * C), scale_part = lane / (16 * C);
     const int64_t scale_row = (col0 + min(scale_col, last_col)) * a.blocks + 16 * scale_part;
     auto load_scales = [&](int32_t step) __attribute__((always_inline)) {
         typedef u32x4 u32x4_bytes __attribute__((aligned(1)));
-        const int64_t at = scale_row + 4 * step, total = a.cols * a.blocks;
+        const int64_t at = scale_row + STEP_BLOCKS * step, total = a.cols * a.blocks;
         u32x4 s;
         if (at + 16 <= total) {
             s = *reinterpret_cast<const u32x4_bytes*>(a.scales + at);
@@ -174,12 +186,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 #pragma unroll
         for (int o = 0; o < T; ++o) acc[c][o] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // x of a step: four values of rows 2 pair + half, 32 lanes a row. Rows past the last are the
+    // x of every Jth block of a step: four values of rows 2 pair + half, 32 lanes a row. Rows past the last are the
     // last again, written to its place.
     f32x4 x[PAIRS];
     const int half = lane >> 5, quad = 4 * (lane & 31);
-    auto load_x = [&](int32_t step) __attribute__((always_inline)) {
-        const int64_t k = int64_t(step) * kStep + quad;
+    auto load_x = [&](int32_t step, int j) __attribute__((always_inline)) {
+        const int64_t k = int64_t(step) * (STEP_BLOCKS * kBlock) + J * (quad & ~31) + 32 * j + (quad & 31);
 #pragma unroll
         for (int pair = 0; pair < PAIRS; ++pair)
             x[pair] = load4<Q>(a.x + min(2 * pair + half, rows - 1) * a.inner, k, a.inner, true);
@@ -190,10 +202,10 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 #pragma unroll
     for (int o = 0; o < T; ++o) part_read[o] = min(16 * o + n, PARTS * rows - 1) * PART_ROW + g * (2 * kBlock);
 
-    u32x4 next[C], next_scales;
+    u32x4 next[J][C], next_scales;
     if (begin < end) {
         next_scales = load_scales(begin);
-        load_x(begin);
+        load_x(begin, 0);
         load(begin, next);
     }
     for (int32_t step = begin; step < end; ++step) {
@@ -204,40 +216,46 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
                 *reinterpret_cast<uint32_t*>(wave_lds + ((4 * scale_part + i) * (16 * C) + scale_col) * 4) = next_scales[i];
             if (step + RUN < end) next_scales = load_scales(step + RUN);
         }
-        wave_lds_order();
 #pragma unroll
-        for (int pair = 0; pair < PAIRS; ++pair) {
-            u32x2 split[PARTS];
-            split_four<PARTS>(x[pair], upper, split);
+        for (int j = 0; j < J; ++j) {
+            wave_lds_order();
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q)
-                *reinterpret_cast<u32x2*>(parts + (q * rows + min(2 * pair + half, rows - 1)) * PART_ROW + 2 * quad) =
-                    split[q];
-        }
-        wave_lds_order();
-        u32x4 now[C];
+            for (int pair = 0; pair < PAIRS; ++pair) {
+                u32x2 split[PARTS];
+                split_four<PARTS>(x[pair], upper, split);
 #pragma unroll
-        for (int c = 0; c < C; ++c) now[c] = next[c];
-        if (step + 1 < end) {
-            load_x(step + 1);  // first: the next step splits x while its codes may be on their way
-            load(step + 1, next);
-        }
-        float factor[C];
+                for (int q = 0; q < PARTS; ++q)
+                    *reinterpret_cast<u32x2*>(parts + (q * rows + min(2 * pair + half, rows - 1)) * PART_ROW + 2 * quad) =
+                        split[q];
+            }
+            wave_lds_order();
+            u32x4 now[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-            factor[c] = factor_of(uint8_t(
-                wave_lds[(in_run * (16 * C) + 16 * c + n) * 4 + min(g, blocks - 1 - 4 * step)]));
+            for (int c = 0; c < C; ++c) now[c] = next[j][c];
+            if (j + 1 < J) {
+                load_x(step, j + 1);
+            } else if (step + 1 < end) {
+                load_x(step + 1, 0);  // first: the next step splits x while its codes may be on their way
+                load(step + 1, next);
+            }
+            float factor[C];
+            const int32_t block = min(J * g + j, blocks - 1 - STEP_BLOCKS * step);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bf16x8 xf[T];
+            for (int c = 0; c < C; ++c)
+                factor[c] = factor_of(uint8_t(
+                    wave_lds[((J * in_run + block / 4) * (16 * C) + 16 * c + n) * 4 + block % 4]));
 #pragma unroll
-            for (int o = 0; o < T; ++o) xf[o] = *reinterpret_cast<const bf16x8*>(parts + part_read[o] + 16 * i);
+            for (int i = 0; i < 4; ++i) {
+                bf16x8 xf[T];
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const bf16x8 wf = fragment_of(now[c][i], factor[c]);
+                for (int o = 0; o < T; ++o) xf[o] = *reinterpret_cast<const bf16x8*>(parts + part_read[o] + 16 * i);
 #pragma unroll
-                for (int o = 0; o < T; ++o)
-                    acc[c][o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[o], acc[c][o], 0, 0, 0);
+                for (int c = 0; c < C; ++c) {
+                    const bf16x8 wf = fragment_of(now[c][i], factor[c]);
+#pragma unroll
+                    for (int o = 0; o < T; ++o)
+                        acc[c][o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[o], acc[c][o], 0, 0, 0);
+                }
             }
         }
     }
@@ -432,7 +450,9 @@ __global__ __launch_bounds__(256) void slice_sums_kernel(ProductArgs a, TileLaun
 }
 
 template <int C, int T, int PAIRS, int PARTS>
-hipError_t few_rows(const ProductArgs& a, int waves, hipStream_t stream) {
+hipError_t few_rows(const ProductArgs& a, hipStream_t stream) {
+    const int64_t steps = (a.blocks + 4 * blocks_of_lane(C, T) - 1) / (4 * blocks_of_lane(C, T));
+    const int waves = int(std::min<int64_t>(kMaxWaves, steps));
     const dim3 grid(unsigned((a.cols + 16 * C - 1) / (16 * C)));
     const size_t lds =
         waves * std::max<size_t>(C * T * 256 * sizeof(float), kScaleBytes + PARTS * a.rows * 2 * (kStep + 8));
@@ -509,11 +529,10 @@ hipError_t many_rows(const ProductArgs& a, hipStream_t stream) {
 //   12288 columns:  9.0,  9.3,  9.2        27.3, 20.5, 15.3
 template <int T, int PAIRS, int PARTS>
 hipError_t few_rows_by_columns(const ProductArgs& a, hipStream_t stream) {
-    const int waves = int(std::max<int64_t>(1, std::min<int64_t>(kMaxWaves, (a.blocks + 3) / 4)));
     const int64_t tiles = (a.cols + 15) / 16;
-    if (tiles >= 3 * a.cu_count) return few_rows<4, T, PAIRS, PARTS>(a, waves, stream);
-    if (4 * tiles >= 5 * a.cu_count) return few_rows<2, T, PAIRS, PARTS>(a, waves, stream);
-    return few_rows<1, T, PAIRS, PARTS>(a, waves, stream);
+    if (tiles >= 3 * a.cu_count) return few_rows<4, T, PAIRS, PARTS>(a, stream);
+    if (4 * tiles >= 5 * a.cu_count) return few_rows<2, T, PAIRS, PARTS>(a, stream);
+    return few_rows<1, T, PAIRS, PARTS>(a, stream);
 }
 
 }  // namespace

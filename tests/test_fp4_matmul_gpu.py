@@ -88,6 +88,18 @@ def test_long_and_wide(gpu, rows, inner, cols):
     assert error < MatmulKernel.MfmaF32.tolerance()
 
 
+@pytest.mark.parametrize("cols", [5201, 12301])
+@pytest.mark.parametrize("inner", [4, 33, 300, 1100])
+@pytest.mark.parametrize("rows,bf16", [(1, False), (2, True), (5, False), (7, True), (9, False), (16, False)])
+def test_few_rows_of_wide_weights(gpu, rows, bf16, inner, cols):
+    """Two and four column tiles a wave, the last ones partial; blocks that end inside a step."""
+    rng = np.random.default_rng(inner)
+    codes, scales, w = weights(cols, inner, inner)
+    x = rng.standard_normal((rows, inner)).astype(np.float32)
+    spec = MatmulSpec.new(rows, cols, inner).with_precision(Precision.Bf16 if bf16 else Precision.F32)
+    check(run(gpu, spec, x, codes, scales, offset=rows % 2), to_bf16(x) if bf16 else x, w, inner)
+
+
 @pytest.mark.parametrize("rows,inner,cols,bf16", [
     (2000, 203, 3900, False),   # tiles of 128 x 256, quads shifted at the rows' ends
     (1990, 64, 4001, False),    # the same, one stage
