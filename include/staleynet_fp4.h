@@ -32,8 +32,9 @@
  *
  * Buffers are bytes in device memory (sn_alloc_bytes, sn_upload_bytes, or any
  * other). Code buffers are 16-byte aligned (SN_ERR_UNSUPPORTED otherwise).
- * Every call is asynchronous on the context's stream, allocates nothing and
- * may be captured into a graph.
+ * The calls on them are asynchronous on the context's stream, allocate nothing
+ * and may be captured into a graph; those that make, copy and free them are as
+ * their fp32 forms.
  */
 #ifndef STALEYNET_FP4_H
 #define STALEYNET_FP4_H

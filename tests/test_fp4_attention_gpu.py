@@ -115,7 +115,7 @@ def test_chunk(gpu, head_dim, heads, kv_heads, queries):
 
 
 def test_many_rows(gpu):
-    """Enough rows that each wave takes rows of its own."""
+    """More tiles of 16 rows than the CUs take at once (four waves each)."""
     case = Case(2, 24, 6, 333, 400, 64, [333, 390], seed=4)
     case.check(case.run(gpu))
 
@@ -153,6 +153,19 @@ def test_many_sequences(gpu, batch, longest, head_dim):
     lengths[[0, 63, 64, batch - 1]] = [longest, 0, longest, longest - 1]
     case = Case(batch, 2, 1, 1, longest, head_dim, lengths, seed=batch)
     case.check(case.run(gpu))
+
+
+@pytest.mark.parametrize("head_dim", [32, 64, 128])
+@pytest.mark.parametrize("queries,length", [(1, 900), (40, 200)])
+def test_a_cache_inside_larger_buffers(gpu, head_dim, queries, length):
+    """Codes at any multiple of 16 bytes, scales at any byte."""
+    case = Case(2, 6, 2, queries, length + 5, head_dim, [length, length // 2], seed=head_dim)
+    buffers = []
+    for codes, scales in zip(case.codes, case.scales):
+        for a, ahead in ((codes, 48), (scales, 3)):
+            whole = gpu.upload_bytes(np.concatenate([np.full(ahead, 255, np.uint8), a.ravel()]))
+            buffers.append(View(whole, ahead, a.size, 1))
+    case.check(case.run(gpu, cache=Fp4Cache(2, 2, length + 5, head_dim, *buffers)))
 
 
 def test_one_length_for_all(gpu):

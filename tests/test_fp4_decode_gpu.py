@@ -147,3 +147,39 @@ def test_a_captured_step_replays(gpu):
     finally:
         gpu.synchronize()
         graph.close()
+
+
+def test_two_graphs_on_one_context(gpu):
+    """A sliced product and a decode step whose keys workgroups share both keep partial sums in the context's
+    workspace: captured apart and replayed in turn, each replay leaves the eager bits."""
+    rng = np.random.default_rng(8)
+    rows, inner, cols, n = 40, 4096, 320, 3000
+    w = gpu.fp4_matrix(cols, inner)
+    gpu.quantize_fp4(gpu.upload(Shape(inner, cols), rng.standard_normal((inner, cols))), w)
+    x, y = gpu.upload(Shape(rows, inner), rng.standard_normal((rows, inner))), gpu.zeros(Shape(rows, cols))
+    cache = gpu.fp4_cache(2, 2, n, 64)
+    packed = gpu.upload(Shape(2 * n, 256), rng.standard_normal((2 * n, 256)))
+    gpu.fp4_cache_append(cache, packed, n, 256, 0, 128)
+    q, out = gpu.upload(Shape(8, 64), rng.standard_normal((8, 64))), gpu.zeros(Shape(8, 64))
+    lengths = gpu.upload_tokens([n, n // 2])
+    calls = (lambda: gpu.matmul_fp4(MatmulSpec.new(rows, cols, inner).right_transposed(), x, w, y),
+             lambda: gpu.fp4_attention(cache, q, out, 4, 1, 0.125, lengths=lengths))
+    eager = []
+    for call, result in zip(calls, (y, out)):
+        call()
+        eager.append(gpu.download(result))
+    assert all(np.isfinite(e).all() and e.any() for e in eager)
+    graphs = [HipGraph(gpu.stream, call) for call in calls]
+    try:
+        for _ in range(3):
+            for buffer in (y, out):
+                gpu.fill_zero(buffer)
+            for graph in graphs:
+                graph.launch()
+            for result, expected in zip((y, out), eager):
+                assert np.array_equal(gpu.download(result), expected)
+            gpu.matmul(MatmulSpec.new(64, 64, 2), q, q, gpu.zeros(Shape(64, 64)))
+    finally:
+        gpu.synchronize()
+        for graph in graphs:
+            graph.close()

@@ -116,6 +116,21 @@ def test_tiles(gpu, rows, inner, cols, bf16):
     check(run(gpu, spec, x, codes, scales, bias=bias, offset=1), to_bf16(x) if bf16 else x, w, inner, bias=bias)
 
 
+@pytest.mark.parametrize("rows", [1, 9, 40])
+@pytest.mark.parametrize("offset", [1, 2, 7])
+def test_scales_at_any_byte(gpu, rows, offset):
+    """Scale bytes need no alignment, and none past the last is read: what surrounds them is NaN's."""
+    rng = np.random.default_rng(offset)
+    inner, cols = 700, 65
+    codes, scales, w = weights(cols, inner, offset)
+    x = rng.standard_normal((rows, inner)).astype(np.float32)
+    around = gpu.upload_bytes(np.concatenate([np.full(offset, 255, np.uint8), scales.ravel(), np.full(40, 255, np.uint8)]))
+    matrix = Fp4Matrix(cols, inner, gpu.upload_bytes(codes), View(around, offset, scales.size, 1))
+    out = gpu.zeros(Shape.new(rows, cols))
+    gpu.matmul_fp4(MatmulSpec.new(rows, cols, inner).right_transposed(), gpu.upload(Shape.new(rows, inner), x), matrix, out)
+    check(gpu.download(out).reshape(rows, cols), x, w, inner)
+
+
 @pytest.mark.parametrize("rows", [1, 5, 9, 40, 100])
 @pytest.mark.parametrize("with_bias", [False, True])
 def test_scale_accumulate_and_bias(gpu, rows, with_bias):
