@@ -28,7 +28,7 @@
  * Limits, past which a call is SN_ERR_OVERFLOW: columns and inner length of a
  * matrix to quantize under 2^31; of a product, columns under 2^28 and inner
  * length under 2^25; a cache's batch * kv_heads under 2^21 and its capacity
- * under 2^30; batch * heads * queries of an attention call under 2^28.
+ * under 2^30; batch * heads * queries of an attention call under 2^27.
  *
  * Buffers are bytes in device memory (sn_alloc_bytes, sn_upload_bytes, or any
  * other). Code buffers are 16-byte aligned (SN_ERR_UNSUPPORTED otherwise).

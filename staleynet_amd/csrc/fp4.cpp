@@ -30,8 +30,10 @@ constexpr size_t kLimit = size_t(1) << 60;
 constexpr size_t kMaxDimension = size_t(1) << 31;
 constexpr size_t kMaxCols = size_t(1) << 28;       // of a product: 2^32 threads a launch
 constexpr size_t kMaxInner = size_t(1) << 25;      // of a product: its kernels count blocks in 32 bits
-constexpr size_t kMaxRows = size_t(1) << 28;        // query rows of an attention call
-constexpr size_t kMaxHeads = size_t(1) << 21;       // of a cache, over its sequences: 2^32 threads a launch
+// Query rows of an attention call and heads of a cache, over their sequences: at most 2^23 + 2^21 tiles of
+// 16 rows, of 256 threads each, where a launch holds 2^32.
+constexpr size_t kMaxRows = size_t(1) << 27;
+constexpr size_t kMaxHeads = size_t(1) << 21;
 constexpr size_t kMaxPositions = size_t(1) << 30;  // of a cache: attention counts them in 32 bits
 
 int status(hipError_t err) { return err == hipSuccess ? SN_OK : int(err); }

@@ -111,7 +111,7 @@ struct Rows {
 __device__ __forceinline__ Rows rows_of(const KernelArgs& p, int64_t b, int64_t kv_head, int32_t tile, int32_t length,
                                         int n) {
     Rows r;
-    const uint32_t group = uint32_t(p.group), rows = uint32_t(p.a.queries) * group;  // under 2^31
+    const uint32_t group = uint32_t(p.group), rows = uint32_t(p.a.queries) * group;  // under 2^27
     const uint32_t first = uint32_t(tile) * kRows, row = first + n;
     r.b = b;
     r.kv_head = kv_head;
@@ -600,7 +600,6 @@ hipError_t launch(const AttentionArgs& a, KernelArgs p, hipStream_t stream) {
         p.workgroups = int32_t(wanted);
         grid = std::min(wanted + tiles, tiles * ((longest + p.least_keys - 1) / p.least_keys));
     }
-    if (grid > INT32_MAX) return hipErrorInvalidValue;
     // Tiles that fill the CUs by themselves need no eight waves each: of 3000 keys with h = 128, 400 tiles
     // take 45.4 us of eight waves and 41.2 of four, 1600 tiles 147 and 125. (Fewer tiles are
     // shared where the workspace allows it, else each has what one workgroup can give; 48 of 300 keys: 6.8

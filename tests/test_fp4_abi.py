@@ -145,8 +145,8 @@ def test_limits():
         assert call(cache=dict(batch=1 << 20, kv_heads=2)) == over
         assert call(cache=dict(capacity=1 << 30)) == over
         assert call(cache=dict(capacity=(1 << 30) - 1)) == gemm.SN_ERR_NULL_ARGUMENT  # the context
-    assert attention(queries=1 << 25) == over  # 2 * 6 heads
-    assert attention(queries=1 << 24) == gemm.SN_ERR_LENGTH_MISMATCH
+    assert attention(queries=1 << 24) == over  # 2 * 6 heads
+    assert attention(queries=1 << 23) == gemm.SN_ERR_LENGTH_MISMATCH
 
 
 def test_the_reference_form_on_known_blocks():
