@@ -85,7 +85,7 @@ int sn_dequantize_fp4(sn_context *context, size_t cols, size_t inner, uint32_t s
  * fp32. Infinities and NaN follow IEEE arithmetic. Deterministic; a row's bits
  * do not depend on the values of the other rows. Lengths and codes as
  * sn_matmul_bias; codes or scales too short is SN_ERR_RIGHT_TOO_SMALL. Products
- * of more than 16 rows whose output is too small to fill the GPU slice the inner
+ * of more than 16 rows (32 rounded to bf16) whose output is too small to fill the GPU slice the inner
  * dimension, with partial sums in the context's workspace (so calls on one
  * context must not overlap); with a smaller workspace they slice less, or not. */
 int sn_matmul_fp4(sn_context *context, const sn_matmul_spec *spec, const float *left, size_t left_len,

@@ -12,7 +12,7 @@
 // block g of the step for column n, or two); the workgroup's waves take consecutive runs, and add
 // their sums through LDS in wave order. The parts of all rows, 3 rows (bf16: 1) to each row
 // of x, are the rows of T operands of 16: at most 5 rows need one matrix instruction for
-// 512 weights, 10 two, 16 three. The wave splits a step's x once, four values a lane, and
+// 512 weights, 10 two, 16 three (bf16: 16 one, 32 two). The wave splits a step's x once, four values a lane, and
 // passes the parts through LDS of its own. D = W x^T: a lane holds four consecutive
 // columns of one part's sums. The codes and the x of the next step are on their way
 // while this one's are used.
@@ -539,10 +539,14 @@ hipError_t few_rows_by_columns(const ProductArgs& a, hipStream_t stream) {
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
     if (a.rows == 0 || a.cols == 0) return hipSuccess;
-    if (a.rows <= 16 && a.inner >= 4) {
+    if (a.rows <= (a.bf16 ? 32 : 16) && a.inner >= 4) {
         // As few operands and loads of x as hold the rows (4096 x 8192: 2 rows 6.7 us, as 16 would be 11.3; one
-        // rounded to bf16 6.1, and 7.4).
-        if (a.bf16) return a.rows <= 2 ? few_rows_by_columns<1, 1, 1>(a, stream) : few_rows_by_columns<1, 8, 1>(a, stream);
+        // rounded to bf16 6.1, and 7.4). 24 rows in bf16: 9.8 us at 4096 x 4096 and 14.8 at 4096 x 14336, where tiles take
+        // 15.9 and 19.3; in fp32 they would be five operands or six, 18.6 and 47.7, tiles 17.4 and 25.1.
+        if (a.bf16)
+            return a.rows <= 2    ? few_rows_by_columns<1, 1, 1>(a, stream)
+                   : a.rows <= 16 ? few_rows_by_columns<1, 8, 1>(a, stream)
+                                  : few_rows_by_columns<2, 16, 1>(a, stream);
         return a.rows <= 2    ? few_rows_by_columns<1, 1, 3>(a, stream)
                : a.rows <= 5  ? few_rows_by_columns<1, 3, 3>(a, stream)
                : a.rows <= 10 ? few_rows_by_columns<2, 5, 3>(a, stream)

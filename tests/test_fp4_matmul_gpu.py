@@ -88,11 +88,12 @@ def test_long_and_wide(gpu, rows, inner, cols):
     assert error < MatmulKernel.MfmaF32.tolerance()
 
 
-@pytest.mark.parametrize("cols", [5201, 12301])
+@pytest.mark.parametrize("cols", [50, 5201, 12301])
 @pytest.mark.parametrize("inner", [4, 33, 300, 1100])
-@pytest.mark.parametrize("rows,bf16", [(1, False), (2, True), (5, False), (7, True), (9, False), (16, False)])
+@pytest.mark.parametrize("rows,bf16", [(1, False), (2, True), (5, False), (7, True), (9, False), (16, False), (17, True),
+                                       (25, True), (32, True)])
 def test_few_rows_of_wide_weights(gpu, rows, bf16, inner, cols):
-    """Two and four column tiles a wave, the last ones partial; blocks that end inside a step."""
+    """One, two and four column tiles a wave, the last ones partial; blocks that end inside a step."""
     rng = np.random.default_rng(inner)
     codes, scales, w = weights(cols, inner, inner)
     x = rng.standard_normal((rows, inner)).astype(np.float32)
