@@ -284,10 +284,11 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 // staged in LDS, 64 inner values at a time, in two stages: while the matrix cores work
 // on one, the next is split and written, and the one after is on its way in registers. A
 // lane's 16 bytes of codes are a block of one column: 64 inner values of 32 columns a
-// load. D = x W: a lane holds one column. 2048 x 4096 x 4096 with fp32 inputs: 181 us, 380 TFLOP/s of products
-// (1140 of bf16 ones, matrix cores busy half the cycles; 130 us without any load, 150 without x's, and 175 to 177 with
-// the next stage's split spread between the matrix instructions, which costs one part a tenth). Inner value 8 i + j of half h of a stage is
+// load. D = x W: a lane holds one column. Inner value 8 i + j of half h of a stage is
 // element j of operand i of lanes h (as the block's words hold the codes).
+//   2048 x 4096 x 4096 with fp32 inputs: 181 us, 380 TFLOP/s of products (1140 of bf16 ones, matrix cores busy half the
+// cycles; 130 us without any load, 150 without x's, and 175 to 177 with the next stage's split spread between the
+// matrix instructions, which costs one part a tenth).
 template <int RT, int CT, int WR, int WC, int PARTS, int SUBS>
 struct TileShape {
     static constexpr int THREADS = 64 * WR * WC;
