@@ -79,7 +79,8 @@ int sn_dequantize_fp4(sn_context *context, size_t cols, size_t inner, uint32_t s
  * it. The spec is sn_matmul's: left_storage SN_ROW_MAJOR, right_storage
  * SN_TRANSPOSED (each column's values are contiguous), batch_count 1, no mask
  * (SN_ERR_UNSUPPORTED otherwise). The left operand's fp32 values are used in
- * full, as the exact sum of three bf16 values (SN_PRECISION_F32, and the
+ * full, subnormals too, as the exact sum of three bf16 values and of what those leave of
+ * values under 2^-110 (SN_PRECISION_F32, and the
  * default with every context kernel but SN_KERNEL_MFMA_BF16), or rounded to
  * bf16 (SN_PRECISION_BF16, or that kernel); products are exact and summed in
  * fp32. Infinities and NaN follow IEEE arithmetic. Deterministic; a row's bits

@@ -48,9 +48,9 @@ __device__ __forceinline__ bf16x8 fragment_of(uint32_t word, float factor) {
 
 // An fp32 value as the exact sum of three bf16 values of its sign, each the
 // leading 8 significant bits of what is left (cut off, not rounded: the largest
-// float stays finite, and 24 = 8 + 8 + 8). Exact from 2^-110 on; below, what is
-// lost is under 2^-133. An infinity or NaN leaves NaN in the
-// rest, which one comparison a pair finds; then it is its own first part
+// float stays finite, and 24 = 8 + 8 + 8). Exact from 2^-110 on; below, rest_of has
+// what they leave. An infinity or NaN leaves NaN after the first part, which one
+// comparison a pair finds; then it is its own first part
 // and the others are 0, so that products follow IEEE arithmetic.
 __device__ __forceinline__ uint32_t upper_halves(float x0, float x1) {
     return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x1), __builtin_bit_cast(uint32_t, x0), 0x07060302u);
@@ -61,6 +61,25 @@ __device__ __forceinline__ float cut(float x, uint32_t upper) {
 __device__ __forceinline__ float quiet(float x) {  // a NaN whose upper half is one
     return x != x ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) | 0x00400000u) : x;
 }
+// What the three parts leave of a value, times 2^100: 0 but for magnitudes under 2^-110, whose bits under 2^-133
+// (bf16's smallest subnormal, at which the last cut ends) the third part cannot hold. There are at most 16 of
+// them, down to 2^-149, so that two parts hold them once they are lifted. notice() gathers, from the value
+// the third part is cut from, whether there are any: those bits are the lower half of its word, and 0 in every
+// other value, which has at most 8 bits left there.
+constexpr float kRestLift = 0x1p100f;
+__device__ __forceinline__ float rest_of(float x, uint32_t upper) {
+#pragma clang fp contract(off)
+    const float x1 = x - cut(x, upper);
+    const float a1 = x1 != x1 ? 0.f : x1;
+    const float a2 = a1 - cut(a1, upper);
+    return (a2 - cut(a2, upper)) * kRestLift;
+}
+__device__ __forceinline__ void notice(uint32_t& left, float third0, float third1) {
+    left |= __builtin_bit_cast(uint32_t, third0) | __builtin_bit_cast(uint32_t, third1);
+    asm("" : "+v"(left));  // one running value: values gathered first would take registers
+}
+__device__ __forceinline__ bool noticed(uint32_t left) { return (left & 0xffffu) != 0; }
+
 __device__ __forceinline__ SplitVector split_vector_of(const u32x4 (&w)[kParts]) {
     SplitVector out;
 #pragma unroll

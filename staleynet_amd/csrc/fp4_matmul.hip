@@ -6,7 +6,9 @@
 // bf16 products, each exact, summed in fp32 by the matrix cores: where fp32 times
 // fp32 takes six (gemm_f32.h). A 16-byte load is one block of one column, and its
 // 32 codes become matrix operands with 16 conversions, scale included; nothing is
-// multiplied per group.
+// multiplied per group. A workgroup whose x holds values under 2^-110, of which three parts may leave
+// something, goes over its share a second time with that and adds the sums to its output. (Where none does, to look
+// for them costs one OR a value: 1 x 8192 x 28672 29.6 us and 29.2 without, others under 1 %.)
 //
 // Few rows: a wave takes 16 C columns and a run of steps of 128 or 256 inner values (lane n, g:
 // block g of the step for column n, or two); the workgroup's waves take consecutive runs, and add
@@ -20,7 +22,7 @@
 // address units as much as the codes do (1 x 8192 x 28672: 39 us, 28 without any; 31.5 so). So a
 // lane reads 16 of one column at once, for the next steps, and the bytes
 // pass through LDS.
-//   What bounds it: W's bytes where there are many (1 x 8192 x 28672: 29.3 us, 125 MB at 4.3 TB/s), one
+//   What bounds it: W's bytes where there are many (1 x 8192 x 28672: 29.6 us, 125 MB at 4.2 TB/s), one
 // launch where there are few (1 x 768 x 2304: 3.8 us), and at 16 rows (16 x 4096 x 14336: 15.3 us
 // for 31 MB) the vector units, busy half the cycles with the split of x, which every workgroup does again.
 // More rows: tiles staged in LDS, below.
@@ -50,6 +52,11 @@ __device__ __forceinline__ void store_output(const ProductArgs& a, int64_t row, 
     if (a.accumulate) out = *y + out;
     if (a.bias != nullptr) out = out + a.bias[col];
     *y = out;
+}
+// A sum of what the parts of x left, to the output that theirs went to. A sum of 0 changes no bit.
+__device__ __forceinline__ void add_rest(const ProductArgs& a, int64_t row, int64_t col, float sum) {
+#pragma clang fp contract(off)
+    if (sum != 0.f) a.y[row * a.cols + col] = a.y[row * a.cols + col] + a.scale * (sum * (1.f / kRestLift));
 }
 
 // How rows of x are read, four values from k (a multiple of 4) on, zeros where `ok` is not
@@ -84,12 +91,21 @@ __device__ __forceinline__ f32x4 load4(const float* row, int64_t k, int64_t inne
 }
 Quads quads_of(int64_t inner) { return inner < 4 ? Quads::kSingle : inner % 4 == 0 ? Quads::kWhole : Quads::kShifted; }
 
-// Four values as PARTS parts, packed in pairs (split_exact has the arithmetic).
-template <int PARTS>
-__device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[PARTS]) {
+// Four values as PARTS parts, packed in pairs (split_exact has the arithmetic), `left` noticing what three parts leave;
+// or, where REST is set, that, lifted.
+template <int PARTS, bool REST>
+__device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[PARTS], uint32_t& left) {
 #pragma clang fp contract(off)
     if constexpr (PARTS == 1) {
         w[0] = u32x2{pack2_bf16(x[0], x[1]), pack2_bf16(x[2], x[3])};
+    } else if constexpr (REST) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float a = rest_of(x[2 * i], upper), b = rest_of(x[2 * i + 1], upper);
+            w[0][i] = upper_halves(a, b);
+            w[1][i] = upper_halves(a - cut(a, upper), b - cut(b, upper));
+            w[2][i] = 0;
+        }
     } else {
         float a[4], a1[4];
 #pragma unroll
@@ -108,7 +124,9 @@ __device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[P
         for (int i = 0; i < 2; ++i) {
             w[0][i] = upper_halves(a[2 * i], a[2 * i + 1]);
             w[1][i] = upper_halves(a1[2 * i], a1[2 * i + 1]);
-            w[2][i] = upper_halves(a1[2 * i] - cut(a1[2 * i], upper), a1[2 * i + 1] - cut(a1[2 * i + 1], upper));
+            const float a2 = a1[2 * i] - cut(a1[2 * i], upper), b2 = a1[2 * i + 1] - cut(a1[2 * i + 1], upper);
+            notice(left, a2, b2);
+            w[2][i] = upper_halves(a2, b2);
         }
     }
 }
@@ -120,17 +138,17 @@ __device__ __forceinline__ void split_four(f32x4 x, uint32_t upper, u32x2 (&w)[P
 // as much or more (16 x 4096 x 14336: 15.8 and 16.2 us; 1 x 4096 x 8192: 6.7 and 7.2).
 constexpr int blocks_of_lane(int c, int t) { return c == 4 && t == 1 ? 2 : 1; }
 
-// At most 2 PAIRS rows, which PARTS (3, or 1 for x rounded to bf16) make at most 16 T.
-template <int C, int T, int PAIRS, int PARTS, Quads Q>
-__global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a) {
+// The columns' sums over the parts of x, to the output; or, where REST is set, over what those leave, added to it.
+// At most 2 PAIRS rows, which PARTS (3, or 1 for x rounded to bf16) make at most 16 T. Returns whether the parts leave
+// something in the workgroup.
+template <int C, int T, int PAIRS, int PARTS, Quads Q, bool REST>
+__device__ __forceinline__ bool few_rows_pass(const ProductArgs& a, char* lds, uint64_t& waves_left, int tid) {
     constexpr int J = blocks_of_lane(C, T);
     constexpr int STEP_BLOCKS = 4 * J;
-    // Scales and parts [wave][PARTS rows][kStep + 8], then the waves' sums [wave][C][T][16 parts][16 columns].
-    extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int PART_ROW = 2 * (kStep + 8);
     constexpr int SCALES = kScaleBytes;  // [four blocks of the run][column][block]
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int waves = blockDim.x >> 6;
     const int n = lane & 15, g = lane >> 4;
     const uint32_t upper = upper_half_mask();
@@ -180,12 +198,6 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
         return s;
     };
 
-    f32x4 acc[C][T];
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int o = 0; o < T; ++o) acc[c][o] = f32x4{0.f, 0.f, 0.f, 0.f};
-
     // x of every Jth block of a step: four values of rows 2 pair + half, 32 lanes a row. Rows past the last are the
     // last again, written to its place.
     f32x4 x[PAIRS];
@@ -202,6 +214,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 #pragma unroll
     for (int o = 0; o < T; ++o) part_read[o] = min(16 * o + n, PARTS * rows - 1) * PART_ROW + g * (2 * kBlock);
 
+    f32x4 acc[C][T];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int o = 0; o < T; ++o) acc[c][o] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint32_t left = 0;
     u32x4 next[J][C], next_scales;
     if (begin < end) {
         next_scales = load_scales(begin);
@@ -222,7 +240,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 #pragma unroll
             for (int pair = 0; pair < PAIRS; ++pair) {
                 u32x2 split[PARTS];
-                split_four<PARTS>(x[pair], upper, split);
+                split_four<PARTS, REST>(x[pair], upper, split, left);
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q)
                     *reinterpret_cast<u32x2*>(parts + (q * rows + min(2 * pair + half, rows - 1)) * PART_ROW + 2 * quad) =
@@ -267,8 +285,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 #pragma unroll
         for (int o = 0; o < T; ++o)
             *reinterpret_cast<f32x4*>(&sums[wave * WAVE_SUMS + (c * T + o) * 256 + n * 16 + 4 * g]) = acc[c][o];
+    constexpr bool NOTICES = PARTS == 3 && !REST;
+    if (NOTICES) {
+        const bool any = __any(noticed(left));
+        if (lane == 0) reinterpret_cast<uint8_t*>(&waves_left)[wave] = any;
+    }
     __syncthreads();
-    for (int e = threadIdx.x; e < rows * 16 * C; e += blockDim.x) {
+    const uint64_t any_left = NOTICES ? waves_left & (~uint64_t(0) >> (64 - 8 * waves)) : 0;
+    for (int e = tid; e < rows * 16 * C; e += blockDim.x) {
         const int row = e / (16 * C), c = e / 16 % C;
         const int64_t col = col0 + e % (16 * C);
         if (col >= a.cols) continue;
@@ -276,7 +300,27 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
         float sum = 0.f;
         for (int w = 0; w < waves; ++w, from += WAVE_SUMS)
             sum += PARTS == 1 ? from[0] : from[0] + (from[16 * rows] + from[32 * rows]);
-        store_output(a, row, col, sum);
+        if constexpr (REST)
+            add_rest(a, row, col, sum);
+        else
+            store_output(a, row, col, sum);
+    }
+    return any_left != 0;
+}
+
+template <int C, int T, int PAIRS, int PARTS, Quads Q>
+__global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a) {
+    // Scales and parts [wave][PARTS rows][kStep + 8], then the waves' sums [wave][C][T][16 parts][16 columns].
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ uint64_t waves_left;  // a byte a wave: whether the parts of its x leave something
+    static_assert(kMaxWaves == 8, "a byte a wave");
+    int tid = threadIdx.x;
+    const bool any = few_rows_pass<C, T, PAIRS, PARTS, Q, false>(a, lds, waves_left, tid);
+    if constexpr (PARTS == 3) {
+        if (!any) return;     // of the workgroup
+        __syncthreads();      // the parts take the sums' place
+        asm("" : "+v"(tid));  // addresses worked out again, not kept in registers through the first pass
+        few_rows_pass<C, T, PAIRS, PARTS, Q, true>(a, lds, waves_left, tid);
     }
 }
 
@@ -307,11 +351,12 @@ struct TileLaunch {
     float* sums;
 };
 
-template <int RT, int CT, int WR, int WC, int PARTS, int SUBS, Quads Q>
-__global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileLaunch launch) {
+// As few_rows_pass.
+template <int RT, int CT, int WR, int WC, int PARTS, int SUBS, Quads Q, bool REST>
+__device__ __forceinline__ void tile_pass(const ProductArgs& a, const TileLaunch& launch, char* stages,
+                                          uint32_t* waves_left, int tid) {
     using S = TileShape<RT, CT, WR, WC, PARTS, SUBS>;
-    __shared__ __attribute__((aligned(16))) char stages[2 * S::STAGE];
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
     const uint32_t upper = upper_half_mask();
@@ -337,11 +382,12 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
             x[u] = load4<Q>(a.x + (row < a.rows ? row : 0) * a.inner, k, a.inner, row < a.rows);
         }
     };
+    uint32_t left = 0;
     auto store_x = [&](char* stage) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < S::QUADS; ++u) {
             u32x2 w[PARTS];
-            split_four<PARTS>(x[u], upper, w);
+            split_four<PARTS, REST>(x[u], upper, w, left);
 #pragma unroll
             for (int q = 0; q < PARTS; ++q)
                 *reinterpret_cast<u32x2*>(stage + q * S::PART + (first_row + u * APART) * S::ROW + 2 * quad) = w[q];
@@ -422,6 +468,10 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
         }
         __syncthreads();
     }
+    if (PARTS == 3 && !REST) {
+        const bool any = __any(noticed(left));
+        if (lane == 0) waves_left[wave] = any;
+    }
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         const int64_t col = wave_col + 32 * c + n;
@@ -432,11 +482,33 @@ __global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileL
             for (int e = 0; e < 16; ++e) {
                 const int64_t row = row0 + wave_row + 32 * r + 8 * (e / 4) + 4 * h + e % 4;
                 if (row >= a.rows) continue;
-                if (launch.slices > 1)
-                    launch.sums[(slice * a.rows + row) * a.cols + col] = acc[r][c][e];
+                float* const sum = &launch.sums[(slice * a.rows + row) * a.cols + col];
+                if (REST && launch.slices > 1)
+                    *sum = *sum + acc[r][c][e] * (1.f / kRestLift);
+                else if (REST)
+                    add_rest(a, row, col, acc[r][c][e]);
+                else if (launch.slices > 1)
+                    *sum = acc[r][c][e];
                 else
                     store_output(a, row, col, acc[r][c][e]);
             }
+    }
+}
+
+template <int RT, int CT, int WR, int WC, int PARTS, int SUBS, Quads Q>
+__global__ __launch_bounds__(64 * WR * WC) void tile_kernel(ProductArgs a, TileLaunch launch) {
+    __shared__ __attribute__((aligned(16))) char stages[2 * TileShape<RT, CT, WR, WC, PARTS, SUBS>::STAGE];
+    __shared__ uint32_t waves_left[WR * WC];
+    int tid = threadIdx.x;
+    tile_pass<RT, CT, WR, WC, PARTS, SUBS, Q, false>(a, launch, stages, waves_left, tid);
+    if constexpr (PARTS == 3) {
+        __syncthreads();
+        uint32_t any = 0;
+#pragma unroll
+        for (int w = 0; w < WR * WC; ++w) any |= waves_left[w];
+        if (any == 0) return;
+        asm("" : "+v"(tid));
+        tile_pass<RT, CT, WR, WC, PARTS, SUBS, Q, true>(a, launch, stages, waves_left, tid);
     }
 }
 
