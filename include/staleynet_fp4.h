@@ -164,7 +164,8 @@ typedef struct sn_fp4_attention_shape {
  * query that sees no position (a sequence of length 0; padding ahead of a
  * shorter prompt) gives zeros; one whose scores are all -inf gives NaN. Positions a query does not see do not enter its
  * result, whatever they hold (also NaN blocks). fp32 arithmetic as in
- * sn_matmul_fp4. lengths over the capacity count as the capacity; `keys` over
+ * sn_matmul_fp4: q times scale log2 e is rounded to fp32, and that is used in full, subnormals
+ * too. lengths over the capacity count as the capacity; `keys` over
  * it is SN_ERR_SHAPE. Buffers too short for the strides are SN_ERR_LENGTH_MISMATCH; out
  * overlapping q or the cache, and out strides by which two outputs share memory,
  * are SN_ERR_ALIASING. Long caches are split over workgroups whose partial

@@ -8,7 +8,8 @@
 //  * S^T = K q^T: keys are the rows of the matrix instruction's result, queries its
 //    columns, so lane (n, g) holds for query n the scores of keys 4 g .. + 3 of each
 //    16. K's codes are converted from the loaded words as they are (lane (n, g):
-//    quarter g of key n); q is split exactly in three bf16 parts (fp4_device.h).
+//    quarter g of key n); q is split exactly in three bf16 parts (fp4_device.h; what they leave of
+//    values under 2^-110 is a product more, by workgroups that have such values).
 //  * The softmax is per lane but for the maximum over the four lanes of a query.
 //  * O^T += V^T P^T: a lane's eight probabilities, split, are the right operand as
 //    they are, the operand's inner index being keys 4 g .. + 3 of the first 16 and
@@ -126,15 +127,28 @@ __device__ __forceinline__ Rows rows_of(const KernelArgs& p, int64_t b, int64_t 
     return r;
 }
 
-// Fragment i of this lane's query, split: head dims g H / 4 + 8 i .. + 7, as K's words hold them.
+// Fragment i of this lane's query, split: head dims g H / 4 + 8 i .. + 7, as K's words hold them. `left` notices what the
+// parts leave of them; query_rest has that, lifted, as two parts.
 template <int H>
-__device__ __forceinline__ SplitVector query_fragment(const KernelArgs& p, const Rows& r, int g, int i,
-                                                      uint32_t upper) {
+__device__ __forceinline__ void query_values(const KernelArgs& p, const Rows& r, int g, int i, float (&x)[8]) {
     const float* from = p.a.q + r.b * p.a.q_sequence + r.head * p.a.q_head + r.t * p.a.q_row + g * (H / 4) + 8 * i;
-    float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = r.ok ? from[e] * p.q_scale : 0.f;
-    return split_exact(x, upper);
+}
+template <int H>
+__device__ __forceinline__ SplitVector query_fragment(const KernelArgs& p, const Rows& r, int g, int i,
+                                                      uint32_t upper, uint32_t& left) {
+    float x[8];
+    query_values<H>(p, r, g, i, x);
+    return split_exact(x, upper, left);
+}
+template <int H>
+__device__ __forceinline__ SplitVector query_rest(const KernelArgs& p, const Rows& r, int g, int i, uint32_t upper) {
+    float x[8];
+    query_values<H>(p, r, g, i, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = rest_of(x[e], upper);
+    return split_finite(x, upper);
 }
 
 // The running softmax of a wave's rows: m and the unscaled O of this lane's query (dims
@@ -150,7 +164,8 @@ struct Running {
 // matrix cores and the vector units have work of their own; codes are loaded two steps
 // (K) and one (V) ahead. m is raised only where a score passes it by 8 (numerators up to
 // 2^8 are as exact), which after a few steps is never: O is hardly rescaled.
-// ready() makes them usable, while the first codes are on their way.
+// ready() makes them usable, while the first codes are on their way, and tells whether they leave something of q; then
+// each step's scores are corrected by a product with that, from codes loaded again.
 template <int H, class Ready, class Query>
 __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t key0, int32_t step, int32_t end,
                                      char* stage, int n, int g, uint32_t upper, Ready&& ready, Query&& q,
@@ -229,13 +244,30 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
         load(a.k_codes, a.k_scales, key0, k_next);
         load(a.v_codes, a.v_scales, key0, v_next);
     }
-    ready();
+    const bool left = ready();
     if (key0 >= end) return;
     Scores s_next = scores(k_next);
     load(a.k_codes, a.k_scales, min(key0 + step, end - 1), k_next);
     for (; key0 < end; key0 += step) {
         Scores s = s_next;
         Words v = v_next;
+        if (left) {
+            Words k;
+            load(a.k_codes, a.k_scales, key0, k);
+            f32x4 rest[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int i = 0; i < NF; ++i) {
+                const SplitVector x = query_rest<H>(p, r, g, i, upper);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int part = 1; part >= 0; --part)
+                        rest[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fragment_of(k.w[u][i], factor_of(k.s[u])),
+                                                                          x.part[part], rest[u], 0, 0, 0);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) s.s[u] = s.s[u] + rest[u] * (1.f / kRestLift);
+        }
         // What queries do not see is replaced: -inf for its scores, 0 for its values, since
         // 0 x NaN would reach them. NaN blocks of keys that some queries see are taken out as
         // well, and those queries given NaN below.
@@ -427,6 +459,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
     __shared__ __attribute__((aligned(16))) char stages[W * Stage::BYTES];
     __shared__ __attribute__((aligned(16))) char q_lds[Stage::Q_BYTES];
     __shared__ uint32_t arrived_last;
+    __shared__ uint32_t fragments_left;  // a byte each: whether its parts leave something of q
     const AttentionArgs& a = p.a;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -444,12 +477,16 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2))) voi
             [&]() __attribute__((always_inline)) {  // q's fragments, one a wave
                 static_assert(H / 32 <= W, "a wave has at most one");
                 if (wave < H / 32) {
-                    const SplitVector x = query_fragment<H>(p, r, g, wave, upper);
+                    uint32_t left = 0;
+                    const SplitVector x = query_fragment<H>(p, r, g, wave, upper, left);
+                    const bool any = __any(noticed(left));
+                    if (lane == 0) reinterpret_cast<uint8_t*>(&fragments_left)[wave] = any;
 #pragma unroll
                     for (int part = 0; part < kParts; ++part)
                         *reinterpret_cast<bf16x8*>(q_lds + ((wave * kParts + part) * 64 + lane) * 16) = x.part[part];
                 }
                 __syncthreads();
+                return (__builtin_amdgcn_readfirstlane(fragments_left) & (~0u >> (32 - H / 4))) != 0;
             },
             [&](int i, int part) __attribute__((always_inline)) {
                 return *reinterpret_cast<const bf16x8*>(q_lds + ((i * kParts + part) * 64 + lane) * 16);

@@ -100,7 +100,7 @@ __device__ __forceinline__ SplitVector split_finite(const float (&x)[8], uint32_
     }
     return split_vector_of(w);
 }
-__device__ __forceinline__ SplitVector split_exact(const float (&x)[8], uint32_t upper) {
+__device__ __forceinline__ SplitVector split_exact(const float (&x)[8], uint32_t upper, uint32_t& left) {
 #pragma clang fp contract(off)
     u32x4 w[kParts];
     bool odd = false;
@@ -111,9 +111,12 @@ __device__ __forceinline__ SplitVector split_exact(const float (&x)[8], uint32_t
         odd |= __builtin_isunordered(a1, b1);
         w[0][p] = upper_halves(a, b);
         w[1][p] = upper_halves(a1, b1);
-        w[2][p] = upper_halves(a1 - cut(a1, upper), b1 - cut(b1, upper));
+        const float a2 = a1 - cut(a1, upper), b2 = b1 - cut(b1, upper);
+        notice(left, a2, b2);
+        w[2][p] = upper_halves(a2, b2);
     }
     if (__any(odd)) {
+        left = ~0u;  // NaN among them
 #pragma unroll
         for (int p = 0; p < 4; ++p) {
             float part[2][kParts];
