@@ -165,7 +165,9 @@ typedef struct sn_fp4_attention_shape {
  * shorter prompt) gives zeros; one whose scores are all -inf gives NaN. Positions a query does not see do not enter its
  * result, whatever they hold (also NaN blocks). fp32 arithmetic as in
  * sn_matmul_fp4: q times scale log2 e is rounded to fp32, and that is used in full, subnormals
- * too. lengths over the capacity count as the capacity; `keys` over
+ * too. Values are summed with weights of up to 2^8, their sum divided by the weights' at the end: where the
+ * number of positions times the largest |value| passes 2^119, sums may overflow to infinities and NaN. A weight
+ * under 2^-118 of the query's largest may count as 0. lengths over the capacity count as the capacity; `keys` over
  * it is SN_ERR_SHAPE. Buffers too short for the strides are SN_ERR_LENGTH_MISMATCH; out
  * overlapping q or the cache, and out strides by which two outputs share memory,
  * are SN_ERR_ALIASING. Long caches are split over workgroups whose partial
