@@ -196,8 +196,8 @@ bool strided_need(const size_t (&counts)[3], const size_t (&strides)[3], size_t 
     return true;
 }
 
-// Whether no two of those rows share an element: each stride passes what the smaller ones span.
-bool distinct(const size_t (&counts)[3], const size_t (&strides)[3], size_t head_dim) {
+// Whether the strides nest, each at least what the smaller ones span, so that no two of those rows share an element.
+bool nested(const size_t (&counts)[3], const size_t (&strides)[3], size_t head_dim) {
     int order[3] = {0, 1, 2};
     std::sort(order, order + 3, [&](int i, int j) { return strides[i] < strides[j]; });
     size_t span = head_dim;
@@ -375,7 +375,7 @@ int sn_fp4_attention(sn_context* ctx, const sn_fp4_cache_shape* cache, const sn_
     if (all_rows == 0) return SN_OK;
     if (q == nullptr || out == nullptr) return SN_ERR_NULL_ARGUMENT;
     const size_t out_bytes = out_need * sizeof(float);
-    if (!distinct(counts, out_strides, cache->head_dim) || overlaps(out, out_bytes, q, q_need * sizeof(float)) ||
+    if (!nested(counts, out_strides, cache->head_dim) || overlaps(out, out_bytes, q, q_need * sizeof(float)) ||
         overlaps(out, out_bytes, lengths, cache->batch * sizeof(uint32_t)))
         return SN_ERR_ALIASING;
     for (const Bytes& b : buffers)

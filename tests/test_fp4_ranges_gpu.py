@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import fp4_reference as ref
+from staleynet_amd.gemm import GpuError, Shape
 from test_fp4_attention_gpu import Case
 
 pytestmark = pytest.mark.gpu
@@ -31,3 +32,38 @@ def test_large_values(gpu, head_dim, heads, queries, length, spread):
     case = Case(2, heads, 2, queries, length, head_dim, [length, length - 3], seed=length, spread=spread)
     case.scales[1][:, :, :length - 3] = 127 + (108 if length == 250 else 103)
     case.check(case.run(gpu))
+
+
+@pytest.mark.parametrize("strides,accepted", [
+    ((192, 32, 64), True), ((192, 32, 63), False), ((191, 32, 64), False), ((192, 31, 64), False),  # (time, head)
+    ((96, 192, 32), True), ((95, 192, 32), False), ((96, 191, 32), False),                          # (head, sequence, time)
+    ((400, 96, 64), False)])  # heads at 0, 96, rows at 0, 64, 128: shares nothing but does not nest
+def test_output_strides_nest(gpu, strides, accepted):
+    """Two sequences of two heads and three queries, 32 floats each: the least strides, one under them, and strides that
+    interleave. Accepted ones leave what lies between the outputs as it was."""
+    case = Case(2, 2, 2, 3, 9, 32, [9, 5], seed=1)
+    q = gpu.upload(Shape.vector(case.q.size), case.q)
+    filled = np.full(1000, 7, np.float32)
+    out = gpu.upload(Shape.vector(1000), filled)
+    call = lambda: gpu.fp4_attention(case.cache(gpu), q, out, 2, 3, case.scale, 0, gpu.upload_tokens(case.lengths),
+                                     out_strides=strides)
+    if not accepted:
+        with pytest.raises(GpuError, match="overlaps"):
+            call()
+        assert (gpu.download(out) == 7).all()
+        return
+    call()
+    at = sum(np.arange(n).reshape([-1 if i == j else 1 for j in range(4)]) * s
+             for i, (n, s) in enumerate(zip((2, 2, 3, 32), (*strides, 1))))
+    got = gpu.download(out)
+    case.check(got[at])
+    filled[at] = got[at]
+    assert np.array_equal(got, filled)
+
+
+def test_strides_of_single_counts_are_not_used(gpu):
+    case = Case(1, 1, 1, 1, 9, 32, [9], seed=2)
+    out = gpu.zeros(Shape.vector(32))
+    gpu.fp4_attention(case.cache(gpu), gpu.upload(Shape.vector(32), case.q), out, 1, 1, case.scale, 9, q_strides=(0, 0, 0),
+                      out_strides=(0, 0, 0))
+    case.check(gpu.download(out).reshape(case.q.shape))
