@@ -494,6 +494,8 @@ def library() -> ctypes.CDLL:
 
 def fp4_sizes(rows: int, inner: int) -> tuple[int, int]:
     """``sn_fp4_sizes``: bytes of the codes and of the scales of ``rows`` rows of ``inner`` values."""
+    if not (0 <= rows < 1 << 64 and 0 <= inner < 1 << 64):  # ctypes would pass the lower 64 bits
+        raise GpuError(SN_ERR_OVERFLOW, "fp4_sizes")
     codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
     rc = _library().sn_fp4_sizes(rows, inner, ctypes.byref(codes), ctypes.byref(scales))
     if rc != SN_OK:

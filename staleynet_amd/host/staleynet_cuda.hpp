@@ -522,8 +522,11 @@ class Gpu {
         return Fp4Matrix{cols, inner, zeros_bytes(codes), zeros_bytes(scales)};
     }
     Fp4Cache fp4_cache(const sn_fp4_cache_shape& shape) const {
-        size_t codes = 0, scales = 0;
-        check(sn_fp4_sizes(shape.batch * shape.kv_heads * shape.capacity, shape.head_dim, &codes, &scales));
+        size_t rows = 0, codes = 0, scales = 0;
+        if (__builtin_mul_overflow(shape.batch, shape.kv_heads, &rows) ||
+            __builtin_mul_overflow(rows, shape.capacity, &rows))
+            check(SN_ERR_OVERFLOW);
+        check(sn_fp4_sizes(rows, shape.head_dim, &codes, &scales));
         return Fp4Cache{shape, zeros_bytes(codes), zeros_bytes(scales), zeros_bytes(codes), zeros_bytes(scales)};
     }
 
