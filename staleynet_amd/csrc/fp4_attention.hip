@@ -316,10 +316,9 @@ __device__ __forceinline__ void walk(const KernelArgs& p, const Rows& r, int32_t
         const float base = run.m == -INFINITY ? 0.f : run.m;
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            x[e] = exp2_of(s.s[e / 4][e % 4] - base);
-            run.l = run.l + x[e];
-        }
+        for (int e = 0; e < 8; ++e) x[e] = exp2_of(s.s[e / 4][e % 4] - base);
+        // The step's sum first: one by one, a lane's sum of equal weights would end at 2^24 of them.
+        run.l = run.l + (((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])));
         const SplitVector pr = split_finite(x, upper);  // a NaN reaches the result through l
         wave_lds_order();
 #pragma unroll

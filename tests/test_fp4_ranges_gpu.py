@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import fp4_reference as ref
-from staleynet_amd.gemm import GpuError, Shape
+from staleynet_amd.gemm import Gpu, GpuError, Shape
 from test_fp4_attention_gpu import Case
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +67,22 @@ def test_strides_of_single_counts_are_not_used(gpu):
     gpu.fp4_attention(case.cache(gpu), gpu.upload(Shape.vector(32), case.q), out, 1, 1, case.scale, 9, q_strides=(0, 0, 0),
                       out_strides=(0, 0, 0))
     case.check(gpu.download(out).reshape(case.q.shape))
+
+
+def test_weights_of_a_very_long_cache_are_all_counted():
+    """3 x 2^28 positions that one workgroup takes (no workspace), 3 x 2^23 a lane: the sum of their equal weights, which
+    are 1, is exact, so the output is within a few roundings of the values' sum by the positions."""
+    gpu = Gpu(0, workspace_bytes=0)
+    try:
+        capacity, time = 3 << 28, 40
+        cache = gpu.fp4_cache(1, 1, capacity, 32)
+        packed = np.random.default_rng(31).standard_normal((time, 64)).astype(np.float32)
+        gpu.fp4_cache_append(cache, gpu.upload(Shape(time, 64), packed), time, 64, 0, 32, position=capacity - time)
+        values = ref.dequantize(*ref.quantize(packed[:, 32:]))
+        q, out = gpu.zeros(Shape(1, 32)), gpu.zeros(Shape(1, 32))
+        gpu.fp4_attention(cache, q, out, 1, 1, 1.0, keys=capacity)
+        want = values.sum(0) / capacity
+        assert (np.abs(gpu.download(out) - want) <= 2.0 ** -19 * np.abs(values).sum(0) / capacity).all()
+        del cache, q, out
+    finally:
+        gpu.close()
