@@ -415,7 +415,7 @@ __device__ __forceinline__ Share share_of(const KernelArgs& p, int lane) {
     const int64_t even = sum_over([](int32_t n) { return n / kKeys; }) * tiles / p.workgroups * kKeys;
     int32_t keys = max(p.least_keys, int32_t((min(even, a.capacity) + kUnit - 1) / kUnit) * kUnit);
     auto splits_of = [&](int32_t n) __attribute__((always_inline)) {
-        return n <= 2 * p.least_keys ? 1 : (n + keys - 1) / keys;
+        return n <= 2 * p.least_keys ? 1 : (n - 1) / keys + 1;  // n + keys may pass 2^31
     };
     auto filled = [&](int32_t n) __attribute__((always_inline)) { return n > keys / 2 ? splits_of(n) : 0; };
     while (keys < a.capacity && sum_over(filled) * tiles > p.workgroups)

@@ -86,3 +86,37 @@ def test_weights_of_a_very_long_cache_are_all_counted():
         del cache, q, out
     finally:
         gpu.close()
+
+
+def test_the_largest_capacity(gpu):
+    """2^30 - 1 positions, all held, and so many rows that each tile's keys are one workgroup's share: a share of the
+    capacity and the keys held are together 2^31. Positions never written hold zeros, so a query's result is known from
+    the 40 that all queries see and that are written."""
+    capacity, head_dim, heads, queries, time = (1 << 30) - 1, 32, 4, 1028, 40
+    rng = np.random.default_rng(30)
+    cache = gpu.fp4_cache(1, 1, capacity, head_dim)
+    packed = rng.standard_normal((time, 64)).astype(np.float32)
+    first = capacity - queries - time
+    gpu.fp4_cache_append(cache, gpu.upload(Shape(time, 64), packed), time, 64, 0, 32, position=first)
+    k, v = (ref.dequantize(*ref.quantize(packed[:, i:i + 32])) for i in (0, 32))
+    q = rng.standard_normal((heads * queries, head_dim)).astype(np.float32)
+    q[::4] = 0
+    out = gpu.upload(Shape(heads * queries, head_dim), np.full(q.size, 7, np.float32))
+    gpu.fp4_attention(cache, gpu.upload(Shape(heads * queries, head_dim), q), out, heads, queries, 6.0,
+                      lengths=gpu.upload_tokens([capacity]))
+    got = gpu.download(out).reshape(q.shape)
+    s = q.astype(np.float64) @ k.T * 6
+    top = np.maximum(s.max(1, keepdims=True), 0)
+    p = np.exp(s - top)
+    seen = capacity - queries + 1 + np.arange(heads * queries) % queries  # head by head
+    others = (seen[:, None] - time) * np.exp(-top)
+    total = p.sum(1, keepdims=True) + others
+    # Queries of zeros have weights of 1, whose sums are exact. A score of the others is a sum of magnitudes of under 300, so off
+    # by (3 + 66) 2^-23 of that, 2^-8.6, which numerator and sum each have; equal weights that are no powers of two are
+    # chains of 2^22 additions a lane, each off by 2^-24 of the sum so far: by 2^-2 of their share.
+    assert 6 * (np.abs(q) @ np.abs(k).T).max() < 300
+    off = np.where(q.any(1, keepdims=True), 2.0 ** -6 + 2.0 ** -2 * others / total, 2.0 ** -18)
+    # And each of the 40 weights counts as 0 where it is under 2^-118 of the largest: where the
+    # largest one's value is 0, that may be all there is of an output.
+    bound = off * (p @ np.abs(v)) / total + time * 2.0 ** -118 * np.abs(v).max()
+    assert (np.abs(got - p @ v / total) <= bound).all()
