@@ -11,7 +11,8 @@ import numpy as np
 import pytest
 
 import fp4_reference as ref
-from staleynet_amd.gemm import MatmulSpec, Precision
+from bench import HipGraph
+from staleynet_amd.gemm import Fp4Matrix, MatmulSpec, Precision, Shape
 from test_fp4_matmul_gpu import run, to_bf16
 
 pytestmark = pytest.mark.gpu
@@ -108,3 +109,28 @@ def test_small_values_rounded_to_bf16(gpu, rows, inner, cols):
         x, codes, scales, w = operands(rows, inner, cols, shift, rows + shift)
         got = run(gpu, MatmulSpec.new(rows, cols, inner).with_precision(Precision.Bf16), x, codes, scales)
         check(got, to_bf16(x), w, inner)
+
+
+@pytest.mark.parametrize("rows,inner,cols", [(1, 300, 50), (16, 300, 50), (40, 2100, 100)])
+def test_a_captured_product_meets_small_values_later(gpu, rows, inner, cols):
+    """Captured on ordinary values and replayed on small ones, on ordinary ones again and on both: the eager bits."""
+    x, codes, scales, w = operands(rows, inner, cols, 2, rows)
+    ordinary = np.random.default_rng(rows).standard_normal(x.shape).astype(np.float32)
+    spec = MatmulSpec.new(rows, cols, inner)
+    matrix = Fp4Matrix(cols, inner, gpu.upload_bytes(codes), gpu.upload_bytes(scales))
+    left, out = gpu.upload(Shape(rows, inner), ordinary), gpu.zeros(Shape(rows, cols))
+    call = lambda: gpu.matmul_fp4(spec.right_transposed(), left, matrix, out)
+    call()
+    gpu.synchronize()
+    graph = HipGraph(gpu.stream, call)
+    try:
+        for values in (x, ordinary, np.where(np.arange(inner) % 2, x, ordinary), x):
+            gpu.copy_from_host(left, values)
+            graph.launch()
+            got = gpu.download(out).reshape(rows, cols)
+            eager = run(gpu, spec, values, codes, scales)  # infinities and NaN among the ordinary ones'
+            assert np.array_equal(got.view(np.uint32), eager.view(np.uint32))
+        check(got, x, w, inner)
+    finally:
+        gpu.synchronize()
+        graph.close()
