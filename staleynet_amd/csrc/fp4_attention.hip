@@ -21,9 +21,9 @@
 // rows of their own, each walking over all keys, left two waves a SIMD in step with the
 // longest sequence: 292 us for two 1000-query chunks against up to 6001 positions, 197 so.)
 // Where there are few rows (a decode step) workgroups share a tile's keys as well.
-//   What bounds it: 64 heads on 8 of 131071 keys, 143 MB, 37 us (3.9 TB/s); 16 sequences of up to 8192 keys, 12.6 us,
+//   What bounds it: 64 heads on 8 of 131071 keys, 143 MB, 37 to 41 us (3.5 to 3.9 TB/s); 16 sequences of up to 8192 keys, 12.6 us,
 // and 12 heads on 701 keys, 8.2 us: one launch and a chain of loads, steps and the merge. Chunks of 1000
-// queries against 6001 keys: 195 us, 0.9 PFLOP/s of bf16 products, where conversions, exponentials, splits and LDS
+// queries against 6001 keys: 195 to 210 us, 0.8 to 0.9 PFLOP/s of bf16 products, where conversions, exponentials, splits and LDS
 // each take about as long as the matrix cores, which are busy 42 % of the cycles.
 #include <hip/hip_runtime.h>
 

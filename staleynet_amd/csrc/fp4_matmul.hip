@@ -23,7 +23,7 @@
 // lane reads 16 of one column at once, for the next steps, and the bytes
 // pass through LDS.
 //   What bounds it: W's bytes where there are many (1 x 8192 x 28672: 29.6 us, 125 MB at 4.2 TB/s), one
-// launch where there are few (1 x 768 x 2304: 3.8 us), and at 16 rows (16 x 4096 x 14336: 15.3 us
+// launch where there are few (1 x 768 x 2304: 3.8 us), and at 16 rows (16 x 4096 x 14336: 15.4 to 16.1 us
 // for 31 MB) the vector units, busy half the cycles with the split of x, which every workgroup does again.
 // More rows: tiles staged in LDS, below.
 #include <hip/hip_runtime.h>
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void few_rows_kernel(ProductArgs a)
 // lane's 16 bytes of codes are a block of one column: 64 inner values of 32 columns a
 // load. D = x W: a lane holds one column. Inner value 8 i + j of half h of a stage is
 // element j of operand i of lanes h (as the block's words hold the codes).
-//   2048 x 4096 x 4096 with fp32 inputs: 181 us, 380 TFLOP/s of products (1140 of bf16 ones, matrix cores busy half the
+//   2048 x 4096 x 4096 with fp32 inputs: 181 to 196 us, 350 to 380 TFLOP/s of products (1050 to 1140 of bf16 ones, matrix cores busy half the
 // cycles; 130 us without any load, 150 without x's, and 175 to 177 with the next stage's split spread between the
 // matrix instructions, which costs one part a tenth).
 template <int RT, int CT, int WR, int WC, int PARTS, int SUBS>

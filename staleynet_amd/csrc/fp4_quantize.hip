@@ -12,11 +12,11 @@
 // All are bound by memory: 4 bytes a value on the fp32 side against 0.53. Where the fp32 values of
 // a block are contiguous four lanes take it, eight values each: 32-byte loads or stores, a word of
 // codes a lane, so a wave's codes are 256 contiguous bytes; the maximum is exchanged over
-// four lanes. 8192 x 28672 weights: 183 us (5.8 TB/s) to 4 bits, 198 back, transposed; 308 and 232
+// four lanes. 8192 x 28672 weights: 184 us (5.8 TB/s) to 4 bits, 199 back, transposed; 301 to 321 and 232 to 253
 // with contiguous columns, where a wave writes 16 bytes each to 64 rows of codes (blocks taken in
 // runs of 4, 8 or 16 by a thread, to fill those rows' lines sooner: 331 to 342).
-// Cache rows: 4 x 2000 rows of 8 heads of 64, appended in 9.2 us and read in 11.5 (4.0 and 3.2 TB/s); 16 single
-// rows, 2.7 us each way.
+// Cache rows: 4 x 2000 rows of 8 heads of 64, appended in 8.8 us and read in 10.8 (4.2 and 3.4 TB/s, traced); 16 single
+// rows, 2.6 us each way.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
