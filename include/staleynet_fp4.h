@@ -169,11 +169,12 @@ typedef struct sn_fp4_attention_shape {
  * number of positions times the largest |value| passes 2^119, sums may overflow to infinities and NaN. A weight
  * under 2^-118 of the query's largest may count as 0. lengths over the capacity count as the capacity; `keys` over
  * it is SN_ERR_SHAPE. Buffers too short for the strides are SN_ERR_LENGTH_MISMATCH; out
- * overlapping q, the cache or the lengths is SN_ERR_ALIASING, and so are out strides that do not nest: sorted, each
- * has to be at least what the smaller ones span (head_dim floats and the steps by them; strides of counts of one are not used), so
- * that no two outputs share memory. Strides that interleave without sharing are refused as well. Long caches are split over workgroups whose partial
- * results go through the context's workspace and are merged in a fixed order, so
- * calls on one context must not overlap; with a smaller workspace they are split
+ * overlapping q, the cache or the lengths is SN_ERR_ALIASING, and so are out strides that do
+ * not nest: sorted, each has to be at least what the smaller ones span (head_dim floats and the
+ * steps by them; strides of counts of one are not used), so that no two outputs share memory.
+ * Strides that interleave without sharing are refused as well. Long caches are split over
+ * workgroups whose partial results go through the context's workspace and are merged in a fixed
+ * order, so calls on one context must not overlap; with a smaller workspace they are split
  * less, or not. Deterministic. */
 int sn_fp4_attention(sn_context *context, const sn_fp4_cache_shape *cache, const sn_fp4_attention_shape *shape,
                      const float *q, size_t q_len, const uint8_t *k_codes, size_t k_codes_len,

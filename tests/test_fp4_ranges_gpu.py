@@ -1,10 +1,14 @@
-"""The ends of the range of attention over a 4-bit cache (``sn_fp4_attention``), as its header states them."""
+"""The ends of the ranges that the header of the 4-bit operators states: values, strides, lengths, the capacity of a cache
+and the inner dimension of a product."""
 import numpy as np
 import pytest
 
 import fp4_reference as ref
-from staleynet_amd.gemm import Gpu, GpuError, Shape
+from fp4_reference import View
+from staleynet_amd.gemm import Fp4Matrix, Gpu, GpuError, MatmulSpec, Precision, Shape, Storage
 from test_fp4_attention_gpu import Case
+from test_fp4_matmul_gpu import check as check_product
+from test_fp4_matmul_gpu import to_bf16
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +124,29 @@ def test_the_largest_capacity(gpu):
     # largest one's value is 0, that may be all there is of an output.
     bound = off * (p @ np.abs(v)) / total + time * 2.0 ** -118 * np.abs(v).max()
     assert (np.abs(got - p @ v / total) <= bound).all()
+
+
+@pytest.mark.parametrize("rows,bf16", [(1, False), (5, False), (16, False), (30, True), (40, False), (40, True)])
+def test_the_longest_inner_dimension(gpu, rows, bf16):
+    """2^25 - 1 values a column, 5 GB of codes, zeros but for the first and the last two blocks of some columns: a product of 95
+    values, as exact as that."""
+    inner, cols = (1 << 25) - 1, 300
+    blocks = ref.blocks_of(inner)
+    rng = np.random.default_rng(rows)
+    matrix = gpu.fp4_matrix(cols, inner)
+    w = np.zeros((cols, 95))
+    for c in (0, 1, 63, 64, 127, 255, 256, 299):
+        for first, at, count in ((0, 0, 32), (blocks - 2, 32, 63)):
+            place, size = c * blocks + first, -(-count // 32)
+            part = Fp4Matrix(1, count, View(matrix.codes, place * 16, size * 16, 1), View(matrix.scales, place, size, 1))
+            gpu.quantize_fp4(gpu.upload(Shape.vector(count), rng.standard_normal(count)), part, Storage.Transposed)
+            w[c, at:at + count] = ref.dequantize(gpu.download_bytes(part.codes), gpu.download_bytes(part.scales), count)
+    x = gpu.zeros(Shape(rows, inner))
+    values = rng.standard_normal((rows, 95)).astype(np.float32)
+    for r in range(rows):
+        gpu.copy_from_host(View(x, r * inner, 32), values[r, :32])
+        gpu.copy_from_host(View(x, (r + 1) * inner - 63, 63), values[r, 32:])
+    spec = MatmulSpec.new(rows, cols, inner).right_transposed()
+    out = gpu.upload(Shape(rows, cols), np.full(rows * cols, 9, np.float32))
+    gpu.matmul_fp4(spec.with_precision(Precision.Bf16 if bf16 else Precision.F32), x, matrix, out)
+    check_product(gpu.download(out).reshape(rows, cols), to_bf16(values) if bf16 else values, w, 95)
