@@ -335,7 +335,7 @@ def _calls(s):
                 keep.append(a)
                 flat.append(ctypes.byref(a))
             else:
-                flat.append(ctypes.c_size_t(a))
+                flat.append(a)
         return getattr(library, name), tuple(flat), keep
 
     kind = case["kind"]
@@ -359,7 +359,6 @@ def _calls(s):
                 call("sn_dequantize_fp8", case["rows"], case["inner"], storage, "codes", "scales", "back")], s["back"]
     if kind == "product":
         spec = gemm.MatmulSpec.new(case["rows"], case["cols"], case["inner"]).right_transposed()
-        spec = spec.accumulate() if case["accumulate"] else spec
         return [call("sn_matmul_fp8", spec.to_c(), "left_codes", "left_scales", "right_codes", "right_scales", "bias",
                      "y")], s["y"]
     shape = gemm.CLogprobShape(case["rows"], case["offset"] + case["heads"] * case["classes"], case["offset"],
