@@ -281,8 +281,26 @@ class CFp4AttentionShape(ctypes.Structure):
         [("scale", ctypes.c_float)]
 
 
+FP8_BLOCK = 128  # SN_FP8_BLOCK (include/staleynet_fp8.h): values of an 8-bit block
+LOGPROBS_LARGEST_TOP = 32  # SN_LOGPROBS_LARGEST_TOP (include/staleynet_logprobs.h)
+
+
+class CRmsNormShape(ctypes.Structure):
+    """``sn_rms_norm_shape`` (include/staleynet_norm.h)."""
+
+    _fields_ = [("rows", ctypes.c_size_t), ("width", ctypes.c_size_t), ("epsilon", ctypes.c_float)]
+
+
+class CLogprobShape(ctypes.Structure):
+    """``sn_logprob_shape`` (include/staleynet_logprobs.h)."""
+
+    _fields_ = [(name, ctypes.c_size_t) for name in ("rows", "cols", "column_offset", "classes", "heads",
+                                                     "token_stride", "token_offset", "top")] + \
+        [("scale", ctypes.c_float)]
+
+
 class ByteBuffer:
-    """Bytes in device memory: the codes or the scales of 4-bit blocks."""
+    """Bytes in device memory: the codes or the scales of 4-bit or 8-bit blocks."""
 
     def __init__(self, gpu: "Gpu", pointer: int, count: int):
         self._gpu = gpu
@@ -313,6 +331,42 @@ class Fp4Matrix:
     inner: int
     codes: ByteBuffer
     scales: ByteBuffer
+
+
+@dataclass(frozen=True)
+class Fp8Matrix:
+    """An operand of a product in 8 bits (include/staleynet_fp8.h): ``rows`` rows of ``inner`` values, each
+    ``ceil(inner / 128)`` blocks of 128 bytes of codes, and one scale byte a block, a row's padded to fours."""
+
+    rows: int
+    inner: int
+    codes: ByteBuffer
+    scales: ByteBuffer
+
+    def buffers(self) -> list:
+        """The two buffers as the C ABI takes them: pointer and bytes each."""
+        return [ctypes.c_void_p(self.codes.pointer), len(self.codes), ctypes.c_void_p(self.scales.pointer),
+                len(self.scales)]
+
+
+@dataclass(frozen=True)
+class LogprobHeads:
+    """Which columns of a logits row the classifiers own (``heads`` of ``classes`` from ``column_offset`` on),
+    and which tokens of a token row are theirs; ``scale`` is an inverse temperature (``sn_logprob_shape``)."""
+
+    classes: int
+    heads: int = 1
+    column_offset: int = 0
+    token_stride: int | None = None  # None: the heads
+    token_offset: int = 0
+    scale: float = 1.0
+
+    def to_c(self, rows: int, cols: int, top: int = 0) -> CLogprobShape:
+        stride = self.heads if self.token_stride is None else self.token_stride
+        _check_sizes("token_logprobs", rows, cols, self.column_offset, self.classes, self.heads, stride,
+                     self.token_offset, top)
+        return CLogprobShape(rows, cols, self.column_offset, self.classes, self.heads, stride, self.token_offset, top,
+                             self.scale)
 
 
 @dataclass(frozen=True)
@@ -468,6 +522,16 @@ def _library() -> ctypes.CDLL:
         lib.sn_fp4_cache_read.argtypes = cache_and_rows + operand * 7
         lib.sn_fp4_attention.argtypes = [ctx, ctypes.POINTER(CFp4CacheShape), ctypes.POINTER(CFp4AttentionShape)] + \
             operand * 7
+        lib.sn_fp8_sizes.argtypes = lib.sn_fp4_sizes.argtypes
+        lib.sn_quantize_fp8.argtypes = lib.sn_quantize_fp4.argtypes
+        lib.sn_dequantize_fp8.argtypes = lib.sn_quantize_fp4.argtypes
+        lib.sn_matmul_fp8.argtypes = [ctx, ctypes.POINTER(CMatmulSpec)] + operand * 6
+        norm = [ctx, ctypes.POINTER(CRmsNormShape)]
+        lib.sn_rms_norm.argtypes = norm + operand * 6
+        lib.sn_rms_norm_fp8.argtypes = norm + operand * 6
+        lib.sn_rms_norm_backward.argtypes = norm + operand * 7
+        lib.sn_token_logprobs.argtypes = [ctx, ctypes.POINTER(CLogprobShape)] + operand * 7
+        lib.sn_token_logprobs_backward.argtypes = [ctx, ctypes.POINTER(CLogprobShape)] + operand * 7
         u32p = ctypes.POINTER(ctypes.c_uint32)
         lib.sn_tile_map.argtypes = [ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, u32p, u32p,
                                     u32p, u32p]
@@ -481,7 +545,9 @@ def _library() -> ctypes.CDLL:
                      "sn_causal_attention_score_grad", "sn_plan_matmul", "sn_plan_matmul_column_sums", "sn_matmul_column_sums", "sn_tile_map", "sn_matmul_noalloc", "sn_causal_attention_with_stats",
                      "sn_causal_attention_backward", "sn_alloc_bytes", "sn_upload_bytes", "sn_download_bytes",
                      "sn_free_bytes", "sn_fp4_sizes", "sn_quantize_fp4", "sn_dequantize_fp4", "sn_matmul_fp4",
-                     "sn_fp4_cache_append", "sn_fp4_cache_read", "sn_fp4_attention"):
+                     "sn_fp4_cache_append", "sn_fp4_cache_read", "sn_fp4_attention", "sn_fp8_sizes", "sn_quantize_fp8",
+                     "sn_dequantize_fp8", "sn_matmul_fp8", "sn_rms_norm", "sn_rms_norm_fp8", "sn_rms_norm_backward",
+                     "sn_token_logprobs", "sn_token_logprobs_backward"):
             getattr(lib, name).restype = ctypes.c_int
         _lib = lib
     return _lib
@@ -490,6 +556,27 @@ def _library() -> ctypes.CDLL:
 def library() -> ctypes.CDLL:
     """The loaded ``libstaleynet_gemm.so`` (raises if it has not been built)."""
     return _library()
+
+
+def _operand(buffer) -> list:
+    """A tensor or buffer, or none, as the C ABI takes it: pointer and elements."""
+    return [None, 0] if buffer is None else [ctypes.c_void_p(buffer.pointer), len(buffer)]
+
+
+def _check_sizes(what: str, *sizes: int) -> None:
+    """Refuses sizes past 64 bits, of which ctypes would pass the lower 64."""
+    if not all(0 <= size < 1 << 64 for size in sizes):
+        raise GpuError(SN_ERR_OVERFLOW, what)
+
+
+def fp8_sizes(rows: int, inner: int) -> tuple[int, int]:
+    """``sn_fp8_sizes``: bytes of the codes and of the scales of ``rows`` rows of ``inner`` values."""
+    _check_sizes("fp8_sizes", rows, inner)
+    codes, scales = ctypes.c_size_t(), ctypes.c_size_t()
+    rc = _library().sn_fp8_sizes(rows, inner, ctypes.byref(codes), ctypes.byref(scales))
+    if rc != SN_OK:
+        raise GpuError(rc, "fp8_sizes")
+    return codes.value, scales.value
 
 
 def fp4_sizes(rows: int, inner: int) -> tuple[int, int]:
@@ -970,6 +1057,102 @@ class Gpu:
         if rc in _VALIDATION_CODES:
             raise MatmulPanic(rc)
         self._check(rc, "matmul_fp4")
+
+    def fp8_matrix(self, rows: int, inner: int) -> Fp8Matrix:
+        """An ``Fp8Matrix`` of zeros."""
+        codes, scales = fp8_sizes(rows, inner)
+        return Fp8Matrix(rows, inner, self.zeros_bytes(codes), self.zeros_bytes(scales))
+
+    def quantize_fp8(self, source: Tensor, matrix: Fp8Matrix, storage: Storage = Storage.RowMajor) -> None:
+        """``sn_quantize_fp8``: an operand rounded to 8-bit blocks along ``inner``; the source is
+        ``[rows, inner]`` (``RowMajor``: activations) or ``[inner, rows]`` (``Transposed``: a weight as Linear
+        keeps it)."""
+        rc = _library().sn_quantize_fp8(self._ctx, matrix.rows, matrix.inner, int(storage),
+                                        ctypes.c_void_p(source.pointer), len(source), *matrix.buffers())
+        if rc in _VALIDATION_CODES:
+            raise MatmulPanic(rc)
+        self._check(rc, "quantize_fp8")
+
+    def dequantize_fp8(self, matrix: Fp8Matrix, output: Tensor, storage: Storage = Storage.RowMajor) -> None:
+        """``sn_dequantize_fp8``: the values ``matrix`` stands for, exactly, stored as ``storage`` says."""
+        rc = _library().sn_dequantize_fp8(self._ctx, matrix.rows, matrix.inner, int(storage), *matrix.buffers(),
+                                          ctypes.c_void_p(output.pointer), len(output))
+        if rc in _VALIDATION_CODES:
+            raise MatmulPanic(rc)
+        self._check(rc, "dequantize_fp8")
+
+    def matmul_fp8(self, spec: MatmulSpec, left: Fp8Matrix, right: Fp8Matrix, output: Tensor,
+                   bias: Tensor | None = None) -> None:
+        """``matmul`` (with ``bias``: ``matmul_bias``) of two 8-bit operands (``sn_matmul_fp8``): ``left`` holds
+        the rows, ``right`` the columns; the spec's ``right`` is ``Transposed``."""
+        if (left.rows, left.inner) != (spec.rows, spec.inner):
+            raise MatmulPanic(SN_ERR_LEFT_TOO_SMALL)
+        if (right.rows, right.inner) != (spec.cols, spec.inner):
+            raise MatmulPanic(SN_ERR_RIGHT_TOO_SMALL)
+        c = spec.to_c()
+        rc = _library().sn_matmul_fp8(self._ctx, ctypes.byref(c), *left.buffers(), *right.buffers(), *_operand(bias),
+                                      ctypes.c_void_p(output.pointer), len(output))
+        if rc in _VALIDATION_CODES:
+            raise MatmulPanic(rc)
+        self._check(rc, "matmul_fp8")
+
+    def rms_norm(self, x: Tensor, weight: Tensor, out: Tensor | Fp8Matrix, epsilon: float, rows: int,
+                 residual: Tensor | None = None, sum: Tensor | None = None, inverse: Tensor | None = None) -> None:
+        """The residual addition and norm of ``rows`` rows (``sn_rms_norm``): ``sum = x + residual``, ``out =
+        weight * sum / sqrt(mean(sum^2) + epsilon)``, and ``inverse``, the factors of the backward. With an
+        ``Fp8Matrix`` as ``out``, rounded to 8-bit blocks (``sn_rms_norm_fp8``; no ``inverse``)."""
+        _check_sizes("rms_norm", rows)
+        shape = CRmsNormShape(rows, len(weight), epsilon)
+        args = [self._ctx, ctypes.byref(shape), *_operand(x), *_operand(residual), *_operand(weight), *_operand(sum)]
+        if isinstance(out, Fp8Matrix):
+            if (out.rows, out.inner) != (rows, len(weight)) or inverse is not None:
+                raise AssertionError("rms_norm: the 8-bit output does not fit the rows, or inverse is asked for with it")
+            rc = _library().sn_rms_norm_fp8(*args, *out.buffers())
+        else:
+            rc = _library().sn_rms_norm(*args, *_operand(out), *_operand(inverse))
+        self._check_lengths(rc, "rms_norm")
+
+    def rms_norm_backward(self, sum: Tensor, inverse: Tensor, weight: Tensor, d_out: Tensor, d_x: Tensor, rows: int,
+                          d_sum: Tensor | None = None, d_weight: Tensor | None = None) -> None:
+        """The norm's gradients (``sn_rms_norm_backward``): ``d_x`` (with ``d_sum``, what reaches the sum past the
+        norm, added) and ``d_weight +=``."""
+        _check_sizes("rms_norm_backward", rows)
+        shape = CRmsNormShape(rows, len(weight), 0.0)
+        rc = _library().sn_rms_norm_backward(self._ctx, ctypes.byref(shape), *_operand(sum), *_operand(inverse),
+                                             *_operand(weight), *_operand(d_out), *_operand(d_sum), *_operand(d_x),
+                                             *_operand(d_weight))
+        self._check_lengths(rc, "rms_norm_backward")
+
+    def token_logprobs(self, logits: Tensor, heads: LogprobHeads, tokens: TokenBuffer | None = None,
+                       logprobs: Tensor | None = None, entropies: Tensor | None = None, stats: Tensor | None = None,
+                       top: int = 0, top_tokens: TokenBuffer | None = None, top_logprobs: Tensor | None = None) -> None:
+        """Log probabilities of given tokens, entropies, what the backward needs and the ``top`` likeliest classes
+        of every row and head (``sn_token_logprobs``), each where a tensor is given for it."""
+        shape = logits.shape()
+        c = heads.to_c(shape.rows, shape.cols, top)
+        rc = _library().sn_token_logprobs(self._ctx, ctypes.byref(c), *_operand(logits), *_operand(tokens),
+                                          *_operand(logprobs), *_operand(entropies), *_operand(stats),
+                                          *_operand(top_tokens), *_operand(top_logprobs))
+        self._check_lengths(rc, "token_logprobs")
+
+    def token_logprobs_backward(self, logits: Tensor, heads: LogprobHeads, stats: Tensor, grad: Tensor,
+                                tokens: TokenBuffer | None = None, d_logprobs: Tensor | None = None,
+                                entropies: Tensor | None = None, d_entropies: Tensor | None = None) -> None:
+        """The gradient of the logits (``sn_token_logprobs_backward``) from those of the log probabilities and of
+        the entropies; ``grad`` may be ``logits``."""
+        shape = logits.shape()
+        c = heads.to_c(shape.rows, shape.cols)
+        rc = _library().sn_token_logprobs_backward(self._ctx, ctypes.byref(c), *_operand(logits), *_operand(tokens),
+                                                   *_operand(stats), *_operand(entropies), *_operand(d_logprobs),
+                                                   *_operand(d_entropies), *_operand(grad))
+        self._check_lengths(rc, "token_logprobs_backward")
+
+    def _check_lengths(self, rc: int, what: str) -> None:
+        if rc == SN_ERR_SHAPE:
+            raise AssertionError(f"{what}: heads run past a row")
+        if rc == SN_ERR_LENGTH_MISMATCH:
+            raise AssertionError(f"{what}: a buffer is too small for the shape")
+        self._check(rc, what)
 
     def fp4_cache(self, batch: int, kv_heads: int, capacity: int, head_dim: int) -> Fp4Cache:
         """An ``Fp4Cache`` of zeros."""
