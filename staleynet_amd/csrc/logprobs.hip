@@ -4,9 +4,20 @@
 // With m the largest logit, z = a (x - m) and rest = the sum of e^z without one
 // term of the largest: T = log(1 + rest), logprob = z_token - T, H = T + W / (1 +
 // rest), W = the sum of e^z (-z), all of whose terms are positive. e^z is 2^(z log2 e)
-// on the transcendental unit (v_exp_f32, about 1 ulp); rounding z log2 e adds
-// at most |z| 2^-24 to a term's relative error. Bound by memory: 4 bytes a logit
-// forward, 8 backward.
+// on the transcendental unit (v_exp_f32, about 1 ulp); the factor a log2 e and its
+// product with x - m add at most 2^-23 |z| to a term's relative error.
+//
+// Bound by memory: 4 bytes a logit forward, 8 backward. A wave holds up to 2048
+// classes of a row's head in registers, so a logit is read once: their maximum,
+// then the sums, then the likeliest. Longer rows are chunks of 2048 whose {m,
+// rest, W} are merged, and where rows are few the chunks go to several waves,
+// whose parts a second kernel merges in order.
+//
+// The likeliest k of a chunk: the k-th largest of the 64 lanes' maxima, found by
+// bisection over ballots, is a bound that at least k values reach and few
+// others do; those are gathered in LDS and each finds its rank by comparing
+// with all. Where too many reach it (many equal values) they are taken one by
+// one instead.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -18,27 +29,38 @@
 namespace sn {
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_unaligned __attribute__((aligned(4)));
+
+constexpr int kWaves = 4;          // of a workgroup, each on its own
+constexpr int kChunk = 2048;       // classes a wave holds
+constexpr int kLargestTop = SN_LOGPROBS_LARGEST_TOP;
+constexpr int kCandidates = 96;    // gathered at once
+constexpr int kListed = kCandidates + kLargestTop;
 constexpr uint32_t kEmptyToken = SN_EMPTY_TOKEN;
-constexpr float kLog2e = 1.44269504088896340736f;
-__device__ __forceinline__ float exp_of(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // An order of logits as integers: NaN is the largest, -0 equals 0; 0 is below all.
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t bits = __builtin_bit_cast(uint32_t, x + 0.f);
-    if (x != x) return 0xffffffffu;
-    return bits ^ (uint32_t(int32_t(bits) >> 31) | 0x80000000u);
+    return x != x ? 0xffffffffu : bits ^ (uint32_t(int32_t(bits) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float logit_of(uint32_t key) {
     return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 // A class with its logit, ordered by the logit and then with the lower class ahead; all are above 0 and below ~0.
 constexpr uint32_t kClassMask = 0x7fffffffu;
-__device__ __forceinline__ uint64_t entry_of(float x, uint32_t c) { return uint64_t(key_of(x)) << 32 | (kClassMask - c); }
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t c) { return uint64_t(key) << 32 | (kClassMask - c); }
 __device__ __forceinline__ uint32_t class_of(uint64_t entry) { return kClassMask - uint32_t(entry); }
 
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int step = 1; step < 64; step <<= 1) v = v + __shfl_xor(v, step);
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int step = 1; step < 64; step <<= 1) v = fmaxf(v, __shfl_xor(v, step));
     return v;
 }
 __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
@@ -49,91 +71,341 @@ __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
     }
     return v;
 }
+// Between a wave's writes of LDS and its other lanes' reads of them, and back: the hardware
+// keeps the order of one wave's accesses, the fences the compiler's.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
 
-// One wave a row and head.
-__global__ __launch_bounds__(64) void logprobs_kernel(LogprobArgs a) {
-#pragma clang fp contract(off)
-    const int lane = threadIdx.x;
-    const int64_t place = blockIdx.x, row = place / a.heads, head = place - row * a.heads;
-    const float* x = a.logits + row * a.cols + a.column_offset + head * a.classes;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int64_t c = lane; c < a.classes; c += 64) {
-        nan |= x[c] != x[c];
-        m = fmaxf(m, x[c]);
+// The largest logit of some classes, the sum of the others' e^z and W over them, in units of log2 e.
+struct Sums {
+    float m, rest, weighted;
+};
+// Those of both. A part without a finite logit has m = -inf and rest = 0, or NaN.
+__device__ __forceinline__ Sums merged(Sums a, Sums b, float factor) {
+    if (b.m > a.m) {
+        const Sums t = a;
+        a = b;
+        b = t;
     }
+    if (b.m == -INFINITY) {
+        a.rest += b.rest;
+        return a;
+    }
+    const float away = (a.m - b.m) * factor, e = __builtin_amdgcn_exp2f(-away);
+    a.rest += e * (1.f + b.rest);
+    a.weighted += e > 0.f ? e * (b.weighted + (1.f + b.rest) * away) : 0.f;
+    return a;
+}
+
+// The `top` largest entries of a wave's, sorted, in list[0 .. top), of which the first `held` are there already and are
+// among them; returns how many there are. N keys a lane (0: none), class(i) the class of key i; a key has to
+// be above `above`. The list has room for kListed entries.
+template <int N, class ClassOf>
+__device__ __forceinline__ int select_top(const uint32_t (&key)[N], ClassOf class_at, int top, uint64_t* list, int held,
+                                          uint32_t above) {
+    const int lane = threadIdx.x & 63;
+    uint32_t largest = 0;
 #pragma unroll
-    for (int step = 1; step < 64; step <<= 1) m = fmaxf(m, __shfl_xor(m, step));
-    float rest = 0.f, weighted = 0.f, equal = 0.f;
-    for (int64_t c = lane; c < a.classes; c += 64) {
-        const float z = (x[c] - m) * a.scale, e = exp_of(z);
-        rest += x[c] < m ? e : 0.f;
-        equal += x[c] == m ? 1.f : 0.f;
-        weighted += e > 0.f ? e * -z : 0.f;
+    for (int i = 0; i < N; ++i) largest = max(largest, key[i]);
+    if (!__any(largest > above)) return held;
+    // The bound, to 16 bits: the `top`-th largest of the lanes' maxima (0 where fewer lanes have values).
+    uint32_t bound = 0;
+#pragma unroll
+    for (uint32_t bit = 0x80000000u; bit >= 0x00010000u; bit >>= 1)
+        if (__popcll(__ballot(largest >= (bound | bit))) >= top) bound |= bit;
+    bound = max(bound, above + 1);
+    int count = held;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint64_t mask = __ballot(key[i] >= bound);
+        if (mask == 0) continue;
+        const int at = count + __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
+        if (key[i] >= bound && at < kListed) list[at] = entry_of(key[i], class_at(i));
+        count += __popcll(mask);
     }
-    rest = wave_sum(rest) + (wave_sum(equal) - 1.f);
-    weighted = wave_sum(weighted);
-    if (__any(nan) || !(fabsf(m) < INFINITY)) rest = m = NAN;
-    const float log_total = log1pf(rest);
+    wave_lds_order();
+    if (count > kListed) {
+        // One by one: the largest below the last, of the lanes' keys and of the list's first `held`.
+        uint64_t own = lane < held ? list[lane] : 0, mine = 0, last = ~uint64_t(0);
+        wave_lds_order();
+        int found = 0;
+        for (; found < top; ++found) {
+            uint64_t best = own < last ? own : 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const uint64_t entry = key[i] > above ? entry_of(key[i], class_at(i)) : 0;
+                if (entry < last && entry > best) best = entry;
+            }
+            last = wave_largest(best);
+            if (last == 0) break;
+            if (lane == found) mine = last;
+        }
+        if (lane < found) list[lane] = mine;
+        wave_lds_order();
+        return found;
+    }
+    // Two entries a lane find their ranks.
+    const uint64_t first = lane < count ? list[lane] : 0, second = lane + 64 < count ? list[lane + 64] : 0;
+    int rank1 = 0, rank2 = 0;
+    for (int i = 0; i < count; ++i) {
+        const uint64_t other = list[i];
+        rank1 += other > first;
+        rank2 += other > second;
+    }
+    wave_lds_order();
+    if (lane < count && rank1 < top) list[rank1] = first;
+    if (lane + 64 < count && rank2 < top) list[rank2] = second;
+    wave_lds_order();
+    return min(count, top);
+}
+static_assert(kListed <= 128, "two entries a lane");
+
+// A place's results: from its sums and its list.
+__device__ __forceinline__ void finish(const LogprobArgs& a, int64_t place, Sums s, const uint64_t* list, int found) {
+#pragma clang fp contract(off)
+    const int lane = threadIdx.x & 63;
+    if (!(fabsf(s.m) < INFINITY) || s.rest != s.rest) s.m = s.rest = NAN;
+    const float log_total = log1pf(s.rest);
     if (lane == 0) {
         if (a.logprobs != nullptr) {
+            const int64_t row = place / a.heads, head = place - row * a.heads;
             const uint32_t token = a.tokens[row * a.token_stride + a.token_offset + head];
             float lp = 0.f;
-            if (token != kEmptyToken) lp = token < uint64_t(a.classes) ? (x[token] - m) * a.scale - log_total : NAN;
+            if (token != kEmptyToken) {
+                lp = NAN;
+                if (token < uint64_t(a.classes))
+                    lp = (a.logits[row * a.cols + a.column_offset + head * a.classes + token] - s.m) * a.scale - log_total;
+            }
             a.logprobs[place] = lp;
         }
-        if (a.entropies != nullptr) a.entropies[place] = log_total + weighted / (1.f + rest);
-        if (a.stats != nullptr) a.stats[2 * place] = m, a.stats[2 * place + 1] = log_total;
+        if (a.entropies != nullptr) a.entropies[place] = log_total + s.weighted * kLn2 / (1.f + s.rest);
+        if (a.stats != nullptr) a.stats[2 * place] = s.m, a.stats[2 * place + 1] = log_total;
     }
-    // The likeliest, one pass each: the largest of (key, lower class first) below the last.
-    uint64_t last = ~uint64_t(0);
-    for (int i = 0; i < a.top; ++i) {
-        uint64_t best = 0;
-        for (int64_t c = lane; c < a.classes; c += 64) {
-            const uint64_t entry = entry_of(x[c], uint32_t(c));
-            if (entry < last && entry > best) best = entry;
+    if (lane < a.top) {
+        const bool none = lane >= found;
+        const uint64_t entry = none ? 0 : list[lane];
+        if (a.top_tokens != nullptr) a.top_tokens[place * a.top + lane] = none ? kEmptyToken : class_of(entry);
+        if (a.top_logprobs != nullptr)
+            a.top_logprobs[place * a.top + lane] =
+                none ? -INFINITY : (logit_of(uint32_t(entry >> 32)) - s.m) * a.scale - log_total;
+    }
+}
+
+// Bytes of workspace a part leaves: its sums and its list.
+__host__ __device__ constexpr int64_t part_bytes(int top) { return 16 + 16 * int64_t((top + 1) / 2); }
+
+// VECTORS vectors of four classes a lane; a wave an item: part `item % parts` of place `item / parts`, the chunks from
+// part * chunks_per_part on.
+template <int VECTORS, bool TOP>
+__global__ __launch_bounds__(64 * kWaves) void logprobs_kernel(LogprobArgs a, int64_t items, int parts,
+                                                               int chunks_per_part) {
+    __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? kListed : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint64_t* list = lists[TOP ? wave : 0];
+    for (int64_t item = int64_t(blockIdx.x) * kWaves + wave; item < items; item += int64_t(gridDim.x) * kWaves) {
+        const int64_t place = item / parts, row = place / a.heads, head = place - row * a.heads;
+        const int part = int(item - place * parts);
+        const float* x = a.logits + row * a.cols + a.column_offset + head * a.classes;
+        const int64_t begin = int64_t(part) * chunks_per_part * (256 * VECTORS);
+        const int64_t end = min(begin + int64_t(chunks_per_part) * (256 * VECTORS), a.classes);
+        const float factor = a.scale * kLog2e;
+        Sums total = {-INFINITY, 0.f, 0.f};
+        int found = 0;
+        for (int64_t chunk = begin; chunk < end; chunk += 256 * VECTORS) {
+            float v[4 * VECTORS];
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i) {
+                const int64_t c = chunk + 4 * (lane + 64 * i);
+                if (c + 4 <= end) {
+                    const f32x4 loaded = *reinterpret_cast<const f32x4_unaligned*>(x + c);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[4 * i + j] = loaded[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[4 * i + j] = c + j < end ? x[c + j] : -INFINITY;
+                }
+            }
+            Sums s = {-INFINITY, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4 * VECTORS; ++i) s.m = fmaxf(s.m, v[i]);
+            s.m = wave_max(s.m);
+            // A NaN is no maximum, but its term makes `rest` NaN. Equal ones to the maximum count 1 each, without one of them.
+            int equal = 0;
+#pragma unroll
+            for (int i = 0; i < 4 * VECTORS; ++i) {
+                const float z = (v[i] - s.m) * factor, e = __builtin_amdgcn_exp2f(z);
+                s.rest += v[i] == s.m ? 0.f : e;
+                equal += v[i] == s.m ? 1 : 0;
+                s.weighted -= e > 0.f ? e * z : 0.f;
+            }
+            s.rest = wave_sum(s.rest);
+            if (s.m != -INFINITY) s.rest += wave_sum(float(equal)) - 1.f;
+            s.weighted = wave_sum(s.weighted);
+            total = merged(total, s, factor);
+            if constexpr (TOP) {
+                uint32_t key[4 * VECTORS];
+#pragma unroll
+                for (int i = 0; i < 4 * VECTORS; ++i)
+                    key[i] = chunk + 4 * (lane + 64 * (i / 4)) + i % 4 < end ? key_of(v[i]) : 0;
+                // Later chunks' classes are higher: an equal key is no candidate.
+                const uint32_t above = found == a.top ? uint32_t(list[a.top - 1] >> 32) : 0;
+                const auto class_at = [&](int i) { return uint32_t(chunk) + 4 * (lane + 64 * (i / 4)) + i % 4; };
+                found = select_top(key, class_at, a.top, list, found, above);
+            }
         }
-        last = wave_largest(best);
-        if (lane == 0) {
-            const bool none = last == 0;
-            if (a.top_tokens != nullptr) a.top_tokens[place * a.top + i] = none ? kEmptyToken : class_of(last);
-            if (a.top_logprobs != nullptr)
-                a.top_logprobs[place * a.top + i] =
-                    none ? -INFINITY : (logit_of(uint32_t(last >> 32)) - m) * a.scale - log_total;
+        if (parts == 1) {
+            finish(a, place, total, list, found);
+        } else {
+            char* out = reinterpret_cast<char*>(a.workspace) + item * part_bytes(a.top);
+            if (lane == 0) *reinterpret_cast<f32x4*>(out) = f32x4{total.m, total.rest, total.weighted, 0.f};
+            if (TOP && lane < a.top) reinterpret_cast<uint64_t*>(out + 16)[lane] = lane < found ? list[lane] : 0;
         }
     }
 }
 
-// One wave a row and head.
-__global__ __launch_bounds__(64) void logprobs_backward_kernel(LogprobBackwardArgs a) {
+// A wave a place: its parts merged, in order.
+template <bool TOP>
+__global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, int64_t places, int parts) {
+    __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? kListed : 1];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int64_t place = int64_t(blockIdx.x) * kWaves + wave; place < places; place += int64_t(gridDim.x) * kWaves) {
+        const char* in = reinterpret_cast<const char*>(a.workspace) + place * parts * part_bytes(a.top);
+        const float factor = a.scale * kLog2e;
+        Sums total = {-INFINITY, 0.f, 0.f};
+        for (int p = lane; p < parts; p += 64) {
+            const f32x4 s = *reinterpret_cast<const f32x4*>(in + p * part_bytes(a.top));
+            total = merged(total, Sums{s[0], s[1], s[2]}, factor);
+        }
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1)
+            total = merged(total, Sums{__shfl_xor(total.m, step), __shfl_xor(total.rest, step), __shfl_xor(total.weighted, step)},
+                           factor);
+        total = Sums{__shfl(total.m, 0), __shfl(total.rest, 0), __shfl(total.weighted, 0)};
+        int found = 0;
+        if constexpr (TOP) {
+            constexpr int N = kChunk / 64;  // parts * top is at most kChunk
+            const int entries = parts * a.top;
+            uint32_t key[N], low[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int e = lane + 64 * i;
+                uint64_t entry = 0;
+                if (e < entries) {
+                    const int p = e / a.top;
+                    entry = reinterpret_cast<const uint64_t*>(in + p * part_bytes(a.top) + 16)[e - p * a.top];
+                }
+                key[i] = uint32_t(entry >> 32);
+                low[i] = class_of(entry);
+            }
+            found = select_top(key, [&](int i) { return low[i]; }, a.top, lists[wave], 0, 0);
+        }
+        finish(a, place, total, lists[TOP ? wave : 0], found);
+    }
+}
+
+// VECTORS vectors of four classes a lane, a wave an item: chunk `item % chunks` of place `item / chunks`.
+template <int VECTORS>
+__global__ __launch_bounds__(64 * kWaves) void logprobs_backward_kernel(LogprobBackwardArgs a, int64_t items, int chunks) {
 #pragma clang fp contract(off)
-    const int64_t place = blockIdx.x, row = place / a.heads, head = place - row * a.heads;
-    const int64_t first = row * a.cols + a.column_offset + head * a.classes;
-    const float *x = a.logits + first, m = a.stats[2 * place], log_total = a.stats[2 * place + 1];
-    float d_logprob = 0.f, d_entropy = 0.f, entropy = 0.f;
-    uint32_t token = kEmptyToken;
-    if (a.d_logprobs != nullptr) {
-        token = a.tokens[row * a.token_stride + a.token_offset + head];
-        if (token != kEmptyToken) d_logprob = a.d_logprobs[place];
+    const int lane = threadIdx.x & 63;
+    for (int64_t item = int64_t(blockIdx.x) * kWaves + (threadIdx.x >> 6); item < items; item += int64_t(gridDim.x) * kWaves) {
+        const int64_t place = item / chunks, row = place / a.heads, head = place - row * a.heads;
+        const int64_t chunk = (item - place * chunks) * (256 * VECTORS);
+        const int64_t first = row * a.cols + a.column_offset + head * a.classes;
+        const float *x = a.logits + first, m = a.stats[2 * place], log_total = a.stats[2 * place + 1];
+        float* grad = a.grad + first;
+        float d_logprob = 0.f, d_entropy = 0.f, entropy = 0.f;
+        uint32_t token = kEmptyToken;
+        if (a.d_logprobs != nullptr) {
+            token = a.tokens[row * a.token_stride + a.token_offset + head];
+            if (token != kEmptyToken) d_logprob = a.d_logprobs[place];
+        }
+        if (a.d_entropies != nullptr) d_entropy = a.d_entropies[place], entropy = a.entropies[place];
+        auto grad_of = [&](float logit, int64_t c) {
+            const float log_p = (logit - m) * a.scale - log_total, p = __builtin_amdgcn_exp2f(log_p * kLog2e);
+            const float one = uint64_t(c) == token ? d_logprob : 0.f;
+            const float more = p > 0.f ? d_entropy * (log_p + entropy) : 0.f;
+            return (one - p * (d_logprob + more)) * a.scale;
+        };
+        f32x4 v[VECTORS];
+#pragma unroll
+        for (int i = 0; i < VECTORS; ++i) {
+            const int64_t c = chunk + 4 * (lane + 64 * i);
+            if (c + 4 <= a.classes) v[i] = *reinterpret_cast<const f32x4_unaligned*>(x + c);
+        }
+#pragma unroll
+        for (int i = 0; i < VECTORS; ++i) {
+            const int64_t c = chunk + 4 * (lane + 64 * i);
+            if (c + 4 <= a.classes) {
+                f32x4 g;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) g[j] = grad_of(v[i][j], c + j);
+                *reinterpret_cast<f32x4_unaligned*>(grad + c) = g;
+            } else {
+                for (int64_t k = c; k < a.classes; ++k) grad[k] = grad_of(x[k], k);
+            }
+        }
     }
-    if (a.d_entropies != nullptr) d_entropy = a.d_entropies[place], entropy = a.entropies[place];
-    for (int64_t c = threadIdx.x; c < a.classes; c += 64) {
-        const float log_p = (x[c] - m) * a.scale - log_total, p = exp_of(log_p);
-        const float one = uint64_t(c) == token ? d_logprob : 0.f;
-        const float more = p > 0.f ? d_entropy * (log_p + entropy) : 0.f;
-        a.grad[first + c] = (one - p * (d_logprob + more)) * a.scale;
-    }
+}
+
+// Workgroups for that many waves' items, within the 2^32 threads of a launch; the kernels' waves loop over the rest.
+unsigned groups_of(int64_t items) { return unsigned(std::min<int64_t>((items + kWaves - 1) / kWaves, 1 << 22)); }
+
+template <int VECTORS>
+void launch_forward(const LogprobArgs& a, int64_t items, int parts, int chunks_per_part, hipStream_t stream) {
+    const dim3 grid(groups_of(items)), block(64 * kWaves);
+    if (a.top > 0)
+        hipLaunchKernelGGL((logprobs_kernel<VECTORS, true>), grid, block, 0, stream, a, items, parts, chunks_per_part);
+    else
+        hipLaunchKernelGGL((logprobs_kernel<VECTORS, false>), grid, block, 0, stream, a, items, parts, chunks_per_part);
 }
 
 }  // namespace
 
 hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(logprobs_kernel, dim3(unsigned(a.rows * a.heads)), dim3(64), 0, stream, a);
+    const int64_t places = a.rows * a.heads;
+    if (a.classes <= kChunk) {
+        if (a.classes <= 256)
+            launch_forward<1>(a, places, 1, 1, stream);
+        else if (a.classes <= 512)
+            launch_forward<2>(a, places, 1, 1, stream);
+        else if (a.classes <= 1024)
+            launch_forward<4>(a, places, 1, 1, stream);
+        else
+            launch_forward<8>(a, places, 1, 1, stream);
+        return hipGetLastError();
+    }
+    // Parts: enough waves to fill the GPU twice over (32 a CU), as many as the merge takes and the workspace holds.
+    const int64_t chunks = (a.classes + kChunk - 1) / kChunk;
+    int64_t parts = std::min(chunks, (64 * int64_t(a.cu_count) + places - 1) / places);
+    parts = std::min<int64_t>(parts, a.top > 0 ? kChunk / a.top : kChunk);
+    parts = std::min<int64_t>(parts, int64_t(a.workspace_bytes) / (places * part_bytes(a.top)));
+    parts = std::max<int64_t>(parts, 1);
+    const int64_t chunks_per_part = (chunks + parts - 1) / parts;
+    parts = (chunks + chunks_per_part - 1) / chunks_per_part;
+    launch_forward<8>(a, places * parts, int(parts), int(chunks_per_part), stream);
+    if (parts > 1) {
+        if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+        const dim3 grid(groups_of(places)), block(64 * kWaves);
+        if (a.top > 0)
+            hipLaunchKernelGGL(merge_kernel<true>, grid, block, 0, stream, a, places, int(parts));
+        else
+            hipLaunchKernelGGL(merge_kernel<false>, grid, block, 0, stream, a, places, int(parts));
+    }
     return hipGetLastError();
 }
 
 hipError_t launch_token_logprobs_backward(const LogprobBackwardArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(logprobs_backward_kernel, dim3(unsigned(a.rows * a.heads)), dim3(64), 0, stream, a);
+    const int64_t places = a.rows * a.heads, chunks = (a.classes + 1023) / 1024;
+    const dim3 block(64 * kWaves);
+    if (a.classes <= 512)
+        hipLaunchKernelGGL(logprobs_backward_kernel<2>, dim3(groups_of(places)), block, 0, stream, a, places, 1);
+    else
+        hipLaunchKernelGGL(logprobs_backward_kernel<4>, dim3(groups_of(places * chunks)), block, 0, stream, a,
+                           places * chunks, int(chunks));
     return hipGetLastError();
 }
 

@@ -74,37 +74,202 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(RmsNormArgs a) {
     }
 }
 
-// d_x, one workgroup a row.
-__global__ __launch_bounds__(256) void rms_norm_grad_kernel(RmsNormBackwardArgs a) {
-    __shared__ float partial[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+// The gradients: THREADS threads a row, THREADS / 64 of a workgroup's waves; VECTORS vectors of eight values a thread, the
+// same columns in every row it takes, so that d_weight's sums stay in its registers until the workgroup's are
+// added up in LDS (in the order of its row groups) and left as its row of `partial`.
+template <int THREADS, int VECTORS, bool WEIGHT>
+__global__ __launch_bounds__(THREADS > 512 ? THREADS : 512) void rms_norm_grad_kernel(RmsNormBackwardArgs a,
+                                                                                              float* partial) {
+#pragma clang fp contract(off)
+    constexpr int kGroup = THREADS > 512 ? THREADS : 512, kRows = kGroup / THREADS, kSpan = 8 * THREADS * VECTORS;
+    __shared__ float dots[kGroup / 64];
+    __shared__ __attribute__((aligned(16))) float sums[WEIGHT && kRows > 1 ? kSpan : 4];
+    const int thread = threadIdx.x % THREADS, group = threadIdx.x / THREADS, wave = threadIdx.x >> 6;
+    float w[VECTORS][8], d_w[VECTORS][8];
+#pragma unroll
+    for (int i = 0; i < VECTORS; ++i) {
+        load8(a.weight, 8 * (thread + THREADS * i), a.width, w[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d_w[i][j] = 0.f;
+    }
+    const float by_width = 1.f / float(a.width);
+    const int64_t groups = (a.rows + kRows - 1) / kRows;
+    for (int64_t rows = blockIdx.x; rows < groups; rows += gridDim.x) {
+        // The last group's rows past the end are the last row again, without its results.
+        const int64_t row = min(rows * kRows + group, a.rows - 1);
+        const bool live = rows * kRows + group < a.rows;
         const float inverse = a.inverse[row];
-        const float *s = a.sum + row * a.width, *d_out = a.d_out + row * a.width;
+        float n[VECTORS][8], g[VECTORS][8], before[VECTORS][8];
         float dot = 0.f;
-        for (int64_t k = threadIdx.x; k < a.width; k += 256) dot += d_out[k] * a.weight[k] * (s[k] * inverse);
+#pragma unroll
+        for (int i = 0; i < VECTORS; ++i) {
+            const int64_t k = 8 * (thread + THREADS * i);
+            load8(a.sum + row * a.width, k, a.width, n[i]);
+            load8(a.d_out + row * a.width, k, a.width, g[i]);
+            if (a.d_sum != nullptr) load8(a.d_sum + row * a.width, k, a.width, before[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < VECTORS; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                n[i][j] *= inverse;
+                if (WEIGHT && live) d_w[i][j] += g[i][j] * n[i][j];
+                g[i][j] *= w[i][j];
+                dot += g[i][j] * n[i][j];
+            }
 #pragma unroll
         for (int step = 1; step < 64; step <<= 1) dot += __shfl_xor(dot, step);
-        if (lane == 0) partial[wave] = dot;
-        __syncthreads();
-        dot = ((partial[0] + partial[1]) + (partial[2] + partial[3])) / float(a.width);
-        __syncthreads();
-        for (int64_t k = threadIdx.x; k < a.width; k += 256) {
-            const float n = s[k] * inverse, g = d_out[k] * a.weight[k];
-            const float before = a.d_sum == nullptr ? 0.f : a.d_sum[row * a.width + k];
-            a.d_x[row * a.width + k] = before + inverse * (g - n * dot);
+        if constexpr (THREADS > 64) {
+            if ((threadIdx.x & 63) == 0) dots[wave] = dot;
+            __syncthreads();
+            dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < THREADS / 64; ++i) dot += dots[group * (THREADS / 64) + i];
+            __syncthreads();
+        }
+        dot *= by_width;
+        if (live) {
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i) {
+                float d_x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    d_x[j] = (a.d_sum != nullptr ? before[i][j] : 0.f) + inverse * (g[i][j] - n[i][j] * dot);
+                store8(a.d_x + row * a.width, 8 * (thread + THREADS * i), a.width, d_x);
+            }
+        }
+    }
+    if constexpr (WEIGHT) {
+        if constexpr (kRows > 1) {
+            for (int turn = 0; turn < kRows; ++turn) {
+                if (group == turn) {
+#pragma unroll
+                    for (int i = 0; i < VECTORS; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            f32x4* at = reinterpret_cast<f32x4*>(&sums[8 * (thread + THREADS * i) + 4 * h]);
+                            f32x4 v = turn == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : *at;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                v[j] += d_w[i][4 * h + j];
+                                d_w[i][4 * h + j] = v[j];
+                            }
+                            *at = v;
+                        }
+                }
+                __syncthreads();
+            }
+        }
+        if (group == kRows - 1) {
+#pragma unroll
+            for (int i = 0; i < VECTORS; ++i)
+                store8(partial + int64_t(blockIdx.x) * a.width, 8 * (thread + THREADS * i), a.width, d_w[i]);
         }
     }
 }
 
-// d_weight, one thread a column.
-__global__ __launch_bounds__(256) void rms_norm_weight_grad_kernel(RmsNormBackwardArgs a) {
-    const int64_t k = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (k >= a.width) return;
+// d_weight from `count` rows of partial sums: 64 columns a workgroup, each of its 16 waves every sixteenth row.
+__global__ __launch_bounds__(1024) void rms_norm_weight_grad_kernel(const float* partial, int64_t count, int64_t width,
+                                                                    float* d_weight) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t k = int64_t(blockIdx.x) * 64 + lane;
     float total = 0.f;
-    for (int64_t row = 0; row < a.rows; ++row)
-        total += a.d_out[row * a.width + k] * (a.sum[row * a.width + k] * a.inverse[row]);
-    a.d_weight[k] += total;
+    if (k < width) {
+#pragma unroll 8
+        for (int64_t row = wave; row < count; row += 16) total += partial[row * width + k];
+    }
+    sums[wave][lane] = total;
+    __syncthreads();
+    if (wave == 0 && k < width) {
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) total += sums[i][lane];
+        d_weight[k] += total;
+    }
+}
+
+// Rows wider than a workgroup holds: d_x, one workgroup a row, read twice.
+__global__ __launch_bounds__(512) void rms_norm_wide_grad_kernel(RmsNormBackwardArgs a) {
+    __shared__ float dots[8];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float inverse = a.inverse[row];
+        const float *s = a.sum + row * a.width, *d_out = a.d_out + row * a.width;
+        float dot = 0.f;
+        for (int64_t k = 8 * threadIdx.x; k < a.width; k += 8 * 512) {
+            float n[8], g[8], w[8];
+            load8(s, k, a.width, n);
+            load8(d_out, k, a.width, g);
+            load8(a.weight, k, a.width, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dot += g[j] * w[j] * (n[j] * inverse);
+        }
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1) dot += __shfl_xor(dot, step);
+        if ((threadIdx.x & 63) == 0) dots[threadIdx.x >> 6] = dot;
+        __syncthreads();
+        dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dot += dots[i];
+        dot *= 1.f / float(a.width);
+        __syncthreads();
+        for (int64_t k = 8 * threadIdx.x; k < a.width; k += 8 * 512) {
+            float n[8], g[8], w[8], d_x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            load8(s, k, a.width, n);
+            load8(d_out, k, a.width, g);
+            load8(a.weight, k, a.width, w);
+            if (a.d_sum != nullptr) load8(a.d_sum + row * a.width, k, a.width, d_x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d_x[j] += inverse * (g[j] * w[j] - n[j] * inverse * dot);
+            store8(a.d_x + row * a.width, k, a.width, d_x);
+        }
+    }
+}
+
+// And their d_weight, or any width's where the workspace holds no partial sums: 64 columns a workgroup, each of its 16
+// waves a sixteenth of the rows.
+__global__ __launch_bounds__(1024) void rms_norm_direct_weight_grad_kernel(RmsNormBackwardArgs a) {
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t k = int64_t(blockIdx.x) * 64 + lane;
+    float total = 0.f;
+    if (k < a.width) {
+#pragma unroll 4
+        for (int64_t row = wave; row < a.rows; row += 16)
+            total += a.d_out[row * a.width + k] * (a.sum[row * a.width + k] * a.inverse[row]);
+    }
+    sums[wave][lane] = total;
+    __syncthreads();
+    if (wave == 0 && k < a.width) {
+        total = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) total += sums[i][lane];
+        a.d_weight[k] += total;
+    }
+}
+
+template <int THREADS, int VECTORS>
+hipError_t launch_grad(const RmsNormBackwardArgs& a, hipStream_t stream) {
+    constexpr int kGroup = THREADS > 512 ? THREADS : 512, kRows = kGroup / THREADS;
+    const int64_t groups = (a.rows + kRows - 1) / kRows;
+    // Workgroups to fill the GPU with waves, four a SIMD, and no more partial sums than the workspace holds.
+    int64_t grid = std::min<int64_t>(groups, 1024 / kGroup * a.cu_count);
+    const dim3 block(kGroup);
+    if (a.d_weight == nullptr) {
+        hipLaunchKernelGGL((rms_norm_grad_kernel<THREADS, VECTORS, false>), dim3(unsigned(grid)), block, 0, stream, a, nullptr);
+        return hipGetLastError();
+    }
+    const int64_t held = int64_t(a.workspace_bytes) / (4 * a.width);
+    const dim3 columns(unsigned((a.width + 63) / 64));
+    if (held < std::min<int64_t>(grid, 64)) {  // too few to be worth it
+        hipLaunchKernelGGL(rms_norm_direct_weight_grad_kernel, columns, dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL((rms_norm_grad_kernel<THREADS, VECTORS, false>), dim3(unsigned(grid)), block, 0, stream, a, nullptr);
+        return hipGetLastError();
+    }
+    grid = std::min(grid, held);
+    hipLaunchKernelGGL((rms_norm_grad_kernel<THREADS, VECTORS, true>), dim3(unsigned(grid)), block, 0, stream, a, a.workspace);
+    hipLaunchKernelGGL(rms_norm_weight_grad_kernel, columns, dim3(1024), 0, stream, a.workspace, grid, a.width, a.d_weight);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -119,11 +284,15 @@ hipError_t launch_rms_norm(const RmsNormArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_rms_norm_backward(const RmsNormBackwardArgs& a, hipStream_t stream) {
-    if (a.d_weight != nullptr) {  // before d_x, which may be written over d_sum but over no input of this one
-        hipLaunchKernelGGL(rms_norm_weight_grad_kernel, dim3(unsigned((a.width + 255) / 256)), dim3(256), 0, stream, a);
-        if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
-    }
-    hipLaunchKernelGGL(rms_norm_grad_kernel, dim3(unsigned(std::min<int64_t>(a.rows, 1 << 20))), dim3(256), 0, stream, a);
+    if (a.width <= 512) return launch_grad<64, 1>(a, stream);
+    if (a.width <= 1024) return launch_grad<64, 2>(a, stream);
+    if (a.width <= 2048) return launch_grad<256, 1>(a, stream);
+    if (a.width <= 4096) return launch_grad<512, 1>(a, stream);
+    if (a.width <= 8192) return launch_grad<1024, 1>(a, stream);
+    if (a.width <= 16384) return launch_grad<1024, 2>(a, stream);
+    if (a.d_weight != nullptr)  // before d_x, which may be written over d_sum but over no input of this one
+        hipLaunchKernelGGL(rms_norm_direct_weight_grad_kernel, dim3(unsigned((a.width + 63) / 64)), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL(rms_norm_wide_grad_kernel, dim3(unsigned(std::min<int64_t>(a.rows, 1 << 20))), dim3(512), 0, stream, a);
     return hipGetLastError();
 }
 
