@@ -84,19 +84,224 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
             }
 }
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void* lds_pointer;
+typedef const __attribute__((address_space(1))) void* global_pointer;
+
+// Values of a tile's step along the inner dimension: half a block.
+constexpr int kStep = 64;
+
+// Waits until at most PENDING of this wave's vector-memory instructions are
+// outstanding (vmcnt; expcnt and lgkmcnt left at their maxima).
+template <int PENDING>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(PENDING >= 0 && PENDING < 64, "vmcnt is 6 bits");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (PENDING & 15) | ((PENDING >> 4) << 14));
+}
+// A barrier that leaves the loads of later steps in flight (a fence would wait for them); this wave's reads of LDS are done.
+__device__ __forceinline__ void stage_barrier() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); vmcnt and expcnt left at their maxima
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Block id -> slice and tile. Consecutive ids land on different XCDs, each with an L2 of its own: ids are regrouped so
+// that an XCD takes a contiguous range, and tiles are walked in bands of 8 tile rows.
+__device__ __forceinline__ void tile_of(int id, int count, int tiles_m, int tiles_n, int& slice, int& tile_m, int& tile_n) {
+    constexpr int kXcds = 8, kBand = 8;
+    const int xcd = id % kXcds, per = count / kXcds, more = count % kXcds;
+    const int linear = (xcd < more ? xcd * (per + 1) : more * (per + 1) + (xcd - more) * per) + id / kXcds;
+    slice = linear / (tiles_m * tiles_n);
+    const int in_slice = linear - slice * (tiles_m * tiles_n);
+    const int band = in_slice / (kBand * tiles_n), first = band * kBand, height = min(kBand, tiles_m - first);
+    const int within = in_slice - first * tiles_n;
+    tile_n = within / height;
+    tile_m = first + within - tile_n * height;
+}
+
+// Where a tile's 64-byte row pieces are in LDS: the 16-byte chunk c of row r is in slot c ^ swizzle(r), so that the
+// rows a fragment read takes at once are in different banks.
+__device__ __forceinline__ int swizzle(int row) { return ((row >> 1) ^ (row >> 3)) & 3; }
+
+// Many rows: a BM x BN tile of the output a workgroup of four waves, each a quarter of it in 32 x 32 blocks.
+template <int BM, int BN>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(ProductArgs a, int tiles_m,
+                                                                                              int tiles_n,
+                                                                                              int blocks_per_slice) {
+    constexpr int FM = BM / 64, FN = BN / 64;
+    constexpr int kLoads = (BM + BN) / 64;  // of 16 rows each, a wave
+    __shared__ __attribute__((aligned(16))) uint8_t stage0[(BM + BN) * kStep], stage1[(BM + BN) * kStep],
+        stage2[(BM + BN) * kStep];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, row = lane & 31;
+    int slice, tile_m, tile_n;
+    tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, slice, tile_m, tile_n);
+    const int64_t m0 = int64_t(tile_m) * BM, n0 = int64_t(tile_n) * BN;
+    const int64_t block0 = int64_t(slice) * blocks_per_slice;
+    const int blocks = int(min(int64_t(blocks_per_slice), a.blocks - block0));
+    const uint32_t stride = uint32_t(a.blocks * kBlock);
+    const int64_t scale_row = scale_stride(a.blocks);
+
+    // Load i of a wave brings rows 16 (4 i + wave) .. + 15 of the tile's rows, then columns: lane l the chunk that slot l %
+    // 4 of row l / 4 holds. Rows past the last are the last again.
+    const uint8_t* x = a.x + m0 * stride + block0 * kBlock;
+    const uint8_t* w = a.w + n0 * stride + block0 * kBlock;
+    const int last_m = int(min(int64_t(BM), a.rows - m0)) - 1, last_n = int(min(int64_t(BN), a.cols - n0)) - 1;
+    uint32_t from[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int r = 16 * (4 * i + wave) + lane / 4, chunk = (lane & 3) ^ swizzle(r);
+        const int source = r < BM ? min(r, last_m) : min(r - BM, last_n);
+        from[i] = uint32_t(source) * stride + 16 * chunk;
+    }
+    const int steps = 2 * blocks;
+    auto load = [&](uint8_t* stage, int step) {
+        const int k = kStep * min(step, steps - 1);  // past the end: the last step again, not used
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const bool left = 16 * 4 * i < BM;  // BM is a multiple of 64
+            __builtin_amdgcn_global_load_lds((global_pointer)((left ? x : w) + k + from[i]),
+                                             (lds_pointer)(stage + (4 * i + wave) * 16 * kStep), 16, 0, 0);
+        }
+    };
+
+    // This wave's fragments: rows of the tile, and their scale bytes.
+    const int wave_m = (wave >> 1) * (BM / 2), wave_n = (wave & 1) * (BN / 2);
+    int at[FM + FN];
+    const uint8_t* scales[FM + FN];
+#pragma unroll
+    for (int i = 0; i < FM + FN; ++i) {
+        const bool left = i < FM;
+        const int r = left ? wave_m + 32 * i + row : wave_n + 32 * (i - FM) + row;
+        const int in_stage = left ? r : BM + r;
+        at[i] = in_stage * kStep + 16 * ((2 * half) ^ swizzle(in_stage));
+        scales[i] = left ? a.x_scales + (m0 + min(r, last_m)) * scale_row + block0
+                         : a.w_scales + (n0 + min(r, last_n)) * scale_row + block0;
+    }
+    f32x16 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    float factor[FM + FN];
+    uint32_t next_scale[FM + FN];
+    // Step `step`'s products from its stage: chunk q of a lane is 16 consecutive values, of two matrix instructions.
+    auto multiply = [&](const uint8_t* stage) {
+        u32x4 codes[2][FM + FN];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int i = 0; i < FM + FN; ++i) codes[q][i] = *reinterpret_cast<const u32x4*>(stage + (at[i] ^ (16 * q)));
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                bf16x8 f[FM + FN];
+#pragma unroll
+                for (int i = 0; i < FM + FN; ++i) f[i] = fragment_of(codes[q][i][2 * h], codes[q][i][2 * h + 1], factor[i]);
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], f[FM + j], acc[i][j], 0, 0, 0);
+            }
+    };
+    // A step: its loads were started two steps ago; at the barrier every wave's have landed and every wave has read the
+    // stage before, which takes the loads of two steps ahead.
+    auto step = [&](uint8_t* stage, uint8_t* before, int t) {
+        wait_loads<kLoads>();
+        stage_barrier();
+        if ((t & 1) == 0) {
+#pragma unroll
+            for (int i = 0; i < FM + FN; ++i) {
+                factor[i] = factor_of(next_scale[i]);
+                next_scale[i] = scales[i][min((t >> 1) + 1, blocks - 1)];
+            }
+        }
+        load(before, t + 2);
+        multiply(stage);
+    };
+    if (blocks > 0) {
+#pragma unroll
+        for (int i = 0; i < FM + FN; ++i) next_scale[i] = scales[i][0];
+        load(stage0, 0);
+        load(stage1, 1);
+        int t = 0;
+        for (; t + 3 <= steps; t += 3) {
+            step(stage0, stage2, t);
+            step(stage1, stage0, t + 1);
+            step(stage2, stage1, t + 2);
+        }
+        if (t < steps) step(stage0, stage2, t);
+        if (t + 1 < steps) step(stage1, stage0, t + 1);
+        wait_loads<0>();
+    }
+    float* partial = gridDim.x > unsigned(tiles_m * tiles_n) ? a.workspace + int64_t(slice) * a.rows * a.cols : nullptr;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t y_row = m0 + wave_m + 32 * i + 8 * (r / 4) + 4 * half + r % 4;
+                const int64_t col = n0 + wave_n + 32 * j + row;
+                if (y_row >= a.rows || col >= a.cols) continue;
+                const int64_t place = y_row * a.cols + col;
+                if (partial != nullptr) {
+                    partial[place] = acc[i][j][r];
+                    continue;
+                }
+                float v = a.scale * acc[i][j][r];
+                if (a.accumulate) v = a.y[place] + v;
+                if (a.bias != nullptr) v = v + a.bias[col];
+                a.y[place] = v;
+            }
+}
+
+// The slices' sums, in order.
+__global__ __launch_bounds__(256) void slices_kernel(ProductArgs a, int slices) {
+    const int64_t count = a.rows * a.cols;
+    for (int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x; e < count; e += int64_t(gridDim.x) * 256) {
+        float total = 0.f;
+        for (int s = 0; s < slices; ++s) total += a.workspace[s * count + e];
+        float v = a.scale * total;
+        if (a.accumulate) v = a.y[e] + v;
+        if (a.bias != nullptr) v = v + a.bias[e % a.cols];
+        a.y[e] = v;
+    }
+}
+
+template <int BM, int BN>
+hipError_t launch_tiles(const ProductArgs& a, hipStream_t stream) {
+    const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN, tiles = tiles_m * tiles_n;
+    // Slices of the inner dimension until there are two workgroups a CU, of eight blocks at least.
+    int64_t slices = std::min<int64_t>({2 * a.cu_count / tiles, a.blocks / 8, 32});
+    slices = std::min<int64_t>(slices, int64_t(a.workspace_bytes / sizeof(float)) / (a.rows * a.cols));
+    slices = std::max<int64_t>(slices, 1);
+    const int64_t per_slice = (a.blocks + slices - 1) / slices;
+    slices = a.blocks == 0 ? 1 : (a.blocks + per_slice - 1) / per_slice;
+    hipLaunchKernelGGL((tile_kernel<BM, BN>), dim3(unsigned(tiles * slices)), dim3(256), 0, stream, a, int(tiles_m),
+                       int(tiles_n), int(per_slice));
+    if (slices > 1) {
+        if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+        const int64_t groups = std::min<int64_t>((a.rows * a.cols + 255) / 256, 16 * a.cu_count);
+        hipLaunchKernelGGL(slices_kernel, dim3(unsigned(groups)), dim3(256), 0, stream, a, int(slices));
+    }
+    return hipGetLastError();
+}
+
 }  // namespace
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
-    const int64_t tiles_m = (a.rows + 63) / 64, tiles_n = (a.cols + 63) / 64;
-    for (int64_t first = 0; first < tiles_m; first += 65535) {
-        ProductArgs part = a;
-        part.x += first * 64 * a.blocks * kBlock;
-        part.x_scales += first * 64 * scale_stride(a.blocks);
-        part.y += first * 64 * a.cols;
-        part.rows = std::min<int64_t>(a.rows - first * 64, 65535 * 64);
-        const dim3 grid{unsigned(tiles_n), unsigned((part.rows + 63) / 64)};
-        hipLaunchKernelGGL(product_kernel, grid, dim3(256), 0, stream, part);
+    if (a.rows > 64) {
+        if (a.rows > 512) return launch_tiles<128, 256>(a, stream);
+        return launch_tiles<64, 128>(a, stream);
     }
+    const int64_t tiles_m = (a.rows + 63) / 64, tiles_n = (a.cols + 63) / 64;
+    hipLaunchKernelGGL(product_kernel, dim3(unsigned(tiles_n), unsigned(tiles_m)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
