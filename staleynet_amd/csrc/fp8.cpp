@@ -19,7 +19,7 @@ using namespace sn::fp8;
 
 constexpr size_t kMaxDimension = size_t(1) << 31;
 constexpr size_t kMaxRows = size_t(1) << 28;   // and columns, of a product: 32-bit tile counters
-constexpr size_t kMaxInner = size_t(1) << 24;  // of a product: 256 rows of codes lie within 32-bit offsets
+constexpr size_t kMaxInner = size_t(1) << 23;  // of a product: 256 rows of codes lie within 32-bit offsets
 
 int operand_call(sn_context* ctx, bool quantize, size_t rows, size_t inner, uint32_t storage, const float* values,
                  size_t values_len, const uint8_t* codes, size_t codes_len, const uint8_t* scales,

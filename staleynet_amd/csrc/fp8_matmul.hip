@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "fp8_device.h"
 #include "fp8_internal.h"
@@ -86,7 +87,6 @@ __global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* lds_pointer;
-typedef const __attribute__((address_space(1))) void* global_pointer;
 
 // Values of a tile's step along the inner dimension: half a block.
 constexpr int kStep = 64;
@@ -116,29 +116,35 @@ __device__ __forceinline__ void tile_of(int id, int count, int tiles_m, int tile
     const int in_slice = linear - slice * (tiles_m * tiles_n);
     const int band = in_slice / (kBand * tiles_n), first = band * kBand, height = min(kBand, tiles_m - first);
     const int within = in_slice - first * tiles_n;
-    tile_n = within / height;
-    tile_m = first + within - tile_n * height;
+    // The divisions leave vector registers; what is the same in all lanes is kept in scalar ones.
+    slice = __builtin_amdgcn_readfirstlane(slice);
+    tile_n = __builtin_amdgcn_readfirstlane(within / height);
+    tile_m = __builtin_amdgcn_readfirstlane(first + within - tile_n * height);
 }
 
-// Where a tile's 64-byte row pieces are in LDS: the 16-byte chunk c of row r is in slot c ^ swizzle(r), so that the
+// Where a tile's 64-byte row pieces are in LDS: the 16-byte chunk c of row r is in slot c ^ swizzle(r), so that the 16
 // rows a fragment read takes at once are in different banks.
-__device__ __forceinline__ int swizzle(int row) { return ((row >> 1) ^ (row >> 3)) & 3; }
+__device__ __forceinline__ int swizzle(int row) { return (row >> 2) & 3; }
 
 // Many rows: a BM x BN tile of the output a workgroup of four waves, each a quarter of it in 32 x 32 blocks.
+//
+// Bound by the matrix cores, with the conversions beside them: a wave converts 24 pairs a lane for eight matrix instructions
+// of 32 cycles. A step of 64 along the inner dimension is four units of one 32x32x16 instruction a block; while a
+// unit is multiplied the next one's codes are converted and the chunk after that is read from LDS. The one barrier of a
+// step is in its middle: there every wave has read all of the step's stage, which takes the loads of three steps
+// ahead, and every wave's loads of the next stage have landed.
 template <int BM, int BN>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(ProductArgs a, int tiles_m,
-                                                                                              int tiles_n,
-                                                                                              int blocks_per_slice) {
-    constexpr int FM = BM / 64, FN = BN / 64;
+__device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m, int tiles_n, int blocks_per_slice) {
+    constexpr int FM = BM / 64, FN = BN / 64, F = FM + FN;
     constexpr int kLoads = (BM + BN) / 64;  // of 16 rows each, a wave
     __shared__ __attribute__((aligned(16))) uint8_t stage0[(BM + BN) * kStep], stage1[(BM + BN) * kStep],
         stage2[(BM + BN) * kStep];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, row = lane & 31;
+    const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int slice, tile_m, tile_n;
     tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, slice, tile_m, tile_n);
     const int64_t m0 = int64_t(tile_m) * BM, n0 = int64_t(tile_n) * BN;
-    const int64_t block0 = int64_t(slice) * blocks_per_slice;
-    const int blocks = int(min(int64_t(blocks_per_slice), a.blocks - block0));
+    const int block0 = slice * blocks_per_slice, blocks = min(blocks_per_slice, int(a.blocks) - block0);
     const uint32_t stride = uint32_t(a.blocks * kBlock);
     const int64_t scale_row = scale_stride(a.blocks);
 
@@ -155,29 +161,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         from[i] = uint32_t(source) * stride + 16 * chunk;
     }
     const int steps = 2 * blocks;
+    // Steps past the last load nothing (a buffer of no bytes), which keeps the count of loads, and so the waits, fixed.
     auto load = [&](uint8_t* stage, int step) {
-        const int k = kStep * min(step, steps - 1);  // past the end: the last step again, not used
+        const int bytes = -max(0, min(1, steps - step));  // all, or none
+        const __amdgpu_buffer_rsrc_t left = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x), 0, bytes, 0x00020000);
+        const __amdgpu_buffer_rsrc_t right = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w), 0, bytes, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const bool left = 16 * 4 * i < BM;  // BM is a multiple of 64
-            __builtin_amdgcn_global_load_lds((global_pointer)((left ? x : w) + k + from[i]),
-                                             (lds_pointer)(stage + (4 * i + wave) * 16 * kStep), 16, 0, 0);
-        }
+        for (int i = 0; i < kLoads; ++i)  // BM is a multiple of 64: a load is of rows or of columns
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(16 * 4 * i < BM ? left : right,
+                                                     (lds_pointer)(stage + (4 * i + wave) * 16 * kStep), 16, from[i],
+                                                     kStep * step, 0, 0);
     };
 
-    // This wave's fragments: rows of the tile, and their scale bytes.
+    // This wave's fragments: 32 of the tile's rows each (the swizzle is the same 32 rows on), and their scale bytes.
     const int wave_m = (wave >> 1) * (BM / 2), wave_n = (wave & 1) * (BN / 2);
-    int at[FM + FN];
-    const uint8_t* scales[FM + FN];
+    const int at_m = (wave_m + row) * kStep + 16 * ((2 * half) ^ swizzle(row));
+    const int at_n = (BM + wave_n + row) * kStep + 16 * ((2 * half) ^ swizzle(row));
+    uint32_t scales[F];
 #pragma unroll
-    for (int i = 0; i < FM + FN; ++i) {
-        const bool left = i < FM;
-        const int r = left ? wave_m + 32 * i + row : wave_n + 32 * (i - FM) + row;
-        const int in_stage = left ? r : BM + r;
-        at[i] = in_stage * kStep + 16 * ((2 * half) ^ swizzle(in_stage));
-        scales[i] = left ? a.x_scales + (m0 + min(r, last_m)) * scale_row + block0
-                         : a.w_scales + (n0 + min(r, last_n)) * scale_row + block0;
-    }
+    for (int i = 0; i < F; ++i)
+        scales[i] = uint32_t(i < FM ? min(wave_m + 32 * i + row, last_m) : min(wave_n + 32 * (i - FM) + row, last_n)) *
+                    uint32_t(scale_row);
+    const uint8_t* x_scales = a.x_scales + m0 * scale_row + block0;
+    const uint8_t* w_scales = a.w_scales + n0 * scale_row + block0;
     f32x16 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -186,57 +192,102 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    float factor[FM + FN];
-    uint32_t next_scale[FM + FN];
-    // Step `step`'s products from its stage: chunk q of a lane is 16 consecutive values, of two matrix instructions.
-    auto multiply = [&](const uint8_t* stage) {
-        u32x4 codes[2][FM + FN];
+    float factor[F];
+    uint32_t next_scale[F];
+    u32x4 chunk0[F], chunk1[F];  // 16 consecutive values of a lane, of two units: a step's first and its second half's
+    bf16x8 even[F], odd[F];      // the fragments of units 0 and 2, and of 1 and 3
+    auto read = [&](const uint8_t* stage, int q, u32x4(&chunk)[F]) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int i = 0; i < FM + FN; ++i) codes[q][i] = *reinterpret_cast<const u32x4*>(stage + (at[i] ^ (16 * q)));
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                bf16x8 f[FM + FN];
-#pragma unroll
-                for (int i = 0; i < FM + FN; ++i) f[i] = fragment_of(codes[q][i][2 * h], codes[q][i][2 * h + 1], factor[i]);
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int j = 0; j < FN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], f[FM + j], acc[i][j], 0, 0, 0);
-            }
+        for (int i = 0; i < F; ++i)
+            chunk[i] = *reinterpret_cast<const u32x4*>(
+                stage + (i < FM ? (at_m ^ (16 * q)) + 32 * kStep * i : (at_n ^ (16 * q)) + 32 * kStep * (i - FM)));
     };
-    // A step: its loads were started two steps ago; at the barrier every wave's have landed and every wave has read the
-    // stage before, which takes the loads of two steps ahead.
-    auto step = [&](uint8_t* stage, uint8_t* before, int t) {
+    auto convert = [&](const u32x4(&chunk)[F], int h, bf16x8(&f)[F]) {
+#pragma unroll
+        for (int i = 0; i < F; ++i) f[i] = fragment_of(chunk[i][2 * h], chunk[i][2 * h + 1], factor[i]);
+    };
+    auto multiply = [&](const bf16x8(&f)[F]) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], f[FM + j], acc[i][j], 0, 0, 0);
+    };
+    auto load_scales = [&](int block) {
+#pragma unroll
+        for (int i = 0; i < F; ++i) next_scale[i] = ((i < FM ? x_scales : w_scales) + min(block, blocks - 1))[scales[i]];
+    };
+    auto take_scales = [&] {
+#pragma unroll
+        for (int i = 0; i < F; ++i) factor[i] = factor_of(next_scale[i]);
+    };
+    // Spreads a unit's conversions, LDS reads and loads over its matrix instructions.
+    auto interleave = [&](auto reads, auto loads) {
+        constexpr int kProducts = FM * FN;
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, (4 * F + kProducts - 1) / kProducts, 0);
+            if (decltype(reads)::value && i < F) __builtin_amdgcn_sched_group_barrier(0x100, (F + kProducts - 1) / kProducts, 0);
+            if (decltype(loads)::value && i < kLoads) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    // Step t on its stage; `next` is the next step's. Entered with unit 0 converted and chunk 0 read.
+    auto step = [&](uint8_t* stage, const uint8_t* next, int t, auto second) {
+        __builtin_amdgcn_sched_barrier(0);
+        read(stage, 1, chunk1);
+        convert(chunk0, 1, odd);
+        multiply(even);
+        interleave(Yes{}, No{});
+        convert(chunk1, 0, even);
+        multiply(odd);
+        interleave(No{}, No{});
         wait_loads<kLoads>();
         stage_barrier();
-        if ((t & 1) == 0) {
-#pragma unroll
-            for (int i = 0; i < FM + FN; ++i) {
-                factor[i] = factor_of(next_scale[i]);
-                next_scale[i] = scales[i][min((t >> 1) + 1, blocks - 1)];
-            }
+        convert(chunk1, 1, odd);
+        if constexpr (decltype(second)::value) {  // of a block: what is converted from here on is the next one's
+            take_scales();
+            load_scales((t >> 1) + 2);
         }
-        load(before, t + 2);
-        multiply(stage);
+        load(stage, t + 3);
+        read(next, 0, chunk0);
+        multiply(even);
+        interleave(Yes{}, Yes{});
+        convert(chunk0, 0, even);
+        multiply(odd);
+        interleave(No{}, No{});
     };
     if (blocks > 0) {
-#pragma unroll
-        for (int i = 0; i < FM + FN; ++i) next_scale[i] = scales[i][0];
+        load_scales(0);
         load(stage0, 0);
         load(stage1, 1);
+        load(stage2, 2);
+        take_scales();
+        load_scales(1);
+        wait_loads<0>();
+        stage_barrier();
+        read(stage0, 0, chunk0);
+        convert(chunk0, 0, even);
         int t = 0;
-        for (; t + 3 <= steps; t += 3) {
-            step(stage0, stage2, t);
-            step(stage1, stage0, t + 1);
-            step(stage2, stage1, t + 2);
+        for (; t + 6 <= steps; t += 6) {
+            step(stage0, stage1, t, No{});
+            step(stage1, stage2, t + 1, Yes{});
+            step(stage2, stage0, t + 2, No{});
+            step(stage0, stage1, t + 3, Yes{});
+            step(stage1, stage2, t + 4, No{});
+            step(stage2, stage0, t + 5, Yes{});
         }
-        if (t < steps) step(stage0, stage2, t);
-        if (t + 1 < steps) step(stage1, stage0, t + 1);
+        if (t < steps) {  // two or four more
+            step(stage0, stage1, t, No{});
+            step(stage1, stage2, t + 1, Yes{});
+            if (t + 2 < steps) {
+                step(stage2, stage0, t + 2, No{});
+                step(stage0, stage1, t + 3, Yes{});
+            }
+        }
         wait_loads<0>();
     }
     float* partial = gridDim.x > unsigned(tiles_m * tiles_n) ? a.workspace + int64_t(slice) * a.rows * a.cols : nullptr;
@@ -259,6 +310,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                 if (a.bias != nullptr) v = v + a.bias[col];
                 a.y[place] = v;
             }
+}
+
+template <int BM, int BN>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(ProductArgs a, int tiles_m,
+                                                                                              int tiles_n,
+                                                                                              int blocks_per_slice) {
+    multiply_tile<BM, BN>(a, tiles_m, tiles_n, blocks_per_slice);
 }
 
 // The slices' sums, in order.
