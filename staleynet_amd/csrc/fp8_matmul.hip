@@ -133,10 +133,11 @@ __device__ __forceinline__ int swizzle(int row) { return (row >> 2) & 3; }
 // unit is multiplied the next one's codes are converted and the chunk after that is read from LDS. The one barrier of a
 // step is in its middle: there every wave has read all of the step's stage, which takes the loads of three steps
 // ahead, and every wave's loads of the next stage have landed.
-template <int BM, int BN>
+template <int BM, int BN, int WAVES_M, int WAVES_N>
 __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m, int tiles_n, int blocks_per_slice) {
-    constexpr int FM = BM / 64, FN = BN / 64, F = FM + FN;
-    constexpr int kLoads = (BM + BN) / 64;  // of 16 rows each, a wave
+    constexpr int kWaves = WAVES_M * WAVES_N, FM = BM / (32 * WAVES_M), FN = BN / (32 * WAVES_N), F = FM + FN;
+    constexpr int kLoads = (BM + BN) / (16 * kWaves);  // of 16 rows each, a wave
+    static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0, "a load is of rows or of columns");
     __shared__ __attribute__((aligned(16))) uint8_t stage0[(BM + BN) * kStep], stage1[(BM + BN) * kStep],
         stage2[(BM + BN) * kStep];
     const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
@@ -148,7 +149,7 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
     const uint32_t stride = uint32_t(a.blocks * kBlock);
     const int64_t scale_row = scale_stride(a.blocks);
 
-    // Load i of a wave brings rows 16 (4 i + wave) .. + 15 of the tile's rows, then columns: lane l the chunk that slot l %
+    // Load i of a wave brings rows 16 (kWaves i + wave) .. + 15 of the tile's rows, then columns: lane l the chunk that slot l %
     // 4 of row l / 4 holds. Rows past the last are the last again.
     const uint8_t* x = a.x + m0 * stride + block0 * kBlock;
     const uint8_t* w = a.w + n0 * stride + block0 * kBlock;
@@ -156,25 +157,31 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
     uint32_t from[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-        const int r = 16 * (4 * i + wave) + lane / 4, chunk = (lane & 3) ^ swizzle(r);
+        const int r = 16 * (kWaves * i + wave) + lane / 4, chunk = (lane & 3) ^ swizzle(r);
         const int source = r < BM ? min(r, last_m) : min(r - BM, last_n);
         from[i] = uint32_t(source) * stride + 16 * chunk;
     }
     const int steps = 2 * blocks;
-    // Steps past the last load nothing (a buffer of no bytes), which keeps the count of loads, and so the waits, fixed.
-    auto load = [&](uint8_t* stage, int step) {
+    // Loads FIRST to LAST of a step. Steps past the last load nothing (a buffer of no bytes), which keeps the count of
+    // loads, and so the waits, fixed.
+    auto load = [&](uint8_t* stage, int step, auto first, auto last) {
         const int bytes = -max(0, min(1, steps - step));  // all, or none
         const __amdgpu_buffer_rsrc_t left = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x), 0, bytes, 0x00020000);
         const __amdgpu_buffer_rsrc_t right = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w), 0, bytes, 0x00020000);
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i)  // BM is a multiple of 64: a load is of rows or of columns
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(16 * 4 * i < BM ? left : right,
-                                                     (lds_pointer)(stage + (4 * i + wave) * 16 * kStep), 16, from[i],
+        for (int i = decltype(first)::value; i < decltype(last)::value; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(16 * kWaves * i < BM ? left : right,
+                                                     (lds_pointer)(stage + (kWaves * i + wave) * 16 * kStep), 16, from[i],
                                                      kStep * step, 0, 0);
     };
+    using L0 = std::integral_constant<int, 0>;
+    using L1 = std::integral_constant<int, (kLoads + 3) / 4>;
+    using L2 = std::integral_constant<int, (kLoads + 1) / 2>;
+    using L3 = std::integral_constant<int, kLoads - kLoads / 4>;
+    using L4 = std::integral_constant<int, kLoads>;
 
     // This wave's fragments: 32 of the tile's rows each (the swizzle is the same 32 rows on), and their scale bytes.
-    const int wave_m = (wave >> 1) * (BM / 2), wave_n = (wave & 1) * (BN / 2);
+    const int wave_m = wave / WAVES_N * (32 * FM), wave_n = wave % WAVES_N * (32 * FN);
     const int at_m = (wave_m + row) * kStep + 16 * ((2 * half) ^ swizzle(row));
     const int at_n = (BM + wave_n + row) * kStep + 16 * ((2 * half) ^ swizzle(row));
     uint32_t scales[F];
@@ -223,28 +230,30 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
     };
     // Spreads a unit's conversions, LDS reads and loads over its matrix instructions.
     auto interleave = [&](auto reads, auto loads) {
-        constexpr int kProducts = FM * FN;
+        constexpr int kProducts = FM * FN, kLoaded = decltype(loads)::value;
 #pragma unroll
         for (int i = 0; i < kProducts; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x002, (4 * F + kProducts - 1) / kProducts, 0);
             if (decltype(reads)::value && i < F) __builtin_amdgcn_sched_group_barrier(0x100, (F + kProducts - 1) / kProducts, 0);
-            if (decltype(loads)::value && i < kLoads) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            if (i < kLoaded) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
     using Yes = std::true_type;
     using No = std::false_type;
-    // Step t on its stage; `next` is the next step's. Entered with unit 0 converted and chunk 0 read.
-    auto step = [&](uint8_t* stage, const uint8_t* next, int t, auto second) {
+    // Step t on its stage; `next` is the next step's, `before` the last's. Entered with unit 0 converted and chunk 0 read.
+    auto step = [&](uint8_t* stage, const uint8_t* next, uint8_t* before, int t, auto second) {
         __builtin_amdgcn_sched_barrier(0);
+        load(before, t + 2, L2{}, L3{});
         read(stage, 1, chunk1);
         convert(chunk0, 1, odd);
         multiply(even);
-        interleave(Yes{}, No{});
+        interleave(Yes{}, std::integral_constant<int, L3::value - L2::value>{});
+        load(before, t + 2, L3{}, L4{});
         convert(chunk1, 0, even);
         multiply(odd);
-        interleave(No{}, No{});
+        interleave(No{}, std::integral_constant<int, L4::value - L3::value>{});
         wait_loads<kLoads>();
         stage_barrier();
         convert(chunk1, 1, odd);
@@ -252,19 +261,20 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
             take_scales();
             load_scales((t >> 1) + 2);
         }
-        load(stage, t + 3);
+        load(stage, t + 3, L0{}, L1{});
         read(next, 0, chunk0);
         multiply(even);
-        interleave(Yes{}, Yes{});
+        interleave(Yes{}, L1{});
+        load(stage, t + 3, L1{}, L2{});
         convert(chunk0, 0, even);
         multiply(odd);
-        interleave(No{}, No{});
+        interleave(No{}, std::integral_constant<int, L2::value - L1::value>{});
     };
     if (blocks > 0) {
         load_scales(0);
-        load(stage0, 0);
-        load(stage1, 1);
-        load(stage2, 2);
+        load(stage0, 0, L0{}, L4{});
+        load(stage1, 1, L0{}, L4{});
+        load(stage2, 2, L0{}, L2{});
         take_scales();
         load_scales(1);
         wait_loads<0>();
@@ -273,50 +283,70 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
         convert(chunk0, 0, even);
         int t = 0;
         for (; t + 6 <= steps; t += 6) {
-            step(stage0, stage1, t, No{});
-            step(stage1, stage2, t + 1, Yes{});
-            step(stage2, stage0, t + 2, No{});
-            step(stage0, stage1, t + 3, Yes{});
-            step(stage1, stage2, t + 4, No{});
-            step(stage2, stage0, t + 5, Yes{});
+            step(stage0, stage1, stage2, t, No{});
+            step(stage1, stage2, stage0, t + 1, Yes{});
+            step(stage2, stage0, stage1, t + 2, No{});
+            step(stage0, stage1, stage2, t + 3, Yes{});
+            step(stage1, stage2, stage0, t + 4, No{});
+            step(stage2, stage0, stage1, t + 5, Yes{});
         }
         if (t < steps) {  // two or four more
-            step(stage0, stage1, t, No{});
-            step(stage1, stage2, t + 1, Yes{});
+            step(stage0, stage1, stage2, t, No{});
+            step(stage1, stage2, stage0, t + 1, Yes{});
             if (t + 2 < steps) {
-                step(stage2, stage0, t + 2, No{});
-                step(stage0, stage1, t + 3, Yes{});
+                step(stage2, stage0, stage1, t + 2, No{});
+                step(stage0, stage1, stage2, t + 3, Yes{});
             }
         }
         wait_loads<0>();
     }
-    float* partial = gridDim.x > unsigned(tiles_m * tiles_n) ? a.workspace + int64_t(slice) * a.rows * a.cols : nullptr;
+    // A buffer of each 32 rows' outputs (or of the slice's sums): places past the last row or column are out of its
+    // range, which stores nothing. A lane's sixteen values of a block are rows 8 (r / 4) + 4 half + r % 4 of one column.
+    const bool partial = gridDim.x > unsigned(tiles_m * tiles_n);
+    float* y = partial ? a.workspace + int64_t(slice) * a.rows * a.cols : a.y;
+    const uint32_t pitch = uint32_t(a.cols) * 4;
+    uint32_t place[FN];
+    float bias[FN];
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int j = 0; j < FN; ++j) {
+        const int64_t col = n0 + wave_n + 32 * j + row;
+        place[j] = col < a.cols ? uint32_t(4 * half) * pitch + uint32_t(col) * 4 : 0xffffffffu;
+        bias[j] = a.bias != nullptr && !partial && col < a.cols ? a.bias[col] : 0.f;
+    }
 #pragma unroll
-        for (int j = 0; j < FN; ++j)
+    for (int i = 0; i < FM; ++i) {
+        const int64_t first = m0 + wave_m + 32 * i;
+        const int64_t held = min(max(a.rows - first, int64_t(0)), int64_t(32));
+        const __amdgpu_buffer_rsrc_t out =
+            __builtin_amdgcn_make_buffer_rsrc(y + first * a.cols, 0, int(uint32_t(held) * pitch), 0x00020000);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            float before[16];
+            if (a.accumulate && !partial) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    before[r] = __builtin_bit_cast(
+                        float, __builtin_amdgcn_raw_buffer_load_b32(out, place[j], (8 * (r / 4) + r % 4) * pitch, 0));
+            }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int64_t y_row = m0 + wave_m + 32 * i + 8 * (r / 4) + 4 * half + r % 4;
-                const int64_t col = n0 + wave_n + 32 * j + row;
-                if (y_row >= a.rows || col >= a.cols) continue;
-                const int64_t place = y_row * a.cols + col;
-                if (partial != nullptr) {
-                    partial[place] = acc[i][j][r];
-                    continue;
+                float v = acc[i][j][r];
+                if (!partial) {
+                    v = a.scale * v;
+                    if (a.accumulate) v = before[r] + v;
+                    if (a.bias != nullptr) v = v + bias[j];
                 }
-                float v = a.scale * acc[i][j][r];
-                if (a.accumulate) v = a.y[place] + v;
-                if (a.bias != nullptr) v = v + a.bias[col];
-                a.y[place] = v;
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), out, place[j],
+                                                      (8 * (r / 4) + r % 4) * pitch, 0);
             }
+        }
+    }
 }
 
-template <int BM, int BN>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(ProductArgs a, int tiles_m,
-                                                                                              int tiles_n,
-                                                                                              int blocks_per_slice) {
-    multiply_tile<BM, BN>(a, tiles_m, tiles_n, blocks_per_slice);
+template <int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(
+    ProductArgs a, int tiles_m, int tiles_n, int blocks_per_slice) {
+    multiply_tile<BM, BN, WAVES_M, WAVES_N>(a, tiles_m, tiles_n, blocks_per_slice);
 }
 
 // The slices' sums, in order.
@@ -332,7 +362,7 @@ __global__ __launch_bounds__(256) void slices_kernel(ProductArgs a, int slices) 
     }
 }
 
-template <int BM, int BN>
+template <int BM, int BN, int WAVES_M, int WAVES_N>
 hipError_t launch_tiles(const ProductArgs& a, hipStream_t stream) {
     const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN, tiles = tiles_m * tiles_n;
     // Slices of the inner dimension until there are two workgroups a CU, of eight blocks at least.
@@ -341,7 +371,7 @@ hipError_t launch_tiles(const ProductArgs& a, hipStream_t stream) {
     slices = std::max<int64_t>(slices, 1);
     const int64_t per_slice = (a.blocks + slices - 1) / slices;
     slices = a.blocks == 0 ? 1 : (a.blocks + per_slice - 1) / per_slice;
-    hipLaunchKernelGGL((tile_kernel<BM, BN>), dim3(unsigned(tiles * slices)), dim3(256), 0, stream, a, int(tiles_m),
+    hipLaunchKernelGGL((tile_kernel<BM, BN, WAVES_M, WAVES_N>), dim3(unsigned(tiles * slices)), dim3(64 * WAVES_M * WAVES_N), 0, stream, a, int(tiles_m),
                        int(tiles_n), int(per_slice));
     if (slices > 1) {
         if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
@@ -355,8 +385,8 @@ hipError_t launch_tiles(const ProductArgs& a, hipStream_t stream) {
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
     if (a.rows > 64) {
-        if (a.rows > 512) return launch_tiles<128, 256>(a, stream);
-        return launch_tiles<64, 128>(a, stream);
+        if (a.rows > 512) return launch_tiles<128, 256, 2, 2>(a, stream);
+        return launch_tiles<64, 128, 2, 2>(a, stream);
     }
     const int64_t tiles_m = (a.rows + 63) / 64, tiles_n = (a.cols + 63) / 64;
     hipLaunchKernelGGL(product_kernel, dim3(unsigned(tiles_n), unsigned(tiles_m)), dim3(256), 0, stream, a);

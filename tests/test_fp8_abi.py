@@ -101,7 +101,7 @@ def test_product_refusals():
     for other in (spec, spec.right_transposed().left_transposed(), spec.right_transposed().causal_left(),
                   spec.right_transposed().batched(gemm.BatchStrides(2, 0, 0, 0))):
         assert product(other) == gemm.SN_ERR_UNSUPPORTED
-    for rows, cols, inner in ((1 << 28, 1, 1), (1, 1 << 28, 1), (1, 1, 1 << 23), (1 << 31, 1, 1)):
+    for rows, cols, inner in ((1 << 28, 1, 1), (1, 1 << 25, 1), (1, 1, 1 << 23), (1 << 31, 1, 1)):
         assert product(MatmulSpec.new(rows, cols, inner).right_transposed(), out=(6, 1 << 31)) == gemm.SN_ERR_OVERFLOW
     assert product(MatmulSpec.new(1, 1, (1 << 23) - 1).right_transposed()) == gemm.SN_ERR_LEFT_TOO_SMALL
     assert gemm.library().sn_matmul_fp8(None, None, *[None, 0] * 6) == gemm.SN_ERR_NULL_ARGUMENT
