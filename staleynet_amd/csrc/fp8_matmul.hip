@@ -22,67 +22,131 @@ namespace sn {
 namespace fp8 {
 namespace {
 
-// One wave a 32 x 32 tile of the output, operands read from memory as they are
-// needed. Lane l holds row l % 16 of a 16-row fragment and bytes 32 (l / 16) .. + 31
-// of a block; the four 32-deep steps of a block take eight of them each,
-// for both operands the same.
-__global__ __launch_bounds__(256) void product_kernel(ProductArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row0 = (int64_t(blockIdx.y) * 2 + wave / 2) * 32, col0 = (int64_t(blockIdx.x) * 2 + wave % 2) * 32;
-    if (row0 >= a.rows || col0 >= a.cols) return;
-    const int64_t stride = a.blocks * kBlock, scale_row = scale_stride(a.blocks);
-    f32x4 acc[2][2] = {};
-    // Rows and columns past the last read the last one's; their results are not stored.
-    const uint8_t *x[2], *x_scales[2], *w[2], *w_scales[2];
+// An output value from its sum.
+__device__ __forceinline__ void finish(const ProductArgs& a, int64_t place, int64_t col, float sum) {
+    float v = a.scale * sum;
+    if (a.accumulate) v = a.y[place] + v;
+    if (a.bias != nullptr) v = v + a.bias[col];
+    a.y[place] = v;
+}
+
+// Few rows: bound by reading the weights once. A workgroup takes 16 C columns, its waves the blocks of the inner
+// dimension in turn, so that each wave's loads are whole 128-byte lines and none is read twice; their sums are added up
+// in LDS, in the order of the waves. The columns are the left operand of the matrix instructions, up to 16 R rows of x the
+// right one. Lane l holds row (or column) l % 16 of a fragment and bytes 32 (l / 16) .. + 31 of a block; the four
+// 32-deep instructions of a block take eight of them each, for both operands the same.
+template <int R, int C>
+struct FewBlock {
+    u32x4 w[C][2], x[R][2];
+    uint32_t w_scale[C], x_scale[R];
+};
+
+// Waves of a workgroup at most: 16 while their 128 registers suffice.
+template <int R, int C>
+constexpr int few_waves() {
+    return R * C <= 2 ? 16 : 8;
+}
+template <int R, int C>
+__global__ __launch_bounds__((64 * few_waves<R, C>())) void few_rows_kernel(ProductArgs a, int slices) {
+    extern __shared__ __attribute__((aligned(16))) float sums[];  // [wave][C][R][64][4]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int64_t group = blockIdx.x / slices, col0 = group * (16 * C);
+    const int slice = blockIdx.x - int(group) * slices;
+    const int blocks = int(a.blocks), stride = waves * slices;
+    const int64_t row_bytes = a.blocks * kBlock, scale_row = scale_stride(a.blocks);
+    // Columns past the last read the last one's, rows past the last nothing (zeros); neither's results are stored.
+    const uint8_t *w[C], *w_scales[C], *x[R], *x_scales[R];
+    bool held[R];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t row = min(row0 + 16 * i + lane % 16, a.rows - 1), col = min(col0 + 16 * i + lane % 16, a.cols - 1);
-        x[i] = a.x + row * stride + 32 * (lane / 16);
-        w[i] = a.w + col * stride + 32 * (lane / 16);
-        x_scales[i] = a.x_scales + row * scale_row;
-        w_scales[i] = a.w_scales + col * scale_row;
+    for (int c = 0; c < C; ++c) {
+        const int64_t col = min(col0 + 16 * c + lane % 16, a.cols - 1);
+        w[c] = a.w + col * row_bytes + 32 * (lane / 16);
+        w_scales[c] = a.w_scales + col * scale_row;
     }
-    for (int64_t b = 0; b < a.blocks; ++b) {
-        u32x4 xc[2][2], wc[2][2];
-        float xf[2], wf[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < R; ++i) {
+        const int64_t row = 16 * i + lane % 16;
+        held[i] = row < a.rows;
+        x[i] = a.x + (held[i] ? row : 0) * row_bytes + 32 * (lane / 16);
+        x_scales[i] = a.x_scales + (held[i] ? row : 0) * scale_row;
+    }
+    auto load = [&](int b, FewBlock<R, C>& to) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                xc[i][h] = *reinterpret_cast<const u32x4*>(x[i] + b * kBlock + 16 * h);
-                wc[i][h] = *reinterpret_cast<const u32x4*>(w[i] + b * kBlock + 16 * h);
-            }
-            xf[i] = factor_of(x_scales[i][b]);
-            wf[i] = factor_of(w_scales[i][b]);
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) to.w[c][h] = *reinterpret_cast<const u32x4*>(w[c] + int64_t(b) * kBlock + 16 * h);
+            to.w_scale[c] = w_scales[c][b];
         }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            if (held[i]) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) to.x[i][h] = *reinterpret_cast<const u32x4*>(x[i] + int64_t(b) * kBlock + 16 * h);
+                to.x_scale[i] = x_scales[i][b];
+            } else {
+                to.x[i][0] = to.x[i][1] = u32x4{0, 0, 0, 0};
+                to.x_scale[i] = kLeastScale;
+            }
+    };
+    f32x4 acc[C][R];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < R; ++i) acc[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const FewBlock<R, C>& from) {
+        float wf[C], xf[R];
+#pragma unroll
+        for (int c = 0; c < C; ++c) wf[c] = factor_of(from.w_scale[c]);
+#pragma unroll
+        for (int i = 0; i < R; ++i) xf[i] = factor_of(from.x_scale[i]);
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
-            bf16x8 xb[2], wb[2];
+            const int h = step / 2, at = 2 * (step % 2);
+            bf16x8 wb[C], xb[R];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                xb[i] = fragment_of(xc[i][step / 2][2 * (step % 2)], xc[i][step / 2][2 * (step % 2) + 1], xf[i]);
-                wb[i] = fragment_of(wc[i][step / 2][2 * (step % 2)], wc[i][step / 2][2 * (step % 2) + 1], wf[i]);
-            }
+            for (int c = 0; c < C; ++c) wb[c] = fragment_of(from.w[c][h][at], from.w[c][h][at + 1], wf[c]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < R; ++i) xb[i] = fragment_of(from.x[i][h][at], from.x[i][h][at + 1], xf[i]);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[i], wb[j], acc[i][j], 0, 0, 0);
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < R; ++i)
+                    acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[c], xb[i], acc[c][i], 0, 0, 0);
         }
+    };
+    // Two blocks in registers: one arrives while the other is multiplied.
+    FewBlock<R, C> even, odd;
+    int b = slice * waves + wave;
+    if (b < blocks) load(b, even);
+    while (b < blocks) {
+        if (b + stride < blocks) load(b + stride, odd);
+        multiply(even);
+        b += stride;
+        if (b >= blocks) break;
+        if (b + stride < blocks) load(b + stride, even);
+        multiply(odd);
+        b += stride;
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t row = row0 + 16 * i + 4 * (lane / 16) + r, col = col0 + 16 * j + lane % 16;
-                if (row >= a.rows || col >= a.cols) continue;
-                float v = a.scale * acc[i][j][r];
-                if (a.accumulate) v = a.y[row * a.cols + col] + v;
-                if (a.bias != nullptr) v = v + a.bias[col];
-                a.y[row * a.cols + col] = v;
-            }
+        for (int i = 0; i < R; ++i)
+            *reinterpret_cast<f32x4*>(&sums[(((wave * C + c) * R + i) * 64 + lane) * 4]) = acc[c][i];
+    __syncthreads();
+    // A value is column 4 (l / 16) + r of its 16 and row l % 16 of its 16: consecutive threads take a row's columns.
+    constexpr int kCols = 16 * C;
+    for (int e = threadIdx.x; e < R * 16 * kCols; e += blockDim.x) {
+        const int row = e / kCols, in_group = e % kCols, c = in_group / 16, i = row / 16;
+        const int64_t col = col0 + in_group;
+        if (row >= a.rows || col >= a.cols) continue;
+        const int at = ((c * R + i) * 64 + in_group % 16 / 4 * 16 + row % 16) * 4 + in_group % 4;
+        float total = 0.f;
+        for (int v = 0; v < waves; ++v) total += sums[v * (C * R * 256) + at];
+        if (slices > 1)
+            a.workspace[(int64_t(slice) * a.rows + row) * a.cols + col] = total;
+        else
+            finish(a, row * a.cols + col, col, total);
+    }
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -133,13 +197,18 @@ __device__ __forceinline__ int swizzle(int row) { return (row >> 2) & 3; }
 // unit is multiplied the next one's codes are converted and the chunk after that is read from LDS. The one barrier of a
 // step is in its middle: there every wave has read all of the step's stage, which takes the loads of three steps
 // ahead, and every wave's loads of the next stage have landed.
-template <int BM, int BN, int WAVES_M, int WAVES_N>
+template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
 __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m, int tiles_n, int blocks_per_slice) {
     constexpr int kWaves = WAVES_M * WAVES_N, FM = BM / (32 * WAVES_M), FN = BN / (32 * WAVES_N), F = FM + FN;
     constexpr int kLoads = (BM + BN) / (16 * kWaves);  // of 16 rows each, a wave
+    constexpr int kBytes = (BM + BN) * kStep;  // of a stage
     static_assert(BM % (16 * kWaves) == 0 && BN % (16 * kWaves) == 0, "a load is of rows or of columns");
-    __shared__ __attribute__((aligned(16))) uint8_t stage0[(BM + BN) * kStep], stage1[(BM + BN) * kStep],
-        stage2[(BM + BN) * kStep];
+    static_assert(STAGES >= 3 && STAGES <= 6 && STAGES != 5, "steps in rounds of an even number of stages");
+    // An array a stage, named by constants, so that the compiler knows which stage a read of LDS may depend on.
+    __shared__ __attribute__((aligned(16))) uint8_t stage0[kBytes], stage1[kBytes], stage2[kBytes];
+    __shared__ __attribute__((aligned(16))) uint8_t stage3[STAGES > 3 ? kBytes : 16], stage4[STAGES > 4 ? kBytes : 16],
+        stage5[STAGES > 4 ? kBytes : 16];
+    uint8_t* const stages[6] = {stage0, stage1, stage2, stage3, stage4, stage5};
     const int lane = threadIdx.x & 63, half = lane >> 5, row = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int slice, tile_m, tile_n;
@@ -242,62 +311,64 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
     };
     using Yes = std::true_type;
     using No = std::false_type;
-    // Step t on its stage; `next` is the next step's, `before` the last's. Entered with unit 0 converted and chunk 0 read.
-    auto step = [&](uint8_t* stage, const uint8_t* next, uint8_t* before, int t, auto second) {
+    // Step t, on stage t % STAGES = S. Entered with unit 0 converted and chunk 0 read. SECOND: of a block.
+    auto step = [&](auto at, auto second, int t) {
+        constexpr int S = decltype(at)::value;
+        uint8_t *const stage = stages[S], *const next = stages[(S + 1) % STAGES], *const last = stages[(S + STAGES - 1) % STAGES];
         __builtin_amdgcn_sched_barrier(0);
-        load(before, t + 2, L2{}, L3{});
+        load(last, t + STAGES - 1, L2{}, L3{});
         read(stage, 1, chunk1);
         convert(chunk0, 1, odd);
         multiply(even);
         interleave(Yes{}, std::integral_constant<int, L3::value - L2::value>{});
-        load(before, t + 2, L3{}, L4{});
+        load(last, t + STAGES - 1, L3{}, L4{});
         convert(chunk1, 0, even);
         multiply(odd);
         interleave(No{}, std::integral_constant<int, L4::value - L3::value>{});
-        wait_loads<kLoads>();
+        wait_loads<kLoads * (STAGES - 2)>();
         stage_barrier();
         convert(chunk1, 1, odd);
-        if constexpr (decltype(second)::value) {  // of a block: what is converted from here on is the next one's
+        if constexpr (decltype(second)::value) {  // what is converted from here on is the next block's
             take_scales();
             load_scales((t >> 1) + 2);
         }
-        load(stage, t + 3, L0{}, L1{});
+        load(stage, t + STAGES, L0{}, L1{});
         read(next, 0, chunk0);
         multiply(even);
         interleave(Yes{}, L1{});
-        load(stage, t + 3, L1{}, L2{});
+        load(stage, t + STAGES, L1{}, L2{});
         convert(chunk0, 0, even);
         multiply(odd);
         interleave(No{}, std::integral_constant<int, L2::value - L1::value>{});
     };
+    constexpr int kRound = STAGES % 2 == 0 ? STAGES : 2 * STAGES;  // an even number of steps that ends on the last stage
+    // Two steps, a block, at a time while there are such in the round.
+    auto round = [&](int t) {
+        auto block = [&](auto pair) {
+            constexpr int P = 2 * decltype(pair)::value;
+            if constexpr (P < kRound) {
+                if (t + P < steps) {
+                    step(std::integral_constant<int, P % STAGES>{}, No{}, t + P);
+                    step(std::integral_constant<int, (P + 1) % STAGES>{}, Yes{}, t + P + 1);
+                }
+            }
+        };
+        block(std::integral_constant<int, 0>{});
+        block(std::integral_constant<int, 1>{});
+        block(std::integral_constant<int, 2>{});
+    };
     if (blocks > 0) {
         load_scales(0);
-        load(stage0, 0, L0{}, L4{});
-        load(stage1, 1, L0{}, L4{});
-        load(stage2, 2, L0{}, L2{});
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) load(stages[i], i, L0{}, L4{});
+        load(stages[STAGES - 1], STAGES - 1, L0{}, L2{});
+        wait_loads<kLoads * (STAGES - 2) + L2::value>();
         take_scales();
         load_scales(1);
-        wait_loads<0>();
         stage_barrier();
         read(stage0, 0, chunk0);
         convert(chunk0, 0, even);
-        int t = 0;
-        for (; t + 6 <= steps; t += 6) {
-            step(stage0, stage1, stage2, t, No{});
-            step(stage1, stage2, stage0, t + 1, Yes{});
-            step(stage2, stage0, stage1, t + 2, No{});
-            step(stage0, stage1, stage2, t + 3, Yes{});
-            step(stage1, stage2, stage0, t + 4, No{});
-            step(stage2, stage0, stage1, t + 5, Yes{});
-        }
-        if (t < steps) {  // two or four more
-            step(stage0, stage1, stage2, t, No{});
-            step(stage1, stage2, stage0, t + 1, Yes{});
-            if (t + 2 < steps) {
-                step(stage2, stage0, stage1, t + 2, No{});
-                step(stage0, stage1, stage2, t + 3, Yes{});
-            }
-        }
+        for (int t = 0; t < steps; t += kRound) round(t);
         wait_loads<0>();
     }
     // A buffer of each 32 rows' outputs (or of the slice's sums): places past the last row or column are out of its
@@ -343,10 +414,11 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
     }
 }
 
-template <int BM, int BN, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(
+// Waves a SIMD: two of the large tiles, whose sums take half of its registers.
+template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) __attribute__((amdgpu_waves_per_eu(BM * BN > 16384 ? 2 : 3))) void tile_kernel(
     ProductArgs a, int tiles_m, int tiles_n, int blocks_per_slice) {
-    multiply_tile<BM, BN, WAVES_M, WAVES_N>(a, tiles_m, tiles_n, blocks_per_slice);
+    multiply_tile<BM, BN, STAGES, WAVES_M, WAVES_N>(a, tiles_m, tiles_n, blocks_per_slice);
 }
 
 // The slices' sums, in order.
@@ -355,42 +427,56 @@ __global__ __launch_bounds__(256) void slices_kernel(ProductArgs a, int slices) 
     for (int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x; e < count; e += int64_t(gridDim.x) * 256) {
         float total = 0.f;
         for (int s = 0; s < slices; ++s) total += a.workspace[s * count + e];
-        float v = a.scale * total;
-        if (a.accumulate) v = a.y[e] + v;
-        if (a.bias != nullptr) v = v + a.bias[e % a.cols];
-        a.y[e] = v;
+        finish(a, e, e % a.cols, total);
     }
 }
+hipError_t launch_slices(const ProductArgs& a, int slices, hipStream_t stream) {
+    const int64_t groups = std::min<int64_t>((a.rows * a.cols + 255) / 256, 16 * a.cu_count);
+    hipLaunchKernelGGL(slices_kernel, dim3(unsigned(groups)), dim3(256), 0, stream, a, slices);
+    return hipGetLastError();
+}
+// At most as many as the workspace holds sums of.
+int64_t held_slices(const ProductArgs& a, int64_t slices) {
+    return std::max<int64_t>(1, std::min<int64_t>(slices, int64_t(a.workspace_bytes / sizeof(float)) / (a.rows * a.cols)));
+}
 
-template <int BM, int BN, int WAVES_M, int WAVES_N>
+template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
 hipError_t launch_tiles(const ProductArgs& a, hipStream_t stream) {
     const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN, tiles = tiles_m * tiles_n;
     // Slices of the inner dimension until there are two workgroups a CU, of eight blocks at least.
-    int64_t slices = std::min<int64_t>({2 * a.cu_count / tiles, a.blocks / 8, 32});
-    slices = std::min<int64_t>(slices, int64_t(a.workspace_bytes / sizeof(float)) / (a.rows * a.cols));
-    slices = std::max<int64_t>(slices, 1);
+    const int64_t slices_wanted = std::min<int64_t>({2 * int64_t(a.cu_count) / tiles, a.blocks / 8, 32});
+    int64_t slices = held_slices(a, slices_wanted);
     const int64_t per_slice = (a.blocks + slices - 1) / slices;
     slices = a.blocks == 0 ? 1 : (a.blocks + per_slice - 1) / per_slice;
-    hipLaunchKernelGGL((tile_kernel<BM, BN, WAVES_M, WAVES_N>), dim3(unsigned(tiles * slices)), dim3(64 * WAVES_M * WAVES_N), 0, stream, a, int(tiles_m),
+    hipLaunchKernelGGL((tile_kernel<BM, BN, STAGES, WAVES_M, WAVES_N>), dim3(unsigned(tiles * slices)), dim3(64 * WAVES_M * WAVES_N), 0, stream, a, int(tiles_m),
                        int(tiles_n), int(per_slice));
-    if (slices > 1) {
-        if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
-        const int64_t groups = std::min<int64_t>((a.rows * a.cols + 255) / 256, 16 * a.cu_count);
-        hipLaunchKernelGGL(slices_kernel, dim3(unsigned(groups)), dim3(256), 0, stream, a, int(slices));
-    }
-    return hipGetLastError();
+    const hipError_t err = hipGetLastError();
+    return err != hipSuccess || slices == 1 ? err : launch_slices(a, int(slices), stream);
+}
+
+template <int R, int C>
+hipError_t launch_few_rows(const ProductArgs& a, hipStream_t stream) {
+    constexpr int64_t kWaveBytes = C * R * 1024;  // of a wave's sums
+    const int64_t groups = (a.cols + 16 * C - 1) / (16 * C);
+    // Waves of a workgroup until there are 24 a CU, a block each at least.
+    int64_t waves = (24 * int64_t(a.cu_count) + groups - 1) / groups;
+    waves = std::max<int64_t>(1, std::min<int64_t>({std::max<int64_t>(waves, 4), few_waves<R, C>(), a.blocks}));
+    // Then slices of the inner dimension over workgroups until there are 8 a CU, of two blocks a wave at least.
+    const int64_t wanted = 8 * int64_t(a.cu_count) / (groups * waves);
+    const int64_t slices = held_slices(a, std::min<int64_t>({wanted, a.blocks / (2 * waves), 32}));
+    hipLaunchKernelGGL((few_rows_kernel<R, C>), dim3(unsigned(groups * slices)), dim3(unsigned(64 * waves)),
+                       unsigned(waves * kWaveBytes), stream, a, int(slices));
+    const hipError_t err = hipGetLastError();
+    return err != hipSuccess || slices == 1 ? err : launch_slices(a, int(slices), stream);
 }
 
 }  // namespace
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
-    if (a.rows > 64) {
-        if (a.rows > 512) return launch_tiles<128, 256, 2, 2>(a, stream);
-        return launch_tiles<64, 128, 2, 2>(a, stream);
-    }
-    const int64_t tiles_m = (a.rows + 63) / 64, tiles_n = (a.cols + 63) / 64;
-    hipLaunchKernelGGL(product_kernel, dim3(unsigned(tiles_n), unsigned(tiles_m)), dim3(256), 0, stream, a);
-    return hipGetLastError();
+    if (a.rows > 512) return launch_tiles<128, 256, 3, 2, 2>(a, stream);
+    if (a.rows > 16) return launch_tiles<64, 128, 4, 2, 2>(a, stream);
+    // Two 16-column fragments a wave where x would be read as often as the weights, or columns are many.
+    return a.rows > 4 || a.cols >= 16384 ? launch_few_rows<1, 2>(a, stream) : launch_few_rows<1, 1>(a, stream);
 }
 
 }  // namespace fp8
