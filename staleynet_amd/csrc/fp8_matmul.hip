@@ -416,7 +416,7 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
 
 // Waves a SIMD: two of the large tiles, whose sums take half of its registers.
 template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) __attribute__((amdgpu_waves_per_eu(BM * BN > 16384 ? 2 : 3))) void tile_kernel(
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) __attribute__((amdgpu_waves_per_eu(BM * BN > 8192 ? 2 : 3))) void tile_kernel(
     ProductArgs a, int tiles_m, int tiles_n, int blocks_per_slice) {
     multiply_tile<BM, BN, STAGES, WAVES_M, WAVES_N>(a, tiles_m, tiles_n, blocks_per_slice);
 }
@@ -443,9 +443,15 @@ int64_t held_slices(const ProductArgs& a, int64_t slices) {
 template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
 hipError_t launch_tiles(const ProductArgs& a, hipStream_t stream) {
     const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN, tiles = tiles_m * tiles_n;
-    // Slices of the inner dimension until there are two workgroups a CU, of eight blocks at least.
-    const int64_t slices_wanted = std::min<int64_t>({2 * int64_t(a.cu_count) / tiles, a.blocks / 8, 32});
-    int64_t slices = held_slices(a, slices_wanted);
+    // Slices of the inner dimension where tiles are few: a block takes about 0.8 us, the second kernel 5 us and 2 us more per
+    // million sums.
+    int64_t slices = 1;
+    double least = 0.8 * double(a.blocks);
+    const int64_t most = held_slices(a, std::min<int64_t>({3 * int64_t(a.cu_count) / tiles, a.blocks / 2, 32}));
+    for (int64_t n = 2; n <= most; ++n) {
+        const double cost = 0.8 * double((a.blocks + n - 1) / n) + 5 + 2e-6 * double(n * a.rows * a.cols);
+        if (cost < least) least = cost, slices = n;
+    }
     const int64_t per_slice = (a.blocks + slices - 1) / slices;
     slices = a.blocks == 0 ? 1 : (a.blocks + per_slice - 1) / per_slice;
     hipLaunchKernelGGL((tile_kernel<BM, BN, STAGES, WAVES_M, WAVES_N>), dim3(unsigned(tiles * slices)), dim3(64 * WAVES_M * WAVES_N), 0, stream, a, int(tiles_m),
@@ -473,10 +479,24 @@ hipError_t launch_few_rows(const ProductArgs& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
-    if (a.rows > 512) return launch_tiles<128, 256, 3, 2, 2>(a, stream);
-    if (a.rows > 16) return launch_tiles<64, 128, 4, 2, 2>(a, stream);
-    // Two 16-column fragments a wave where x would be read as often as the weights, or columns are many.
-    return a.rows > 4 || a.cols >= 16384 ? launch_few_rows<1, 2>(a, stream) : launch_few_rows<1, 1>(a, stream);
+    // Few rows: the more 16-column fragments a wave, the less often x is read beside the weights, while three workgroups for
+    // four CUs are left. Up to 64 rows of narrow outputs too, where a tile's steps one after the other take longer than
+    // reading x for every 16 columns: 60 x 1000 x 1300 (inner 1000) 5.6 us against 8.6, 64 x 8192 x 8192 58.6 against 29.5.
+    const bool wide = a.cols >= 48 * a.cu_count, narrow = a.cols < 24 * a.cu_count;
+    if (a.rows <= 16) {
+        if (wide) return launch_few_rows<1, 4>(a, stream);
+        return narrow ? launch_few_rows<1, 1>(a, stream) : launch_few_rows<1, 2>(a, stream);
+    }
+    if (a.rows <= 32) return wide ? launch_few_rows<2, 4>(a, stream) : launch_few_rows<2, 2>(a, stream);
+    if (a.rows <= 64 && narrow) return launch_few_rows<4, 1>(a, stream);
+    // The largest tile that there are two of for each CU.
+    auto fills = [&](int64_t m, int64_t n) {
+        return ((a.rows + m - 1) / m) * ((a.cols + n - 1) / n) >= 2 * a.cu_count;
+    };
+    if (fills(128, 256)) return launch_tiles<128, 256, 3, 2, 2>(a, stream);
+    if (fills(128, 128)) return launch_tiles<128, 128, 3, 2, 2>(a, stream);
+    if (fills(64, 128)) return launch_tiles<64, 128, 3, 2, 2>(a, stream);
+    return launch_tiles<64, 64, 6, 2, 2>(a, stream);
 }
 
 }  // namespace fp8
