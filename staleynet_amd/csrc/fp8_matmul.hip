@@ -342,12 +342,12 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
         interleave(No{}, std::integral_constant<int, L2::value - L1::value>{});
     };
     constexpr int kRound = STAGES % 2 == 0 ? STAGES : 2 * STAGES;  // an even number of steps that ends on the last stage
-    // Two steps, a block, at a time while there are such in the round.
-    auto round = [&](int t) {
+    // The blocks (of two steps) of a round, all of them or the `left` first.
+    auto round = [&](int t, auto whole, int left) {
         auto block = [&](auto pair) {
             constexpr int P = 2 * decltype(pair)::value;
             if constexpr (P < kRound) {
-                if (t + P < steps) {
+                if (decltype(whole)::value || P < left) {
                     step(std::integral_constant<int, P % STAGES>{}, No{}, t + P);
                     step(std::integral_constant<int, (P + 1) % STAGES>{}, Yes{}, t + P + 1);
                 }
@@ -368,7 +368,9 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
         stage_barrier();
         read(stage0, 0, chunk0);
         convert(chunk0, 0, even);
-        for (int t = 0; t < steps; t += kRound) round(t);
+        int t = 0;
+        for (; t + kRound <= steps; t += kRound) round(t, Yes{}, 0);
+        round(t, No{}, steps - t);
         wait_loads<0>();
     }
     // A buffer of each 32 rows' outputs (or of the slice's sums): places past the last row or column are out of its
