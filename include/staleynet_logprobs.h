@@ -30,7 +30,7 @@ extern "C" {
  * there are heads). Token h of a row is at row * token_stride + token_offset + h.
  * top: alternatives to list, at most 32 (SN_ERR_UNSUPPORTED otherwise, as is a
  * scale that is not positive and finite). rows * heads is under 2^31, classes
- * under 2^30 (SN_ERR_OVERFLOW). */
+ * under 2^30, rows * cols under 2^40 (SN_ERR_OVERFLOW). */
 typedef struct sn_logprob_shape {
     size_t rows;
     size_t cols;

@@ -48,20 +48,35 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float logit_of(uint32_t key) {
     return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
+constexpr uint32_t kLeastKey = 0x007fffffu;  // of -inf
 // A class with its logit, ordered by the logit and then with the lower class ahead; all are above 0 and below ~0.
 constexpr uint32_t kClassMask = 0x7fffffffu;
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t c) { return uint64_t(key) << 32 | (kClassMask - c); }
 __device__ __forceinline__ uint32_t class_of(uint64_t entry) { return kClassMask - uint32_t(entry); }
 
+// Reductions over a wave by lane moves within the vector unit (DPP: 1, 2, 4 and 8 lanes within a row of 16, then the
+// rows' last lanes to the next rows): lane 63 has the result, which a scalar register takes. A move's lanes without a
+// source keep `rest`.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ float moved(float v, float rest) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, rest), __builtin_bit_cast(int, v),
+                                                                 CONTROL, ROWS, 0xf, false));
+}
+template <class Op>
+__device__ __forceinline__ float wave_reduce(float v, float rest, Op op) {
+    v = op(v, moved<0x111, 0xf>(v, rest));
+    v = op(v, moved<0x112, 0xf>(v, rest));
+    v = op(v, moved<0x114, 0xf>(v, rest));
+    v = op(v, moved<0x118, 0xf>(v, rest));
+    v = op(v, moved<0x142, 0xa>(v, rest));
+    v = op(v, moved<0x143, 0xc>(v, rest));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int step = 1; step < 64; step <<= 1) v = v + __shfl_xor(v, step);
-    return v;
+    return wave_reduce(v, 0.f, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int step = 1; step < 64; step <<= 1) v = fmaxf(v, __shfl_xor(v, step));
-    return v;
+    return wave_reduce(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
 #pragma unroll
@@ -100,43 +115,59 @@ __device__ __forceinline__ Sums merged(Sums a, Sums b, float factor) {
     return a;
 }
 
-// The `top` largest entries of a wave's, sorted, in list[0 .. top), of which the first `held` are there already and are
-// among them; returns how many there are. N keys a lane (0: none), class(i) the class of key i; a key has to
-// be above `above`. The list has room for kListed entries.
-template <int N, class ClassOf>
-__device__ __forceinline__ int select_top(const uint32_t (&key)[N], ClassOf class_at, int top, uint64_t* list, int held,
-                                          uint32_t above) {
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
+    return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32 |
+           uint32_t(__builtin_amdgcn_readlane(int(v), lane));
+}
+
+// The `top` largest entries of a wave's values and of the `held` sorted ones in list[0 .. held), sorted, to list[0 .. top);
+// returns how many there are. again(i, c) is value i and its class once more, from memory. Lane l's value i is of class class_at(i), none from `end` on; `largest` is the lane's largest,
+// NaN aside, and `nan` says, the same in all lanes, whether there is one. Where `top` are held, a value has to be above the
+// last of them (its class is higher). The list has room for kListed entries.
+template <int N, class ClassAt, class Again>
+__device__ __forceinline__ int select_top(const float (&value)[N], ClassAt class_at, Again again, uint32_t end, float largest,
+                                          bool nan, int top, uint64_t* list, int held) {
     const int lane = threadIdx.x & 63;
-    uint32_t largest = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) largest = max(largest, key[i]);
-    if (!__any(largest > above)) return held;
-    // The bound, to 16 bits: the `top`-th largest of the lanes' maxima (0 where fewer lanes have values).
-    uint32_t bound = 0;
-#pragma unroll
-    for (uint32_t bit = 0x80000000u; bit >= 0x00010000u; bit >>= 1)
-        if (__popcll(__ballot(largest >= (bound | bit))) >= top) bound |= bit;
-    bound = max(bound, above + 1);
+    // Keys from `bound` on are candidates. At first what is above the held ones, or any (-inf's key is the least).
+    uint32_t bound = held == top ? uint32_t(__builtin_amdgcn_readfirstlane(int(list[top - 1] >> 32))) : kLeastKey - 1;
+    if (bound == 0xffffffffu) return held;  // as many NaN
+    ++bound;
     int count = held;
+    if (!nan) {
+        const uint32_t key = key_of(largest);
+        if (!__any(key >= bound)) return held;
+        // The `top`-th largest of the lanes' maxima, to 16 bits: `top` values reach it, and few more.
+        uint32_t reached = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint64_t mask = __ballot(key[i] >= bound);
-        if (mask == 0) continue;
-        const int at = count + __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
-        if (key[i] >= bound && at < kListed) list[at] = entry_of(key[i], class_at(i));
-        count += __popcll(mask);
+        for (uint32_t bit = 0x80000000u; bit >= 0x00010000u; bit >>= 1)
+            if (__popcll(__ballot(key >= (reached | bit))) >= top) reached |= bit;
+        bound = max(bound, reached);
+        const float least = logit_of(bound);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (__ballot(value[i] >= least) == 0) continue;
+            const bool candidate = value[i] >= least && class_at(i) < end;
+            const uint64_t mask = __ballot(candidate);
+            const int at = count + __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
+            if (candidate && at < kListed)  // made an entry below, once for all
+                list[at] = uint64_t(__builtin_bit_cast(uint32_t, value[i])) << 32 | class_at(i);
+            count += __popcll(mask);
+        }
+        wave_lds_order();
     }
-    wave_lds_order();
-    if (count > kListed) {
-        // One by one: the largest below the last, of the lanes' keys and of the list's first `held`.
-        uint64_t own = lane < held ? list[lane] : 0, mine = 0, last = ~uint64_t(0);
+    if (nan || count > kListed) {
+        // One by one: the largest below the last, of the lanes' values and of the list's first `held`.
+        const uint64_t own = lane < held ? list[lane] : 0;
+        uint64_t mine = 0, last = ~uint64_t(0);
         wave_lds_order();
         int found = 0;
         for (; found < top; ++found) {
             uint64_t best = own < last ? own : 0;
-#pragma unroll
+#pragma nounroll
             for (int i = 0; i < N; ++i) {
-                const uint64_t entry = key[i] > above ? entry_of(key[i], class_at(i)) : 0;
+                uint32_t c;
+                const uint32_t key = key_of(again(i, c));
+                const uint64_t entry = key >= bound && c < end ? entry_of(key, c) : 0;
                 if (entry < last && entry > best) best = entry;
             }
             last = wave_largest(best);
@@ -147,68 +178,96 @@ __device__ __forceinline__ int select_top(const uint32_t (&key)[N], ClassOf clas
         wave_lds_order();
         return found;
     }
-    // Two entries a lane find their ranks.
-    const uint64_t first = lane < count ? list[lane] : 0, second = lane + 64 < count ? list[lane + 64] : 0;
-    int rank1 = 0, rank2 = 0;
-    for (int i = 0; i < count; ++i) {
-        const uint64_t other = list[i];
-        rank1 += other > first;
-        rank2 += other > second;
+    // Each lane's entries, two at most, find their ranks.
+    const auto made = [&](int at) {
+        const uint64_t found = list[at];
+        return at < held ? found : entry_of(key_of(__builtin_bit_cast(float, uint32_t(found >> 32))), uint32_t(found));
+    };
+    const uint64_t first = lane < count ? made(lane) : 0;
+    int rank1 = 0;
+    for (int i = 0; i < min(count, 64); ++i) rank1 += lane_value(first, i) > first;
+    if (count > 64) {
+        const uint64_t second = lane + 64 < count ? made(lane + 64) : 0;
+        int rank2 = 0;
+        for (int i = 0; i < 64; ++i) rank2 += lane_value(first, i) > second;
+        for (int i = 0; i < count - 64; ++i) {
+            const uint64_t other = lane_value(second, i);
+            rank1 += other > first;
+            rank2 += other > second;
+        }
+        wave_lds_order();
+        if (lane + 64 < count && rank2 < top) list[rank2] = second;
     }
     wave_lds_order();
     if (lane < count && rank1 < top) list[rank1] = first;
-    if (lane + 64 < count && rank2 < top) list[rank2] = second;
     wave_lds_order();
     return min(count, top);
 }
 static_assert(kListed <= 128, "two entries a lane");
 
+// Where a place's head starts in the logits and its token in the tokens.
+struct Place {
+    int64_t logits, token;
+};
+template <class Args>
+__device__ __forceinline__ Place place_of(const Args& a, uint32_t place) {
+    uint32_t row = place, head = 0;
+    if (a.heads > 1) {
+        row = place / uint32_t(a.heads);
+        head = place - row * uint32_t(a.heads);
+    }
+    return Place{row * a.cols + a.column_offset + head * a.classes, row * a.token_stride + a.token_offset + head};
+}
+
 // A place's results: from its sums and its list.
-__device__ __forceinline__ void finish(const LogprobArgs& a, int64_t place, Sums s, const uint64_t* list, int found) {
+__device__ __forceinline__ void finish(const LogprobArgs& a, uint32_t place, const Place& at, Sums s, const uint64_t* list,
+                                       int found) {
 #pragma clang fp contract(off)
     const int lane = threadIdx.x & 63;
     if (!(fabsf(s.m) < INFINITY) || s.rest != s.rest) s.m = s.rest = NAN;
     const float log_total = log1pf(s.rest);
     if (lane == 0) {
         if (a.logprobs != nullptr) {
-            const int64_t row = place / a.heads, head = place - row * a.heads;
-            const uint32_t token = a.tokens[row * a.token_stride + a.token_offset + head];
+            const uint32_t token = a.tokens[at.token];
             float lp = 0.f;
             if (token != kEmptyToken) {
                 lp = NAN;
-                if (token < uint64_t(a.classes))
-                    lp = (a.logits[row * a.cols + a.column_offset + head * a.classes + token] - s.m) * a.scale - log_total;
+                if (token < uint64_t(a.classes)) lp = (a.logits[at.logits + token] - s.m) * a.scale - log_total;
             }
             a.logprobs[place] = lp;
         }
         if (a.entropies != nullptr) a.entropies[place] = log_total + s.weighted * kLn2 / (1.f + s.rest);
-        if (a.stats != nullptr) a.stats[2 * place] = s.m, a.stats[2 * place + 1] = log_total;
+        if (a.stats != nullptr) a.stats[2 * int64_t(place)] = s.m, a.stats[2 * int64_t(place) + 1] = log_total;
     }
     if (lane < a.top) {
         const bool none = lane >= found;
         const uint64_t entry = none ? 0 : list[lane];
-        if (a.top_tokens != nullptr) a.top_tokens[place * a.top + lane] = none ? kEmptyToken : class_of(entry);
+        if (a.top_tokens != nullptr) a.top_tokens[int64_t(place) * a.top + lane] = none ? kEmptyToken : class_of(entry);
         if (a.top_logprobs != nullptr)
-            a.top_logprobs[place * a.top + lane] =
+            a.top_logprobs[int64_t(place) * a.top + lane] =
                 none ? -INFINITY : (logit_of(uint32_t(entry >> 32)) - s.m) * a.scale - log_total;
     }
 }
 
-// Bytes of workspace a part leaves: its sums and its list.
-__host__ __device__ constexpr int64_t part_bytes(int top) { return 16 + 16 * int64_t((top + 1) / 2); }
+// What the parts leave in the workspace: their sums, [place][part] of four floats, then their lists, [place][part][top].
+__host__ __device__ constexpr int64_t part_bytes(int top) { return 16 + 8 * int64_t(top); }
+__device__ __forceinline__ uint64_t* lists_of(const LogprobArgs& a, int64_t parts) {
+    return reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(a.workspace) + 16 * parts);
+}
 
 // VECTORS vectors of four classes a lane; a wave an item: part `item % parts` of place `item / parts`, the chunks from
 // part * chunks_per_part on.
 template <int VECTORS, bool TOP>
-__global__ __launch_bounds__(64 * kWaves) void logprobs_kernel(LogprobArgs a, int64_t items, int parts,
-                                                               int chunks_per_part) {
+__global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))) void logprobs_kernel(LogprobArgs a, uint32_t items,
+                                                                                                       int parts, int chunks_per_part) {
     __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? kListed : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint64_t* list = lists[TOP ? wave : 0];
-    for (int64_t item = int64_t(blockIdx.x) * kWaves + wave; item < items; item += int64_t(gridDim.x) * kWaves) {
-        const int64_t place = item / parts, row = place / a.heads, head = place - row * a.heads;
-        const int part = int(item - place * parts);
-        const float* x = a.logits + row * a.cols + a.column_offset + head * a.classes;
+    for (uint32_t item = blockIdx.x * kWaves + wave; item < items; item += gridDim.x * kWaves) {
+        const uint32_t place = parts == 1 ? item : item / uint32_t(parts);
+        const int part = int(item - place * uint32_t(parts));
+        const Place at = place_of(a, place);
+        const float* x = a.logits + at.logits;
         const int64_t begin = int64_t(part) * chunks_per_part * (256 * VECTORS);
         const int64_t end = min(begin + int64_t(chunks_per_part) * (256 * VECTORS), a.classes);
         const float factor = a.scale * kLog2e;
@@ -216,10 +275,11 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_kernel(LogprobArgs a, in
         int found = 0;
         for (int64_t chunk = begin; chunk < end; chunk += 256 * VECTORS) {
             float v[4 * VECTORS];
+            const bool whole = chunk + 256 * VECTORS <= end;
 #pragma unroll
             for (int i = 0; i < VECTORS; ++i) {
                 const int64_t c = chunk + 4 * (lane + 64 * i);
-                if (c + 4 <= end) {
+                if (whole || c + 4 <= end) {
                     const f32x4 loaded = *reinterpret_cast<const f32x4_unaligned*>(x + c);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[4 * i + j] = loaded[j];
@@ -231,52 +291,67 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_kernel(LogprobArgs a, in
             Sums s = {-INFINITY, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 4 * VECTORS; ++i) s.m = fmaxf(s.m, v[i]);
+            const float largest = s.m;
             s.m = wave_max(s.m);
             // A NaN is no maximum, but its term makes `rest` NaN. Equal ones to the maximum count 1 each, without one of them.
-            int equal = 0;
+            int equal = 0;  // over the wave
 #pragma unroll
             for (int i = 0; i < 4 * VECTORS; ++i) {
                 const float z = (v[i] - s.m) * factor, e = __builtin_amdgcn_exp2f(z);
                 s.rest += v[i] == s.m ? 0.f : e;
-                equal += v[i] == s.m ? 1 : 0;
+                equal += __popcll(__ballot(v[i] == s.m));
                 s.weighted -= e > 0.f ? e * z : 0.f;
             }
             s.rest = wave_sum(s.rest);
-            if (s.m != -INFINITY) s.rest += wave_sum(float(equal)) - 1.f;
+            if (s.m != -INFINITY) s.rest += float(equal - 1);
             s.weighted = wave_sum(s.weighted);
             total = merged(total, s, factor);
             if constexpr (TOP) {
-                uint32_t key[4 * VECTORS];
-#pragma unroll
-                for (int i = 0; i < 4 * VECTORS; ++i)
-                    key[i] = chunk + 4 * (lane + 64 * (i / 4)) + i % 4 < end ? key_of(v[i]) : 0;
-                // Later chunks' classes are higher: an equal key is no candidate.
-                const uint32_t above = found == a.top ? uint32_t(list[a.top - 1] >> 32) : 0;
                 const auto class_at = [&](int i) { return uint32_t(chunk) + 4 * (lane + 64 * (i / 4)) + i % 4; };
-                found = select_top(key, class_at, a.top, list, found, above);
+                const auto again = [&](int i, uint32_t& c) {
+                    c = class_at(i);
+                    return c < uint32_t(end) ? x[c] : -INFINITY;
+                };
+                found = select_top(v, class_at, again, uint32_t(end), largest, __any(s.rest != s.rest), a.top, list, found);
             }
         }
         if (parts == 1) {
-            finish(a, place, total, list, found);
+            finish(a, place, at, total, list, found);
         } else {
-            char* out = reinterpret_cast<char*>(a.workspace) + item * part_bytes(a.top);
-            if (lane == 0) *reinterpret_cast<f32x4*>(out) = f32x4{total.m, total.rest, total.weighted, 0.f};
-            if (TOP && lane < a.top) reinterpret_cast<uint64_t*>(out + 16)[lane] = lane < found ? list[lane] : 0;
+            if (lane == 0) reinterpret_cast<f32x4*>(a.workspace)[item] = f32x4{total.m, total.rest, total.weighted, 0.f};
+            if (TOP && lane < a.top) lists_of(a, items)[int64_t(item) * a.top + lane] = lane < found ? list[lane] : 0;
         }
     }
 }
 
 // A wave a place: its parts merged, in order.
 template <bool TOP>
-__global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, int64_t places, int parts) {
+__global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, uint32_t places, int parts) {
     __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? kListed : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t place = int64_t(blockIdx.x) * kWaves + wave; place < places; place += int64_t(gridDim.x) * kWaves) {
-        const char* in = reinterpret_cast<const char*>(a.workspace) + place * parts * part_bytes(a.top);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t place = blockIdx.x * kWaves + wave; place < places; place += gridDim.x * kWaves) {
+        const f32x4* in = reinterpret_cast<const f32x4*>(a.workspace) + int64_t(place) * parts;
         const float factor = a.scale * kLog2e;
+        // The likeliest of the parts' lists: parts * top is at most kChunk. Their values as logits, NaN's too, and 0
+        // for no entry, which is no class.
+        constexpr int N = kChunk / 64;
+        float value[TOP ? N : 1], largest = -INFINITY;
+        uint32_t classes[TOP ? N : 1];
+        const uint64_t* entries = lists_of(a, int64_t(places) * parts) + int64_t(place) * parts * a.top;
+        const auto value_at = [&](int i, uint32_t& c) {
+            const int e = lane + 64 * i;
+            const uint64_t entry = e < parts * a.top ? entries[e] : 0;
+            c = entry != 0 ? class_of(entry) : ~0u;
+            return entry != 0 ? logit_of(uint32_t(entry >> 32)) : -INFINITY;
+        };
+        bool nan = false;
+        if constexpr (TOP) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) value[i] = value_at(i, classes[i]);
+        }
         Sums total = {-INFINITY, 0.f, 0.f};
         for (int p = lane; p < parts; p += 64) {
-            const f32x4 s = *reinterpret_cast<const f32x4*>(in + p * part_bytes(a.top));
+            const f32x4 s = in[p];
             total = merged(total, Sums{s[0], s[1], s[2]}, factor);
         }
 #pragma unroll
@@ -286,41 +361,36 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, int64
         total = Sums{__shfl(total.m, 0), __shfl(total.rest, 0), __shfl(total.weighted, 0)};
         int found = 0;
         if constexpr (TOP) {
-            constexpr int N = kChunk / 64;  // parts * top is at most kChunk
-            const int entries = parts * a.top;
-            uint32_t key[N], low[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int e = lane + 64 * i;
-                uint64_t entry = 0;
-                if (e < entries) {
-                    const int p = e / a.top;
-                    entry = reinterpret_cast<const uint64_t*>(in + p * part_bytes(a.top) + 16)[e - p * a.top];
-                }
-                key[i] = uint32_t(entry >> 32);
-                low[i] = class_of(entry);
+                largest = fmaxf(largest, value[i]);
+                nan |= value[i] != value[i];
             }
-            found = select_top(key, [&](int i) { return low[i]; }, a.top, lists[wave], 0, 0);
+            const auto class_at = [&](int i) { return classes[i]; };
+            const auto again = [&](int i, uint32_t& c) { return value_at(i, c); };
+            found = select_top(value, class_at, again, ~0u, largest, __any(nan), a.top, lists[wave], 0);
         }
-        finish(a, place, total, lists[TOP ? wave : 0], found);
+        finish(a, place, place_of(a, place), total, lists[TOP ? wave : 0], found);
     }
 }
 
 // VECTORS vectors of four classes a lane, a wave an item: chunk `item % chunks` of place `item / chunks`.
 template <int VECTORS>
-__global__ __launch_bounds__(64 * kWaves) void logprobs_backward_kernel(LogprobBackwardArgs a, int64_t items, int chunks) {
+__global__ __launch_bounds__(64 * kWaves) void logprobs_backward_kernel(LogprobBackwardArgs a, uint32_t items,
+                                                                        uint32_t chunks) {
 #pragma clang fp contract(off)
-    const int lane = threadIdx.x & 63;
-    for (int64_t item = int64_t(blockIdx.x) * kWaves + (threadIdx.x >> 6); item < items; item += int64_t(gridDim.x) * kWaves) {
-        const int64_t place = item / chunks, row = place / a.heads, head = place - row * a.heads;
-        const int64_t chunk = (item - place * chunks) * (256 * VECTORS);
-        const int64_t first = row * a.cols + a.column_offset + head * a.classes;
-        const float *x = a.logits + first, m = a.stats[2 * place], log_total = a.stats[2 * place + 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (uint32_t item = blockIdx.x * kWaves + wave; item < items; item += gridDim.x * kWaves) {
+        const uint32_t place = chunks == 1 ? item : item / chunks;
+        const int64_t chunk = int64_t(item - place * chunks) * (256 * VECTORS);
+        const Place at = place_of(a, place);
+        const int64_t first = at.logits;
+        const float *x = a.logits + first, m = a.stats[2 * int64_t(place)], log_total = a.stats[2 * int64_t(place) + 1];
         float* grad = a.grad + first;
         float d_logprob = 0.f, d_entropy = 0.f, entropy = 0.f;
         uint32_t token = kEmptyToken;
         if (a.d_logprobs != nullptr) {
-            token = a.tokens[row * a.token_stride + a.token_offset + head];
+            token = a.tokens[at.token];
             if (token != kEmptyToken) d_logprob = a.d_logprobs[place];
         }
         if (a.d_entropies != nullptr) d_entropy = a.d_entropies[place], entropy = a.entropies[place];
@@ -352,15 +422,17 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_backward_kernel(LogprobB
 }
 
 // Workgroups for that many waves' items, within the 2^32 threads of a launch; the kernels' waves loop over the rest.
+// Items are counted in 32 bits: at most 2^31 places, of one part where they are many, or the 1024 logits' chunks of at most
+// 2^42 logits.
 unsigned groups_of(int64_t items) { return unsigned(std::min<int64_t>((items + kWaves - 1) / kWaves, 1 << 22)); }
 
 template <int VECTORS>
 void launch_forward(const LogprobArgs& a, int64_t items, int parts, int chunks_per_part, hipStream_t stream) {
     const dim3 grid(groups_of(items)), block(64 * kWaves);
     if (a.top > 0)
-        hipLaunchKernelGGL((logprobs_kernel<VECTORS, true>), grid, block, 0, stream, a, items, parts, chunks_per_part);
+        hipLaunchKernelGGL((logprobs_kernel<VECTORS, true>), grid, block, 0, stream, a, uint32_t(items), parts, chunks_per_part);
     else
-        hipLaunchKernelGGL((logprobs_kernel<VECTORS, false>), grid, block, 0, stream, a, items, parts, chunks_per_part);
+        hipLaunchKernelGGL((logprobs_kernel<VECTORS, false>), grid, block, 0, stream, a, uint32_t(items), parts, chunks_per_part);
 }
 
 }  // namespace
@@ -378,9 +450,9 @@ hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream) {
             launch_forward<8>(a, places, 1, 1, stream);
         return hipGetLastError();
     }
-    // Parts: enough waves to fill the GPU twice over (32 a CU), as many as the merge takes and the workspace holds.
+    // Parts: enough waves to fill the GPU (32 a CU), as many as the merge takes and the workspace holds.
     const int64_t chunks = (a.classes + kChunk - 1) / kChunk;
-    int64_t parts = std::min(chunks, (64 * int64_t(a.cu_count) + places - 1) / places);
+    int64_t parts = std::min(chunks, (32 * int64_t(a.cu_count) + places - 1) / places);
     parts = std::min<int64_t>(parts, a.top > 0 ? kChunk / a.top : kChunk);
     parts = std::min<int64_t>(parts, int64_t(a.workspace_bytes) / (places * part_bytes(a.top)));
     parts = std::max<int64_t>(parts, 1);
@@ -391,9 +463,9 @@ hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream) {
         if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
         const dim3 grid(groups_of(places)), block(64 * kWaves);
         if (a.top > 0)
-            hipLaunchKernelGGL(merge_kernel<true>, grid, block, 0, stream, a, places, int(parts));
+            hipLaunchKernelGGL(merge_kernel<true>, grid, block, 0, stream, a, uint32_t(places), int(parts));
         else
-            hipLaunchKernelGGL(merge_kernel<false>, grid, block, 0, stream, a, places, int(parts));
+            hipLaunchKernelGGL(merge_kernel<false>, grid, block, 0, stream, a, uint32_t(places), int(parts));
     }
     return hipGetLastError();
 }
@@ -402,10 +474,10 @@ hipError_t launch_token_logprobs_backward(const LogprobBackwardArgs& a, hipStrea
     const int64_t places = a.rows * a.heads, chunks = (a.classes + 1023) / 1024;
     const dim3 block(64 * kWaves);
     if (a.classes <= 512)
-        hipLaunchKernelGGL(logprobs_backward_kernel<2>, dim3(groups_of(places)), block, 0, stream, a, places, 1);
+        hipLaunchKernelGGL(logprobs_backward_kernel<2>, dim3(groups_of(places)), block, 0, stream, a, uint32_t(places), 1u);
     else
         hipLaunchKernelGGL(logprobs_backward_kernel<4>, dim3(groups_of(places * chunks)), block, 0, stream, a,
-                           places * chunks, int(chunks));
+                           uint32_t(places * chunks), uint32_t(chunks));
     return hipGetLastError();
 }
 

@@ -23,6 +23,7 @@ using namespace sn::abi;
 
 constexpr size_t kMaxHeads = size_t(1) << 31;    // over the rows
 constexpr size_t kMaxClasses = size_t(1) << 30;
+constexpr size_t kMaxLogits = size_t(1) << 40;   // of a call: the kernels count chunks of them in 32 bits
 
 struct Needs {
     size_t logits, places, tokens;
@@ -33,7 +34,7 @@ int check_shape(const sn_logprob_shape* shape, bool tokens, Needs* need) {
     const sn_logprob_shape& s = *shape;
     size_t columns, end;
     if (!product(s.rows, s.cols, &need->logits) || !product(s.rows, s.heads, &need->places) ||
-        need->places >= kMaxHeads || s.classes >= kMaxClasses || !product(s.heads, s.classes, &columns) ||
+        need->logits >= kMaxLogits || need->places >= kMaxHeads || s.classes >= kMaxClasses || !product(s.heads, s.classes, &columns) ||
         !sum(columns, s.column_offset, &end))
         return SN_ERR_OVERFLOW;
     if (end > s.cols || (s.heads > 0 && s.classes == 0)) return SN_ERR_SHAPE;
