@@ -64,6 +64,7 @@ struct RmsNormArgs {
     uint8_t* scales = nullptr;
     int64_t rows = 0, width = 0;
     float epsilon = 0.f;
+    int cu_count = 256;
 };
 hipError_t launch_rms_norm(const RmsNormArgs& args, hipStream_t stream);
 

@@ -75,6 +75,7 @@ int forward(sn_context* ctx, const sn_rms_norm_shape* shape, const float* x, siz
     args.rows = int64_t(shape->rows);
     args.width = int64_t(shape->width);
     args.epsilon = shape->epsilon;
+    args.cu_count = ctx->env.cu_count;
     hipError_t err = hipSetDevice(ctx->device);
     if (err == hipSuccess) err = sn::launch_rms_norm(args, ctx->stream);
     return status(err);
