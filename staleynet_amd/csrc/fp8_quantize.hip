@@ -51,66 +51,74 @@ __global__ __launch_bounds__(kThreads) void dequantize_rows_kernel(OperandArgs a
     }
 }
 
-// Columns of a row-major source, [inner, rows]: a workgroup takes a block of 64
-// neighbouring rows of the format, a wave 32 of its 128 values of each, so that
-// loads and stores on the fp32 side are 256 contiguous bytes a wave.
+// Columns of a row-major source, [inner, rows]: a workgroup takes a block of 64 neighbouring rows of the format, a wave 32
+// of its 128 values of each, so that loads and stores on the fp32 side are 256 contiguous bytes a wave. The codes are turned
+// in LDS, so that eight lanes store a row's 128 bytes (14336 x 4096: 51 us, 5.8 TB/s, against 77 where each lane
+// stored its own 32).
+constexpr int kTurned = 128 + 16;  // bytes of a row in LDS: 16 rows' chunks are in different banks
 __global__ __launch_bounds__(kThreads) void quantize_columns_kernel(OperandArgs a) {
     __shared__ uint32_t largest[4][64];
-    const int64_t blocks = blocks_of(a.inner);
+    __shared__ __attribute__((aligned(16))) uint8_t turned[64 * kTurned];
+    const int64_t blocks = blocks_of(a.inner), row_groups = (a.rows + 63) / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = int64_t(blockIdx.x) * 64 + lane;
-    for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
-        const int64_t k0 = b * kBlock + 32 * wave;
-        const float* from = a.source + k0 * a.rows + row;
-        float v[32];
-        uint32_t magnitude = 0;
+    for (int64_t group = blockIdx.x; group < row_groups; group += gridDim.x)
+        for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
+            const int64_t row0 = group * 64, row = row0 + lane;
+            const int64_t k0 = b * kBlock + 32 * wave;
+            const float* from = a.source + k0 * a.rows + row;
+            float v[32];
+            uint32_t magnitude = 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            v[i] = row < a.rows && k0 + i < a.inner ? from[i * a.rows] : 0.f;
-            magnitude = max(magnitude, magnitude_of(v[i]));
-        }
-        largest[wave][lane] = magnitude;
-        __syncthreads();
-        magnitude = max(max(largest[0][lane], largest[1][lane]), max(largest[2][lane], largest[3][lane]));
-        __syncthreads();
-        if (row >= a.rows) continue;
-        const uint32_t s = scale_byte(magnitude);
-        u32x4 words[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-        if (s <= kLargestScale) {
+            for (int i = 0; i < 32; ++i) v[i] = row < a.rows && k0 + i < a.inner ? from[i * a.rows] : 0.f;
 #pragma unroll
-            for (int w = 0; w < 8; ++w) words[w / 4][w % 4] = codes_of(&v[4 * w], factor_of(s));
+            for (int i = 0; i < 32; ++i) magnitude = max(magnitude, magnitude_of(v[i]));
+            largest[wave][lane] = magnitude;
+            __syncthreads();
+            magnitude = max(max(largest[0][lane], largest[1][lane]), max(largest[2][lane], largest[3][lane]));
+            const uint32_t s = scale_byte(magnitude);
+            u32x4 words[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            if (s <= kLargestScale) {
+#pragma unroll
+                for (int w = 0; w < 8; ++w) words[w / 4][w % 4] = codes_of(&v[4 * w], factor_of(s));
+            }
+            u32x4* to = reinterpret_cast<u32x4*>(turned + lane * kTurned + 32 * wave);
+            to[0] = words[0];
+            to[1] = words[1];
+            __syncthreads();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = 32 * h + threadIdx.x / 8, chunk = threadIdx.x % 8;
+                if (row0 + r < a.rows)
+                    *reinterpret_cast<u32x4*>(a.codes + ((row0 + r) * blocks + b) * kBlock + 16 * chunk) =
+                        *reinterpret_cast<const u32x4*>(turned + r * kTurned + 16 * chunk);
+            }
+            if (wave == 0 && row < a.rows) {
+                uint8_t* scales = a.scales + row * scale_stride(blocks);
+                scales[b] = uint8_t(s);
+                if (b == blocks - 1)
+                    for (int64_t pad = blocks; pad < scale_stride(blocks); ++pad) scales[pad] = 0;
+            }
         }
-        u32x4* to = reinterpret_cast<u32x4*>(a.codes + (row * blocks + b) * kBlock + 32 * wave);
-        to[0] = words[0];
-        to[1] = words[1];
-        if (wave == 0) {
-            uint8_t* scales = a.scales + row * scale_stride(blocks);
-            scales[b] = uint8_t(s);
-            if (b == blocks - 1)
-                for (int64_t pad = blocks; pad < scale_stride(blocks); ++pad) scales[pad] = 0;
-        }
-    }
 }
 __global__ __launch_bounds__(kThreads) void dequantize_columns_kernel(OperandArgs a) {
-    const int64_t blocks = blocks_of(a.inner);
+    const int64_t blocks = blocks_of(a.inner), row_groups = (a.rows + 63) / 64;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = int64_t(blockIdx.x) * 64 + lane;
-    if (row >= a.rows) return;
-    for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
-        const int64_t k0 = b * kBlock + 32 * wave;
-        if (k0 >= a.inner) continue;
-        const u32x4* from = reinterpret_cast<const u32x4*>(a.codes + (row * blocks + b) * kBlock + 32 * wave);
-        const u32x4 words[2] = {from[0], from[1]};
-        const float factor = factor_of(a.scales[row * scale_stride(blocks) + b]);
-        float* to = a.output + k0 * a.rows + row;
+    for (int64_t group = blockIdx.x; group < row_groups; group += gridDim.x)
+        for (int64_t b = blockIdx.y; b < blocks; b += gridDim.y) {
+            const int64_t row = group * 64 + lane, k0 = b * kBlock + 32 * wave;
+            if (row >= a.rows || k0 >= a.inner) continue;
+            const u32x4* from = reinterpret_cast<const u32x4*>(a.codes + (row * blocks + b) * kBlock + 32 * wave);
+            const u32x4 words[2] = {from[0], from[1]};
+            const float factor = factor_of(a.scales[row * scale_stride(blocks) + b]);
+            float* to = a.output + k0 * a.rows + row;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            const f32x4 v = values_of(words[w / 4][w % 4], factor);
+            for (int w = 0; w < 8; ++w) {
+                const f32x4 v = values_of(words[w / 4][w % 4], factor);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (k0 + 4 * w + i < a.inner) to[(4 * w + i) * a.rows] = v[i];
+                for (int i = 0; i < 4; ++i)
+                    if (k0 + 4 * w + i < a.inner) to[(4 * w + i) * a.rows] = v[i];
+            }
         }
-    }
 }
 
 }  // namespace
@@ -118,7 +126,7 @@ __global__ __launch_bounds__(kThreads) void dequantize_columns_kernel(OperandArg
 hipError_t launch_operand(const OperandArgs& a, bool quantize, hipStream_t stream) {
     const int64_t blocks = blocks_of(a.inner);
     if (a.transposed) {
-        const dim3 grid(unsigned((a.rows + 63) / 64), unsigned(std::min<int64_t>(blocks, 65535)));
+        const dim3 grid(unsigned(std::min<int64_t>((a.rows + 63) / 64, 1 << 20)), unsigned(std::min<int64_t>(blocks, 256)));
         if (quantize)
             hipLaunchKernelGGL(quantize_columns_kernel, grid, dim3(kThreads), 0, stream, a);
         else
