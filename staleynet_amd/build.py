@@ -75,7 +75,7 @@ def build_oracle() -> str:
     return os.path.join(oracle_dir, "liboracle.so")
 
 
-CPP_TESTS = ["kernels_match_reference", "fp4_calls", "fp4_shapes"]
+CPP_TESTS = ["kernels_match_reference", "fp4_calls", "fp4_shapes", "fp8_calls"]
 
 
 def build_cpp_tests() -> list[str]:

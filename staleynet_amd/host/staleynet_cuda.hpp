@@ -30,6 +30,9 @@
 //   ByteBuffer, Fp4Matrix, Fp4Cache, Gpu::quantize_fp4 / dequantize_fp4 / matmul_fp4 /
 //   fp4_cache_append / fp4_cache_read / fp4_attention (4-bit weights and cache, staleynet_fp4.h; no
 //                     reference counterpart)
+//   Fp8Matrix, Gpu::quantize_fp8 / dequantize_fp8 / matmul_fp8 (8-bit operands, staleynet_fp8.h), Gpu::rms_norm /
+//   rms_norm_fp8 / rms_norm_backward (staleynet_norm.h), Gpu::token_logprobs / token_logprobs_backward
+//                     (staleynet_logprobs.h; no reference counterpart)
 // The reference panics on undersized operands; here that is a thrown
 // staleynet_cuda::Panic carrying the same message. Driver errors (the
 // reference's Err(DriverError)) are thrown as staleynet_cuda::GpuError.
@@ -44,7 +47,10 @@
 #include <vector>
 
 #include "staleynet_fp4.h"
+#include "staleynet_fp8.h"
 #include "staleynet_gemm.h"
+#include "staleynet_logprobs.h"
+#include "staleynet_norm.h"
 
 namespace staleynet_cuda {
 
@@ -234,6 +240,7 @@ class TokenBuffer {
 
     size_t len() const { return count_; }
     const uint32_t* data() const { return buffer_; }
+    uint32_t* data() { return buffer_; }
 
    private:
     void release() {
@@ -245,7 +252,7 @@ class TokenBuffer {
     size_t count_ = 0;
 };
 
-// Bytes in device memory: the codes or the scales of 4-bit blocks; owns its buffer (move-only).
+// Bytes in device memory: the codes or the scales of 4-bit or 8-bit blocks; owns its buffer (move-only).
 class ByteBuffer {
    public:
     ByteBuffer() = default;
@@ -281,6 +288,12 @@ class ByteBuffer {
 // A product's right operand [inner, cols] in 4 bits (staleynet_fp4.h).
 struct Fp4Matrix {
     size_t cols = 0, inner = 0;
+    ByteBuffer codes, scales;
+};
+
+// An operand of a product in 8 bits: `rows` rows of `inner` values (staleynet_fp8.h).
+struct Fp8Matrix {
+    size_t rows = 0, inner = 0;
     ByteBuffer codes, scales;
 };
 
@@ -583,9 +596,92 @@ class Gpu {
                                lengths ? lengths->len() : 0, out.data(), out.len()));
     }
 
+    Fp8Matrix fp8_matrix(size_t rows, size_t inner) const {
+        size_t codes = 0, scales = 0;
+        check(sn_fp8_sizes(rows, inner, &codes, &scales));
+        return Fp8Matrix{rows, inner, zeros_bytes(codes), zeros_bytes(scales)};
+    }
+
+    // An operand to 8 bits and back, stored as `storage` says: [rows, inner], or a weight's [inner, rows]
+    // (sn_quantize_fp8, sn_dequantize_fp8).
+    void quantize_fp8(const Tensor& source, Fp8Matrix& matrix, Storage storage = Storage::RowMajor) const {
+        check(sn_quantize_fp8(context_, matrix.rows, matrix.inner, abi_storage(storage), source.data(), source.len(),
+                              matrix.codes.data(), matrix.codes.len(), matrix.scales.data(), matrix.scales.len()));
+    }
+    void dequantize_fp8(const Fp8Matrix& matrix, Tensor& output, Storage storage = Storage::RowMajor) const {
+        check(sn_dequantize_fp8(context_, matrix.rows, matrix.inner, abi_storage(storage), matrix.codes.data(),
+                                matrix.codes.len(), matrix.scales.data(), matrix.scales.len(), output.data(),
+                                output.len()));
+    }
+
+    // `Gpu::matmul`, or with a bias matmul_bias, of two 8-bit operands (sn_matmul_fp8); the spec is right_transposed.
+    void matmul_fp8(const MatmulSpec& spec, const Fp8Matrix& left, const Fp8Matrix& right, Tensor& output,
+                    const Tensor* bias = nullptr) const {
+        if (left.rows != spec.rows || left.inner != spec.inner)
+            throw Panic(SN_ERR_LEFT_TOO_SMALL, "matmul_fp8: the left operand's rows and inner length are not the spec's");
+        if (right.rows != spec.cols || right.inner != spec.inner)
+            throw Panic(SN_ERR_RIGHT_TOO_SMALL, "matmul_fp8: the right operand's columns and inner length are not the spec's");
+        const sn_matmul_spec c = spec.to_ffi();
+        check(sn_matmul_fp8(context_, &c, left.codes.data(), left.codes.len(), left.scales.data(), left.scales.len(),
+                            right.codes.data(), right.codes.len(), right.scales.data(), right.scales.len(),
+                            bias ? bias->data() : nullptr, bias ? bias->len() : 0, output.data(), output.len()));
+    }
+
+    // sum = x + residual and out = its root-mean-square norm (sn_rms_norm); residual, sum and inverse may be null, and
+    // sum may be x or residual.
+    void rms_norm(const sn_rms_norm_shape& shape, const Tensor& x, const Tensor* residual, const Tensor& weight,
+                  Tensor* sum, Tensor& out, Tensor* inverse = nullptr) const {
+        check(sn_rms_norm(context_, &shape, x.data(), x.len(), data_of(residual), len_of(residual), weight.data(),
+                          weight.len(), data_of(sum), len_of(sum), out.data(), out.len(), data_of(inverse),
+                          len_of(inverse)));
+    }
+    // The same rounded to 8-bit rows (sn_rms_norm_fp8).
+    void rms_norm_fp8(const sn_rms_norm_shape& shape, const Tensor& x, const Tensor* residual, const Tensor& weight,
+                      Tensor* sum, Fp8Matrix& out) const {
+        if (out.rows != shape.rows || out.inner != shape.width)
+            throw Panic(SN_ERR_LENGTH_MISMATCH, "rms_norm_fp8: the 8-bit rows are not the shape's");
+        check(sn_rms_norm_fp8(context_, &shape, x.data(), x.len(), data_of(residual), len_of(residual), weight.data(),
+                              weight.len(), data_of(sum), len_of(sum), out.codes.data(), out.codes.len(),
+                              out.scales.data(), out.scales.len()));
+    }
+    // The norm's gradients (sn_rms_norm_backward); d_sum and d_weight may be null, and d_x may be d_sum.
+    void rms_norm_backward(const sn_rms_norm_shape& shape, const Tensor& sum, const Tensor& inverse,
+                           const Tensor& weight, const Tensor& d_out, const Tensor* d_sum, Tensor& d_x,
+                           Tensor* d_weight) const {
+        check(sn_rms_norm_backward(context_, &shape, sum.data(), sum.len(), inverse.data(), inverse.len(),
+                                   weight.data(), weight.len(), d_out.data(), d_out.len(), data_of(d_sum),
+                                   len_of(d_sum), d_x.data(), d_x.len(), data_of(d_weight), len_of(d_weight)));
+    }
+
+    // Log probabilities of tokens, entropies, the backward's stats and the likeliest classes (sn_token_logprobs), each
+    // where it is given.
+    void token_logprobs(const sn_logprob_shape& shape, const Tensor& logits, const TokenBuffer* tokens,
+                        Tensor* logprobs, Tensor* entropies, Tensor* stats, TokenBuffer* top_tokens = nullptr,
+                        Tensor* top_logprobs = nullptr) const {
+        check(sn_token_logprobs(context_, &shape, logits.data(), logits.len(), tokens ? tokens->data() : nullptr,
+                                tokens ? tokens->len() : 0, data_of(logprobs), len_of(logprobs), data_of(entropies),
+                                len_of(entropies), data_of(stats), len_of(stats),
+                                top_tokens ? top_tokens->data() : nullptr, top_tokens ? top_tokens->len() : 0,
+                                data_of(top_logprobs), len_of(top_logprobs)));
+    }
+    // The gradient of the logits (sn_token_logprobs_backward); it may be the logits themselves.
+    void token_logprobs_backward(const sn_logprob_shape& shape, const Tensor& logits, const TokenBuffer* tokens,
+                                 const Tensor& stats, const Tensor* entropies, const Tensor* d_logprobs,
+                                 const Tensor* d_entropies, Tensor& grad) const {
+        check(sn_token_logprobs_backward(context_, &shape, logits.data(), logits.len(),
+                                         tokens ? tokens->data() : nullptr, tokens ? tokens->len() : 0, stats.data(),
+                                         stats.len(), data_of(entropies), len_of(entropies), data_of(d_logprobs),
+                                         len_of(d_logprobs), data_of(d_entropies), len_of(d_entropies), grad.data(),
+                                         grad.len()));
+    }
+
     sn_context* raw() const { return context_; }
 
    private:
+    static const float* data_of(const Tensor* t) { return t ? t->data() : nullptr; }
+    static float* data_of(Tensor* t) { return t ? t->data() : nullptr; }
+    static size_t len_of(const Tensor* t) { return t ? t->len() : 0; }
+
     static uint32_t abi_storage(Storage storage) {
         return storage == Storage::Transposed ? SN_TRANSPOSED : SN_ROW_MAJOR;
     }
