@@ -136,12 +136,15 @@ __device__ __forceinline__ int select_top(const float (&value)[N], ClassAt class
     if (!nan) {
         const uint32_t key = key_of(largest);
         if (!__any(key >= bound)) return held;
-        // The `top`-th largest of the lanes' maxima, to 16 bits: `top` values reach it, and few more.
-        uint32_t reached = 0;
+        // The `top`-th largest of the lanes' maxima, to 16 bits: `top` values reach it, and few more. Not needed where
+        // few lanes have anything above the held ones.
+        if (__popcll(__ballot(key >= bound)) > kLargestTop / 2) {
+            uint32_t reached = 0;
 #pragma unroll
-        for (uint32_t bit = 0x80000000u; bit >= 0x00010000u; bit >>= 1)
-            if (__popcll(__ballot(key >= (reached | bit))) >= top) reached |= bit;
-        bound = max(bound, reached);
+            for (uint32_t bit = 0x80000000u; bit >= 0x00010000u; bit >>= 1)
+                if (__popcll(__ballot(key >= (reached | bit))) >= top) reached |= bit;
+            bound = max(bound, reached);
+        }
         const float least = logit_of(bound);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -219,23 +222,29 @@ __device__ __forceinline__ Place place_of(const Args& a, uint32_t place) {
     return Place{row * a.cols + a.column_offset + head * a.classes, row * a.token_stride + a.token_offset + head};
 }
 
+// The given token and its logit (NaN where it is no class), read ahead of what is computed meanwhile.
+struct Given {
+    uint32_t token;
+    float logit;
+};
+__device__ __forceinline__ Given given_of(const LogprobArgs& a, const Place& at) {
+    Given g = {kEmptyToken, NAN};
+    if (a.logprobs == nullptr) return g;
+    g.token = a.tokens[at.token];
+    if (g.token < uint64_t(a.classes)) g.logit = a.logits[at.logits + g.token];
+    return g;
+}
+
 // A place's results: from its sums and its list.
-__device__ __forceinline__ void finish(const LogprobArgs& a, uint32_t place, const Place& at, Sums s, const uint64_t* list,
+__device__ __forceinline__ void finish(const LogprobArgs& a, uint32_t place, const Given& given, Sums s, const uint64_t* list,
                                        int found) {
 #pragma clang fp contract(off)
     const int lane = threadIdx.x & 63;
     if (!(fabsf(s.m) < INFINITY) || s.rest != s.rest) s.m = s.rest = NAN;
     const float log_total = log1pf(s.rest);
     if (lane == 0) {
-        if (a.logprobs != nullptr) {
-            const uint32_t token = a.tokens[at.token];
-            float lp = 0.f;
-            if (token != kEmptyToken) {
-                lp = NAN;
-                if (token < uint64_t(a.classes)) lp = (a.logits[at.logits + token] - s.m) * a.scale - log_total;
-            }
-            a.logprobs[place] = lp;
-        }
+        if (a.logprobs != nullptr)
+            a.logprobs[place] = given.token == kEmptyToken ? 0.f : (given.logit - s.m) * a.scale - log_total;
         if (a.entropies != nullptr) a.entropies[place] = log_total + s.weighted * kLn2 / (1.f + s.rest);
         if (a.stats != nullptr) a.stats[2 * int64_t(place)] = s.m, a.stats[2 * int64_t(place) + 1] = log_total;
     }
@@ -268,6 +277,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
         const int part = int(item - place * uint32_t(parts));
         const Place at = place_of(a, place);
         const float* x = a.logits + at.logits;
+        const Given given = parts == 1 ? given_of(a, at) : Given{};
         const int64_t begin = int64_t(part) * chunks_per_part * (256 * VECTORS);
         const int64_t end = min(begin + int64_t(chunks_per_part) * (256 * VECTORS), a.classes);
         const float factor = a.scale * kLog2e;
@@ -316,7 +326,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
             }
         }
         if (parts == 1) {
-            finish(a, place, at, total, list, found);
+            finish(a, place, given, total, list, found);
         } else {
             if (lane == 0) reinterpret_cast<f32x4*>(a.workspace)[item] = f32x4{total.m, total.rest, total.weighted, 0.f};
             if (TOP && lane < a.top) lists_of(a, items)[int64_t(item) * a.top + lane] = lane < found ? list[lane] : 0;
@@ -331,6 +341,7 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, uint3
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (uint32_t place = blockIdx.x * kWaves + wave; place < places; place += gridDim.x * kWaves) {
         const f32x4* in = reinterpret_cast<const f32x4*>(a.workspace) + int64_t(place) * parts;
+        const Given given = given_of(a, place_of(a, place));
         const float factor = a.scale * kLog2e;
         // The likeliest of the parts' lists: parts * top is at most kChunk. Their values as logits, NaN's too, and 0
         // for no entry, which is no class.
@@ -370,7 +381,7 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, uint3
             const auto again = [&](int i, uint32_t& c) { return value_at(i, c); };
             found = select_top(value, class_at, again, ~0u, largest, __any(nan), a.top, lists[wave], 0);
         }
-        finish(a, place, place_of(a, place), total, lists[TOP ? wave : 0], found);
+        finish(a, place, given, total, lists[TOP ? wave : 0], found);
     }
 }
 
