@@ -66,8 +66,11 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void rms_norm_kernel
     __shared__ double partial[kGroup / 64];
     const int thread = threadIdx.x % THREADS, group = threadIdx.x / THREADS;
     for (int64_t rows = blockIdx.x; rows * kRows < a.rows; rows += gridDim.x) {
-        // Rows past the last are the last again, with the same results.
-        const int64_t row = min(rows * kRows + group, a.rows - 1);
+        // Waves past the last row leave (they are rows of their own, and meet no barrier): the sum may be written over x, so
+        // that no row is anyone else's to read.
+        const int64_t row = rows * kRows + group;
+        static_assert(kRows == 1 || THREADS == 64, "a wave that leaves skips the barriers");
+        if (kRows > 1 && row >= a.rows) break;
         float s[VECTORS][8];
 #pragma unroll
         for (int i = 0; i < VECTORS; ++i) load_sum(a, row, 8 * (thread + THREADS * i), s[i]);

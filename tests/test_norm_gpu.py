@@ -111,6 +111,20 @@ def test_the_stream_updated_in_place(gpu, width, onto):
     assert np.array_equal(gpu.download_bytes(matrix.codes).reshape(6, -1), ref.quantize(fetch(gpu, y, s.shape))[0])
 
 
+@pytest.mark.parametrize("rows,width", [(1, 64), (1, 512), (3, 200), (1027, 512), (1025, 1000), (4099, 768)])
+def test_rows_updated_in_place_are_read_once(gpu, rows, width):
+    """Fewer rows than the workgroups' waves are for: none is read again after its sum was written over it."""
+    x, residual, weight = inputs(rows, width, rows)
+    rt, wt, y = place(gpu, residual), place(gpu, weight), place(gpu, np.zeros(x.size))
+    s, xt = x, place(gpu, x)
+    for _ in range(24):
+        gpu.rms_norm(xt, wt, y, EPSILON, rows, rt, xt)
+        s = s + residual
+    assert np.array_equal(fetch(gpu, xt, s.shape), s)
+    want, _ = expected(s, weight)
+    assert (np.abs(fetch(gpu, y, s.shape) - want) <= (U + 2.0 ** -40) * np.abs(want) + 2.0 ** -150).all()
+
+
 @pytest.mark.parametrize("width", [130, 3000, 50000])
 def test_values_at_the_edges(gpu, width):
     """Rows of zeros, of subnormals, of the largest floats; NaN and infinities stay in their row."""
