@@ -13,7 +13,7 @@
  *   y = weight * s * i                     (computed in 64 bits, rounded once)
  * NaN and infinities follow IEEE arithmetic, and stay in their row. Rows are
  * dense, [rows, width]. epsilon is at least 0 and finite (SN_ERR_UNSUPPORTED
- * otherwise). Limits, past which a call is SN_ERR_OVERFLOW: rows under 2^31,
+ * otherwise). Nothing is written where rows or width is 0. Limits, past which a call is SN_ERR_OVERFLOW: rows under 2^31,
  * width under 2^25. Lengths count elements of their buffer (too short:
  * SN_ERR_LENGTH_MISMATCH). The calls are asynchronous on the context's stream,
  * allocate nothing, may be captured into a graph, and are deterministic.

@@ -19,7 +19,7 @@ using namespace sn::fp8;
 
 constexpr size_t kMaxDimension = size_t(1) << 31;
 constexpr size_t kMaxRows = size_t(1) << 28;   // of a product: 32-bit tile counters
-constexpr size_t kMaxCols = size_t(1) << 25;   // of a product: 32 rows of outputs lie within 32-bit offsets
+constexpr size_t kMaxCols = size_t(1) << 24;   // of a product: 32 rows of outputs are less than 2^31 bytes
 constexpr size_t kMaxInner = size_t(1) << 23;  // of a product: 256 rows of codes lie within 32-bit offsets
 
 int operand_call(sn_context* ctx, bool quantize, size_t rows, size_t inner, uint32_t storage, const float* values,
@@ -128,8 +128,6 @@ int sn_matmul_fp8(sn_context* ctx, const sn_matmul_spec* spec, const uint8_t* le
     args.accumulate = spec->write == SN_ACCUMULATE;
     args.workspace = ctx->env.workspace;
     args.workspace_bytes = ctx->env.workspace_bytes;
-    args.counters = ctx->env.counters;
-    args.counter_count = ctx->env.counter_count;
     args.cu_count = ctx->env.cu_count;
     hipError_t err = hipSetDevice(ctx->device);
     if (err == hipSuccess) err = launch_product(args, ctx->stream);

@@ -44,8 +44,6 @@ struct ProductArgs {
     bool accumulate = false;
     float* workspace = nullptr;
     size_t workspace_bytes = 0;
-    uint32_t* counters = nullptr;  // zero between calls
-    size_t counter_count = 0;
     int cu_count = 256;
 };
 hipError_t launch_product(const ProductArgs& args, hipStream_t stream);

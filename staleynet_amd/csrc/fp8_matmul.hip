@@ -373,8 +373,8 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
         round(t, No{}, steps - t);
         wait_loads<0>();
     }
-    // A buffer of each 32 rows' outputs (or of the slice's sums): places past the last row or column are out of its
-    // range, which stores nothing. A lane's sixteen values of a block are rows 8 (r / 4) + 4 half + r % 4 of one column.
+    // A buffer of each 32 rows' outputs (or of the slice's sums), of less than 2^31 bytes: places past the last row are out
+    // of its range, and so is 2^31 with any row's offset, for columns past the last; such stores do nothing. A lane's sixteen values of a block are rows 8 (r / 4) + 4 half + r % 4 of one column.
     const bool partial = gridDim.x > unsigned(tiles_m * tiles_n);
     float* y = partial ? a.workspace + int64_t(slice) * a.rows * a.cols : a.y;
     const uint32_t pitch = uint32_t(a.cols) * 4;
@@ -383,7 +383,7 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
         const int64_t col = n0 + wave_n + 32 * j + row;
-        place[j] = col < a.cols ? uint32_t(4 * half) * pitch + uint32_t(col) * 4 : 0xffffffffu;
+        place[j] = col < a.cols ? uint32_t(4 * half) * pitch + uint32_t(col) * 4 : 0x80000000u;
         bias[j] = a.bias != nullptr && !partial && col < a.cols ? a.bias[col] : 0.f;
     }
 #pragma unroll

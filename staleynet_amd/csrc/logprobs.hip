@@ -21,6 +21,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 
@@ -94,6 +95,8 @@ __device__ __forceinline__ void wave_lds_order() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
+// a log2 e, finite: at 0 differences it gives 0.
+__device__ __forceinline__ float factor_of(float scale) { return fminf(scale * kLog2e, FLT_MAX); }
 // The largest logit of some classes, the sum of the others' e^z and W over them, in units of log2 e.
 struct Sums {
     float m, rest, weighted;
@@ -280,7 +283,7 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
         const Given given = parts == 1 ? given_of(a, at) : Given{};
         const int64_t begin = int64_t(part) * chunks_per_part * (256 * VECTORS);
         const int64_t end = min(begin + int64_t(chunks_per_part) * (256 * VECTORS), a.classes);
-        const float factor = a.scale * kLog2e;
+        const float factor = factor_of(a.scale);
         Sums total = {-INFINITY, 0.f, 0.f};
         int found = 0;
         for (int64_t chunk = begin; chunk < end; chunk += 256 * VECTORS) {
@@ -342,7 +345,7 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, uint3
     for (uint32_t place = blockIdx.x * kWaves + wave; place < places; place += gridDim.x * kWaves) {
         const f32x4* in = reinterpret_cast<const f32x4*>(a.workspace) + int64_t(place) * parts;
         const Given given = given_of(a, place_of(a, place));
-        const float factor = a.scale * kLog2e;
+        const float factor = factor_of(a.scale);
         // The likeliest of the parts' lists: parts * top is at most kChunk. Their values as logits, NaN's too, and 0
         // for no entry, which is no class.
         constexpr int N = kChunk / 64;

@@ -105,6 +105,8 @@ def test_product_refusals():
         assert product(MatmulSpec.new(rows, cols, inner).right_transposed(), out=(6, 1 << 31)) == gemm.SN_ERR_OVERFLOW
     assert product(MatmulSpec.new(1, 1, (1 << 23) - 1).right_transposed()) == gemm.SN_ERR_LEFT_TOO_SMALL
     assert gemm.library().sn_matmul_fp8(None, None, *[None, 0] * 6) == gemm.SN_ERR_NULL_ARGUMENT
+    assert product(MatmulSpec.new(1, 1 << 24, 1).right_transposed(), out=(6, 1 << 24)) == gemm.SN_ERR_OVERFLOW
+    assert product(MatmulSpec.new(1, (1 << 24) - 1, 1).right_transposed(), out=(6, 1 << 24)) == gemm.SN_ERR_RIGHT_TOO_SMALL
 
 
 def test_norm_refusals():
@@ -164,7 +166,7 @@ def test_logprob_refusals(function, sizes):
     assert logprobs(dict(top=33)) == gemm.SN_ERR_UNSUPPORTED
     for scale in (0.0, -1.0, float("nan"), float("inf")):
         assert logprobs(dict(scale=scale)) == gemm.SN_ERR_UNSUPPORTED
-    for shape in (dict(rows=1 << 31), dict(classes=1 << 30), dict(rows=1 << 40, cols=1 << 40),
+    for shape in (dict(rows=1 << 31), dict(classes=1 << 30), dict(rows=1 << 40, cols=1 << 40), dict(rows=1 << 20, cols=1 << 20),
                   dict(token_stride=1 << 60), dict(column_offset=(1 << 64) - 1)):
         assert logprobs(shape) == gemm.SN_ERR_OVERFLOW
     assert gemm.library().sn_token_logprobs(None, None, *[None, 0] * 7) == gemm.SN_ERR_NULL_ARGUMENT

@@ -132,6 +132,15 @@ def test_forward(gpu, rows, heads, classes, top):
     assert all(np.array_equal(got[n], again[n]) for n in got)
 
 
+@pytest.mark.parametrize("scale", [3.3e38, 1e-40])
+@pytest.mark.parametrize("rows,heads,classes", [(3, 2, 50), (4, 1, 3000), (2, 1, 40000)])
+def test_scales_at_the_ends(gpu, rows, heads, classes, scale):
+    """The largest logit, which several classes have, has log probability -log of their number; or all are alike."""
+    case = Case(rows, heads, classes, scale=scale, seed=classes)
+    case.logits = np.minimum(np.rint(case.logits), 4).astype(np.float32)
+    case.check(case.forward(gpu, 9), 9)
+
+
 @pytest.mark.parametrize("rows,heads,classes", [(3, 2, 50), (4, 1, 3000), (2, 1, 40000)])
 def test_any_of_the_outputs(gpu, rows, heads, classes):
     case = Case(rows, heads, classes, seed=1, stride=heads + 3, token_offset=2)
