@@ -123,72 +123,11 @@ __device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
            uint32_t(__builtin_amdgcn_readlane(int(v), lane));
 }
 
-// The `top` largest entries of a wave's values and of the `held` sorted ones in list[0 .. held), sorted, to list[0 .. top);
-// returns how many there are. again(i, c) is value i and its class once more, from memory. Lane l's value i is of class class_at(i), none from `end` on; `largest` is the lane's largest,
-// NaN aside, and `nan` says, the same in all lanes, whether there is one. Where `top` are held, a value has to be above the
-// last of them (its class is higher). The list has room for kListed entries.
-template <int N, class ClassAt, class Again>
-__device__ __forceinline__ int select_top(const float (&value)[N], ClassAt class_at, Again again, uint32_t end, float largest,
-                                          bool nan, int top, uint64_t* list, int held) {
+// The `top` largest of `count` entries, at most kListed, made(0) .. made(count - 1) from the list, sorted to the list's
+// start: each lane's entries, two at most, find their ranks. Returns how many there are.
+template <class Made>
+__device__ __forceinline__ int rank_entries(uint64_t* list, int count, int top, Made made) {
     const int lane = threadIdx.x & 63;
-    // Keys from `bound` on are candidates. At first what is above the held ones, or any (-inf's key is the least).
-    uint32_t bound = held == top ? uint32_t(__builtin_amdgcn_readfirstlane(int(list[top - 1] >> 32))) : kLeastKey - 1;
-    if (bound == 0xffffffffu) return held;  // as many NaN
-    ++bound;
-    int count = held;
-    if (!nan) {
-        const uint32_t key = key_of(largest);
-        if (!__any(key >= bound)) return held;
-        // The `top`-th largest of the lanes' maxima, to 16 bits: `top` values reach it, and few more. Not needed where
-        // few lanes have anything above the held ones.
-        if (__popcll(__ballot(key >= bound)) > kLargestTop / 2) {
-            uint32_t reached = 0;
-#pragma unroll
-            for (uint32_t bit = 0x80000000u; bit >= 0x00010000u; bit >>= 1)
-                if (__popcll(__ballot(key >= (reached | bit))) >= top) reached |= bit;
-            bound = max(bound, reached);
-        }
-        const float least = logit_of(bound);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (__ballot(value[i] >= least) == 0) continue;
-            const bool candidate = value[i] >= least && class_at(i) < end;
-            const uint64_t mask = __ballot(candidate);
-            const int at = count + __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
-            if (candidate && at < kListed)  // made an entry below, once for all
-                list[at] = uint64_t(__builtin_bit_cast(uint32_t, value[i])) << 32 | class_at(i);
-            count += __popcll(mask);
-        }
-        wave_lds_order();
-    }
-    if (nan || count > kListed) {
-        // One by one: the largest below the last, of the lanes' values and of the list's first `held`.
-        const uint64_t own = lane < held ? list[lane] : 0;
-        uint64_t mine = 0, last = ~uint64_t(0);
-        wave_lds_order();
-        int found = 0;
-        for (; found < top; ++found) {
-            uint64_t best = own < last ? own : 0;
-#pragma nounroll
-            for (int i = 0; i < N; ++i) {
-                uint32_t c;
-                const uint32_t key = key_of(again(i, c));
-                const uint64_t entry = key >= bound && c < end ? entry_of(key, c) : 0;
-                if (entry < last && entry > best) best = entry;
-            }
-            last = wave_largest(best);
-            if (last == 0) break;
-            if (lane == found) mine = last;
-        }
-        if (lane < found) list[lane] = mine;
-        wave_lds_order();
-        return found;
-    }
-    // Each lane's entries, two at most, find their ranks.
-    const auto made = [&](int at) {
-        const uint64_t found = list[at];
-        return at < held ? found : entry_of(key_of(__builtin_bit_cast(float, uint32_t(found >> 32))), uint32_t(found));
-    };
     const uint64_t first = lane < count ? made(lane) : 0;
     int rank1 = 0;
     for (int i = 0; i < min(count, 64); ++i) rank1 += lane_value(first, i) > first;
@@ -210,6 +149,90 @@ __device__ __forceinline__ int select_top(const float (&value)[N], ClassAt class
     return min(count, top);
 }
 static_assert(kListed <= 128, "two entries a lane");
+
+// The `top` largest entries of a chunk's values and of the `held` sorted ones in list[0 .. held), sorted, to list[0 .. top);
+// returns how many there are. Lane l's value i is of class chunk + 4 (l + 64 (i / 4)) + i % 4, in memory at x[class], none
+// from `end` on; `largest` is the lane's largest, NaN aside, and `nan` says, the same in all lanes, whether there is one.
+// Where `top` are held, a value has to be above the last of them (its class is higher). The list has room for kListed
+// entries.
+template <int N>
+__device__ __forceinline__ int select_top(const float (&value)[N], const float* x, uint32_t chunk, uint32_t end, float largest,
+                                          bool nan, int top, uint64_t* list, int held) {
+    const int lane = threadIdx.x & 63;
+    const auto class_at = [&](int i) { return chunk + 4 * (lane + 64 * (i / 4)) + i % 4; };
+    // Keys from `bound` on are candidates. At first what is above the held ones, or any (-inf's key is the least).
+    uint32_t bound = held == top ? uint32_t(__builtin_amdgcn_readfirstlane(int(list[top - 1] >> 32))) : kLeastKey - 1;
+    if (bound == 0xffffffffu) return held;  // as many NaN
+    ++bound;
+    int count = held;
+    if (!nan) {
+        const uint32_t key = key_of(largest);
+        if (!__any(key >= bound)) return held;
+        // The `top`-th largest of the lanes' maxima, to 16 bits: `top` values reach it, and few more. Not needed where
+        // few lanes have anything above the held ones.
+        uint32_t reached = 0;
+        const auto bisect = [&](uint32_t bit) {
+            if (__popcll(__ballot(key >= (reached | bit))) >= top) reached |= bit;
+        };
+        if (__popcll(__ballot(key >= bound)) > kLargestTop / 2) {
+#pragma unroll
+            for (int b = 31; b >= 16; --b) bisect(1u << b);
+            bound = max(bound, reached);
+        }
+        const auto gather = [&](float v, uint32_t c, float least) {
+            const bool candidate = v >= least && c < end;
+            const uint64_t mask = __ballot(candidate);
+            const int at = count + __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
+            if (candidate && at < kListed)  // made an entry below, once for all
+                list[at] = uint64_t(__builtin_bit_cast(uint32_t, v)) << 32 | c;
+            count += __popcll(mask);
+        };
+        const float least = logit_of(bound);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (__ballot(value[i] >= least) != 0) gather(value[i], class_at(i), least);
+        // Too many within 2^-7 of the bound: to all its bits, from memory.
+        if (count > kListed) {
+            reached = 0;
+#pragma nounroll
+            for (int b = 31; b >= 0; --b) bisect(1u << b);
+            bound = max(bound, reached);
+            count = held;
+#pragma nounroll
+            for (int i = 0; i < N; ++i) {
+                const uint32_t c = class_at(i);
+                gather(c < end ? x[c] : -INFINITY, c, logit_of(bound));
+            }
+        }
+        wave_lds_order();
+    }
+    if (nan || count > kListed) {
+        // One by one: the largest below the last, of the lanes' values and of the list's first `held`.
+        const uint64_t own = lane < held ? list[lane] : 0;
+        uint64_t mine = 0, last = ~uint64_t(0);
+        wave_lds_order();
+        int found = 0;
+        for (; found < top; ++found) {
+            uint64_t best = own < last ? own : 0;
+#pragma nounroll
+            for (int i = 0; i < N; ++i) {
+                const uint32_t c = class_at(i), key = c < end ? key_of(x[c]) : 0;
+                const uint64_t entry = key >= bound ? entry_of(key, c) : 0;
+                if (entry < last && entry > best) best = entry;
+            }
+            last = wave_largest(best);
+            if (last == 0) break;
+            if (lane == found) mine = last;
+        }
+        if (lane < found) list[lane] = mine;
+        wave_lds_order();
+        return found;
+    }
+    return rank_entries(list, count, top, [&](int at) {
+        const uint64_t found = list[at];
+        return at < held ? found : entry_of(key_of(__builtin_bit_cast(float, uint32_t(found >> 32))), uint32_t(found));
+    });
+}
 
 // Where a place's head starts in the logits and its token in the tokens.
 struct Place {
@@ -307,26 +330,21 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
             const float largest = s.m;
             s.m = wave_max(s.m);
             // A NaN is no maximum, but its term makes `rest` NaN. Equal ones to the maximum count 1 each, without one of them.
-            int equal = 0;  // over the wave
+            int others = 0;  // over the wave
 #pragma unroll
             for (int i = 0; i < 4 * VECTORS; ++i) {
                 const float z = (v[i] - s.m) * factor, e = __builtin_amdgcn_exp2f(z);
-                s.rest += v[i] == s.m ? 0.f : e;
-                equal += __popcll(__ballot(v[i] == s.m));
-                s.weighted -= e > 0.f ? e * z : 0.f;
+                const bool other = !(v[i] == s.m);
+                s.rest += other ? e : 0.f;
+                others += __popcll(__ballot(other));
+                s.weighted = fmaf(-e, fmaxf(z, -FLT_MAX), s.weighted);  // 0 of z = -inf, and of a NaN what `rest` makes up for
             }
             s.rest = wave_sum(s.rest);
-            if (s.m != -INFINITY) s.rest += float(equal - 1);
+            if (s.m != -INFINITY) s.rest += float(256 * VECTORS - 1 - others);
             s.weighted = wave_sum(s.weighted);
             total = merged(total, s, factor);
-            if constexpr (TOP) {
-                const auto class_at = [&](int i) { return uint32_t(chunk) + 4 * (lane + 64 * (i / 4)) + i % 4; };
-                const auto again = [&](int i, uint32_t& c) {
-                    c = class_at(i);
-                    return c < uint32_t(end) ? x[c] : -INFINITY;
-                };
-                found = select_top(v, class_at, again, uint32_t(end), largest, __any(s.rest != s.rest), a.top, list, found);
-            }
+            if constexpr (TOP)
+                found = select_top(v, x, uint32_t(chunk), uint32_t(end), largest, __any(s.rest != s.rest), a.top, list, found);
         }
         if (parts == 1) {
             finish(a, place, given, total, list, found);
@@ -335,6 +353,69 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
             if (TOP && lane < a.top) lists_of(a, items)[int64_t(item) * a.top + lane] = lane < found ? list[lane] : 0;
         }
     }
+}
+
+// The likeliest of `parts` sorted lists of `top` entries, 0 behind their last: to list[0 .. top), sorted; returns how many
+// there are. A lane a part, 64 at a time: the `top`-th largest of their first eight is a bound that few others reach.
+__device__ __forceinline__ int merge_lists(const uint64_t* entries, int parts, int top, uint64_t* list) {
+    const int lane = threadIdx.x & 63;
+    int found = 0;
+    for (int group = 0; group < parts; group += 64) {
+        const uint64_t* own = entries + int64_t(group + lane) * top;
+        const int size = group + lane < parts ? top : 0;
+        constexpr int kAhead = 8;
+        uint64_t ahead[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) ahead[j] = j < size ? own[j] : 0;
+        const uint64_t above = found == top ? list[top - 1] + 1 : 1;
+        uint64_t bound;
+        int count;
+        const auto gather = [&](uint64_t entry) {
+            const uint64_t mask = __ballot(entry >= bound);
+            const int at = count + __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
+            if (entry >= bound && at < kListed) list[at] = entry;
+            count += __popcll(mask);
+            return mask != 0;
+        };
+        for (int low = 16; low >= 0; low -= 16) {  // to 16 bits, or if that leaves too many, to all
+            uint32_t reached = 0;
+#pragma nounroll
+            for (int b = 31; b >= low; --b) {
+                const uint32_t tried = reached | 1u << b;
+                int reaching = 0;
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) reaching += __popcll(__ballot(uint32_t(ahead[j] >> 32) >= tried));
+                if (reaching >= top) reached = tried;
+            }
+            bound = max(above, uint64_t(reached) << 32);
+            count = found;
+            bool more = true;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) more = gather(ahead[j]);
+            for (int j = kAhead; j < top && more && count <= kListed; ++j) more = gather(j < size ? own[j] : 0);
+            if (count <= kListed) break;
+        }
+        wave_lds_order();
+        if (count <= kListed) {
+            found = rank_entries(list, count, top, [&](int at) { return list[at]; });
+            continue;
+        }
+        // Many equal ones: one by one, the largest of the held ones and of the parts' next.
+        uint64_t held = lane < found ? list[lane] : 0, next = ahead[0], mine = 0;
+        wave_lds_order();
+        int taken = 0, j = 0;
+        for (; taken < top; ++taken) {
+            const uint64_t best = wave_largest(max(held, next));
+            if (best == 0) break;
+            if (lane == taken) mine = best;
+            if (held == best) held = 0;
+            if (next == best) next = ++j < size ? own[j] : 0;
+        }
+        if (lane < taken) list[lane] = mine;
+        wave_lds_order();
+        found = taken;
+    }
+    return found;
 }
 
 // A wave a place: its parts merged, in order.
@@ -346,44 +427,19 @@ __global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, uint3
         const f32x4* in = reinterpret_cast<const f32x4*>(a.workspace) + int64_t(place) * parts;
         const Given given = given_of(a, place_of(a, place));
         const float factor = factor_of(a.scale);
-        // The likeliest of the parts' lists: parts * top is at most kChunk. Their values as logits, NaN's too, and 0
-        // for no entry, which is no class.
-        constexpr int N = kChunk / 64;
-        float value[TOP ? N : 1], largest = -INFINITY;
-        uint32_t classes[TOP ? N : 1];
-        const uint64_t* entries = lists_of(a, int64_t(places) * parts) + int64_t(place) * parts * a.top;
-        const auto value_at = [&](int i, uint32_t& c) {
-            const int e = lane + 64 * i;
-            const uint64_t entry = e < parts * a.top ? entries[e] : 0;
-            c = entry != 0 ? class_of(entry) : ~0u;
-            return entry != 0 ? logit_of(uint32_t(entry >> 32)) : -INFINITY;
-        };
-        bool nan = false;
-        if constexpr (TOP) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) value[i] = value_at(i, classes[i]);
-        }
         Sums total = {-INFINITY, 0.f, 0.f};
         for (int p = lane; p < parts; p += 64) {
             const f32x4 s = in[p];
             total = merged(total, Sums{s[0], s[1], s[2]}, factor);
         }
+        int found = 0;
+        if constexpr (TOP)
+            found = merge_lists(lists_of(a, int64_t(places) * parts) + int64_t(place) * parts * a.top, parts, a.top, lists[wave]);
 #pragma unroll
         for (int step = 1; step < 64; step <<= 1)
             total = merged(total, Sums{__shfl_xor(total.m, step), __shfl_xor(total.rest, step), __shfl_xor(total.weighted, step)},
                            factor);
         total = Sums{__shfl(total.m, 0), __shfl(total.rest, 0), __shfl(total.weighted, 0)};
-        int found = 0;
-        if constexpr (TOP) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                largest = fmaxf(largest, value[i]);
-                nan |= value[i] != value[i];
-            }
-            const auto class_at = [&](int i) { return classes[i]; };
-            const auto again = [&](int i, uint32_t& c) { return value_at(i, c); };
-            found = select_top(value, class_at, again, ~0u, largest, __any(nan), a.top, lists[wave], 0);
-        }
         finish(a, place, given, total, lists[TOP ? wave : 0], found);
     }
 }

@@ -169,6 +169,19 @@ def test_equal_logits_go_by_class(gpu, classes):
         case.check(case.forward(gpu, top), top)
 
 
+@pytest.mark.parametrize("classes", [60, 1000, 2048, 4097, 6200, 20000, 200000])
+@pytest.mark.parametrize("top", [1, 10, 32])
+def test_close_logits(gpu, classes, top):
+    """All within a hundredth of each other, rising, falling, and with few in the lead."""
+    case = Case(4, 1, classes, seed=classes)
+    rng = np.random.default_rng(classes)
+    case.logits[0] = 100 + rng.random(classes) / 100
+    case.logits[1] = -100 + np.arange(classes) * 2.0 ** -14
+    case.logits[2] = 50 - np.arange(classes) * 2.0 ** -14
+    case.logits[3] = np.where(np.arange(classes) % 97 == 0, 3 + rng.random(classes) / 1000, -7)
+    case.check(case.forward(gpu, top), top)
+
+
 @pytest.mark.parametrize("classes", [3, 40, 1024, 2500, 30000])
 def test_masks_infinities_and_nan(gpu, classes):
     case = Case(12, 2, classes, seed=4)
