@@ -32,6 +32,7 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4_unaligned __attribute__((aligned(4)));
+typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;          // of a workgroup, each on its own
 constexpr int kChunk = 2048;       // classes a wave holds
@@ -118,37 +119,30 @@ __device__ __forceinline__ Sums merged(Sums a, Sums b, float factor) {
     return a;
 }
 
-__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
-    return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(v >> 32), lane))) << 32 |
-           uint32_t(__builtin_amdgcn_readlane(int(v), lane));
-}
-
 // The `top` largest of `count` entries, at most kListed, made(0) .. made(count - 1) from the list, sorted to the list's
 // start: each lane's entries, two at most, find their ranks. Returns how many there are.
 template <class Made>
 __device__ __forceinline__ int rank_entries(uint64_t* list, int count, int top, Made made) {
     const int lane = threadIdx.x & 63;
-    const uint64_t first = lane < count ? made(lane) : 0;
-    int rank1 = 0;
-    for (int i = 0; i < min(count, 64); ++i) rank1 += lane_value(first, i) > first;
-    if (count > 64) {
-        const uint64_t second = lane + 64 < count ? made(lane + 64) : 0;
-        int rank2 = 0;
-        for (int i = 0; i < 64; ++i) rank2 += lane_value(first, i) > second;
-        for (int i = 0; i < count - 64; ++i) {
-            const uint64_t other = lane_value(second, i);
-            rank1 += other > first;
-            rank2 += other > second;
-        }
-        wave_lds_order();
-        if (lane + 64 < count && rank2 < top) list[rank2] = second;
+    const uint64_t first = lane < count ? made(lane) : 0, second = lane + 64 < count ? made(lane + 64) : 0;
+    wave_lds_order();
+    list[lane] = first;
+    if (count > 64) list[lane + 64] = second;
+    wave_lds_order();
+    int rank1 = 0, rank2 = 0;
+#pragma unroll 4
+    for (int i = 0; i < count; i += 2) {  // the list read two at once by all lanes, with zeros behind the last
+        const u64x2 others = *reinterpret_cast<const u64x2*>(&list[i]);
+        rank1 += (others[0] > first) + (others[1] > first);
+        if (count > 64) rank2 += (others[0] > second) + (others[1] > second);
     }
     wave_lds_order();
     if (lane < count && rank1 < top) list[rank1] = first;
+    if (lane + 64 < count && rank2 < top) list[rank2] = second;
     wave_lds_order();
     return min(count, top);
 }
-static_assert(kListed <= 128, "two entries a lane");
+static_assert(kListed == 128, "two entries a lane");
 
 // The `top` largest entries of a chunk's values and of the `held` sorted ones in list[0 .. held), sorted, to list[0 .. top);
 // returns how many there are. Lane l's value i is of class chunk + 4 (l + 64 (i / 4)) + i % 4, in memory at x[class], none
@@ -295,7 +289,7 @@ __device__ __forceinline__ uint64_t* lists_of(const LogprobArgs& a, int64_t part
 template <int VECTORS, bool TOP>
 __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))) void logprobs_kernel(LogprobArgs a, uint32_t items,
                                                                                                        int parts, int chunks_per_part) {
-    __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? kListed : 1];
+    __shared__ __attribute__((aligned(16))) uint64_t lists[TOP ? kWaves : 1][TOP ? kListed : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint64_t* list = lists[TOP ? wave : 0];
     for (uint32_t item = blockIdx.x * kWaves + wave; item < items; item += gridDim.x * kWaves) {
@@ -356,7 +350,8 @@ __global__ __launch_bounds__(64 * kWaves) __attribute__((amdgpu_waves_per_eu(4))
 }
 
 // The likeliest of `parts` sorted lists of `top` entries, 0 behind their last: to list[0 .. top), sorted; returns how many
-// there are. A lane a part, 64 at a time: the `top`-th largest of their first eight is a bound that few others reach.
+// there are. A lane a part, 64 at a time: the `top`-th largest of their firsts (or where these are few, of their first eight) is a bound
+// that few others reach.
 __device__ __forceinline__ int merge_lists(const uint64_t* entries, int parts, int top, uint64_t* list) {
     const int lane = threadIdx.x & 63;
     int found = 0;
@@ -367,6 +362,7 @@ __device__ __forceinline__ int merge_lists(const uint64_t* entries, int parts, i
         uint64_t ahead[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) ahead[j] = j < size ? own[j] : 0;
+        const bool few = min(parts - group, 64) < 2 * top;
         const uint64_t above = found == top ? list[top - 1] + 1 : 1;
         uint64_t bound;
         int count;
@@ -382,9 +378,11 @@ __device__ __forceinline__ int merge_lists(const uint64_t* entries, int parts, i
 #pragma nounroll
             for (int b = 31; b >= low; --b) {
                 const uint32_t tried = reached | 1u << b;
-                int reaching = 0;
+                int reaching = __popcll(__ballot(uint32_t(ahead[0] >> 32) >= tried));
+                if (few) {
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j) reaching += __popcll(__ballot(uint32_t(ahead[j] >> 32) >= tried));
+                    for (int j = 1; j < kAhead; ++j) reaching += __popcll(__ballot(uint32_t(ahead[j] >> 32) >= tried));
+                }
                 if (reaching >= top) reached = tried;
             }
             bound = max(above, uint64_t(reached) << 32);
@@ -421,7 +419,7 @@ __device__ __forceinline__ int merge_lists(const uint64_t* entries, int parts, i
 // A wave a place: its parts merged, in order.
 template <bool TOP>
 __global__ __launch_bounds__(64 * kWaves) void merge_kernel(LogprobArgs a, uint32_t places, int parts) {
-    __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? kListed : 1];
+    __shared__ __attribute__((aligned(16))) uint64_t lists[TOP ? kWaves : 1][TOP ? kListed : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (uint32_t place = blockIdx.x * kWaves + wave; place < places; place += gridDim.x * kWaves) {
         const f32x4* in = reinterpret_cast<const f32x4*>(a.workspace) + int64_t(place) * parts;
