@@ -30,125 +30,6 @@ __device__ __forceinline__ void finish(const ProductArgs& a, int64_t place, int6
     a.y[place] = v;
 }
 
-// Few rows: bound by reading the weights once. A workgroup takes 16 C columns, its waves the blocks of the inner
-// dimension in turn, so that each wave's loads are whole 128-byte lines and none is read twice; their sums are added up
-// in LDS, in the order of the waves. The columns are the left operand of the matrix instructions, up to 16 R rows of x the
-// right one. Lane l holds row (or column) l % 16 of a fragment and bytes 32 (l / 16) .. + 31 of a block; the four
-// 32-deep instructions of a block take eight of them each, for both operands the same.
-template <int R, int C>
-struct FewBlock {
-    u32x4 w[C][2], x[R][2];
-    uint32_t w_scale[C], x_scale[R];
-};
-
-// Waves of a workgroup at most: 16 while their 128 registers suffice.
-template <int R, int C>
-constexpr int few_waves() {
-    return R * C <= 2 ? 16 : 8;
-}
-template <int R, int C>
-__global__ __launch_bounds__((64 * few_waves<R, C>())) void few_rows_kernel(ProductArgs a, int slices) {
-    extern __shared__ __attribute__((aligned(16))) float sums[];  // [wave][C][R][64][4]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int64_t group = blockIdx.x / slices, col0 = group * (16 * C);
-    const int slice = blockIdx.x - int(group) * slices;
-    const int blocks = int(a.blocks), stride = waves * slices;
-    const int64_t row_bytes = a.blocks * kBlock, scale_row = scale_stride(a.blocks);
-    // Columns past the last read the last one's, rows past the last nothing (zeros); neither's results are stored.
-    const uint8_t *w[C], *w_scales[C], *x[R], *x_scales[R];
-    bool held[R];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int64_t col = min(col0 + 16 * c + lane % 16, a.cols - 1);
-        w[c] = a.w + col * row_bytes + 32 * (lane / 16);
-        w_scales[c] = a.w_scales + col * scale_row;
-    }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t row = 16 * i + lane % 16;
-        held[i] = row < a.rows;
-        x[i] = a.x + (held[i] ? row : 0) * row_bytes + 32 * (lane / 16);
-        x_scales[i] = a.x_scales + (held[i] ? row : 0) * scale_row;
-    }
-    auto load = [&](int b, FewBlock<R, C>& to) {
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) to.w[c][h] = *reinterpret_cast<const u32x4*>(w[c] + int64_t(b) * kBlock + 16 * h);
-            to.w_scale[c] = w_scales[c][b];
-        }
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-            if (held[i]) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) to.x[i][h] = *reinterpret_cast<const u32x4*>(x[i] + int64_t(b) * kBlock + 16 * h);
-                to.x_scale[i] = x_scales[i][b];
-            } else {
-                to.x[i][0] = to.x[i][1] = u32x4{0, 0, 0, 0};
-                to.x_scale[i] = kLeastScale;
-            }
-    };
-    f32x4 acc[C][R];
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < R; ++i) acc[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](const FewBlock<R, C>& from) {
-        float wf[C], xf[R];
-#pragma unroll
-        for (int c = 0; c < C; ++c) wf[c] = factor_of(from.w_scale[c]);
-#pragma unroll
-        for (int i = 0; i < R; ++i) xf[i] = factor_of(from.x_scale[i]);
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-            const int h = step / 2, at = 2 * (step % 2);
-            bf16x8 wb[C], xb[R];
-#pragma unroll
-            for (int c = 0; c < C; ++c) wb[c] = fragment_of(from.w[c][h][at], from.w[c][h][at + 1], wf[c]);
-#pragma unroll
-            for (int i = 0; i < R; ++i) xb[i] = fragment_of(from.x[i][h][at], from.x[i][h][at + 1], xf[i]);
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int i = 0; i < R; ++i)
-                    acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[c], xb[i], acc[c][i], 0, 0, 0);
-        }
-    };
-    // Two blocks in registers: one arrives while the other is multiplied.
-    FewBlock<R, C> even, odd;
-    int b = slice * waves + wave;
-    if (b < blocks) load(b, even);
-    while (b < blocks) {
-        if (b + stride < blocks) load(b + stride, odd);
-        multiply(even);
-        b += stride;
-        if (b >= blocks) break;
-        if (b + stride < blocks) load(b + stride, even);
-        multiply(odd);
-        b += stride;
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-            *reinterpret_cast<f32x4*>(&sums[(((wave * C + c) * R + i) * 64 + lane) * 4]) = acc[c][i];
-    __syncthreads();
-    // A value is column 4 (l / 16) + r of its 16 and row l % 16 of its 16: consecutive threads take a row's columns.
-    constexpr int kCols = 16 * C;
-    for (int e = threadIdx.x; e < R * 16 * kCols; e += blockDim.x) {
-        const int row = e / kCols, in_group = e % kCols, c = in_group / 16, i = row / 16;
-        const int64_t col = col0 + in_group;
-        if (row >= a.rows || col >= a.cols) continue;
-        const int at = ((c * R + i) * 64 + in_group % 16 / 4 * 16 + row % 16) * 4 + in_group % 4;
-        float total = 0.f;
-        for (int v = 0; v < waves; ++v) total += sums[v * (C * R * 256) + at];
-        if (slices > 1)
-            a.workspace[(int64_t(slice) * a.rows + row) * a.cols + col] = total;
-        else
-            finish(a, row * a.cols + col, col, total);
-    }
-}
-
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* lds_pointer;
 
@@ -168,6 +49,140 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+}
+
+// Few rows: bound by reading the weights once. A workgroup takes 16 C columns, its W waves the blocks of the inner
+// dimension in turn, each with LDS of its own for two blocks; their sums are added up in the end, in the order of
+// the waves. The columns are the left operand of the matrix instructions, up to 16 R rows of x the right one. Lane l
+// holds row (or column) l % 16 of a fragment and bytes 32 (l / 16) .. + 31 of a block; the four 32-deep instructions of
+// a block take eight of them each, for both operands the same. Loading them so from memory would have each lane of a
+// load in another line than its neighbours, 64 lookups an instruction; through LDS eight lanes load a line together
+// (16 x 4096 x 14336, weights
+// from HBM: 14.9 us, 3.9 TB/s, against 20.4).
+template <int R, int C, int W>
+__device__ __forceinline__ void multiply_few(const ProductArgs& a, int slices) {
+    constexpr int F = C + R, kPerWave = F * 16 * int(kBlock), kLoads = 2 * F;  // of eight rows each, a block
+    // An array a stage, named by constants, so that the compiler knows which stage a read of LDS may depend on.
+    __shared__ __attribute__((aligned(16))) uint8_t stage0[W * kPerWave], stage1[W * kPerWave];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint8_t* const stages[2] = {stage0 + wave * kPerWave, stage1 + wave * kPerWave};
+    const int group = int(blockIdx.x) / slices, slice = int(blockIdx.x) - group * slices;
+    const int64_t col0 = int64_t(group) * (16 * C);
+    const int blocks = int(a.blocks), stride = W * slices, first = slice * W + wave;
+    const uint32_t row_bytes = uint32_t(a.blocks * kBlock);
+    const int64_t scale_row = scale_stride(a.blocks);
+    // Columns and rows past the last are the last again; their results are not stored.
+    const int last_col = int(min(int64_t(16 * C), a.cols - col0)) - 1, last_row = int(a.rows) - 1;
+    const uint8_t* w = a.w + col0 * row_bytes;
+    uint32_t from[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int r = 8 * i + lane / 8;
+        from[i] = uint32_t(i < 2 * C ? min(r, last_col) : min(r - 16 * C, last_row)) * row_bytes + 16 * ((lane % 8) ^ (lane / 8));
+    }
+    // A block's loads; of one past the last, of no bytes, which keeps the count of loads, and so the waits, fixed.
+    auto load = [&](uint8_t* stage, int b) {
+        const int bytes = __builtin_amdgcn_readfirstlane((b - blocks) >> 31);  // all, or none
+        const __amdgpu_buffer_rsrc_t left = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w), 0, bytes, 0x00020000);
+        const __amdgpu_buffer_rsrc_t right = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.x), 0, bytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(i < 2 * C ? left : right, (lds_pointer)(stage + 1024 * i), 16, from[i],
+                                                     int(kBlock) * min(b, blocks), 0, 0);
+    };
+    // The scale bytes of four of this wave's blocks, from b on: lane l's are row (or column) l % 16's of block l / 16 of them.
+    const uint8_t* scales[F];
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+        scales[i] = i < C ? a.w_scales + (col0 + min(16 * i + lane % 16, last_col)) * scale_row
+                          : a.x_scales + min(16 * (i - C) + lane % 16, last_row) * scale_row;
+    uint32_t next[F];
+    auto load_scales = [&](int b) {
+        const int at = min(b + stride * (lane / 16), blocks - 1);
+#pragma unroll
+        for (int i = 0; i < F; ++i) next[i] = scales[i][at];
+    };
+    const int at = lane % 16 * int(kBlock) + 16 * ((lane / 16 * 2) ^ (lane % 8));
+    f32x4 acc[C][R];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < R; ++i) acc[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (first < blocks) {
+        load_scales(first);
+        load(stages[0], first);
+        load(stages[1], first + stride);
+        for (int b0 = first; b0 < blocks; b0 += 4 * stride) {
+            float factors[F];
+#pragma unroll
+            for (int i = 0; i < F; ++i) factors[i] = factor_of(next[i]);
+            load_scales(b0 + 4 * stride);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int b = b0 + u * stride;
+                if (b >= blocks) break;
+                uint8_t* const stage = stages[u % 2];
+                wait_loads<kLoads>();  // all but the other stage's
+                asm volatile("" ::: "memory");
+                u32x4 chunk[F][2];
+#pragma unroll
+                for (int i = 0; i < F; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        chunk[i][h] = *reinterpret_cast<const u32x4*>(stage + 16 * int(kBlock) * i + (at ^ (16 * h)));
+                float factor[F];
+#pragma unroll
+                for (int i = 0; i < F; ++i) factor[i] = __shfl(factors[i], lane % 16 + 16 * u);
+                __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage is read
+                asm volatile("" ::: "memory");
+                load(stage, b + 2 * stride);
+#pragma unroll
+                for (int step = 0; step < 4; ++step) {
+                    const int h = step / 2, q = 2 * (step % 2);
+                    bf16x8 f[F];
+#pragma unroll
+                    for (int i = 0; i < F; ++i) f[i] = fragment_of(chunk[i][h][q], chunk[i][h][q + 1], factor[i]);
+#pragma unroll
+                    for (int c = 0; c < C; ++c)
+#pragma unroll
+                        for (int i = 0; i < R; ++i)
+                            acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[c], f[C + i], acc[c][i], 0, 0, 0);
+                }
+            }
+        }
+        wait_loads<0>();
+        asm volatile("" ::: "memory");
+    }
+    // The waves' sums, [wave][C][R][64][4], each in its part of the first stage.
+    constexpr int kWaveFloats = kPerWave / 4;
+    static_assert(kWaveFloats >= 256 * C * R, "a wave's sums fit its part of a stage");
+    float* const sums = reinterpret_cast<float*>(stage0);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            *reinterpret_cast<f32x4*>(&sums[wave * kWaveFloats + ((c * R + i) * 64 + lane) * 4]) = acc[c][i];
+    __syncthreads();
+    // A value is column 4 (l / 16) + r of its 16 and row l % 16 of its 16: consecutive threads take a row's columns.
+    constexpr int kCols = 16 * C;
+    for (int e = threadIdx.x; e < R * 16 * kCols; e += 64 * W) {
+        const int row = e / kCols, in_group = e % kCols, c = in_group / 16, i = row / 16;
+        const int64_t col = col0 + in_group;
+        if (row >= a.rows || col >= a.cols) continue;
+        const int from_lane = ((c * R + i) * 64 + in_group % 16 / 4 * 16 + row % 16) * 4 + in_group % 4;
+        float total = 0.f;
+#pragma unroll 4
+        for (int v = 0; v < W; ++v) total += sums[v * kWaveFloats + from_lane];
+        if (slices > 1)
+            a.workspace[(int64_t(slice) * a.rows + row) * a.cols + col] = total;
+        else
+            finish(a, row * a.cols + col, col, total);
+    }
+}
+
+template <int R, int C, int W>
+__global__ __launch_bounds__(64 * W) void few_rows_kernel(ProductArgs a, int slices) {
+    multiply_few<R, C, W>(a, slices);
 }
 
 // Block id -> slice and tile. Consecutive ids land on different XCDs, each with an L2 of its own: ids are regrouped so
@@ -234,7 +249,7 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
     // Loads FIRST to LAST of a step. Steps past the last load nothing (a buffer of no bytes), which keeps the count of
     // loads, and so the waits, fixed.
     auto load = [&](uint8_t* stage, int step, auto first, auto last) {
-        const int bytes = -max(0, min(1, steps - step));  // all, or none
+        const int bytes = __builtin_amdgcn_readfirstlane((step - steps) >> 31);  // all, or none
         const __amdgpu_buffer_rsrc_t left = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x), 0, bytes, 0x00020000);
         const __amdgpu_buffer_rsrc_t right = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w), 0, bytes, 0x00020000);
 #pragma unroll
@@ -462,18 +477,18 @@ hipError_t launch_tiles(const ProductArgs& a, hipStream_t stream) {
     return err != hipSuccess || slices == 1 ? err : launch_slices(a, int(slices), stream);
 }
 
-template <int R, int C>
+template <int R, int C, int W>
 hipError_t launch_few_rows(const ProductArgs& a, hipStream_t stream) {
-    constexpr int64_t kWaveBytes = C * R * 1024;  // of a wave's sums
     const int64_t groups = (a.cols + 16 * C - 1) / (16 * C);
-    // Waves of a workgroup until there are 24 a CU, a block each at least.
-    int64_t waves = (24 * int64_t(a.cu_count) + groups - 1) / groups;
-    waves = std::max<int64_t>(1, std::min<int64_t>({std::max<int64_t>(waves, 4), few_waves<R, C>(), a.blocks}));
-    // Then slices of the inner dimension over workgroups until there are 8 a CU, of two blocks a wave at least.
-    const int64_t wanted = 8 * int64_t(a.cu_count) / (groups * waves);
-    const int64_t slices = held_slices(a, std::min<int64_t>({wanted, a.blocks / (2 * waves), 32}));
-    hipLaunchKernelGGL((few_rows_kernel<R, C>), dim3(unsigned(groups * slices)), dim3(unsigned(64 * waves)),
-                       unsigned(waves * kWaveBytes), stream, a, int(slices));
+    // Slices of the inner dimension where column groups are few: a workgroup takes about 62 KB of operands in a us, the
+    // second kernel 3 us (16 x 768 x 28672: 12.1 us in five slices, 22.1 in one).
+    int64_t slices = 1;
+    const double whole = double(16 * (R + C) * a.blocks * kBlock) / 62e3;
+    double least = whole;
+    const int64_t most = held_slices(a, std::min<int64_t>({a.cu_count / groups, a.blocks / W, 32}));
+    for (int64_t n = 2; n <= most; ++n)
+        if (whole / double(n) + 3 < least) least = whole / double(n) + 3, slices = n;
+    hipLaunchKernelGGL((few_rows_kernel<R, C, W>), dim3(unsigned(groups * slices)), dim3(64 * W), 0, stream, a, int(slices));
     const hipError_t err = hipGetLastError();
     return err != hipSuccess || slices == 1 ? err : launch_slices(a, int(slices), stream);
 }
@@ -481,16 +496,26 @@ hipError_t launch_few_rows(const ProductArgs& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
-    // Few rows: the more 16-column fragments a wave, the less often x is read beside the weights, while three workgroups for
-    // four CUs are left. Up to 64 rows of narrow outputs too, where a tile's steps one after the other take longer than
-    // reading x for every 16 columns: 60 x 1000 x 1300 (inner 1000) 5.6 us against 8.6, 64 x 8192 x 8192 58.6 against 29.5.
-    const bool wide = a.cols >= 48 * a.cu_count, narrow = a.cols < 24 * a.cu_count;
+    // Few rows. Workgroups of 16 columns while every CU has at most one; beyond, more columns or fewer waves each, so that
+    // the CUs hold all or most of them at once. Measured alternatives in us, inner dimension 14336, 4096 or 8192:
+    //   16 x 4224: <1, 2, 8> 20.9, <1, 1, 4> 23.3, <1, 1, 8> 24.5; 16 x 14336: <1, 1, 4> 16.5, <1, 1, 8> 18.4, <1, 2, 8> 19.0;
+    //   16 x 28672: <1, 4, 4> 37.6, <1, 1, 4> 39.9; 32 x 14336: <2, 2, 4> 18.4, <2, 4, 3> 19.4; 32 x 28672: 56.0, 45.4.
+    // Up to 64 rows too where a tile's steps one after the other take longer than reading x for every 16 or 32 columns:
+    //   64 x 8192: <4, 2, 6> 25.9, tiles 34.5; 64 x 14336: <4, 2, 3> 25.8, tiles 33.1; 64 x 28672: 71.4, tiles 67.7.
+    const int64_t cu = a.cu_count, cols = a.cols;
     if (a.rows <= 16) {
-        if (wide) return launch_few_rows<1, 4>(a, stream);
-        return narrow ? launch_few_rows<1, 1>(a, stream) : launch_few_rows<1, 2>(a, stream);
+        if (cols <= 16 * cu) return launch_few_rows<1, 1, 8>(a, stream);
+        if (cols <= 24 * cu) return launch_few_rows<1, 2, 8>(a, stream);
+        return cols < 48 * cu ? launch_few_rows<1, 1, 4>(a, stream) : launch_few_rows<1, 4, 4>(a, stream);
     }
-    if (a.rows <= 32) return wide ? launch_few_rows<2, 4>(a, stream) : launch_few_rows<2, 2>(a, stream);
-    if (a.rows <= 64 && narrow) return launch_few_rows<4, 1>(a, stream);
+    if (a.rows <= 32) {
+        if (cols <= 16 * cu) return launch_few_rows<2, 1, 12>(a, stream);
+        return cols <= 64 * cu ? launch_few_rows<2, 2, 4>(a, stream) : launch_few_rows<2, 4, 3>(a, stream);
+    }
+    if (a.rows <= 64 && cols <= 64 * cu) {
+        if (cols <= 16 * cu) return launch_few_rows<4, 1, 8>(a, stream);
+        return cols <= 32 * cu ? launch_few_rows<4, 2, 6>(a, stream) : launch_few_rows<4, 2, 3>(a, stream);
+    }
     // The largest tile that there are two of for each CU.
     auto fills = [&](int64_t m, int64_t n) {
         return ((a.rows + m - 1) / m) * ((a.cols + n - 1) / n) >= 2 * a.cu_count;
