@@ -273,8 +273,10 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
     for (int i = 0; i < F; ++i)
         scales[i] = uint32_t(i < FM ? min(wave_m + 32 * i + row, last_m) : min(wave_n + 32 * (i - FM) + row, last_n)) *
                     uint32_t(scale_row);
-    const uint8_t* x_scales = a.x_scales + m0 * scale_row + block0;
-    const uint8_t* w_scales = a.w_scales + n0 * scale_row + block0;
+    const __amdgpu_buffer_rsrc_t x_scales =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.x_scales + m0 * scale_row + block0), 0, -1, 0x00020000);
+    const __amdgpu_buffer_rsrc_t w_scales =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.w_scales + n0 * scale_row + block0), 0, -1, 0x00020000);
     f32x16 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -305,8 +307,10 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], f[FM + j], acc[i][j], 0, 0, 0);
     };
     auto load_scales = [&](int block) {
+        const int at = __builtin_amdgcn_readfirstlane(min(block, blocks - 1));
 #pragma unroll
-        for (int i = 0; i < F; ++i) next_scale[i] = ((i < FM ? x_scales : w_scales) + min(block, blocks - 1))[scales[i]];
+        for (int i = 0; i < F; ++i)
+            next_scale[i] = __builtin_amdgcn_raw_buffer_load_b8(i < FM ? x_scales : w_scales, scales[i], at, 0);
     };
     auto take_scales = [&] {
 #pragma unroll
@@ -431,9 +435,9 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
     }
 }
 
-// Waves a SIMD: two of the large tiles, whose sums take half of its registers.
+// Waves a SIMD: one of the largest tiles, whose sums take half of its registers or more, two of the next.
 template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) __attribute__((amdgpu_waves_per_eu(BM * BN > 8192 ? 2 : 3))) void tile_kernel(
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) __attribute__((amdgpu_waves_per_eu(BM * BN > 32768 ? 1 : BM * BN > 8192 ? 2 : 3))) void tile_kernel(
     ProductArgs a, int tiles_m, int tiles_n, int blocks_per_slice) {
     multiply_tile<BM, BN, STAGES, WAVES_M, WAVES_N>(a, tiles_m, tiles_n, blocks_per_slice);
 }
@@ -457,24 +461,41 @@ int64_t held_slices(const ProductArgs& a, int64_t slices) {
     return std::max<int64_t>(1, std::min<int64_t>(slices, int64_t(a.workspace_bytes / sizeof(float)) / (a.rows * a.cols)));
 }
 
-template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
-hipError_t launch_tiles(const ProductArgs& a, hipStream_t stream) {
-    const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN, tiles = tiles_m * tiles_n;
-    // Slices of the inner dimension where tiles are few: a block takes about 0.8 us, the second kernel 5 us and 2 us more per
-    // million sums.
-    int64_t slices = 1;
-    double least = 0.8 * double(a.blocks);
-    const int64_t most = held_slices(a, std::min<int64_t>({3 * int64_t(a.cu_count) / tiles, a.blocks / 2, 32}));
-    for (int64_t n = 2; n <= most; ++n) {
-        const double cost = 0.8 * double((a.blocks + n - 1) / n) + 5 + 2e-6 * double(n * a.rows * a.cols);
-        if (cost < least) least = cost, slices = n;
-    }
+template <int BM, int BN, int STAGES>
+hipError_t launch_tiles(const ProductArgs& a, int64_t slices, hipStream_t stream) {
+    const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.cols + BN - 1) / BN;
     const int64_t per_slice = (a.blocks + slices - 1) / slices;
     slices = a.blocks == 0 ? 1 : (a.blocks + per_slice - 1) / per_slice;
-    hipLaunchKernelGGL((tile_kernel<BM, BN, STAGES, WAVES_M, WAVES_N>), dim3(unsigned(tiles * slices)), dim3(64 * WAVES_M * WAVES_N), 0, stream, a, int(tiles_m),
-                       int(tiles_n), int(per_slice));
+    hipLaunchKernelGGL((tile_kernel<BM, BN, STAGES, 2, 2>), dim3(unsigned(tiles_m * tiles_n * slices)), dim3(256), 0, stream, a,
+                       int(tiles_m), int(tiles_n), int(per_slice));
     const hipError_t err = hipGetLastError();
     return err != hipSuccess || slices == 1 ? err : launch_slices(a, int(slices), stream);
+}
+
+// Tiles and slices of the inner dimension by their time in us: a CU takes `block` for a block of a tile, whether it has
+// one tile or several at once, and writes outputs at 20 KB a us; the slices' second kernel takes 5 and 2 more per million
+// sums. The larger a tile, the fewer conversions and reads of LDS for each product, and the more its edges and last round
+// waste. The times are of 8192 x 8192 x 8192 and 6001 x 4096 x 14336, where the tiles took, in this order:
+//   817, 887, 918, 1069, 1389, 1736 us and 626, 563, 591, 711, 921, 1104 us.
+struct Tile {
+    int rows, cols;
+    double block;
+};
+constexpr Tile kTiles[] = {{256, 256, 3.0}, {192, 256, 2.42}, {128, 256, 1.70}, {128, 128, 0.99}, {64, 128, 0.65}, {64, 64, 0.41}};
+void choose_tile(const ProductArgs& a, int& tile, int64_t& slices) {
+    double least = 0;
+    tile = -1;
+    for (int i = 0; i < int(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+        const Tile& t = kTiles[i];
+        const int64_t tiles = ((a.rows + t.rows - 1) / t.rows) * ((a.cols + t.cols - 1) / t.cols);
+        const int64_t most = held_slices(a, std::min<int64_t>({2 * int64_t(a.cu_count) / tiles, a.blocks / 2, 32}));
+        for (int64_t n = 1; n <= most; ++n) {
+            const int64_t rounds = (tiles * n + a.cu_count - 1) / a.cu_count, blocks = (a.blocks + n - 1) / n;
+            double cost = double(rounds) * (double(blocks) * t.block + double(t.rows * t.cols) * 4 / 20e3);
+            if (n > 1) cost += 5 + 2e-6 * double(n * a.rows * a.cols);
+            if (tile < 0 || cost < least) least = cost, tile = i, slices = n;
+        }
+    }
 }
 
 template <int R, int C, int W>
@@ -516,14 +537,17 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
         if (cols <= 16 * cu) return launch_few_rows<4, 1, 8>(a, stream);
         return cols <= 32 * cu ? launch_few_rows<4, 2, 6>(a, stream) : launch_few_rows<4, 2, 3>(a, stream);
     }
-    // The largest tile that there are two of for each CU.
-    auto fills = [&](int64_t m, int64_t n) {
-        return ((a.rows + m - 1) / m) * ((a.cols + n - 1) / n) >= 2 * a.cu_count;
-    };
-    if (fills(128, 256)) return launch_tiles<128, 256, 3, 2, 2>(a, stream);
-    if (fills(128, 128)) return launch_tiles<128, 128, 3, 2, 2>(a, stream);
-    if (fills(64, 128)) return launch_tiles<64, 128, 3, 2, 2>(a, stream);
-    return launch_tiles<64, 64, 6, 2, 2>(a, stream);
+    int tile;
+    int64_t slices;
+    choose_tile(a, tile, slices);
+    switch (tile) {
+        case 0: return launch_tiles<256, 256, 3>(a, slices, stream);
+        case 1: return launch_tiles<192, 256, 3>(a, slices, stream);
+        case 2: return launch_tiles<128, 256, 3>(a, slices, stream);
+        case 3: return launch_tiles<128, 128, 3>(a, slices, stream);
+        case 4: return launch_tiles<64, 128, 3>(a, slices, stream);
+        default: return launch_tiles<64, 64, 6>(a, slices, stream);
+    }
 }
 
 }  // namespace fp8
