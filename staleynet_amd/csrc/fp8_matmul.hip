@@ -518,24 +518,24 @@ hipError_t launch_few_rows(const ProductArgs& a, hipStream_t stream) {
 
 hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
     // Few rows. Workgroups of 16 columns while every CU has at most one; beyond, more columns or fewer waves each, so that
-    // the CUs hold all or most of them at once. Measured alternatives in us, inner dimension 14336, 4096 or 8192:
-    //   16 x 4224: <1, 2, 8> 20.9, <1, 1, 4> 23.3, <1, 1, 8> 24.5; 16 x 14336: <1, 1, 4> 16.5, <1, 1, 8> 18.4, <1, 2, 8> 19.0;
-    //   16 x 28672: <1, 4, 4> 37.6, <1, 1, 4> 39.9; 32 x 14336: <2, 2, 4> 18.4, <2, 4, 3> 19.4; 32 x 28672: 56.0, 45.4.
-    // Up to 64 rows too where a tile's steps one after the other take longer than reading x for every 16 or 32 columns:
-    //   64 x 8192: <4, 2, 6> 25.9, tiles 34.5; 64 x 14336: <4, 2, 3> 25.8, tiles 33.1; 64 x 28672: 71.4, tiles 67.7.
+    // the CUs hold all or most of them at once. Alternatives measured in us, rows x inner dimension x columns:
+    //   16 x 14336 x 4224: <1, 2, 8> 20.9, <1, 1, 4> 23.3, <1, 1, 8> 24.5; 16 x 4096 x 14336: <1, 4, 4> 12.7, <1, 1, 4> 15.4;
+    //   32 x 8192 x 28672: <2, 4, 3> 42.5, <2, 2, 4> 57.2, tiles 50.8; 32 x 4096 x 8192: <2, 2, 4> 8.9, tiles 12.3.
+    // Up to 64 rows where 16 columns a workgroup suffice: 64 x 4096 x 4096 10.8, tiles 11.9; 64 x 4096 x 14336 <4, 2, 3>
+    // 21.6, tiles 20.8. Many columns of a short inner dimension are left to the tiles: 16 x 768 x 50304 13.2, tiles 10.9.
     const int64_t cu = a.cu_count, cols = a.cols;
-    if (a.rows <= 16) {
-        if (cols <= 16 * cu) return launch_few_rows<1, 1, 8>(a, stream);
-        if (cols <= 24 * cu) return launch_few_rows<1, 2, 8>(a, stream);
-        return cols < 48 * cu ? launch_few_rows<1, 1, 4>(a, stream) : launch_few_rows<1, 4, 4>(a, stream);
-    }
-    if (a.rows <= 32) {
-        if (cols <= 16 * cu) return launch_few_rows<2, 1, 12>(a, stream);
-        return cols <= 64 * cu ? launch_few_rows<2, 2, 4>(a, stream) : launch_few_rows<2, 4, 3>(a, stream);
-    }
-    if (a.rows <= 64 && cols <= 64 * cu) {
-        if (cols <= 16 * cu) return launch_few_rows<4, 1, 8>(a, stream);
-        return cols <= 32 * cu ? launch_few_rows<4, 2, 6>(a, stream) : launch_few_rows<4, 2, 3>(a, stream);
+    const bool few = a.rows <= 32 ? a.blocks > 8 || cols <= 64 * cu : a.rows <= 64 && cols <= 16 * cu;
+    if (few) {
+        if (a.rows <= 16) {
+            if (cols <= 16 * cu) return launch_few_rows<1, 1, 8>(a, stream);
+            if (cols <= 24 * cu) return launch_few_rows<1, 2, 8>(a, stream);
+            return cols < 48 * cu ? launch_few_rows<1, 1, 4>(a, stream) : launch_few_rows<1, 4, 4>(a, stream);
+        }
+        if (a.rows <= 32) {
+            if (cols <= 16 * cu) return launch_few_rows<2, 1, 12>(a, stream);
+            return cols <= 64 * cu ? launch_few_rows<2, 2, 4>(a, stream) : launch_few_rows<2, 4, 3>(a, stream);
+        }
+        return launch_few_rows<4, 1, 8>(a, stream);
     }
     int tile;
     int64_t slices;

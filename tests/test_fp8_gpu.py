@@ -199,6 +199,24 @@ def test_long_and_wide(gpu, rows, inner, cols):
     assert np.array_equal(got, run(gpu, spec, left, right, bias=bias))  # the same bits again
 
 
+@pytest.mark.parametrize("rows,inner,cols", [
+    (16, 300, 4300), (9, 1000, 6201), (16, 1200, 12301), (3, 130, 12300), (20, 1500, 4097), (32, 1100, 16500), (17, 260, 16401),
+    (16, 9000, 500), (20, 10000, 300), (50, 9000, 700), (64, 2100, 4096),  # of few rows, then tiles of each size
+    (80, 260, 16400), (333, 2000, 3000), (69, 6252, 4186), (1000, 1200, 3001), (520, 9000, 3900), (1500, 1000, 3001)])
+def test_each_form(gpu, rows, inner, cols):
+    left, right = operand(rows, inner, rows), operand(cols, inner, cols)
+    check(run(gpu, MatmulSpec.new(rows, cols, inner), left, right), left[2], right[2], inner)
+
+
+@pytest.mark.parametrize("inner", [1, 130, 300, 500, 640, 700, 900])
+@pytest.mark.parametrize("rows,cols", [(4090, 4081), (2500, 4095)])
+def test_the_largest_tiles(gpu, rows, cols, inner):
+    """One to eight blocks: whole rounds of steps and each remainder."""
+    left, right = operand(rows, inner, rows), operand(cols, inner, cols)
+    got = run(gpu, MatmulSpec.new(rows, cols, inner).accumulate(), left, right, before=np.ones((rows, cols), np.float32))
+    check(got, left[2], right[2], inner, before=np.ones((rows, cols), np.float32))
+
+
 @pytest.mark.parametrize("rows", [1, 5, 16, 40, 100, 300])
 @pytest.mark.parametrize("with_bias", [False, True])
 def test_scale_accumulate_and_bias(gpu, rows, with_bias):
