@@ -78,7 +78,8 @@ __device__ __forceinline__ void multiply_few(const ProductArgs& a, int slices) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
         const int r = 8 * i + lane / 8;
-        from[i] = uint32_t(i < 2 * C ? min(r, last_col) : min(r - 16 * C, last_row)) * row_bytes + 16 * ((lane % 8) ^ (lane / 8));
+        from[i] = uint32_t(i < 2 * C ? min(r, last_col) : min(r - 16 * C, last_row)) * row_bytes +
+                  16 * ((lane % 8) ^ ((r >> 1) & 7));  // the chunk that slot l % 8 of the row holds
     }
     // A block's loads; of one past the last, of no bytes, which keeps the count of loads, and so the waits, fixed.
     auto load = [&](uint8_t* stage, int b) {
@@ -102,7 +103,8 @@ __device__ __forceinline__ void multiply_few(const ProductArgs& a, int slices) {
 #pragma unroll
         for (int i = 0; i < F; ++i) next[i] = scales[i][at];
     };
-    const int at = lane % 16 * int(kBlock) + 16 * ((lane / 16 * 2) ^ (lane % 8));
+    // The 16 rows of a read are in different banks.
+    const int at = lane % 16 * int(kBlock) + 16 * ((lane / 16 * 2) ^ (lane % 16 >> 1));
     f32x4 acc[C][R];
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -521,10 +523,10 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
     // the CUs hold all or most of them at once. Alternatives measured in us, rows x inner dimension x columns:
     //   16 x 14336 x 4224: <1, 2, 8> 20.9, <1, 1, 4> 23.3, <1, 1, 8> 24.5; 16 x 4096 x 14336: <1, 4, 4> 12.7, <1, 1, 4> 15.4;
     //   32 x 8192 x 28672: <2, 4, 3> 42.5, <2, 2, 4> 57.2, tiles 50.8; 32 x 4096 x 8192: <2, 2, 4> 8.9, tiles 12.3.
-    // Up to 64 rows where 16 columns a workgroup suffice: 64 x 4096 x 4096 10.8, tiles 11.9; 64 x 4096 x 14336 <4, 2, 3>
-    // 21.6, tiles 20.8. Many columns of a short inner dimension are left to the tiles: 16 x 768 x 50304 13.2, tiles 10.9.
+    // Up to 64 rows too, for weights that come from HBM: 64 x 8192 x 8192 25.0, tiles 32.6 (25.7 and 24.9 from the last-level
+    // cache). Many columns of a short inner dimension are left to the tiles: 16 x 768 x 50304 13.2, tiles 10.9.
     const int64_t cu = a.cu_count, cols = a.cols;
-    const bool few = a.rows <= 32 ? a.blocks > 8 || cols <= 64 * cu : a.rows <= 64 && cols <= 16 * cu;
+    const bool few = a.rows <= 32 ? a.blocks > 8 || cols <= 64 * cu : a.rows <= 64 && cols <= 64 * cu;
     if (few) {
         if (a.rows <= 16) {
             if (cols <= 16 * cu) return launch_few_rows<1, 1, 8>(a, stream);
@@ -535,7 +537,8 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
             if (cols <= 16 * cu) return launch_few_rows<2, 1, 12>(a, stream);
             return cols <= 64 * cu ? launch_few_rows<2, 2, 4>(a, stream) : launch_few_rows<2, 4, 3>(a, stream);
         }
-        return launch_few_rows<4, 1, 8>(a, stream);
+        if (cols <= 16 * cu) return launch_few_rows<4, 1, 8>(a, stream);
+        return cols <= 32 * cu ? launch_few_rows<4, 2, 6>(a, stream) : launch_few_rows<4, 2, 3>(a, stream);
     }
     int tile;
     int64_t slices;

@@ -201,7 +201,7 @@ def test_long_and_wide(gpu, rows, inner, cols):
 
 @pytest.mark.parametrize("rows,inner,cols", [
     (16, 300, 4300), (9, 1000, 6201), (16, 1200, 12301), (3, 130, 12300), (20, 1500, 4097), (32, 1100, 16500), (17, 260, 16401),
-    (16, 9000, 500), (20, 10000, 300), (50, 9000, 700), (64, 2100, 4096),  # of few rows, then tiles of each size
+    (16, 9000, 500), (20, 10000, 300), (50, 9000, 700), (64, 2100, 4096), (40, 1500, 4097), (64, 900, 9001),  # of few rows, then tiles of each size
     (80, 260, 16400), (333, 2000, 3000), (69, 6252, 4186), (1000, 1200, 3001), (520, 9000, 3900), (1500, 1000, 3001)])
 def test_each_form(gpu, rows, inner, cols):
     left, right = operand(rows, inner, rows), operand(cols, inner, cols)
