@@ -1,5 +1,6 @@
 // Products of two 8-bit operands (sn_matmul_fp8; staleynet_fp8.h has the format):
 //   y = scale * X W (+ y) (+ bias)
+// (sizes below are rows x inner dimension x columns)
 //
 // A code times its block's factor is exact in bf16, and a product of two such
 // values is exact in fp32, so fragments are codes converted in registers and
@@ -57,7 +58,7 @@ __device__ __forceinline__ void stage_barrier() {
 // holds row (or column) l % 16 of a fragment and bytes 32 (l / 16) .. + 31 of a block; the four 32-deep instructions of
 // a block take eight of them each, for both operands the same. Loading them so from memory would have each lane of a
 // load in another line than its neighbours, 64 lookups an instruction; through LDS eight lanes load a line together
-// (16 x 4096 x 14336, weights
+// (16 x 14336 x 4096, weights
 // from HBM: 14.9 us, 3.9 TB/s, against 20.4).
 template <int R, int C, int W>
 __device__ __forceinline__ void multiply_few(const ProductArgs& a, int slices) {
@@ -209,11 +210,13 @@ __device__ __forceinline__ int swizzle(int row) { return (row >> 2) & 3; }
 
 // Many rows: a BM x BN tile of the output a workgroup of four waves, each a quarter of it in 32 x 32 blocks.
 //
-// Bound by the matrix cores, with the conversions beside them: a wave converts 24 pairs a lane for eight matrix instructions
-// of 32 cycles. A step of 64 along the inner dimension is four units of one 32x32x16 instruction a block; while a
-// unit is multiplied the next one's codes are converted and the chunk after that is read from LDS. The one barrier of a
-// step is in its middle: there every wave has read all of the step's stage, which takes the loads of three steps
-// ahead, and every wave's loads of the next stage have landed.
+// Bound by the matrix cores, and at large sizes by the power they draw: 6001 x 4096 x 14336 takes 554 to 589 us by the
+// card (1196 to 1272 TFLOP/s; the library's bf16 product of the same shape 590), 8192 x 8192 x 8192 807 us (1362). A wave
+// of the 256 x 256 tile converts 32 pairs a lane for sixteen matrix instructions of 32 cycles, one of the 128 x 256 tile 24
+// for eight. A step of 64 along the inner dimension is four units of one 32x32x16 instruction a block; while a unit is multiplied the
+// next one's codes are converted and the chunk after that is read from LDS. The one barrier of a step is in its middle:
+// there every wave has read all of the step's stage, which takes the loads of STAGES steps ahead, and every wave's loads of
+// the next stage have landed.
 template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
 __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m, int tiles_n, int blocks_per_slice) {
     constexpr int kWaves = WAVES_M * WAVES_N, FM = BM / (32 * WAVES_M), FN = BN / (32 * WAVES_N), F = FM + FN;
@@ -395,7 +398,8 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
         wait_loads<0>();
     }
     // A buffer of each 32 rows' outputs (or of the slice's sums), of less than 2^31 bytes: places past the last row are out
-    // of its range, and so is 2^31 with any row's offset, for columns past the last; such stores do nothing. A lane's sixteen values of a block are rows 8 (r / 4) + 4 half + r % 4 of one column.
+    // of its range, and so is 2^31 with any row's offset, for columns past the last; such stores do nothing. A lane's
+    // sixteen values of a block are rows 8 (r / 4) + 4 half + r % 4 of one column.
     const bool partial = gridDim.x > unsigned(tiles_m * tiles_n);
     float* y = partial ? a.workspace + int64_t(slice) * a.rows * a.cols : a.y;
     const uint32_t pitch = uint32_t(a.cols) * 4;
@@ -439,7 +443,8 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
 
 // Waves a SIMD: one of the largest tiles, whose sums take half of its registers or more, two of the next.
 template <int BM, int BN, int STAGES, int WAVES_M, int WAVES_N>
-__global__ __launch_bounds__(64 * WAVES_M * WAVES_N) __attribute__((amdgpu_waves_per_eu(BM * BN > 32768 ? 1 : BM * BN > 8192 ? 2 : 3))) void tile_kernel(
+__global__ __launch_bounds__(64 * WAVES_M * WAVES_N)
+    __attribute__((amdgpu_waves_per_eu(BM * BN > 32768 ? 1 : BM * BN > 8192 ? 2 : 3))) void tile_kernel(
     ProductArgs a, int tiles_m, int tiles_n, int blocks_per_slice) {
     multiply_tile<BM, BN, STAGES, WAVES_M, WAVES_N>(a, tiles_m, tiles_n, blocks_per_slice);
 }
@@ -477,13 +482,14 @@ hipError_t launch_tiles(const ProductArgs& a, int64_t slices, hipStream_t stream
 // Tiles and slices of the inner dimension by their time in us: a CU takes `block` for a block of a tile, whether it has
 // one tile or several at once, and writes outputs at 20 KB a us; the slices' second kernel takes 5 and 2 more per million
 // sums. The larger a tile, the fewer conversions and reads of LDS for each product, and the more its edges and last round
-// waste. The times are of 8192 x 8192 x 8192 and 6001 x 4096 x 14336, where the tiles took, in this order:
+// waste. The times are of 8192 x 8192 x 8192 and 6001 x 14336 x 4096, where the tiles took, in this order:
 //   817, 887, 918, 1069, 1389, 1736 us and 626, 563, 591, 711, 921, 1104 us.
 struct Tile {
     int rows, cols;
     double block;
 };
-constexpr Tile kTiles[] = {{256, 256, 3.0}, {192, 256, 2.42}, {128, 256, 1.70}, {128, 128, 0.99}, {64, 128, 0.65}, {64, 64, 0.41}};
+constexpr Tile kTiles[] = {{256, 256, 3.00}, {192, 256, 2.42}, {128, 256, 1.70},
+                           {128, 128, 0.99}, {64, 128, 0.65},  {64, 64, 0.41}};
 void choose_tile(const ProductArgs& a, int& tile, int64_t& slices) {
     double least = 0;
     tile = -1;
@@ -504,7 +510,7 @@ template <int R, int C, int W>
 hipError_t launch_few_rows(const ProductArgs& a, hipStream_t stream) {
     const int64_t groups = (a.cols + 16 * C - 1) / (16 * C);
     // Slices of the inner dimension where column groups are few: a workgroup takes about 62 KB of operands in a us, the
-    // second kernel 3 us (16 x 768 x 28672: 12.1 us in five slices, 22.1 in one).
+    // second kernel 3 us (16 x 28672 x 768: 12.1 us in five slices, 22.1 in one).
     int64_t slices = 1;
     const double whole = double(16 * (R + C) * a.blocks * kBlock) / 62e3;
     double least = whole;

@@ -5,7 +5,8 @@
 // A is at most 464; codes are the values times 2^-e rounded to e4m3, to nearest
 // even. The scaling is by a power of two, so each step is exact but the one
 // rounding. Both ways are bound by memory: 4 bytes a value on the fp32 side
-// against 1.01.
+// against 1.01. 1999 x 4001 take 8.3 us there and 9.3 back (from the last-level
+// cache), 8192 x 4096 30 us back (5.6 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -53,8 +54,8 @@ __global__ __launch_bounds__(kThreads) void dequantize_rows_kernel(OperandArgs a
 
 // Columns of a row-major source, [inner, rows]: a workgroup takes a block of 64 neighbouring rows of the format, a wave 32
 // of its 128 values of each, so that loads and stores on the fp32 side are 256 contiguous bytes a wave. The codes are turned
-// in LDS, so that eight lanes store a row's 128 bytes (14336 x 4096: 51 us, 5.8 TB/s, against 77 where each lane
-// stored its own 32).
+// in LDS, so that eight lanes store a row's 128 bytes (14336 x 4096 from the last-level cache: 51 us, 5.8 TB/s,
+// against 77 where each lane stored its own 32; 78 from HBM, and as long with 512 bytes a wave).
 constexpr int kTurned = 128 + 16;  // bytes of a row in LDS: 16 rows' chunks are in different banks
 __global__ __launch_bounds__(kThreads) void quantize_columns_kernel(OperandArgs a) {
     __shared__ uint32_t largest[4][64];

@@ -34,8 +34,8 @@ int check_shape(const sn_logprob_shape* shape, bool tokens, Needs* need) {
     const sn_logprob_shape& s = *shape;
     size_t columns, end;
     if (!product(s.rows, s.cols, &need->logits) || !product(s.rows, s.heads, &need->places) ||
-        need->logits >= kMaxLogits || need->places >= kMaxHeads || s.classes >= kMaxClasses || !product(s.heads, s.classes, &columns) ||
-        !sum(columns, s.column_offset, &end))
+        need->logits >= kMaxLogits || need->places >= kMaxHeads || s.classes >= kMaxClasses ||
+        !product(s.heads, s.classes, &columns) || !sum(columns, s.column_offset, &end))
         return SN_ERR_OVERFLOW;
     if (end > s.cols || (s.heads > 0 && s.classes == 0)) return SN_ERR_SHAPE;
     if (s.top > SN_LOGPROBS_LARGEST_TOP || !(s.scale > 0.f) || !std::isfinite(s.scale)) return SN_ERR_UNSUPPORTED;

@@ -1,7 +1,8 @@
 // The residual addition with the root-mean-square norm, and its gradients
 // (staleynet_norm.h has the formulas).
 //
-// Bound by memory: 12 to 16 bytes a value against a handful of operations. A row
+// Bound by memory: 12 to 16 bytes a value against a handful of operations. 8192 x 4096 with a residual takes 97 us in fp32
+// (5.5 TB/s) and 88 to 97 with an 8-bit output; its gradients, 8192 x 768, 21 us and 2 to 5 for d_weight's partial sums. A row
 // is read once and stays in registers; its sum of squares and y are formed in 64
 // bits (their products of fp32 values are exact there, and the vector units run
 // them at the fp32 rate), so that y is the correctly rounded one but for
