@@ -454,7 +454,13 @@ __global__ __launch_bounds__(256) void slices_kernel(ProductArgs a, int slices) 
     const int64_t count = a.rows * a.cols;
     for (int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x; e < count; e += int64_t(gridDim.x) * 256) {
         float total = 0.f;
-        for (int s = 0; s < slices; ++s) total += a.workspace[s * count + e];
+        for (int s = 0; s < slices; s += 8) {  // eight in flight
+            float part[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) part[u] = s + u < slices ? a.workspace[(s + u) * count + e] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) total += part[u];
+        }
         finish(a, e, e % a.cols, total);
     }
 }
@@ -480,16 +486,17 @@ hipError_t launch_tiles(const ProductArgs& a, int64_t slices, hipStream_t stream
 }
 
 // Tiles and slices of the inner dimension by their time in us: a CU takes `block` for a block of a tile, whether it has
-// one tile or several at once, and writes outputs at 20 KB a us; the slices' second kernel takes 5 and 2 more per million
-// sums. The larger a tile, the fewer conversions and reads of LDS for each product, and the more its edges and last round
+// one tile or several at once, and writes outputs at 20 KB a us; the slices' second kernel takes 3.5 and 1.5 more per
+// million sums. The larger a tile, the fewer conversions and reads of LDS for each product, and the more its edges and last round
 // waste. The times are of 8192 x 8192 x 8192 and 6001 x 14336 x 4096, where the tiles took, in this order:
-//   817, 887, 918, 1069, 1389, 1736 us and 626, 563, 591, 711, 921, 1104 us.
+//   817, 887, 918, 1069, 1389, 1736 us and 626, 563, 591, 711, 921, 1104 us,
+// and for the two smallest of 100 x 8192 x 8192 and 65 x 4096 x 14336, where a CU has one of them (34.4 and 27.8 us).
 struct Tile {
     int rows, cols;
     double block;
 };
 constexpr Tile kTiles[] = {{256, 256, 3.00}, {192, 256, 2.42}, {128, 256, 1.70},
-                           {128, 128, 0.99}, {64, 128, 0.65},  {64, 64, 0.41}};
+                           {128, 128, 0.99}, {64, 128, 0.75},  {64, 64, 0.475}};
 void choose_tile(const ProductArgs& a, int& tile, int64_t& slices) {
     double least = 0;
     tile = -1;
@@ -500,7 +507,7 @@ void choose_tile(const ProductArgs& a, int& tile, int64_t& slices) {
         for (int64_t n = 1; n <= most; ++n) {
             const int64_t rounds = (tiles * n + a.cu_count - 1) / a.cu_count, blocks = (a.blocks + n - 1) / n;
             double cost = double(rounds) * (double(blocks) * t.block + double(t.rows * t.cols) * 4 / 20e3);
-            if (n > 1) cost += 5 + 2e-6 * double(n * a.rows * a.cols);
+            if (n > 1) cost += 3.5 + 1.5e-6 * double(n * a.rows * a.cols);
             if (tile < 0 || cost < least) least = cost, tile = i, slices = n;
         }
     }
@@ -510,7 +517,7 @@ template <int R, int C, int W>
 hipError_t launch_few_rows(const ProductArgs& a, hipStream_t stream) {
     const int64_t groups = (a.cols + 16 * C - 1) / (16 * C);
     // Slices of the inner dimension where column groups are few: a workgroup takes about 62 KB of operands in a us, the
-    // second kernel 3 us (16 x 28672 x 768: 12.1 us in five slices, 22.1 in one).
+    // second kernel 3 us (16 x 28672 x 768: 11.2 us in five slices, 22.1 in one).
     int64_t slices = 1;
     const double whole = double(16 * (R + C) * a.blocks * kBlock) / 62e3;
     double least = whole;
