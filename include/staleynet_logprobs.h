@@ -69,8 +69,11 @@ int sn_token_logprobs(sn_context *context, const sn_logprob_shape *shape, const 
  *   grad_c = a (d_logprob ([c = token] - p_c) - d_entropy p_c (log p_c + H))
  * written to the heads' columns of grad [rows, cols]; other columns are left
  * alone. An empty token has no d_logprob term, one that is no class no [c =
- * token] term. tokens may be null without d_logprobs. grad may be logits
- * itself; any other overlap is SN_ERR_ALIASING. `top` is not used. */
+ * token] term. A place with no d_logprob term (an empty token, or no
+ * d_logprobs) and no d_entropy, or one of 0, has gradient 0 whatever its
+ * logits; else a head with a NaN or +inf, or without a finite logit, has NaN.
+ * tokens may be null without d_logprobs. grad may be logits itself; any other
+ * overlap is SN_ERR_ALIASING. `top` is not used. */
 int sn_token_logprobs_backward(sn_context *context, const sn_logprob_shape *shape, const float *logits,
                                size_t logits_len, const uint32_t *tokens, size_t tokens_len, const float *stats,
                                size_t stats_len, const float *entropies, size_t entropies_len,

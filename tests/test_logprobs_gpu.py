@@ -422,3 +422,34 @@ def test_captured_calls_replay(gpu):
             gpu.token_logprobs(t[0], case.heads, t[1], out[0], out[1], out[2], 2, ids, out[3])
     finally:
         graph.close()
+
+
+@pytest.mark.parametrize("classes", [1, 40, 513, 1024, 1027, 30000])
+def test_places_without_a_term_have_no_gradient(gpu, classes):
+    """An empty token, or no d_logprobs, with no d_entropy: zeros, in heads without a finite logit or with NaN and
+    infinities too. The other places are the same bits as without such rows."""
+    case = Case(9, 2, classes, column_offset=1, after=2, seed=13, scale=0.7)
+    bad = case.logits[:, 1:-2].reshape(9, 2, classes).copy()
+    bad[0] = -np.inf
+    bad[1, :, classes // 2] = np.nan
+    bad[2, 0, classes - 1], bad[2, 1] = np.inf, np.inf
+    bad[3] = np.nan
+    good = case.logits.copy()
+    case.token_rows[:5] = EMPTY
+    case.token_rows[5, 0], case.token_rows[6, 1] = EMPTY, classes
+    case.d_entropies[:5], case.d_entropies[4, 1] = 0.0, -0.0
+    case.d_logprobs[0], case.d_logprobs[1] = np.nan, np.inf  # an empty token's is not used
+    for which in (("logprobs", "entropies"), ("logprobs",), ("entropies",), ()):
+        case.logits = good
+        forward = case.forward(gpu, 0, want=("entropies", "stats"))
+        want = run_backward(gpu, case, forward["stats"], forward["entropies"], which)
+        case.logits = good.copy()
+        case.logits[:4, 1:-2] = bad.reshape(9, -1)[:4]
+        forward = case.forward(gpu, 0, want=("entropies", "stats"))
+        assert np.isnan(forward["stats"][:4, :, 0]).all()
+        for in_place in (False, True):
+            got = run_backward(gpu, case, forward["stats"], forward["entropies"], which, in_place=in_place)
+            assert (got[:5] == 0).all()
+            assert np.array_equal(got, want)
+        if not which:
+            assert not got.any()
