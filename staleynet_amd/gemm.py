@@ -343,6 +343,9 @@ class Fp8Matrix:
     codes: ByteBuffer
     scales: ByteBuffer
 
+    def __post_init__(self):
+        _check_sizes("Fp8Matrix", self.rows, self.inner)
+
     def buffers(self) -> list:
         """The two buffers as the C ABI takes them: pointer and bytes each."""
         return [ctypes.c_void_p(self.codes.pointer), len(self.codes), ctypes.c_void_p(self.scales.pointer),
