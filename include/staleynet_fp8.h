@@ -24,7 +24,7 @@
  *
  * Limits, past which a call is SN_ERR_OVERFLOW: rows and inner length of a
  * matrix to quantize under 2^31; of a product, rows under 2^28, columns under
- * 2^24 and inner length under 2^23.
+ * 2^24, inner length under 2^23, and tiles of 256 x 256 outputs under 2^24.
  *
  * Buffers are bytes in device memory (sn_alloc_bytes of staleynet_fp4.h, or any
  * other). Code buffers are 16-byte aligned and scale buffers 4-byte aligned

@@ -18,7 +18,7 @@ using namespace sn::abi;
 using namespace sn::fp8;
 
 constexpr size_t kMaxDimension = size_t(1) << 31;
-constexpr size_t kMaxRows = size_t(1) << 28;   // of a product: 32-bit tile counters
+constexpr size_t kMaxRows = size_t(1) << 28;   // of a product; its tiles are counted in the call
 constexpr size_t kMaxCols = size_t(1) << 24;   // of a product: 32 rows of outputs are less than 2^31 bytes
 constexpr size_t kMaxInner = size_t(1) << 23;  // of a product: 256 rows of codes lie within 32-bit offsets
 
@@ -95,7 +95,8 @@ int sn_matmul_fp8(sn_context* ctx, const sn_matmul_spec* spec, const uint8_t* le
     size_t left_codes_need, left_scales_need, right_codes_need, right_scales_need;
     if (sn_fp8_sizes(spec->rows, spec->inner, &left_codes_need, &left_scales_need) != SN_OK ||
         sn_fp8_sizes(spec->cols, spec->inner, &right_codes_need, &right_scales_need) != SN_OK ||
-        spec->inner >= kMaxInner || spec->rows >= kMaxRows || spec->cols >= kMaxCols)
+        spec->inner >= kMaxInner || spec->rows >= kMaxRows || spec->cols >= kMaxCols ||
+        (spec->rows + kLargestTile - 1) / kLargestTile * ((spec->cols + kLargestTile - 1) / kLargestTile) >= kMaxTiles)
         return SN_ERR_OVERFLOW;
     if (left_codes_len < left_codes_need || left_scales_len < left_scales_need) return SN_ERR_LEFT_TOO_SMALL;
     if (right_codes_len < right_codes_need || right_scales_len < right_scales_need) return SN_ERR_RIGHT_TOO_SMALL;

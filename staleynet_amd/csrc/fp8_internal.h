@@ -31,7 +31,9 @@ struct OperandArgs {
 };
 hipError_t launch_operand(const OperandArgs& args, bool quantize, hipStream_t stream);
 
-// Products of two 8-bit operands (fp8_matmul.hip).
+// Products of two 8-bit operands (fp8_matmul.hip): less than kMaxTiles tiles of 256 threads, as a launch is less than 2^32
+// threads; the largest tiles are kLargestTile rows by as many columns.
+constexpr int64_t kMaxTiles = int64_t(1) << 24, kLargestTile = 256;
 struct ProductArgs {
     const uint8_t* x = nullptr;
     const uint8_t* x_scales = nullptr;

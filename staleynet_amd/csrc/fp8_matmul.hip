@@ -498,7 +498,7 @@ struct Tile {
     int rows, cols;
     double block;
 };
-constexpr Tile kTiles[] = {{256, 256, 3.00}, {192, 256, 2.42}, {128, 256, 1.70},
+constexpr Tile kTiles[] = {{kLargestTile, kLargestTile, 3.00}, {192, 256, 2.42}, {128, 256, 1.70},
                            {128, 128, 0.99}, {64, 128, 0.75},  {64, 64, 0.475}};
 void choose_tile(const ProductArgs& a, int& tile, int64_t& slices) {
     double least = 0;
@@ -506,6 +506,7 @@ void choose_tile(const ProductArgs& a, int& tile, int64_t& slices) {
     for (int i = 0; i < int(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
         const Tile& t = kTiles[i];
         const int64_t tiles = ((a.rows + t.rows - 1) / t.rows) * ((a.cols + t.cols - 1) / t.cols);
+        if (tiles >= kMaxTiles) continue;  // never the largest
         const int64_t most = held_slices(a, std::min<int64_t>({2 * int64_t(a.cu_count) / tiles, a.blocks / 2, 32}));
         for (int64_t n = 1; n <= most; ++n) {
             const int64_t rounds = (tiles * n + a.cu_count - 1) / a.cu_count, blocks = (a.blocks + n - 1) / n;

@@ -230,3 +230,18 @@ def test_the_rust_binding_matches_the_headers():
         want = [rust_type(re.fullmatch(r"(.*?)(\w+)", p.strip()).group(1)) for p in " ".join(params.split()).split(",")]
         got = re.search(rf"pub fn {name}\((.*?)\)\s*->\s*c_int;", block, flags=re.S).group(1)
         assert [" ".join(p.split(":", 1)[1].split()) for p in " ".join(got.split()).split(",")] == want, name
+
+
+def test_products_of_more_tiles_than_a_launch_holds_are_refused():
+    """2^24 tiles of 256 x 256 outputs and 256 threads each would be 2^32 threads."""
+    def product(rows, cols):
+        spec = MatmulSpec.new(rows, cols, 1).right_transposed()
+        (x, x_scales), (w, w_scales) = gemm.fp8_sizes(rows, 1), gemm.fp8_sizes(cols, 1)
+        return call("sn_matmul_fp8", spec.to_c(), (1, x), (2, x_scales), (3, w), (4, w_scales), (None, 0), (6, rows * cols))
+
+    assert product(4096 * 256, 4095 * 256) == gemm.SN_ERR_NULL_ARGUMENT  # the context
+    assert product(4096 * 256, 4095 * 256 + 1) == gemm.SN_ERR_OVERFLOW
+    assert product(4095 * 256 + 1, 4096 * 256) == gemm.SN_ERR_OVERFLOW
+    assert product((1 << 28) - 1, (1 << 24) - 1) == gemm.SN_ERR_OVERFLOW
+    assert product((1 << 28) - 1, 64) == gemm.SN_ERR_NULL_ARGUMENT
+    assert product(64, (1 << 24) - 1) == gemm.SN_ERR_NULL_ARGUMENT
