@@ -468,11 +468,6 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_backward_kernel(LogprobB
             if (token != kEmptyToken) d_logprob = a.d_logprobs[place];
         }
         if (a.d_entropies != nullptr) d_entropy = a.d_entropies[place], entropy = a.entropies[place];
-        if (token == kEmptyToken && d_entropy == 0.f) {  // no term, also of a head whose p is NaN
-            const int64_t end = min(chunk + 256 * VECTORS, a.classes);
-            for (int64_t c = chunk + lane; c < end; c += 64) grad[c] = 0.f;
-            continue;
-        }
         auto grad_of = [&](float logit, int64_t c) {
             const float log_p = (logit - m) * a.scale - log_total, p = __builtin_amdgcn_exp2f(log_p * kLog2e);
             const float one = uint64_t(c) == token ? d_logprob : 0.f;
@@ -484,6 +479,13 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_backward_kernel(LogprobB
         for (int i = 0; i < VECTORS; ++i) {
             const int64_t c = chunk + 4 * (lane + 64 * i);
             if (c + 4 <= a.classes) v[i] = *reinterpret_cast<const f32x4_unaligned*>(x + c);
+        }
+        // No term: zeros, also in a head whose p is NaN. (Ahead of the logits' loads the branch had them wait for the token's:
+        // 333 x 50001 23.0 us against 21.4.)
+        if (token == kEmptyToken && d_entropy == 0.f) {
+            const int64_t end = min(chunk + 256 * VECTORS, a.classes);
+            for (int64_t c = chunk + lane; c < end; c += 64) grad[c] = 0.f;
+            continue;
         }
 #pragma unroll
         for (int i = 0; i < VECTORS; ++i) {
