@@ -148,7 +148,8 @@ __global__ __launch_bounds__(THREADS > 512 ? THREADS : 512) void rms_norm_grad_k
     const float by_width = 1.f / float(a.width);
     const int64_t groups = (a.rows + kRows - 1) / kRows;
     for (int64_t rows = blockIdx.x; rows < groups; rows += gridDim.x) {
-        // The last group's rows past the end are the last row again, without its results.
+        // The last group's rows past the end are the last row again, without its results; d_sum, which d_x may be written
+        // over, is not theirs to read.
         const int64_t row = min(rows * kRows + group, a.rows - 1);
         const bool live = rows * kRows + group < a.rows;
         const float inverse = a.inverse[row];
@@ -159,7 +160,7 @@ __global__ __launch_bounds__(THREADS > 512 ? THREADS : 512) void rms_norm_grad_k
             const int64_t k = 8 * (thread + THREADS * i);
             load8(a.sum + row * a.width, k, a.width, n[i]);
             load8(a.d_out + row * a.width, k, a.width, g[i]);
-            if (a.d_sum != nullptr) load8(a.d_sum + row * a.width, k, a.width, before[i]);
+            if (a.d_sum != nullptr && live) load8(a.d_sum + row * a.width, k, a.width, before[i]);
         }
 #pragma unroll
         for (int i = 0; i < VECTORS; ++i) {

@@ -315,3 +315,16 @@ def test_captured_norms_replay(gpu):
             gpu.rms_norm_backward(out[0], out[3], t[3], t[2], out[2], rows, None, out[4])
     finally:
         graph.close()
+
+
+@pytest.mark.parametrize("rows,width", [(1, 300), (9, 500), (3, 768), (4097, 768), (5, 2000), (1025, 1500)])
+def test_gradients_in_place_of_groups_that_are_not_full(gpu, rows, width):
+    """d_x over d_sum, with d_weight, where the last workgroup has more row groups than rows: the bits of other buffers."""
+    s, inverse, weight, d_out, d_sum = grad_inputs(rows, width, rows)
+    before = np.ones(width, np.float32)
+    want, want_w = gradients(gpu, s, inverse, weight, d_out, d_sum, before)
+    d_x, d_x_off, _, _ = backward(s, inverse, weight, d_out, d_sum)
+    assert (np.abs(want - d_x) <= d_x_off).all()
+    for _ in range(3):
+        got, got_w = gradients(gpu, s, inverse, weight, d_out, d_sum, before, onto=True)
+        assert np.array_equal(got, want) and np.array_equal(got_w, want_w)
