@@ -13,10 +13,11 @@
  *   y = weight * s * i                     (computed in 64 bits, rounded once)
  * NaN and infinities follow IEEE arithmetic, and stay in their row. Rows are
  * dense, [rows, width]. epsilon is at least 0 and finite (SN_ERR_UNSUPPORTED
- * otherwise). Nothing is written where rows or width is 0. Limits, past which a call is SN_ERR_OVERFLOW: rows under 2^31,
- * width under 2^25. Lengths count elements of their buffer (too short:
- * SN_ERR_LENGTH_MISMATCH). The calls are asynchronous on the context's stream,
- * allocate nothing, may be captured into a graph, and are deterministic.
+ * otherwise). Nothing is written where rows or width is 0. Limits, past which a
+ * call is SN_ERR_OVERFLOW: rows under 2^31, width under 2^25. Lengths count
+ * elements of their buffer (too short: SN_ERR_LENGTH_MISMATCH). The calls are
+ * asynchronous on the context's stream, allocate nothing, may be captured into a
+ * graph, and are deterministic.
  */
 #ifndef STALEYNET_NORM_H
 #define STALEYNET_NORM_H
@@ -43,7 +44,8 @@ int sn_rms_norm(sn_context *context, const sn_rms_norm_shape *shape, const float
                 size_t sum_len, float *out, size_t out_len, float *inverse, size_t inverse_len);
 
 /* The same with y rounded to 8-bit rows, the left operand of sn_matmul_fp8:
- * the bits that sn_quantize_fp8 would give of sn_rms_norm's output. */
+ * the bits that sn_quantize_fp8 would give of sn_rms_norm's output. It leaves no
+ * inverse: a step that goes back through the norm has it from sn_rms_norm. */
 int sn_rms_norm_fp8(sn_context *context, const sn_rms_norm_shape *shape, const float *x, size_t x_len,
                     const float *residual, size_t residual_len, const float *weight, size_t weight_len, float *sum,
                     size_t sum_len, uint8_t *codes, size_t codes_len, uint8_t *scales, size_t scales_len);

@@ -90,7 +90,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void rms_norm_kernel
             __syncthreads();
         }
         const double inverse = inverse_of(a, squares);
-        if (a.inverse != nullptr && thread == 0) a.inverse[row] = float(inverse);
+        if (!EIGHT && a.inverse != nullptr && thread == 0) a.inverse[row] = float(inverse);
 #pragma unroll
         for (int i = 0; i < VECTORS; ++i) store_results<EIGHT>(a, row, 8 * (thread + THREADS * i), s[i], inverse);
     }
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(512) void rms_norm_wide_kernel(RmsNormArgs a) {
         for (int i = 0; i < 8; ++i) squares += partial[i];
         __syncthreads();
         const double inverse = inverse_of(a, squares);
-        if (a.inverse != nullptr && threadIdx.x == 0) a.inverse[row] = float(inverse);
+        if (!EIGHT && a.inverse != nullptr && threadIdx.x == 0) a.inverse[row] = float(inverse);
         for (int64_t k = 8 * threadIdx.x; k < blocks_of(a.width) * kBlock; k += 8 * 512) {
             float s[8];
             load_sum(a, row, k, s);
