@@ -381,3 +381,32 @@ def test_captured_products_replay(gpu):
             gpu.matmul_fp8(calls[1][0], calls[1][3], calls[1][4], calls[1][5])
     finally:
         graph.close()
+
+
+@pytest.mark.parametrize("rows,inner", [(70, 33000), (1, 40001), (130, 32897)])
+def test_columns_of_more_blocks_than_a_grid_holds(gpu, rows, inner):
+    """Transposed operands of more than 256 blocks, as a batch's tokens are a weight gradient's inner dimension."""
+    test_quantize_and_back(gpu, rows, inner, Storage.Transposed)
+
+
+@pytest.mark.parametrize("rows,inner,cols", [(2701, 2348, 68), (129, 9077, 6403), (4109, 4929, 932)])
+def test_slices_of_the_other_tiles(gpu, rows, inner, cols):
+    """Tiles of 64 x 128, 192 x 256 and 256 x 256 with the inner dimension in slices."""
+    left, right = operand(rows, inner, rows), operand(cols, inner, cols)
+    rng = np.random.default_rng(rows)
+    before, bias = (rng.standard_normal(n).astype(np.float32) for n in ((rows, cols), cols))
+    spec = MatmulSpec.new(rows, cols, inner).scaled(0.25).accumulate()
+    check(run(gpu, spec, left, right, bias, before), left[2], right[2], inner, 0.25, before, bias)
+
+
+@pytest.mark.parametrize("tokens,width,cols", [(1, 40, 70), (333, 200, 300), (1100, 768, 130), (4099, 96, 513)])
+def test_a_weight_gradient(gpu, tokens, width, cols):
+    """dW += X^T dY: both operands transposed to 8-bit blocks along the tokens."""
+    rng = np.random.default_rng(tokens)
+    x, d_y = (rng.standard_normal((tokens, n)).astype(np.float32) for n in (width, cols))
+    before = rng.standard_normal((width, cols)).astype(np.float32)
+    left, right = (same_as_reference(gpu, np.ascontiguousarray(v.T), storage=Storage.Transposed) for v in (x, d_y))
+    out = gpu.upload(Shape(width, cols), before)
+    gpu.matmul_fp8(MatmulSpec.new(width, cols, tokens).right_transposed().accumulate(), left[2], right[2], out)
+    a, b = (ref.dequantize(*m[:2], tokens) for m in (left, right))
+    check(gpu.download(out).reshape(width, cols), a, b, tokens, before=before)

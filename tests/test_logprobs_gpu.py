@@ -453,3 +453,33 @@ def test_places_without_a_term_have_no_gradient(gpu, classes):
             assert np.array_equal(got, want)
         if not which:
             assert not got.any()
+
+
+def test_captured_lists_replay(gpu):
+    """The listed classes of split and unsplit rows, overwritten before each replay."""
+    sets = []
+    for rows, heads, classes in ((4, 16, 1024), (2, 1, 30000)):
+        case = Case(rows, heads, classes, seed=14)
+        n = 6 * rows * heads
+        sets.append((case, Placed(gpu, case.logits), gpu.upload_tokens(np.zeros(n, np.uint32)), gpu.zeros(Shape.vector(n))))
+
+    def step():
+        for case, logits, ids, best in sets:
+            gpu.token_logprobs(logits, case.heads, top=6, top_tokens=ids, top_logprobs=best)
+
+    def results():
+        return [np.asarray(gpu.download_tokens(s[2])) for s in sets] + [gpu.download(s[3]) for s in sets]
+
+    step()
+    want = results()
+    graph = HipGraph(gpu.stream, step)
+    try:
+        for _ in range(3):
+            for case, logits, ids, best in sets:  # other lists: of the negated logits
+                gpu.token_logprobs(Placed(gpu, -case.logits), case.heads, top=6, top_tokens=ids, top_logprobs=best)
+            assert not any(np.array_equal(a, b) for a, b in zip(results(), want))
+            graph.launch()
+            gpu.synchronize()
+            assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+    finally:
+        graph.close()

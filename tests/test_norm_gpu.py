@@ -328,3 +328,59 @@ def test_gradients_in_place_of_groups_that_are_not_full(gpu, rows, width):
     for _ in range(3):
         got, got_w = gradients(gpu, s, inverse, weight, d_out, d_sum, before, onto=True)
         assert np.array_equal(got, want) and np.array_equal(got_w, want_w)
+
+
+@pytest.mark.parametrize("rows,width", [(1100, 768), (1027, 1000), (1025, 513), (1999, 1024)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_many_rows_in_8_bits(gpu, rows, width, in_place):
+    """Rows of two vectors a lane, more of them than four a CU: the quantized fp32 output's bits."""
+    x, residual, weight = inputs(rows, width, rows)
+    wt, y = place(gpu, weight), place(gpu, np.zeros(x.size))
+    gpu.rms_norm(place(gpu, x), wt, y, EPSILON, rows, place(gpu, residual))
+    codes, scales = rows * ref.blocks_of(width) * 128, rows * ref.scale_stride(width)
+    held = [gpu.upload_bytes(np.full(n + 64, 99, np.uint8)) for n in (codes, scales)]
+    matrix = Fp8Matrix(rows, width, View(held[0], 0, codes, 1), View(held[1], 0, scales, 1))
+    xt = place(gpu, x)
+    total = xt if in_place else place(gpu, np.zeros(x.size))
+    gpu.rms_norm(xt, wt, matrix, EPSILON, rows, place(gpu, residual), total)
+    s = x + residual
+    assert np.array_equal(fetch(gpu, total, s.shape), s)
+    got = fetch(gpu, y, s.shape)
+    want, _ = expected(s, weight)
+    assert (np.abs(got - want) <= (U + 2.0 ** -40) * np.abs(want) + 2.0 ** -150).all()
+    got_codes, got_scales = (gpu.download_bytes(b) for b in held)
+    assert (got_codes[codes:] == 99).all() and (got_scales[scales:] == 99).all()
+    want_codes, want_scales = ref.quantize(got)
+    assert np.array_equal(got_scales[:scales].reshape(rows, -1), want_scales)
+    assert np.array_equal(got_codes[:codes].reshape(rows, -1), want_codes)
+
+
+def test_captured_8_bit_norms_replay(gpu):
+    """The codes and scales of captured norms, overwritten before each replay."""
+    sets = []
+    for rows, width in ((1, 768), (600, 300), (1100, 768), (40, 9000), (2, 20000)):
+        x, _, weight = inputs(rows, width, 15)
+        matrix = gpu.fp8_matrix(rows, width)
+        other = gpu.upload(Shape(rows, width), 1 - x)
+        sets.append((rows, gpu.upload(Shape(rows, width), x), gpu.upload(Shape.vector(width), weight), matrix, other))
+
+    def step():
+        for rows, x, weight, matrix, _ in sets:
+            gpu.rms_norm(x, weight, matrix, EPSILON, rows)
+
+    def results():
+        return [gpu.download_bytes(b) for s in sets for b in (s[3].codes, s[3].scales)]
+
+    step()
+    want = results()
+    graph = HipGraph(gpu.stream, step)
+    try:
+        for _ in range(3):
+            for rows, _, weight, matrix, other in sets:
+                gpu.rms_norm(other, weight, matrix, 1e30, rows)  # other codes, and factors far smaller
+            assert not any(np.array_equal(a, b) for a, b in zip(results(), want))
+            graph.launch()
+            gpu.synchronize()
+            assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+    finally:
+        graph.close()
