@@ -11,10 +11,12 @@
  * m, and the scale a (an inverse temperature):
  *   z_c = a (x_c - m),  T = log(sum of e^(z_c)),  log p_c = z_c - T
  *   logprob = log p_token,  entropy = H = -sum of p_c log p_c
- * A logit of -inf has probability 0 and adds nothing to H. A row of a head with
- * a NaN or +inf, or without a finite logit, gives NaN in all but the top
- * tokens. Sums are fp32; T is log(1 + the sum without the largest term), so
- * that log probabilities and entropies near 0 keep their digits.
+ * A logit of -inf has probability 0 and adds nothing to H, and so has one that
+ * is further below m than fp32 reaches. A row of a head with a NaN or +inf, or
+ * without a finite logit, gives NaN in all but the top tokens, an empty token's
+ * log probability (0) and the places past the classes. Sums are fp32; T is
+ * log(1 + the sum without the largest term), so that log probabilities and
+ * entropies near 0 keep their digits.
  */
 #ifndef STALEYNET_LOGPROBS_H
 #define STALEYNET_LOGPROBS_H

@@ -6,9 +6,10 @@
 // values is exact in fp32, so fragments are codes converted in registers and
 // multiplied by the bf16 matrix instructions, which sum in fp32. The 8-bit
 // matrix instructions (v_mfma_scale_f32_16x16x128_f8f6f4 and the 16x16x32 forms)
-// would run twice as fast, but were measured to align the products of
-// neighbouring k to the largest of them and to cut off what lies 13 bits below: random codes
-// come out up to 2^-12 of the largest product wrong, where fp32 sums are
+// would run twice as fast, but were measured to align the products of eight
+// neighbouring k to the largest of them and to cut off what lies more than 13
+// bits below: sums of 128 products of random codes come out up to 2^-11.2 of the
+// largest product wrong (the bf16 instructions' 2^-19.9), where fp32 sums are
 // asked for.
 #include <hip/hip_runtime.h>
 
@@ -213,7 +214,8 @@ __device__ __forceinline__ int swizzle(int row) { return (row >> 2) & 3; }
 // Bound by the matrix cores, and at large sizes by the power they draw: 6001 x 4096 x 14336 takes 554 to 589 us by the
 // card (1196 to 1272 TFLOP/s; the library's bf16 product of the same shape 590), 8192 x 8192 x 8192 807 us (1362). A wave
 // of the 256 x 256 tile converts 32 pairs a lane for sixteen matrix instructions of 32 cycles, one of the 128 x 256 tile 24
-// for eight. A step of 64 along the inner dimension is four units of one 32x32x16 instruction a block; while a unit is multiplied the
+// for eight; it takes all 512 registers of a lane, and 16 of its 256 sums pass through scratch memory between the last
+// product and the stores. A step of 64 along the inner dimension is four units of one 32x32x16 instruction a block; while a unit is multiplied the
 // next one's codes are converted and the chunk after that is read from LDS. The one barrier of a step is in its middle:
 // there every wave has read all of the step's stage, which takes the loads of STAGES steps ahead, and every wave's loads of
 // the next stage have landed.
@@ -398,7 +400,8 @@ __device__ __forceinline__ void multiply_tile(const ProductArgs& a, int tiles_m,
         wait_loads<0>();
     }
     // Outputs of the smaller tiles pass the caches by (nt), which leaves operands in them: 200 x 768 x 16384 10.1 us against 11.5,
-    // 2048 x 768 x 2304 15.0 against 16.5; with the larger ones 4096 x 4096 x 4096 took 118.5 against 114.9.
+    // 2048 x 768 x 2304 15.0 against 16.5; with the larger ones 4096 x 4096 x 4096 took 118.5 against 114.9. Slices' sums too, to
+    // no difference: 100 x 8192 x 8192 30.7 against 30.8, 512 x 14336 x 4096 71.3 to 72.2 against 71.3 to 72.6.
     constexpr int kStreamed = BM * BN <= 128 * 128 ? 2 : 0;
     // A buffer of each 32 rows' outputs (or of the slice's sums), of less than 2^31 bytes: places past the last row are out
     // of its range, and so is 2^31 with any row's offset, for columns past the last; such stores do nothing. A lane's
@@ -540,8 +543,16 @@ hipError_t launch_product(const ProductArgs& a, hipStream_t stream) {
     // the CUs hold all or most of them at once. Alternatives measured in us, rows x inner dimension x columns:
     //   16 x 14336 x 4224: <1, 2, 8> 20.9, <1, 1, 4> 23.3, <1, 1, 8> 24.5; 16 x 4096 x 14336: <1, 4, 4> 12.7, <1, 1, 4> 15.4;
     //   32 x 8192 x 28672: <2, 4, 3> 42.5, <2, 2, 4> 57.2, tiles 50.8; 32 x 4096 x 8192: <2, 2, 4> 8.9, tiles 12.3.
-    // Up to 64 rows too, for weights that come from HBM: 64 x 8192 x 8192 25.0, tiles 32.6 (25.7 and 24.9 from the last-level
-    // cache). Many columns of a short inner dimension are left to the tiles: 16 x 768 x 50304 13.2, tiles 10.9.
+    // Forms that are next to each other in the rule, weights from HBM:
+    //   16 x 4096 x 8192: <1, 2, 8> 10.4, <1, 1, 4> 11.3, <1, 4, 4> 12.3; 16 x 4096 x 12000: <1, 2, 8> 17.1, <1, 1, 4> 14.6, <1, 4, 4> 13.8;
+    //   32 x 4096 x 4096: <2, 1, 12> 9.1, <2, 2, 4> 9.8, <2, 1, 8> 8.7; 32 x 14336 x 4096: <2, 1, 12> 19.6 to 21.1,
+    //   <2, 2, 4> 19.2, <2, 1, 8> 19.5;
+    //   64 x 8192 x 8192: <4, 1, 8> 33.6, <4, 2, 6> 26.6, <4, 2, 3> 26.1; 64 x 14336 x 4096: <4, 1, 8> 27.3, <4, 2, 6> 25.9;
+    //   40 x 4096 x 4096: <4, 1, 8> 10.7, <4, 2, 6> 14.1; 64 x 8192 x 16000: <4, 2, 6> 49.1, <4, 2, 3> 43.
+    // 33 to 64 rows for weights that come from HBM: 40 x 4096 x 4096 10.7, tiles 12.4; 64 x 4096 x 16384 24.7, tiles 28.1 (20.6 and
+    // 20.0 from the last-level cache); 64 x 8192 x 16000 43, tiles 53.6 (40.5 and 36.7). The tiles lead where the inner dimension
+    // is long and columns few: 64 x 8192 x 8192 26.6, tiles 25.4; 64 x 14336 x 4096 27.4, tiles 23.2.
+    // Many columns of a short inner dimension are left to the tiles: 16 x 768 x 50304 13.2, tiles 10.9.
     const int64_t cu = a.cu_count, cols = a.cols;
     const bool few = a.rows <= 32 ? a.blocks > 8 || cols <= 64 * cu : a.rows <= 64 && cols <= 64 * cu;
     if (few) {

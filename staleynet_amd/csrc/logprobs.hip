@@ -503,8 +503,9 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_backward_kernel(LogprobB
 }
 
 // Workgroups for that many waves' items, within the 2^32 threads of a launch; the kernels' waves loop over the rest.
-// Items are counted in 32 bits: at most 2^31 places, of one part where they are many, or the 1024 logits' chunks of at most
-// 2^42 logits.
+// Items are counted in 32 bits, and so is the loop's step past them: places are less than 2^31, with parts only where they
+// are few, and the backward's chunks of 1024 of the less than 2^40 logits are less than 2^30 besides one a place, of which
+// there are less than 2^30 where a head has more than one.
 unsigned groups_of(int64_t items) { return unsigned(std::min<int64_t>((items + kWaves - 1) / kWaves, 1 << 22)); }
 
 template <int VECTORS>
